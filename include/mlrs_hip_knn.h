@@ -448,6 +448,195 @@ typedef struct mlrs_pool_stats {
 int32_t mlrs_pool_stats_get(mlrs_pool_stats *out);
 int32_t mlrs_pool_stats_reset(void);
 
+/*
+ * ---- training an embedding ----
+ * What a table of embeddings is trained with before it is searched: a layer
+ * forwards and backwards, the softmax cross entropy of many classes with its
+ * gradient, and the optimizer step.  No counterpart in the reference.
+ *
+ * Element types: _f32 (float), _f16 (IEEE half) and _bf16 (bfloat16; 16-bit
+ * elements are passed as uint16_t).  Products, sums, softmax statistics and
+ * norms are held in f32 whatever the type; a result is rounded to its type
+ * once, to nearest even.  Matrices are contiguous and row-major, aligned to
+ * their element size; other alignments than 16 bytes (or rows that are no
+ * multiple of 16 bytes) cost a copy of the operand into the workspace.
+ * Results do not depend on the stream or on other calls, and the same call
+ * gives the same bits.  Row, column and class counts are limited to 2^31 - 1
+ * and a row to 2^22 bytes (MLRS_ERR_UNSUPPORTED "features").
+ */
+#define MLRS_ACT_NONE 0
+#define MLRS_ACT_RELU 1
+#define MLRS_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define MLRS_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+#define MLRS_ACT_SILU 4      /* z / (1 + e^-z) */
+
+/*
+ * z = x w^T + bias; y = act(z) + residual.  x is n x d_in, w d_out x d_in,
+ * bias d_out (may be NULL), residual n x d_out (may be NULL), y n x d_out;
+ * preact (n x d_out, may be NULL) receives z.  y may be the residual's buffer.
+ * Errors, in this order:
+ *   ShapeMismatch "x" / "w"       n*d_in != x_len, d_out*d_in != w_len
+ *   ShapeMismatch "features"      d_in < 1 or d_out < 1
+ *   MLRS_ERR_UNSUPPORTED "features" / "rows"  sizes past the limits above
+ *   ShapeMismatch "bias" / "residual" / "out" / "preact"
+ *   MLRS_ERR_UNSUPPORTED "activation"
+ */
+int32_t mlrs_linear_f32(const float *x, int64_t x_len, int64_t n, int64_t d_in, const float *w, int64_t w_len,
+                        int64_t d_out, const float *bias, int64_t bias_len, const float *residual,
+                        int64_t residual_len, int32_t activation, float *y, int64_t y_len, float *preact,
+                        int64_t preact_len, void *stream);
+int32_t mlrs_linear_f16(const uint16_t *x, int64_t x_len, int64_t n, int64_t d_in, const uint16_t *w, int64_t w_len,
+                        int64_t d_out, const uint16_t *bias, int64_t bias_len, const uint16_t *residual,
+                        int64_t residual_len, int32_t activation, uint16_t *y, int64_t y_len, uint16_t *preact,
+                        int64_t preact_len, void *stream);
+int32_t mlrs_linear_bf16(const uint16_t *x, int64_t x_len, int64_t n, int64_t d_in, const uint16_t *w, int64_t w_len,
+                         int64_t d_out, const uint16_t *bias, int64_t bias_len, const uint16_t *residual,
+                         int64_t residual_len, int32_t activation, uint16_t *y, int64_t y_len, uint16_t *preact,
+                         int64_t preact_len, void *stream);
+
+/*
+ * The gradient of mlrs_linear: dz = dy * act'(preact); dx = dz w (n x d_in),
+ * dw = dz^T x (d_out x d_in), dbias = the column sums of dz (d_out); the
+ * residual's gradient is dy.  Any of dx, dw and dbias may be NULL (length 0).
+ * preact is what mlrs_linear kept, NULL (length 0) with MLRS_ACT_NONE.  16-bit
+ * types: dz is rounded to the type before the two products (dbias sums it
+ * unrounded).  n = 0 gives dw = 0 and dbias = 0.
+ * Errors, in this order: as mlrs_linear ("x", "w", "features", "rows"), then
+ *   ShapeMismatch "dy" / "dx" / "dw" / "dbias", MLRS_ERR_UNSUPPORTED
+ *   "activation", ShapeMismatch "preact".
+ */
+int32_t mlrs_linear_grad_f32(const float *dy, int64_t dy_len, const float *x, int64_t x_len, int64_t n, int64_t d_in,
+                             const float *w, int64_t w_len, int64_t d_out, const float *preact, int64_t preact_len,
+                             int32_t activation, float *dx, int64_t dx_len, float *dw, int64_t dw_len, float *dbias,
+                             int64_t dbias_len, void *stream);
+int32_t mlrs_linear_grad_f16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                             int64_t d_in, const uint16_t *w, int64_t w_len, int64_t d_out, const uint16_t *preact,
+                             int64_t preact_len, int32_t activation, uint16_t *dx, int64_t dx_len, uint16_t *dw,
+                             int64_t dw_len, uint16_t *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_linear_grad_bf16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                              int64_t d_in, const uint16_t *w, int64_t w_len, int64_t d_out, const uint16_t *preact,
+                              int64_t preact_len, int32_t activation, uint16_t *dx, int64_t dx_len, uint16_t *dw,
+                              int64_t dw_len, uint16_t *dbias, int64_t dbias_len, void *stream);
+
+/*
+ * Softmax cross entropy of z = h w^T + bias: lse_i = log sum_v e^(z_iv) and
+ * loss_i = lse_i - z_i,target(i), without z in memory.  h is n x d, w
+ * classes x d, bias `classes` long (may be NULL; -inf leaves a class out);
+ * target, loss and lse hold n elements.  A row whose target is `ignore_index`
+ * has loss 0 (its lse is still written); a target that is no class, loss NaN.
+ * A row all of whose logits are -inf has lse -inf, and loss NaN.
+ * Errors, in this order: ShapeMismatch "h" / "w", "features" (d or classes
+ *   < 1), MLRS_ERR_UNSUPPORTED "features" / "rows", ShapeMismatch "bias" /
+ *   "target" / "out".
+ */
+int32_t mlrs_softmax_xent_f32(const float *h, int64_t h_len, int64_t n, int64_t d, const float *w, int64_t w_len,
+                              int64_t classes, const float *bias, int64_t bias_len, const int64_t *target,
+                              int64_t target_len, int64_t ignore_index, float *loss, float *lse, int64_t out_len,
+                              void *stream);
+int32_t mlrs_softmax_xent_f16(const uint16_t *h, int64_t h_len, int64_t n, int64_t d, const uint16_t *w,
+                              int64_t w_len, int64_t classes, const uint16_t *bias, int64_t bias_len,
+                              const int64_t *target, int64_t target_len, int64_t ignore_index, float *loss, float *lse,
+                              int64_t out_len, void *stream);
+int32_t mlrs_softmax_xent_bf16(const uint16_t *h, int64_t h_len, int64_t n, int64_t d, const uint16_t *w,
+                               int64_t w_len, int64_t classes, const uint16_t *bias, int64_t bias_len,
+                               const int64_t *target, int64_t target_len, int64_t ignore_index, float *loss,
+                               float *lse, int64_t out_len, void *stream);
+
+/*
+ * The gradient of sum_i grad_i loss_i: with dz_iv = grad_i (e^(z_iv - lse_i) -
+ * [v = target(i)]), zero in ignored rows, dh = dz w (n x d), dw = dz^T h
+ * (classes x d) and dbias = the column sums of dz.  lse is mlrs_softmax_xent's
+ * of the same operands; z is computed again, in pieces of the vocabulary whose
+ * dz takes at most MLRS_XENT_PIECE_BYTES of workspace.  Any of dh, dw and dbias
+ * may be NULL (length 0).  16-bit types: dz is rounded to the type before the
+ * products (f16: scaled by a power of two first, by the largest |grad|).
+ * n = 0 gives dw = 0 and dbias = 0.
+ * Errors, in this order: as mlrs_softmax_xent ("out" being lse's and grad's
+ *   length), then ShapeMismatch "dh" / "dw" / "dbias".
+ */
+#define MLRS_XENT_PIECE_BYTES 1073741824 /* 1 GiB */
+int32_t mlrs_softmax_xent_grad_f32(const float *h, int64_t h_len, int64_t n, int64_t d, const float *w, int64_t w_len,
+                                   int64_t classes, const float *bias, int64_t bias_len, const int64_t *target,
+                                   int64_t target_len, int64_t ignore_index, const float *lse, const float *grad,
+                                   int64_t out_len, float *dh, int64_t dh_len, float *dw, int64_t dw_len,
+                                   float *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_softmax_xent_grad_f16(const uint16_t *h, int64_t h_len, int64_t n, int64_t d, const uint16_t *w,
+                                   int64_t w_len, int64_t classes, const uint16_t *bias, int64_t bias_len,
+                                   const int64_t *target, int64_t target_len, int64_t ignore_index, const float *lse,
+                                   const float *grad, int64_t out_len, uint16_t *dh, int64_t dh_len, uint16_t *dw,
+                                   int64_t dw_len, uint16_t *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_softmax_xent_grad_bf16(const uint16_t *h, int64_t h_len, int64_t n, int64_t d, const uint16_t *w,
+                                    int64_t w_len, int64_t classes, const uint16_t *bias, int64_t bias_len,
+                                    const int64_t *target, int64_t target_len, int64_t ignore_index, const float *lse,
+                                    const float *grad, int64_t out_len, uint16_t *dh, int64_t dh_len, uint16_t *dw,
+                                    int64_t dw_len, uint16_t *dbias, int64_t dbias_len, void *stream);
+
+#define MLRS_DTYPE_F32 0
+#define MLRS_DTYPE_F16 1
+#define MLRS_DTYPE_BF16 2
+
+typedef struct mlrs_grad_tensor {
+    const void *grad;
+    int64_t len;
+    int32_t dtype; /* MLRS_DTYPE_* */
+} mlrs_grad_tensor;
+
+/*
+ * norm = the root of the sum of squares of every element of `count` gradients;
+ * scale = min(1, max_norm / norm), the factor that clips them, NaN where the
+ * norm is not finite.  Both are single floats on the device, so the step that
+ * takes the factor needs no read-back.  `tensors` is host memory, read before
+ * the call returns.
+ * Errors: MLRS_ERR_NULL_POINTER, ShapeMismatch "tensors" (count < 0 or a
+ *   negative length), MLRS_ERR_UNSUPPORTED "dtype", InvalidParam "max_norm"
+ *   (not > 0).
+ */
+int32_t mlrs_grad_clip_scale(const mlrs_grad_tensor *tensors, int64_t count, double max_norm, float *norm,
+                             float *scale, void *stream);
+
+typedef struct mlrs_adamw_tensor {
+    void *param;          /* f32, or f16 / bf16 with a master */
+    const void *grad;     /* f32, f16 or bf16 */
+    void *exp_avg;        /* 32 bits: f32; 8 bits: codes */
+    void *exp_avg_sq;     /* 32 bits: f32; 8 bits: codes of the root */
+    float *master;        /* f32 value of the parameter; NULL for f32 parameters */
+    float *avg_scale;     /* 8 bits: a scale per MLRS_STATE_BLOCK elements; else NULL */
+    float *avg_sq_scale;  /* likewise */
+    int64_t len;
+    double weight_decay;
+    int32_t param_dtype, grad_dtype; /* MLRS_DTYPE_* */
+} mlrs_adamw_tensor;
+#define MLRS_STATE_BLOCK 256
+
+/*
+ * One AdamW step of `count` tensors in place, `step` counting from 1:
+ *   g = grad * scale;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps)
+ * `scale` is a float on the device (mlrs_grad_clip_scale's, the inverse of a
+ * loss scale; NULL = 1); where it is not finite nothing is changed.
+ * state_bits 32: m and v are f32.  state_bits 8: a block of MLRS_STATE_BLOCK
+ * elements of a tensor has one scale each for m and for sqrt(v), which are kept
+ * as a sign, four bits of exponent and three of fraction (m) and four and four
+ * (the root), rounded up or down at random by `seed`, the tensor's place and
+ * the element's index: give every step another seed.  All codes and scales 0 is
+ * the state before the first step.  `tensors` is host memory, read before the
+ * call returns; no tensor may appear twice.
+ * Errors: MLRS_ERR_NULL_POINTER ("master" for a 16-bit parameter without one),
+ *   ShapeMismatch "tensors", MLRS_ERR_UNSUPPORTED "dtype" / "state_bits",
+ *   InvalidParam "lr" / "betas" / "eps" / "weight_decay" / "step".
+ */
+int32_t mlrs_adamw_step(const mlrs_adamw_tensor *tensors, int64_t count, int32_t state_bits, double lr, double beta1,
+                        double beta2, double eps, int64_t step, const float *scale, uint32_t seed, void *stream);
+
+/*
+ * The values that an 8-bit state stands for: `which` 0 = exp_avg, 1 = the root
+ * of exp_avg_sq.  scales_len = the blocks of `len` elements.
+ * Errors: ShapeMismatch "codes" / "scales" / "out", MLRS_ERR_UNSUPPORTED
+ *   "which", MLRS_ERR_NULL_POINTER.
+ */
+int32_t mlrs_adamw_state_values(const uint8_t *codes, int64_t len, const float *scales, int64_t scales_len,
+                                int32_t which, float *out, int64_t out_len, void *stream);
+
 /* Release the cached device workspace of the current device. */
 int32_t mlrs_release_workspace(void);
 

@@ -85,6 +85,28 @@ class HipError(RuntimeError):
     pass
 
 
+class GradTensor(ctypes.Structure):
+    """mlrs_grad_tensor."""
+    _fields_ = [("grad", ctypes.c_void_p), ("len", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """mlrs_adamw_tensor."""
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("exp_avg", ctypes.c_void_p),
+        ("exp_avg_sq", ctypes.c_void_p),
+        ("master", ctypes.c_void_p),
+        ("avg_scale", ctypes.c_void_p),
+        ("avg_sq_scale", ctypes.c_void_p),
+        ("len", ctypes.c_int64),
+        ("weight_decay", ctypes.c_double),
+        ("param_dtype", ctypes.c_int32),
+        ("grad_dtype", ctypes.c_int32),
+    ]
+
+
 # (name, restype, argtypes) of every exported symbol in include/mlrs_hip_knn.h
 _i32, _i64, _vp, _f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
 SIGNATURES = {
@@ -130,8 +152,22 @@ SIGNATURES = {
     "mlrs_timing_enable": (_i32, [_i32]),
     "mlrs_probe_peak": (_i32, [_i32, _i32, ctypes.POINTER(_f64), _vp]),
     "mlrs_force_path": (_i32, [_i32]),
+    "mlrs_grad_clip_scale": (_i32, [ctypes.POINTER(GradTensor), _i64, _f64, _vp, _vp, _vp]),
+    "mlrs_adamw_step": (_i32, [ctypes.POINTER(AdamwTensor), _i64, _i32, _f64, _f64, _f64, _f64, _i64, _vp,
+                               ctypes.c_uint32, _vp]),
+    "mlrs_adamw_state_values": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp]),
     "mlrs_timing_read": (_i32, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64), ctypes.c_char_p, _i32]),
 }
+
+for _s in ("f32", "f16", "bf16"):
+    SIGNATURES["mlrs_linear_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp,
+                                              _i64, _vp, _i64, _vp])
+    SIGNATURES["mlrs_linear_grad_" + _s] = (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32,
+                                                   _vp, _i64, _vp, _i64, _vp, _i64, _vp])
+    SIGNATURES["mlrs_softmax_xent_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64,
+                                                    _vp, _vp, _i64, _vp])
+    SIGNATURES["mlrs_softmax_xent_grad_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                                         _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp])
 
 _lib = None
 

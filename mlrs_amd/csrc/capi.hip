@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/mlrs_hip_knn.h"
+#include "capi_shared.hpp"
 #include "knn_common.hpp"
 #include "knn_groupmin.hpp"
 #include "knn_kernels.hpp"
@@ -3278,3 +3279,43 @@ int32_t mlrs_release_workspace(void) {
 }
 
 }  // extern "C"
+
+// What the entry points of other files share with this one's.
+namespace mlrs {
+namespace capi {
+
+int32_t run_call(int32_t (*body)(void*), void* ctx) {
+    CallGuard cg;
+    return body(ctx);
+}
+int32_t error(int32_t code, const char* operand, int64_t rows, int64_t cols, int64_t len, const char* message) {
+    return set_err(code, operand, rows, cols, len, 0, "%s", message);
+}
+int32_t shape_error(const char* operand, int64_t rows, int64_t cols, int64_t len) {
+    return shape_err(operand, rows, cols, len);
+}
+int32_t hip_error(hipError_t e, const char* where) { return hip_err(e, where); }
+bool geometry(int64_t rows, int64_t cols, int64_t len) { return geom_ok(rows, cols, len); }
+int32_t scratch(size_t bytes, hipStream_t s, char** out, int* cus) { return workspace(bytes, s, out, cus); }
+int32_t cu_count(int* cus) {
+    int dev = 0;
+    const int32_t rc = current_device(&dev);
+    if (rc) return rc;
+    Arena& A = g_arena[dev];
+    if (A.cus == 0) {
+        int n = 0;
+        const hipError_t e = hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev);
+        if (e != hipSuccess) return hip_err(e, "hipDeviceGetAttribute");
+        A.cus = n > 0 ? n : 1;
+    }
+    *cus = A.cus;
+    return MLRS_OK;
+}
+Timed::Timed(hipStream_t s, const char* name) {
+    static_assert(sizeof(KernelTimer) <= sizeof(room) && alignof(KernelTimer) <= alignof(Timed), "room for the timer");
+    new (room) KernelTimer(s, name);
+}
+Timed::~Timed() { reinterpret_cast<KernelTimer*>(room)->~KernelTimer(); }
+
+}  // namespace capi
+}  // namespace mlrs

@@ -1,0 +1,507 @@
+// C-ABI layer of the training operators: validation (before any launch),
+// packing of operands that the kernels cannot read in place, and dispatch.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mlrs_hip_knn.h"
+#include "capi_shared.hpp"
+#include "train_kernels.hpp"
+
+using namespace mlrs;
+using namespace mlrs::train;
+
+namespace {
+
+constexpr int64_t kMaxCount = 0x7FFFFFFF - 512;  // a tile past it must not overflow
+constexpr int64_t kMaxRowBytes = (int64_t)1 << 22;  // 256 rows of a tile within a buffer descriptor's 2^31
+
+int32_t null_error(const char* operand) {
+    return capi::error(MLRS_ERR_NULL_POINTER, operand, 0, 0, 0, "null pointer");
+}
+
+// Carves a call's scratch: first a pass that only adds up, then one that hands
+// out addresses.
+struct Scratch {
+    char* base = nullptr;
+    size_t used = 0;
+    template <typename T>
+    T* take(size_t n) {
+        used = (used + 255) & ~(size_t)255;
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += n * sizeof(T);
+        return p;
+    }
+};
+
+template <typename T>
+int64_t padded(int64_t cols) {
+    constexpr int64_t E = 16 / (int64_t)sizeof(T);
+    return (cols + E - 1) / E * E;
+}
+
+template <typename T>
+bool readable(const T* p, int64_t cols) {
+    return (uintptr_t)p % 16 == 0 && padded<T>(cols) == cols;
+}
+
+// An operand as the kernels read it: in place, or packed.
+template <typename T>
+struct Op {
+    const T* src;
+    int64_t rows, cols;
+    T* packed = nullptr;
+    Op(const T* p, int64_t r, int64_t c) : src(p), rows(r), cols(c) {}
+    bool in_place() const { return readable(src, cols); }
+    void plan(Scratch& sc) {
+        if (!in_place()) packed = sc.take<T>((size_t)(rows * padded<T>(cols)));
+    }
+    hipError_t pack(hipStream_t s) const {
+        return in_place() ? hipSuccess : launch_pack<T>(src, rows, cols, packed, padded<T>(cols), s);
+    }
+    Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, padded<T>(cols)}; }
+};
+
+// Sizes that both layers of operators share: a (n x d) and w (m x d).
+template <typename T>
+int32_t check_sizes(const char* a_name, int64_t a_len, int64_t n, int64_t d, int64_t w_len, int64_t m) {
+    if (!capi::geometry(n, d, a_len)) return capi::shape_error(a_name, n, d, a_len);
+    if (!capi::geometry(m, d, w_len)) return capi::shape_error("w", m, d, w_len);
+    if (d < 1 || m < 1) return capi::shape_error("features", m, d, 0);
+    if (d > kMaxRowBytes / (int64_t)sizeof(T) || m > kMaxCount)
+        return capi::error(MLRS_ERR_UNSUPPORTED, "features", m, d, 0, "rows are limited to 2^22 bytes");
+    if (n > kMaxCount) return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, d, 0, "row counts are limited to 2^31 - 513");
+    return MLRS_OK;
+}
+
+// A product's grid must fit: tiles of the smallest size, every part of k.
+bool grid_fits(int64_t m, int64_t n) { return ((m + 63) / 64) * ((n + 63) / 64) <= INT32_MAX / 64; }
+int32_t grid_error(int64_t m, int64_t n) {
+    return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, m, 0, "the product has more tiles than a launch");
+}
+
+#define MLRS_TRY(call)                                      \
+    do {                                                    \
+        const hipError_t e_ = (call);                       \
+        if (e_ != hipSuccess) return capi::hip_error(e_, where); \
+    } while (0)
+
+// ---------------------------------------------------------------------------
+template <typename T>
+int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w, int64_t w_len, int64_t m,
+                    const T* bias, int64_t bias_len, const T* residual, int64_t residual_len, int32_t act, T* y,
+                    int64_t y_len, T* z, int64_t z_len, void* stream) {
+    const char* where = "linear";
+    return capi::call([&]() -> int32_t {
+        int32_t rc = check_sizes<T>("x", x_len, n, k, w_len, m);
+        if (rc) return rc;
+        if (bias ? bias_len != m : bias_len != 0) return capi::shape_error("bias", 1, m, bias_len);
+        if (residual ? !capi::geometry(n, m, residual_len) : residual_len != 0)
+            return capi::shape_error("residual", n, m, residual_len);
+        if (!capi::geometry(n, m, y_len)) return capi::shape_error("out", n, m, y_len);
+        if (z ? !capi::geometry(n, m, z_len) : z_len != 0) return capi::shape_error("preact", n, m, z_len);
+        if (act < MLRS_ACT_NONE || act > MLRS_ACT_SILU)
+            return capi::error(MLRS_ERR_UNSUPPORTED, "activation", act, 0, 0, "unknown activation");
+        if (n == 0) return MLRS_OK;
+        if (!x || !w || !y) return null_error(!x ? "x" : !w ? "w" : "out");
+        if (!grid_fits(m, n)) return grid_error(m, n);
+        const hipStream_t s = (hipStream_t)stream;
+        const LinearOut o{bias, residual, y, z, act};
+        if (n <= kFewRows) {
+            capi::Timed timed(s, "linear_few");
+            MLRS_TRY(launch_linear_few<T>(x, w, n, m, k, o, s));
+            return MLRS_OK;
+        }
+        int cus = 0;
+        rc = capi::cu_count(&cus);
+        if (rc) return rc;
+        const Cut cut = choose_cut((int)sizeof(T), m, n, k, cus);
+        Op<T> xo(x, n, k), wo(w, m, k);
+        float* part = nullptr;
+        Scratch sc;
+        for (int pass = 0; pass < 2; ++pass) {
+            xo.plan(sc);
+            wo.plan(sc);
+            part = sc.take<float>(cut.part_bytes(m, n) / 4);
+            if (sc.used == 0) break;
+            if (pass == 0) {
+                rc = capi::scratch(sc.used, s, &sc.base, &cus);
+                if (rc) return rc;
+                sc.used = 0;
+            }
+        }
+        MLRS_TRY(xo.pack(s));
+        MLRS_TRY(wo.pack(s));
+        capi::Timed timed(s, "linear");
+        MLRS_TRY(launch_linear<T>(xo.mat(), wo.mat(), n, m, k, o, cut, part, s));
+        return MLRS_OK;
+    });
+}
+
+template <typename T>
+int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
+                         int64_t w_len, int64_t m, const T* z, int64_t z_len, int32_t act, T* dx, int64_t dx_len,
+                         T* dw, int64_t dw_len, T* db, int64_t db_len, void* stream) {
+    const char* where = "linear_grad";
+    return capi::call([&]() -> int32_t {
+        int32_t rc = check_sizes<T>("x", x_len, n, k, w_len, m);
+        if (rc) return rc;
+        if (m > kMaxRowBytes / (int64_t)sizeof(T))
+            return capi::error(MLRS_ERR_UNSUPPORTED, "features", m, k, 0, "rows are limited to 2^22 bytes");
+        if (!capi::geometry(n, m, dy_len)) return capi::shape_error("dy", n, m, dy_len);
+        if (dx ? !capi::geometry(n, k, dx_len) : dx_len != 0) return capi::shape_error("dx", n, k, dx_len);
+        if (dw ? !capi::geometry(m, k, dw_len) : dw_len != 0) return capi::shape_error("dw", m, k, dw_len);
+        if (db ? db_len != m : db_len != 0) return capi::shape_error("dbias", 1, m, db_len);
+        if (act < MLRS_ACT_NONE || act > MLRS_ACT_SILU)
+            return capi::error(MLRS_ERR_UNSUPPORTED, "activation", act, 0, 0, "unknown activation");
+        if (act == MLRS_ACT_NONE ? z_len != 0 : !capi::geometry(n, m, z_len))
+            return capi::shape_error("preact", n, m, z_len);
+        if (!dx && !dw && !db) return MLRS_OK;
+        if (n > 0) {
+            if (!dy) return null_error("dy");
+            if (dw && !x) return null_error("x");
+            if (act != MLRS_ACT_NONE && !z) return null_error("preact");
+        }
+        if (dx && !w) return null_error("w");
+        if (!grid_fits(k, n) || !grid_fits(k, m)) return grid_error(k, std::max(m, n));
+        const hipStream_t s = (hipStream_t)stream;
+        int cus = 0;
+        rc = capi::cu_count(&cus);
+        if (rc) return rc;
+        const bool products = (dx && n > 0) || dw;
+        // dy itself serves as dz where there is no slope and its rows can be read
+        const bool make_dz = products && n > 0 && (act != MLRS_ACT_NONE || !readable(dy, m));
+        const Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
+        const int parts = column_parts(n, m, cus);
+        Op<T> xo(x, n, k), wo(w, m, k);
+        T* dz = nullptr;
+        float *part = nullptr, *sums = nullptr;
+        Scratch sc;
+        for (int pass = 0; pass < 2; ++pass) {
+            if (dw) xo.plan(sc);
+            if (dx) wo.plan(sc);
+            if (make_dz) dz = sc.take<T>((size_t)(n * padded<T>(m)));
+            if (db) sums = sc.take<float>((size_t)parts * (size_t)m);
+            part = sc.take<float>(std::max(dx ? cx.part_bytes(k, n) : 0, dw ? cw.part_bytes(k, m) : 0) / 4);
+            if (sc.used == 0) break;
+            if (pass == 0) {
+                rc = capi::scratch(sc.used, s, &sc.base, &cus);
+                if (rc) return rc;
+                sc.used = 0;
+            }
+        }
+        if (make_dz || db)
+            MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, padded<T>(m),
+                                        db ? sums : nullptr, parts, s));
+        if (db) MLRS_TRY(launch_sum_parts<T>(sums, parts, m, nullptr, db, s));
+        const Mat dzm = make_dz ? Mat{dz, padded<T>(m)} : Mat{dy, m};
+        capi::Timed timed(s, "linear_grad");
+        if (dx && n > 0) {
+            MLRS_TRY(wo.pack(s));
+            const StoreTo o{dx, k, nullptr, nullptr, 0, nullptr};
+            MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, o, cx, part, s));
+        }
+        if (dw) {
+            MLRS_TRY(xo.pack(s));
+            const StoreTo o{dw, k, nullptr, nullptr, 0, nullptr};
+            MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, o, cw, part, s));
+        }
+        return MLRS_OK;
+    });
+}
+
+// ---------------------------------------------------------------------------
+// The tile of a product that is not split.
+template <typename T>
+int tile_for(int64_t m, int64_t n, int cus) {
+    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), mid = ((m + 127) / 128) * ((n + 127) / 128);
+    return large >= cus ? 0 : mid >= cus ? 1 : 2;
+}
+
+template <typename T>
+int32_t check_xent(int64_t h_len, int64_t n, int64_t d, int64_t w_len, int64_t v, const T* bias, int64_t bias_len,
+                   int64_t target_len, int64_t out_len) {
+    const int32_t rc = check_sizes<T>("h", h_len, n, d, w_len, v);
+    if (rc) return rc;
+    if (bias ? bias_len != v : bias_len != 0) return capi::shape_error("bias", 1, v, bias_len);
+    if (target_len != n) return capi::shape_error("target", n, 1, target_len);
+    if (out_len != n) return capi::shape_error("out", n, 1, out_len);
+    if (!grid_fits(v, n)) return grid_error(v, n);
+    return MLRS_OK;
+}
+
+template <typename T>
+int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, int64_t w_len, int64_t v,
+                  const T* bias, int64_t bias_len, const int64_t* target, int64_t target_len, int64_t ignore,
+                  float* loss, float* lse, int64_t out_len, void* stream) {
+    const char* where = "softmax_xent";
+    return capi::call([&]() -> int32_t {
+        int32_t rc = check_xent<T>(h_len, n, d, w_len, v, bias, bias_len, target_len, out_len);
+        if (rc) return rc;
+        if (n == 0) return MLRS_OK;
+        if (!h || !w || !target || !loss || !lse)
+            return null_error(!h ? "h" : !w ? "w" : !target ? "target" : "out");
+        const hipStream_t s = (hipStream_t)stream;
+        int cus = 0;
+        rc = capi::cu_count(&cus);
+        if (rc) return rc;
+        const int tile = tile_for<T>(v, n, cus);
+        const int64_t parts = stats_parts(tile, v);
+        Op<T> ho(h, n, d), wo(w, v, d);
+        float *top = nullptr, *total = nullptr, *hit = nullptr;
+        Scratch sc;
+        for (int pass = 0; pass < 2; ++pass) {
+            ho.plan(sc);
+            wo.plan(sc);
+            top = sc.take<float>((size_t)(parts * n));
+            total = sc.take<float>((size_t)(parts * n));
+            hit = sc.take<float>((size_t)n);
+            if (pass == 0) {
+                rc = capi::scratch(sc.used, s, &sc.base, &cus);
+                if (rc) return rc;
+                sc.used = 0;
+            }
+        }
+        MLRS_TRY(ho.pack(s));
+        MLRS_TRY(wo.pack(s));
+        capi::Timed timed(s, "softmax_xent");
+        MLRS_TRY(launch_xent_stats<T>(ho.mat(), wo.mat(), bias, target, n, v, d, tile, top, total, hit, s));
+        MLRS_TRY(launch_xent_join(top, total, parts, hit, target, n, v, ignore, loss, lse, s));
+        return MLRS_OK;
+    });
+}
+
+template <typename T>
+int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, int64_t w_len, int64_t v,
+                       const T* bias, int64_t bias_len, const int64_t* target, int64_t target_len, int64_t ignore,
+                       const float* lse, const float* grad, int64_t out_len, T* dh, int64_t dh_len, T* dw,
+                       int64_t dw_len, T* db, int64_t db_len, void* stream) {
+    const char* where = "softmax_xent_grad";
+    return capi::call([&]() -> int32_t {
+        int32_t rc = check_xent<T>(h_len, n, d, w_len, v, bias, bias_len, target_len, out_len);
+        if (rc) return rc;
+        if (dh ? !capi::geometry(n, d, dh_len) : dh_len != 0) return capi::shape_error("dh", n, d, dh_len);
+        if (dw ? !capi::geometry(v, d, dw_len) : dw_len != 0) return capi::shape_error("dw", v, d, dw_len);
+        if (db ? db_len != v : db_len != 0) return capi::shape_error("dbias", 1, v, db_len);
+        if (!dh && !dw && !db) return MLRS_OK;
+        if (!w) return null_error("w");
+        if (n > 0 && (!h || !target || !lse || !grad))
+            return null_error(!h ? "h" : !target ? "target" : !lse ? "lse" : "grad");
+        const hipStream_t s = (hipStream_t)stream;
+        int cus = 0;
+        rc = capi::cu_count(&cus);
+        if (rc) return rc;
+        if (n == 0) {
+            // no rows: the products over them are empty sums
+            if (dw) {
+                const StoreTo o{dw, d, nullptr, nullptr, 0, nullptr};
+                MLRS_TRY(launch_product<T>(Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, false, d, v, 0, o,
+                                           Cut{2, 1, 0}, nullptr, s));
+            }
+            if (db) MLRS_TRY(launch_sum_parts<T>(nullptr, 0, v, nullptr, db, s));
+            return MLRS_OK;
+        }
+        // classes of a piece: a multiple of 256, at least one tile
+        const int64_t fit = MLRS_XENT_PIECE_BYTES / ((int64_t)sizeof(T) * n) / 256 * 256;
+        const int64_t pieces = (v + std::max<int64_t>(fit, 256) - 1) / std::max<int64_t>(fit, 256);
+        const int64_t piece = pieces == 1 ? v : ((v + pieces - 1) / pieces + 255) / 256 * 256;
+        const int64_t ld = padded<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;
+        const bool scaled = sizeof(T) == 2 && std::is_same<T, _Float16>::value;
+        const Cut ch = choose_cut((int)sizeof(T), d, n, std::min(piece, v), cus);
+        const Cut cw = choose_cut((int)sizeof(T), d, std::min(piece, v), n, cus);
+        const int parts = column_parts(n, std::min(piece, v), cus);
+        Op<T> ho(h, n, d), wo(w, v, d);
+        T* dz = nullptr;
+        float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr;
+        Scratch sc;
+        for (int pass = 0; pass < 2; ++pass) {
+            ho.plan(sc);
+            wo.plan(sc);
+            dz = sc.take<T>((size_t)(n * ld));
+            if (dh && pieces > 1) acc = sc.take<float>((size_t)(n * dh_ld));
+            if (db) sums = sc.take<float>((size_t)parts * (size_t)std::min(piece, v));
+            if (scaled) up = sc.take<float>(2);
+            part = sc.take<float>(
+                std::max(dh ? ch.part_bytes(d, n) : 0, dw ? cw.part_bytes(d, std::min(piece, v)) : 0) / 4);
+            if (pass == 0) {
+                rc = capi::scratch(sc.used, s, &sc.base, &cus);
+                if (rc) return rc;
+                sc.used = 0;
+            }
+        }
+        MLRS_TRY(ho.pack(s));
+        MLRS_TRY(wo.pack(s));
+        if (scaled) MLRS_TRY(launch_grad_scale(grad, target, n, ignore, up, s));
+        const float* down = scaled ? up + 1 : nullptr;
+        const Mat hm = ho.mat(), wm = wo.mat();
+        capi::Timed timed(s, "softmax_xent_grad");
+        for (int64_t v0 = 0; v0 < v; v0 += piece) {
+            const int64_t vp = std::min(piece, v - v0);
+            const bool last = v0 + vp == v;
+            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
+                                          tile_for<T>(vp, n, cus), s));
+            const Mat dzm{dz, ld};
+            if (db) {
+                MLRS_TRY(launch_column_sums<T>(dzm, n, vp, sums, parts, s));
+                MLRS_TRY(launch_sum_parts<T>(sums, parts, vp, down, db + v0, s));
+            }
+            if (dw) {
+                const StoreTo o{dw + v0 * d, d, nullptr, nullptr, 0, down};
+                MLRS_TRY(launch_product<T>(hm, dzm, false, d, vp, n, o, cw, part, s));
+            }
+            if (dh) {
+                StoreTo o{};
+                o.ld = d;
+                o.acc = acc;
+                o.acc_ld = dh_ld;
+                o.add = v0 > 0 ? acc : nullptr;
+                if (last) {
+                    o.out = dh;
+                    o.alpha = down;
+                }
+                Cut c = ch;
+                if (vp < piece) c = choose_cut((int)sizeof(T), d, n, vp, cus);
+                if (c.part_bytes(d, n) > ch.part_bytes(d, n)) c = Cut{c.tile, 1, 0};
+                MLRS_TRY(launch_product<T>(Mat{(const T*)wm.p + v0 * wm.ld, wm.ld}, dzm, true, d, n, vp, o, c, part, s));
+            }
+        }
+        return MLRS_OK;
+    });
+}
+
+bool dtype_ok(int32_t t) { return t >= MLRS_DTYPE_F32 && t <= MLRS_DTYPE_BF16; }
+
+}  // namespace
+
+extern "C" {
+
+#define MLRS_TRAIN_ENTRY(SUFFIX, ABI, T)                                                                             \
+    int32_t mlrs_linear_##SUFFIX(const ABI* x, int64_t x_len, int64_t n, int64_t d_in, const ABI* w, int64_t w_len,  \
+                                 int64_t d_out, const ABI* bias, int64_t bias_len, const ABI* residual,              \
+                                 int64_t residual_len, int32_t activation, ABI* y, int64_t y_len, ABI* preact,       \
+                                 int64_t preact_len, void* stream) {                                                 \
+        return linear_impl<T>((const T*)x, x_len, n, d_in, (const T*)w, w_len, d_out, (const T*)bias, bias_len,      \
+                              (const T*)residual, residual_len, activation, (T*)y, y_len, (T*)preact, preact_len,    \
+                              stream);                                                                               \
+    }                                                                                                                \
+    int32_t mlrs_linear_grad_##SUFFIX(                                                                               \
+        const ABI* dy, int64_t dy_len, const ABI* x, int64_t x_len, int64_t n, int64_t d_in, const ABI* w,           \
+        int64_t w_len, int64_t d_out, const ABI* preact, int64_t preact_len, int32_t activation, ABI* dx,            \
+        int64_t dx_len, ABI* dw, int64_t dw_len, ABI* dbias, int64_t dbias_len, void* stream) {                      \
+        return linear_grad_impl<T>((const T*)dy, dy_len, (const T*)x, x_len, n, d_in, (const T*)w, w_len, d_out,     \
+                                   (const T*)preact, preact_len, activation, (T*)dx, dx_len, (T*)dw, dw_len,         \
+                                   (T*)dbias, dbias_len, stream);                                                    \
+    }                                                                                                                \
+    int32_t mlrs_softmax_xent_##SUFFIX(const ABI* h, int64_t h_len, int64_t n, int64_t d, const ABI* w,              \
+                                       int64_t w_len, int64_t classes, const ABI* bias, int64_t bias_len,            \
+                                       const int64_t* target, int64_t target_len, int64_t ignore_index, float* loss, \
+                                       float* lse, int64_t out_len, void* stream) {                                  \
+        return xent_impl<T>((const T*)h, h_len, n, d, (const T*)w, w_len, classes, (const T*)bias, bias_len, target, \
+                            target_len, ignore_index, loss, lse, out_len, stream);                                   \
+    }                                                                                                                \
+    int32_t mlrs_softmax_xent_grad_##SUFFIX(                                                                         \
+        const ABI* h, int64_t h_len, int64_t n, int64_t d, const ABI* w, int64_t w_len, int64_t classes,             \
+        const ABI* bias, int64_t bias_len, const int64_t* target, int64_t target_len, int64_t ignore_index,          \
+        const float* lse, const float* grad, int64_t out_len, ABI* dh, int64_t dh_len, ABI* dw, int64_t dw_len,      \
+        ABI* dbias, int64_t dbias_len, void* stream) {                                                               \
+        return xent_grad_impl<T>((const T*)h, h_len, n, d, (const T*)w, w_len, classes, (const T*)bias, bias_len,    \
+                                 target, target_len, ignore_index, lse, grad, out_len, (T*)dh, dh_len, (T*)dw,       \
+                                 dw_len, (T*)dbias, dbias_len, stream);                                              \
+    }
+MLRS_TRAIN_ENTRY(f32, float, float)
+MLRS_TRAIN_ENTRY(f16, uint16_t, _Float16)
+MLRS_TRAIN_ENTRY(bf16, uint16_t, __bf16)
+
+int32_t mlrs_grad_clip_scale(const mlrs_grad_tensor* tensors, int64_t count, double max_norm, float* norm,
+                             float* scale, void* stream) {
+    const char* where = "grad_clip_scale";
+    return capi::call([&]() -> int32_t {
+        if (count < 0) return capi::shape_error("tensors", count, 1, 0);
+        if (count > 0 && !tensors) return null_error("tensors");
+        for (int64_t i = 0; i < count; ++i) {
+            if (tensors[i].len < 0) return capi::shape_error("tensors", i, 1, tensors[i].len);
+            if (!dtype_ok(tensors[i].dtype))
+                return capi::error(MLRS_ERR_UNSUPPORTED, "dtype", tensors[i].dtype, i, 0, "unknown element type");
+            if (tensors[i].len > 0 && !tensors[i].grad) return null_error("grad");
+        }
+        if (!(max_norm > 0.0))
+            return capi::error(MLRS_ERR_INVALID_PARAM, "max_norm", 0, 0, 0, "max_norm is invalid (must be > 0)");
+        if (!norm || !scale) return null_error("out");
+        const hipStream_t s = (hipStream_t)stream;
+        const int64_t parts = norm_parts(tensors, count);
+        char* ws = nullptr;
+        int cus = 0;
+        const int32_t rc = capi::scratch((size_t)parts * sizeof(double), s, &ws, &cus);
+        if (rc) return rc;
+        capi::Timed timed(s, "grad_clip_scale");
+        MLRS_TRY(launch_clip_scale(tensors, count, max_norm, (double*)ws, norm, scale, s));
+        return MLRS_OK;
+    });
+}
+
+int32_t mlrs_adamw_step(const mlrs_adamw_tensor* tensors, int64_t count, int32_t state_bits, double lr, double beta1,
+                        double beta2, double eps, int64_t step, const float* scale, uint32_t seed, void* stream) {
+    const char* where = "adamw_step";
+    return capi::call([&]() -> int32_t {
+        if (count < 0) return capi::shape_error("tensors", count, 1, 0);
+        if (count > 0 && !tensors) return null_error("tensors");
+        if (state_bits != 32 && state_bits != 8)
+            return capi::error(MLRS_ERR_UNSUPPORTED, "state_bits", state_bits, 0, 0, "states have 32 or 8 bits");
+        auto invalid = [](const char* name, const char* message) {
+            return capi::error(MLRS_ERR_INVALID_PARAM, name, 0, 0, 0, message);
+        };
+        if (!(lr >= 0.0) || std::isinf(lr)) return invalid("lr", "lr is invalid (must be finite and >= 0)");
+        if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
+            return invalid("betas", "betas are invalid (must be in [0, 1))");
+        if (!(eps >= 0.0) || std::isinf(eps)) return invalid("eps", "eps is invalid (must be finite and >= 0)");
+        if (step < 1) return invalid("step", "step is invalid (counts from 1)");
+        for (int64_t i = 0; i < count; ++i) {
+            const mlrs_adamw_tensor& t = tensors[i];
+            if (t.len < 0) return capi::shape_error("tensors", i, 1, t.len);
+            if (!dtype_ok(t.param_dtype) || !dtype_ok(t.grad_dtype))
+                return capi::error(MLRS_ERR_UNSUPPORTED, "dtype", t.param_dtype, t.grad_dtype, 0,
+                                   "unknown element type");
+            if (!(t.weight_decay >= 0.0) || std::isinf(t.weight_decay))
+                return invalid("weight_decay", "weight_decay is invalid (must be finite and >= 0)");
+            if (t.len == 0) continue;
+            if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return null_error("tensors");
+            if (t.param_dtype != MLRS_DTYPE_F32 && !t.master) return null_error("master");
+            if (state_bits == 8 && (!t.avg_scale || !t.avg_sq_scale)) return null_error("scales");
+        }
+        const double c1 = 1.0 - std::pow(beta1, (double)step), c2 = 1.0 - std::pow(beta2, (double)step);
+        AdamwHyper hy;
+        hy.b1 = (float)beta1;
+        hy.c1 = (float)(1.0 - beta1);
+        hy.b2 = (float)beta2;
+        hy.c2 = (float)(1.0 - beta2);
+        hy.step = (float)(lr / c1);
+        hy.root = (float)(1.0 / std::sqrt(c2));
+        hy.eps = (float)eps;
+        hy.lr = lr;
+        hy.seed = seed;
+        const hipStream_t s = (hipStream_t)stream;
+        capi::Timed timed(s, "adamw_step");
+        MLRS_TRY(launch_adamw(tensors, count, state_bits, hy, scale, s));
+        return MLRS_OK;
+    });
+}
+
+int32_t mlrs_adamw_state_values(const uint8_t* codes, int64_t len, const float* scales, int64_t scales_len,
+                                int32_t which, float* out, int64_t out_len, void* stream) {
+    const char* where = "adamw_state_values";
+    return capi::call([&]() -> int32_t {
+        if (len < 0) return capi::shape_error("codes", len, 1, len);
+        if (scales_len != (len + MLRS_STATE_BLOCK - 1) / MLRS_STATE_BLOCK)
+            return capi::shape_error("scales", (len + MLRS_STATE_BLOCK - 1) / MLRS_STATE_BLOCK, 1, scales_len);
+        if (out_len != len) return capi::shape_error("out", len, 1, out_len);
+        if (which != 0 && which != 1)
+            return capi::error(MLRS_ERR_UNSUPPORTED, "which", which, 0, 0, "which is 0 (exp_avg) or 1 (exp_avg_sq)");
+        if (len == 0) return MLRS_OK;
+        if (!codes || !scales || !out) return null_error(!codes ? "codes" : !scales ? "scales" : "out");
+        MLRS_TRY(launch_state_values(codes, scales, len, which, out, (hipStream_t)stream));
+        return MLRS_OK;
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,347 @@
+// The matrix product under the training operators: P[i, j] = sum_k A(i, k) B(j, k)
+// for f32, f16 and bf16 operands, accumulated in f32 on the matrix cores, and
+// handed to an epilogue while it is still in registers.
+//
+// Operands.  Either operand is stored with its contraction index contiguous
+// ("K layout", ptr[row * ld + k]) or with its row index contiguous ("R
+// layout", ptr[k * ld + row]), so the three products of a layer need no
+// transposed copies: x w^T is K x K, dz w is R x K, dz^T x is R x R.  Pointers
+// are 16-byte aligned and ld is a multiple of 16 bytes; the host packs what is
+// not.
+//
+// Tile.  A workgroup computes BM x BN of P, its waves a WM x WN grid of
+// 32 x 32 blocks (v_mfma_f32_32x32x16 for 16-bit types, four
+// v_mfma_f32_32x32x2 for f32).  A is the operand whose index runs along the
+// output's rows in memory: a lane then holds four consecutive elements of one
+// output row.  128 bytes of the contraction axis are staged at a time,
+// straight from HBM into one of two LDS buffers, the other one being read
+// meanwhile; out-of-range elements come back as zeros from the buffer
+// descriptor's bounds check.
+//
+// LDS layout.  K operand: a row's 128 bytes as eight 16-byte chunks, chunk c
+// kept at c ^ (row & 7), so eight rows read at one c touch all banks.  R
+// operand: the tile's elements of one k back to back, their 16-byte chunks
+// kept at c ^ r_swizzle(k): the four k of a transposing read (16-bit types)
+// and the two halves of a wave (f32) then lie in different banks.  The swizzle
+// is applied to the global address of each lane, as the copy into LDS is
+// linear.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace mlrs {
+namespace train {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// The element types by what the kernels need of them.  Conversions to 16 bits
+// round to nearest even.
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    typedef f32x4 Frag;  // 16 bytes of the contraction axis
+    typedef f32x4 Vec4;
+};
+template <>
+struct Elem<_Float16> {
+    typedef f16x8 Frag;
+    typedef f16x4 Vec4;
+};
+template <>
+struct Elem<__bf16> {
+    typedef bf16x8 Frag;
+    typedef bf16x4 Vec4;
+};
+
+struct Operand {
+    const void* p;
+    int64_t ld;  // elements
+};
+
+struct GemmArgs {
+    Operand a, b;
+    int32_t m, n, k;       // P is m x n (a's rows, b's rows)
+    int32_t tiles_m, tiles_n;
+    int32_t splits;        // parts of the contraction axis, a grid's worth of tiles each
+    int32_t k_split;       // elements of k in a part (a multiple of the staged width)
+    int32_t band;          // tiles of m that are walked together (L2 reuse)
+};
+
+constexpr int kStageBytes = 128;  // of the contraction axis, per buffer
+
+template <typename T>
+__host__ __device__ constexpr int stage_elems() {
+    return kStageBytes / (int)sizeof(T);
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+#define MLRS_LDS __attribute__((address_space(3)))
+#else
+#define MLRS_LDS
+#endif
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_step(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (sizeof(T) == 4) {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[0], b[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[1], b[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[2], b[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[3], b[3], c, 0, 0, 0);
+    } else if constexpr (__is_same(T, _Float16)) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+#else
+    (void)a;
+    (void)b;
+#endif
+    return c;
+}
+
+// R layout: what the chunk index of step k is exclusive-ored with.
+template <typename T, int ROWS>
+__device__ __forceinline__ int r_swizzle(int k) {
+    if (sizeof(T) == 4) return (k & 4) << 1;
+    return ROWS * 2 >= 256 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+}
+
+// One operand's copy into LDS: the bytes of ROWS rows (or columns) of one
+// staged width, 1,024 per wave and instruction.
+template <typename T, bool KC, int ROWS, int WAVES>
+struct Stager {
+    static constexpr int kInstr = ROWS * kStageBytes / 1024 / WAVES;
+    static constexpr int kChunks = ROWS * (int)sizeof(T) / 16;  // of one k (R layout)
+    static_assert(kInstr >= 1, "a wave copies at least one kilobyte");
+    const char* base;   // the tile's first element at k = 0
+    int64_t bytes;      // from base to the operand's end
+    int64_t step;       // bytes per element of k
+    int32_t kbytes;     // K layout: 16 * the lane's chunk
+    uint32_t off[kInstr];
+
+    __device__ __forceinline__ void init(const Operand& o, int32_t row0, int32_t rows, int32_t k, int wave, int lane) {
+        const int64_t es = (int64_t)sizeof(T);
+        // whole rows: the bounds check works by 16-byte chunks, which end at ld
+        const int64_t total = (KC ? (int64_t)rows : (int64_t)k) * o.ld * es;
+        const int64_t at = KC ? (int64_t)row0 * o.ld * es : (int64_t)row0 * es;
+        base = reinterpret_cast<const char*>(o.p) + at;
+        bytes = total - at;
+        step = KC ? es : o.ld * es;
+        const uint32_t ldb = (uint32_t)(o.ld * es);
+        kbytes = 0;
+#pragma unroll
+        for (int i = 0; i < kInstr; ++i) {
+            const int q = (wave * kInstr + i) * 64 + lane;
+            if constexpr (KC) {
+                const int r = q >> 3, c = (q & 7) ^ (r & 7);
+                kbytes = 16 * c;
+                off[i] = (uint32_t)r * ldb + 16u * (uint32_t)c;
+            } else {
+                const int kk = q / kChunks;
+                const int c = (q % kChunks) ^ r_swizzle<T, ROWS>(kk);
+                off[i] = (uint32_t)kk * ldb + 16u * (uint32_t)c;
+            }
+        }
+    }
+
+    // Elements k0 .. k0 + the staged width; k is the operand's extent.
+    __device__ __forceinline__ void load(char* lds, int32_t k0, int32_t k, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int64_t skip = (int64_t)k0 * step;
+        const int64_t left = bytes - skip;
+        const uint32_t records = left < 0x7FFFFFFF ? (left > 0 ? (uint32_t)left : 0u) : 0x7FFFFFFFu;
+        __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + skip), (short)0, (int)records, 0x00027000);
+        // chunks past the end of a row would be the next row's
+        const bool out = KC && kbytes >= (k - k0) * (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < kInstr; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (MLRS_LDS void*)(lds + (wave * kInstr + i) * 1024), 16, out ? 0x80000000u : off[i], 0, 0, 0);
+#else
+        (void)lds;
+        (void)k0;
+        (void)k;
+        (void)wave;
+#endif
+    }
+};
+
+// One operand's fragments out of LDS: BLOCKS blocks of 32 rows from row
+// `first`; step s of the four in a staged width.
+template <typename T, bool KC, int ROWS, int BLOCKS>
+struct Reader {
+    int at[KC ? 4 : BLOCKS];
+
+    __device__ __forceinline__ void init(int first, int lane) {
+        const int h = lane >> 5, r = lane & 31;
+        if constexpr (KC) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) at[s] = (first + r) * kStageBytes + (((2 * s + h) ^ (r & 7)) << 4);
+        } else if constexpr (sizeof(T) == 2) {
+            // lane 4 q + p of sixteen addresses four elements of step q of
+            // four; the transposing read hands lane i column i of them
+            const int q = (lane & 15) >> 2, p = lane & 3, side = (lane >> 4) & 1;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) {
+                const int c = ((first >> 5) + b) * 4 + side * 2 + (p >> 1);
+                at[b] = (8 * h + q) * (ROWS * 2) + ((c ^ r_swizzle<T, ROWS>(q)) << 4) + (p & 1) * 8;
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) {
+                const int c = ((first >> 5) + b) * 8 + (r >> 2);
+                at[b] = 4 * h * (ROWS * 4) + ((c ^ r_swizzle<T, ROWS>(4 * h)) << 4) + (r & 3) * 4;
+            }
+        }
+    }
+
+    __device__ __forceinline__ typename Elem<T>::Frag get(const char* lds, int s, int b) const {
+        typedef typename Elem<T>::Frag Frag;
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (KC) {
+            return *reinterpret_cast<const Frag*>(lds + at[s] + b * 32 * kStageBytes);
+        } else if constexpr (sizeof(T) == 2) {
+            const char* q = lds + at[b] + s * 16 * (ROWS * 2);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLRS_LDS s16x4*)q);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLRS_LDS s16x4*)(q + 4 * (ROWS * 2)));
+            return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const char* q = lds + at[b] + s * 8 * (ROWS * 4);
+            Frag f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float*>(q + i * (ROWS * 4));
+            return f;
+        }
+#else
+        (void)lds;
+        (void)s;
+        (void)b;
+        return Frag{};
+#endif
+    }
+};
+
+// What an epilogue is told about the wave's part of the tile.
+struct Place {
+    int32_t m0, n0;    // first row (of a) and column (of b) of the wave's blocks
+    int32_t m, n;      // the extents of P
+    int32_t split;
+    int32_t tile_m;    // the workgroup's tile index along m
+    int lane, wave;
+    int wm, wn;        // the wave's place in the workgroup's grid
+};
+
+// Workgroups go to the eight XCDs in turn; give each XCD a contiguous run of
+// tiles, so that its L2 holds the operand panels that its workgroups share.
+__device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
+    const int32_t per = total >> 3, extra = total & 7;
+    const int32_t x = wg & 7, i = wg >> 3;
+    return x * per + (x < extra ? x : extra) + i;
+}
+
+template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
+__global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 : 2))) void gemm_kernel(GemmArgs g,
+                                                                                                       Epi epi) {
+    constexpr int BM = WM * MB * 32, BN = WN * NB * 32, WAVES = WM * WN;
+    constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
+    constexpr int BK = stage_elems<T>();
+    static_assert(((kA + kB) & (kA + kB - 1)) == 0, "the buffers are toggled by one bit");
+    __shared__ __attribute__((aligned(1024))) char buf[2 * (kA + kB)];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    const int32_t tiles = g.tiles_m * g.tiles_n;
+    const int32_t split = blockIdx.x / tiles;
+    const int32_t t = xcd_tile(blockIdx.x - split * tiles, tiles);
+    // bands of `band` tiles of m, walked along n
+    const int32_t per_band = g.band * g.tiles_n;
+    const int32_t bnd = t / per_band, in = t - bnd * per_band;
+    const int32_t width = g.tiles_m - bnd * g.band < g.band ? g.tiles_m - bnd * g.band : g.band;
+    const int32_t tm = bnd * g.band + in % width, tn = in / width;
+    const int32_t m0 = tm * BM, n0 = tn * BN;
+
+    const int32_t k_lo = split * g.k_split;
+    const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;
+
+    Stager<T, AKC, BM, WAVES> sa;
+    Stager<T, BKC, BN, WAVES> sb;
+    sa.init(g.a, m0, g.m, g.k, wave, lane);
+    sb.init(g.b, n0, g.n, g.k, wave, lane);
+    Reader<T, AKC, BM, MB> ra;
+    Reader<T, BKC, BN, NB> rb;
+    ra.init(wm * MB * 32, lane);
+    rb.init(wn * NB * 32, lane);
+
+    f32x16 acc[MB][NB] = {};
+
+    auto stage = [&](char* to, int32_t k0) {
+        sa.load(to, k0, g.k, wave);
+        sb.load(to + kA, k0, g.k, wave);
+    };
+    auto compute = [&](const char* from) {
+        typename Elem<T>::Frag a[2][MB], b[2][NB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) a[0][i] = ra.get(from, 0, i);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) b[0][j] = rb.get(from + kA, 0, j);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s + 1 < 4) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i) a[(s + 1) & 1][i] = ra.get(from, s + 1, i);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) b[(s + 1) & 1][j] = rb.get(from + kA, s + 1, j);
+            }
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(a[s & 1][i], b[s & 1][j], acc[i][j]);
+        }
+    };
+    // a staged width's copies have landed for every wave, and the other
+    // buffer is no longer read
+    auto publish = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+    };
+
+    int cur = 0;
+    if (k_lo < k_hi) stage(buf, k_lo);
+    for (int32_t k0 = k_lo; k0 < k_hi; k0 += BK) {
+        publish();
+        if (k0 + BK < k_hi) stage(buf + (cur ^ (kA + kB)), k0 + BK);
+        compute(buf + cur);
+        cur ^= kA + kB;
+    }
+
+    Place p;
+    p.m0 = m0 + wm * MB * 32;
+    p.n0 = n0 + wn * NB * 32;
+    p.m = g.m;
+    p.n = g.n;
+    p.split = split;
+    p.tile_m = tm;
+    p.lane = lane;
+    p.wave = wave;
+    p.wm = wm;
+    p.wn = wn;
+    epi.template run<WM, WN, MB, NB>(acc, p, buf);
+}
+
+}  // namespace train
+}  // namespace mlrs

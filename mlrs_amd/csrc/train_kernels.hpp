@@ -1,0 +1,109 @@
+// Host side of the training operators' kernels: what capi_train.hip calls.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/mlrs_hip_knn.h"
+
+namespace mlrs {
+namespace train {
+
+// A row-major matrix the matrix-core kernels can read: 16-byte aligned, rows
+// a multiple of 16 bytes apart.
+struct Mat {
+    const void* p;
+    int64_t ld;
+};
+
+// How a product is cut: the tile, and the parts of its contraction axis.
+struct Cut {
+    int tile;         // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
+    int splits;
+    int32_t k_split;
+    size_t part_bytes(int64_t m, int64_t n) const {
+        return splits > 1 ? (size_t)splits * (size_t)n * (size_t)((m + 3) & ~(int64_t)3) * 4 : 0;
+    }
+};
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus);
+
+// dst (rows x ld, ld >= cols) := src (rows x cols), zeros behind each row.
+template <typename T>
+hipError_t launch_pack(const T* src, int64_t rows, int64_t cols, T* dst, int64_t ld, hipStream_t s);
+
+// y (n x m) = act(x w^T + bias) + residual; z, where not null, x w^T + bias.
+struct LinearOut {
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    int act;
+};
+template <typename T>
+hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
+                         float* part, hipStream_t s);
+// The same for a few rows, straight from the caller's unpacked operands.
+constexpr int kFewRows = 64;
+template <typename T>
+hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
+                             hipStream_t s);
+
+// dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and the
+// column sums of it in parts (sums may be null): parts x m floats.
+int column_parts(int64_t n, int64_t m, int cus);
+template <typename T>
+hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld, float* sums,
+                           int parts, hipStream_t s);
+// The column sums of a packed matrix, in parts.
+template <typename T>
+hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, float* sums, int parts, hipStream_t s);
+// out := alpha * (sum of the parts), in order.
+template <typename T>
+hipError_t launch_sum_parts(const float* sums, int parts, int64_t m, const float* alpha, T* out, hipStream_t s);
+
+// Stores of a product P (m x n, element (i, j) at out[j * ld + i]): a (rows m)
+// with its row index contiguous, b (rows n) with k contiguous (b_k) or not.
+struct StoreTo {
+    void* out;           // of type T, or null: the running sum `acc` is written
+    int64_t ld;
+    const float* add;    // added first; may be null
+    float* acc;          // n x acc_ld
+    int64_t acc_ld;      // a multiple of 4
+    const float* alpha;  // device scalar; may be null
+};
+template <typename T>
+hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
+                          float* part, hipStream_t s);
+
+// Softmax cross entropy: the statistics of every wave's classes, joined into
+// lse and loss; the scale of a half-precision gradient; a piece's gradient.
+int64_t stats_parts(int tile, int64_t classes);
+template <typename T>
+hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target, int64_t n, int64_t classes, int64_t k,
+                             int tile, float* top, float* total, float* hit, hipStream_t s);
+hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
+                            const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
+                            hipStream_t s);
+hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n, int64_t ignore, float* up_down,
+                             hipStream_t s);
+template <typename T>
+hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
+                             const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
+                             int64_t ignore, T* out, int64_t ld, int tile, hipStream_t s);
+
+// Optimizer.
+int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);
+hipError_t launch_clip_scale(const mlrs_grad_tensor* t, int64_t count, double max_norm, double* parts, float* norm,
+                             float* scale, hipStream_t s);
+struct AdamwHyper {
+    float b1, c1, b2, c2, step, root, eps;  // c1 = 1 - b1, c2 = 1 - b2
+    double lr;
+    uint32_t seed;
+};
+hipError_t launch_adamw(const mlrs_adamw_tensor* t, int64_t count, int bits, const AdamwHyper& hy, const float* scale,
+                        hipStream_t s);
+hipError_t launch_state_values(const uint8_t* codes, const float* scales, int64_t len, int which, float* out,
+                               hipStream_t s);
+
+}  // namespace train
+}  // namespace mlrs

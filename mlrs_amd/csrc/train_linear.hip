@@ -1,0 +1,379 @@
+// A layer forwards and backwards: y = act(x w^T + bias) + residual, and the
+// products dz w and dz^T x of its gradient.
+#include <cmath>
+
+#include "train_launch.hpp"
+
+namespace mlrs {
+namespace train {
+
+// ---------------------------------------------------------------------------
+// how a product is cut
+// ---------------------------------------------------------------------------
+// Cycles of a staged width (128 bytes of k) of a tile with its resident
+// neighbours on the CU, and how many those are.
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus) {
+    const double stage[3] = {elem_bytes == 2 ? 3000.0 : 18000.0, elem_bytes == 2 ? 2000.0 : 9500.0,
+                             elem_bytes == 2 ? 1800.0 : 5500.0};
+    const int resident[3] = {1, 2, 4};
+    const int64_t per = kStageBytes / elem_bytes;
+    const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
+    Cut best{0, 1, 0};
+    double best_cost = 1e300;
+    for (int t = 0; t < 3; ++t) {
+        const int rows = kTileRows[t];
+        const int64_t tiles = ((m + rows - 1) / rows) * ((n + rows - 1) / rows);
+        for (int64_t sp = 1; sp <= 64 && sp <= stages; sp = sp < 4 ? sp + 1 : sp * 2) {
+            const int64_t each = (stages + sp - 1) / sp;
+            if (sp > 1 && (each < 4 || (sp - 1) * each >= stages)) continue;
+            const int64_t wgs = tiles * sp;
+            const double rounds = std::ceil((double)wgs / (double)(cus * resident[t]));
+            // a CU that holds fewer than its neighbours runs them faster
+            const double fill = std::min(1.0, std::max(0.4, (double)wgs / (double)(cus * resident[t])));
+            double cost = rounds * (each * stage[t] * (rounds > 1 ? 1.0 : fill) + 6000.0);
+            if (sp > 1) cost += 8000.0 + (double)sp * (double)m * (double)n * 8.0 / 2000.0;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best.tile = t;
+                best.splits = (int)sp;
+                best.k_split = (int32_t)(each * per);
+            }
+        }
+    }
+    return best;
+}
+
+// ---------------------------------------------------------------------------
+// packing
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
+                                                   T* __restrict__ dst, int64_t ld) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t chunks = ld / E, total = rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * E;
+        const T* from = src + r * cols;
+        typename Elem<T>::Frag v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = c + e < cols ? from[c + e] : (T)0.0f;
+        *reinterpret_cast<typename Elem<T>::Frag*>(dst + r * ld + c) = v;
+    }
+}
+
+template <typename T>
+hipError_t launch_pack(const T* src, int64_t rows, int64_t cols, T* dst, int64_t ld, hipStream_t s) {
+    const int64_t total = rows * (ld / (16 / (int64_t)sizeof(T)));
+    if (total == 0) return hipSuccess;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
+    pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, s>>>(src, rows, cols, dst, ld);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// the parts of a split contraction, joined in order
+// ---------------------------------------------------------------------------
+template <typename Point>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t stride,
+                                                   int64_t part_ld, int64_t m, int64_t n, Point point) {
+    const int64_t quads = part_ld / 4, total = quads * n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / quads, c = (i - r * quads) * 4;
+        const float* at = part + r * part_ld + c;
+        f32x4 v = *reinterpret_cast<const f32x4*>(at);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(at + s * stride);
+        point(r, c, m, v);
+    }
+}
+
+template <typename Point>
+static hipError_t launch_join(const float* part, int splits, int64_t m, int64_t n, const Point& point, hipStream_t s) {
+    const int64_t part_ld = (m + 3) & ~(int64_t)3;
+    const int64_t total = part_ld / 4 * n;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
+    join_kernel<Point><<<dim3((unsigned)blocks), 256, 0, s>>>(part, splits, n * part_ld, part_ld, m, n, point);
+    return hipGetLastError();
+}
+
+template <typename T>
+struct LinearPoint {
+    LinearEpi<T> e;
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const { e.point(n, c, m, v); }
+};
+template <typename T>
+struct StorePoint {
+    StoreEpi<T> e;
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
+        if (e.out) {
+            e.finish(n, c, m, v);
+        } else {
+            if (e.add) v += load4(e.add + n * e.part_ld, c, m, true);
+            store4(e.part + n * e.part_ld, c, m, true, v);
+        }
+    }
+};
+
+template <typename T>
+static StoreEpi<T> parts_epi(float* part, int64_t m, int64_t n) {
+    StoreEpi<T> e{};
+    e.part = part;
+    e.part_ld = (m + 3) & ~(int64_t)3;
+    e.part_stride = n * e.part_ld;
+    e.wide = true;
+    return e;
+}
+
+// ---------------------------------------------------------------------------
+// forwards
+// ---------------------------------------------------------------------------
+template <typename T>
+static LinearEpi<T> linear_epi(const LinearOut& o, int64_t m) {
+    LinearEpi<T> e;
+    e.bias = (const T*)o.bias;
+    e.residual = (const T*)o.residual;
+    e.y = (T*)o.y;
+    e.z = (T*)o.z;
+    e.ld = m;
+    e.act = o.act;
+    e.wide = wide_rows<T>(o.y, m) && (!o.z || wide_rows<T>(o.z, m)) && (!o.residual || wide_rows<T>(o.residual, m));
+    return e;
+}
+
+template <typename T>
+hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
+                         float* part, hipStream_t s) {
+    const LinearEpi<T> e = linear_epi<T>(o, m);
+    if (cut.splits == 1) return launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, 1, 0, e, s);
+    const hipError_t r = launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, cut.splits, cut.k_split,
+                                                    parts_epi<T>(part, m, n), s);
+    if (r != hipSuccess) return r;
+    return launch_join(part, cut.splits, m, n, LinearPoint<T>{e}, s);
+}
+
+// A few rows: the weights are read once, straight into registers as the
+// fragments of v_mfma_f32_16x16x32 (f32: 16x16x4).  A workgroup computes
+// sixteen outputs of every row; its waves take the contraction axis in turn
+// and their sums are joined in LDS, in the order of the waves.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16_step(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    } else if constexpr (__is_same(T, _Float16)) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    } else {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+#else
+    (void)a;
+    (void)b;
+#endif
+    return c;
+}
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ typename Elem<T>::Frag chunk_at(const T* row, int64_t c, int64_t k) {
+    constexpr int E = 16 / (int)sizeof(T);
+    typename Elem<T>::Frag f;
+    if constexpr (ALIGNED) {  // k is a multiple of E
+        if (c < k)
+            f = *reinterpret_cast<const typename Elem<T>::Frag*>(row + c);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = (T)0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = c + e < k ? row[c + e] : (T)0.0f;
+    }
+    return f;
+}
+
+template <typename T, bool ALIGNED, int NB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                                int32_t n, int32_t m, int64_t k, LinearEpi<T> epi) {
+    constexpr int E = 16 / (int)sizeof(T);
+    constexpr int STEP = 4 * E;  // of k per wave and step
+    __shared__ f32x4 sums[WAVES][NB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const int32_t m0 = blockIdx.x * 16;
+    const T* wr = w + (int64_t)(m0 + r < m ? m0 + r : m - 1) * k;
+    const T* xr[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) xr[b] = x + (int64_t)(b * 16 + r < n ? b * 16 + r : n - 1) * k;
+    f32x4 acc[NB] = {};
+    constexpr int U = 4;  // steps in flight
+    for (int64_t k0 = (int64_t)wave * (U * STEP); k0 < k; k0 += (int64_t)WAVES * (U * STEP)) {
+        typename Elem<T>::Frag a[U], bx[NB][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[u] = chunk_at<T, ALIGNED>(wr, k0 + u * STEP + q * E, k);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < U; ++u) bx[b][u] = chunk_at<T, ALIGNED>(xr[b], k0 + u * STEP + q * E, k);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < U; ++u) acc[b] = mfma16_step<T>(a[u], bx[b][u], acc[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) sums[wave][b][lane] = acc[b];
+    __syncthreads();
+    // wave b joins the sums of rows 16 b .. 16 b + 15
+    for (int b = wave; b < NB; b += WAVES) {
+        f32x4 v = sums[0][b][lane];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v += sums[i][b][lane];
+        const int32_t row = b * 16 + r, c = m0 + 4 * q;
+        if (row < n && c < m) epi.point(row, c, m, v);
+    }
+}
+
+template <typename T, bool ALIGNED, int NB>
+static hipError_t launch_few_nb(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearEpi<T>& e,
+                                hipStream_t s) {
+    linear_few_kernel<T, ALIGNED, NB, 8>
+        <<<dim3((unsigned)((m + 15) / 16)), 512, 0, s>>>(x, w, (int32_t)n, (int32_t)m, k, e);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
+                             hipStream_t s) {
+    const LinearEpi<T> e = linear_epi<T>(o, m);
+    const bool al = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && (k * (int64_t)sizeof(T)) % 16 == 0;
+    if (n <= 16) return al ? launch_few_nb<T, true, 1>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 1>(x, w, n, m, k, e, s);
+    if (n <= 32) return al ? launch_few_nb<T, true, 2>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 2>(x, w, n, m, k, e, s);
+    return al ? launch_few_nb<T, true, 4>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 4>(x, w, n, m, k, e, s);
+}
+
+// ---------------------------------------------------------------------------
+// backwards
+// ---------------------------------------------------------------------------
+// A workgroup takes 256 columns (four per lane) and every parts-th run of
+// rows; its four waves take rows in turn and their sums are joined in order.
+int column_parts(int64_t n, int64_t m, int cus) {
+    const int64_t across = std::max<int64_t>(1, (m + 255) / 256);
+    const int64_t want = std::max<int64_t>(1, (int64_t)cus * 8 / across);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 15) / 16));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, int64_t dy_ld,
+                                                       const T* __restrict__ z, int act, int64_t n, int64_t m,
+                                                       T* __restrict__ dz, int64_t ld, float* __restrict__ sums,
+                                                       int64_t rows_per, bool wide) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per;
+    const int64_t r1 = r0 + rows_per < n ? r0 + rows_per : n;
+    f32x4 sum = {};
+    if (c < (dz ? ld : m)) {
+        for (int64_t r = r0 + wave; r < r1; r += 4) {
+            f32x4 v = load4(dy + r * dy_ld, c, m, wide);
+            if (z) {
+                const f32x4 zz = load4(z + r * m, c, m, wide);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= activate_slope(zz[e], act);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e >= m) v[e] = 0.0f;
+            sum += v;
+            if (dz) store4(dz + r * ld, c, ld, true, v);
+        }
+    }
+    if (!sums) return;
+    __shared__ f32x4 join[4][64];
+    join[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && c < m) {
+        f32x4 v = join[0][lane];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) v += join[i][lane];
+        store4(sums + (int64_t)blockIdx.y * m, c, m, false, v);
+    }
+}
+
+template <typename T>
+static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
+                           float* sums, int parts, hipStream_t s) {
+    const int64_t across = ((dz ? ld : m) + 255) / 256;
+    if (across == 0 || (n == 0 && !sums)) return hipSuccess;
+    const int64_t rows_per = (n + parts - 1) / parts;
+    const bool wide = wide_rows<T>(dy, dy_ld) && (!z || wide_rows<T>(z, m));
+    act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)parts), 256, 0, s>>>(dy, dy_ld, z, act, n, m, dz, ld, sums,
+                                                                             rows_per, wide);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld, float* sums,
+                           int parts, hipStream_t s) {
+    return act_grad<T>(dy, m, z, act, n, m, dz, ld, sums, parts, s);
+}
+
+template <typename T>
+hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, float* sums, int parts, hipStream_t s) {
+    return act_grad<T>((const T*)a.p, a.ld, nullptr, kActNone, n, m, nullptr, 0, sums, parts, s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ sums, int parts, int64_t m,
+                                                        const float* __restrict__ alpha, T* __restrict__ out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= m) return;
+    float v = 0.0f;
+    for (int p = 0; p < parts; ++p) v += sums[(int64_t)p * m + c];
+    if (alpha) v *= *alpha;
+    out[c] = (T)v;
+}
+
+template <typename T>
+hipError_t launch_sum_parts(const float* sums, int parts, int64_t m, const float* alpha, T* out, hipStream_t s) {
+    if (m == 0) return hipSuccess;
+    sum_parts_kernel<T><<<dim3((unsigned)((m + 255) / 256)), 256, 0, s>>>(sums, parts, m, alpha, out);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
+                          float* part, hipStream_t s) {
+    StoreEpi<T> e{};
+    e.out = (T*)o.out;
+    e.part = o.acc;
+    e.add = o.add;
+    e.alpha = o.alpha;
+    e.ld = o.ld;
+    e.part_ld = o.acc_ld;
+    e.part_stride = 0;
+    e.wide = o.out && wide_rows<T>(o.out, o.ld);
+    if (cut.splits == 1)
+        return b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, 1, 0, e, s)
+                   : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, 1, 0, e, s);
+    const StoreEpi<T> pe = parts_epi<T>(part, m, n);
+    const hipError_t r = b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, pe, s)
+                             : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, pe, s);
+    if (r != hipSuccess) return r;
+    return launch_join(part, cut.splits, m, n, StorePoint<T>{e}, s);
+}
+
+#define MLRS_INST(T)                                                                                               \
+    template hipError_t launch_pack<T>(const T*, int64_t, int64_t, T*, int64_t, hipStream_t);                      \
+    template hipError_t launch_linear<T>(Mat, Mat, int64_t, int64_t, int64_t, const LinearOut&, const Cut&, float*, \
+                                         hipStream_t);                                                             \
+    template hipError_t launch_linear_few<T>(const T*, const T*, int64_t, int64_t, int64_t, const LinearOut&,      \
+                                             hipStream_t);                                                         \
+    template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t, float*, int,    \
+                                           hipStream_t);                                                           \
+    template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, float*, int, hipStream_t);                    \
+    template hipError_t launch_sum_parts<T>(const float*, int, int64_t, const float*, T*, hipStream_t);            \
+    template hipError_t launch_product<T>(Mat, Mat, bool, int64_t, int64_t, int64_t, const StoreTo&, const Cut&,   \
+                                          float*, hipStream_t);
+MLRS_INST(float)
+MLRS_INST(_Float16)
+MLRS_INST(__bf16)
+
+}  // namespace train
+}  // namespace mlrs

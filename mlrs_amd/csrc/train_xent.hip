@@ -1,0 +1,121 @@
+// Softmax cross entropy of h w^T + bias over many classes, without the logits
+// in memory.  Forwards, a tile of logits is reduced in registers to the
+// largest and the sum of exponentials of each row; backwards, the gradient of
+// a piece of the vocabulary is made from recomputed logits and goes into the
+// two products of the gradient before the next piece.
+#include "train_launch.hpp"
+
+namespace mlrs {
+namespace train {
+
+static const int kWaveRows[3] = {128, 64, 32};  // classes of a wave, by tile
+
+int64_t stats_parts(int tile, int64_t classes) {
+    const int rows = kTileRows[tile];
+    return (classes + rows - 1) / rows * (rows / kWaveRows[tile]);
+}
+
+template <typename T>
+hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target, int64_t n, int64_t classes, int64_t k,
+                             int tile, float* top, float* total, float* hit, hipStream_t s) {
+    const StatsEpi<T> e{bias, target, top, total, hit};
+    return launch_gemm<T, true, true>(tile, w, h, classes, n, k, 1, 0, e, s);
+}
+
+// A workgroup joins the parts of 32 rows: eight threads take every eighth part
+// of a row, then one of them joins the eight.  Fixed order, so a row's loss
+// does not depend on the others.
+__global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict__ top, const float* __restrict__ total,
+                                                        int64_t parts, const float* __restrict__ hit,
+                                                        const int64_t* __restrict__ target, int64_t n,
+                                                        int64_t classes, int64_t ignore, float* __restrict__ loss,
+                                                        float* __restrict__ lse) {
+    __shared__ float tops[8][32], sums[8][32];
+    const int c = threadIdx.x & 31, p0 = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + c;
+    const float none = -__builtin_huge_valf();
+    float mx = none, sum = 0.0f;
+    if (i < n) {
+        for (int64_t p = p0; p < parts; p += 8) mx = fmaxf(mx, top[p * n + i]);
+        const float base = mx == none ? 0.0f : mx;
+        for (int64_t p = p0; p < parts; p += 8) sum += total[p * n + i] * exp_fast(top[p * n + i] - base);
+    }
+    tops[p0][c] = mx;
+    sums[p0][c] = sum;
+    __syncthreads();
+    if (p0 != 0 || i >= n) return;
+#pragma unroll
+    for (int p = 1; p < 8; ++p) mx = fmaxf(mx, tops[p][c]);
+    const float base = mx == none ? 0.0f : mx;
+    sum = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) sum += sums[p][c] * exp_fast(tops[p][c] - base);
+    const float l = base + logf(sum);
+    lse[i] = l;
+    const int64_t t = target[i];
+    float v = 0.0f;
+    if (t != ignore) v = t >= 0 && t < classes ? l - hit[i] : __builtin_nanf("");
+    loss[i] = v;
+}
+
+hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
+                            const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
+                            hipStream_t s) {
+    xent_join_kernel<<<dim3((unsigned)((n + 31) / 32)), 256, 0, s>>>(top, total, parts, hit, target, n, classes,
+                                                                    ignore, loss, lse);
+    return hipGetLastError();
+}
+
+// up_down[0]: the power of two that brings the largest |gradient| of a kept row
+// to 2^13 .. 2^14, so that the products of it with probabilities down to 2^-28
+// are normal numbers of half precision; up_down[1]: its inverse.
+__global__ __launch_bounds__(1024) void grad_scale_kernel(const float* __restrict__ grad,
+                                                          const int64_t* __restrict__ target, int64_t n,
+                                                          int64_t ignore, float* __restrict__ up_down) {
+    __shared__ float most[16];
+    float mx = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 1024)
+        if (target[i] != ignore) mx = fmaxf(mx, fabsf(grad[i]));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, most[i]);
+    int e = (int)((__float_as_uint(mx) >> 23) & 255u) - 127;  // mx in 2^e .. 2^(e+1)
+    // nothing to scale, or nothing finite; and both factors stay normal
+    if (mx == 0.0f || e == 128) e = 13;
+    e = 13 - e;
+    e = e < -120 ? -120 : e > 120 ? 120 : e;
+    up_down[0] = __uint_as_float((uint32_t)(127 + e) << 23);
+    up_down[1] = __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n, int64_t ignore, float* up_down,
+                             hipStream_t s) {
+    grad_scale_kernel<<<1, 1024, 0, s>>>(grad, target, n, ignore, up_down);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
+                             const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
+                             int64_t ignore, T* out, int64_t ld, int tile, hipStream_t s) {
+    const LogitGradEpi<T> e{bias ? bias + first : nullptr, target, lse, grad, up, out, ld, ignore, (int32_t)first,
+                            (int32_t)classes};
+    const Mat wp{(const T*)w.p + first * w.ld, w.ld};
+    return launch_gemm<T, true, true>(tile, wp, h, piece, n, k, 1, 0, e, s);
+}
+
+#define MLRS_INST(T)                                                                                              \
+    template hipError_t launch_xent_stats<T>(Mat, Mat, const T*, const int64_t*, int64_t, int64_t, int64_t, int,  \
+                                             float*, float*, float*, hipStream_t);                                \
+    template hipError_t launch_logit_grad<T>(Mat, Mat, const T*, const int64_t*, const float*, const float*,      \
+                                             const float*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,  \
+                                             T*, int64_t, int, hipStream_t);
+MLRS_INST(float)
+MLRS_INST(_Float16)
+MLRS_INST(__bf16)
+
+}  // namespace train
+}  // namespace mlrs

@@ -21,6 +21,19 @@ Geometry is validated by the C ABI before any launch; a violation raises
 | ``knn_classify``    | KNeighborsClassifier's host vote, crates/mlrs-algos/src/neighbors/classifier.rs:782-930 |
 | ``device_copy``     | device_copy, crates/mlrs-backend/src/prims/knn.rs:358-386         |
 | ``pool_stats``      | BufferPool::stats (PoolStats), crates/mlrs-backend/src/pool.rs:27-56,97 |
+
+What a table of embeddings is trained with has no counterpart in the reference;
+it takes float32, float16 and bfloat16 tensors:
+
+| function                 | what                                                       |
+|--------------------------|------------------------------------------------------------|
+| ``linear``               | ``act(x w^T + bias) + residual``                           |
+| ``linear_grad``          | its gradient                                               |
+| ``softmax_xent``         | softmax cross entropy of many classes, no logits in memory |
+| ``softmax_xent_grad``    | its gradient, in pieces of the vocabulary                  |
+| ``clip_scale``           | the norm of many gradients and the factor that clips it    |
+| ``adamw_step``           | AdamW over many tensors, states in 32 or 8 bits            |
+| ``adamw_state_values``   | the values that an 8-bit state stands for                  |
 """
 import ctypes
 
@@ -415,3 +428,265 @@ def knn_classify(y_class, n_classes, idx, dist=None, weighted=False, dtype=torch
         _ptr(labels), labels.numel(), _stream(yc.device))
     _lib.check(rc)
     return proba, labels.to(torch.int64)
+
+
+# ---- training an embedding ----
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+STATE_BLOCK = 256  # elements of a tensor that share a scale of an 8-bit state
+_TRAIN_DT = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+_TRAIN_ID = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _train_suffix(t):
+    try:
+        return _TRAIN_DT[t.dtype]
+    except KeyError:
+        raise TypeError("the training operators take float32, float16 or bfloat16 tensors, got %s" % t.dtype)
+
+
+def _activation_id(name):
+    try:
+        return ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError("unknown activation %r (expected one of %s)" % (name, sorted(ACTIVATIONS)))
+
+
+def _layer_operands(a, w, a_name, **others):
+    """The checks a layer and a loss share: device, contiguity, one element
+    type, two dimensions.  The C ABI checks the sizes."""
+    given = [t for t in others.values() if t is not None]
+    _dev_check(a, w, *given)
+    s = _train_suffix(a)
+    for name, t in dict(w=w, **others).items():
+        if t is not None and t.dtype != a.dtype:
+            raise TypeError("%s and %s dtypes differ (%s, %s)" % (a_name, name, a.dtype, t.dtype))
+    if a.dim() != 2 or w.dim() != 2:
+        raise ValueError("%s and w must have two dimensions, got %s and %s"
+                         % (a_name, tuple(a.shape), tuple(w.shape)))
+    if a.shape[1] != w.shape[1]:
+        raise ValueError("%s has %d columns, w %d" % (a_name, a.shape[1], w.shape[1]))
+    return s
+
+
+def _len(t):
+    return t.numel() if t is not None else 0
+
+
+def linear(x, w, bias=None, activation="none", residual=None, keep_preact=False, out=None):
+    """A layer, ``act(x w^T + bias) + residual`` (mlrs_linear_*).
+
+    ``x`` (n, d_in), ``w`` (d_out, d_in), ``bias`` (d_out,) and ``residual``
+    (n, d_out) share one dtype, float32, float16 or bfloat16; sums are held in
+    float32 and each output rounded once.  ``activation``: "none", "relu",
+    "gelu" (the erf form), "gelu_tanh" or "silu".  Returns ``y`` (n, d_out), or
+    ``(y, z)`` with ``keep_preact``: z = x w^T + bias, what ``linear_grad``
+    takes.  ``out`` receives y (it may be ``residual`` itself)."""
+    s = _layer_operands(x, w, "x", bias=bias, residual=residual)
+    act = _activation_id(activation)
+    n, d_in = x.shape
+    d_out = w.shape[0]
+    if out is None:
+        y = torch.empty((n, d_out), dtype=x.dtype, device=x.device)
+    else:
+        _check_out(out, "out", (x.dtype,), n * d_out, x.device)
+        y = out
+    z = torch.empty((n, d_out), dtype=x.dtype, device=x.device) if keep_preact else None
+    _lib.check(getattr(_lib.load(), "mlrs_linear_" + s)(
+        _ptr(x), x.numel(), n, d_in, _ptr(w), w.numel(), d_out, _ptr(bias), _len(bias), _ptr(residual), _len(residual),
+        act, _ptr(y), y.numel(), _ptr(z), _len(z), _stream(x.device)))
+    return (y, z) if keep_preact else y
+
+
+def linear_grad(dy, x, w, preact=None, activation="none", bias=True, need_dx=True, need_dw=True):
+    """The gradient of ``linear`` (mlrs_linear_grad_*): ``(dx, dw, dbias)``, None
+    in the place of what is not asked for.
+
+    ``dy`` (n, d_out) is the gradient of y; ``preact`` is the z that ``linear``
+    kept (not used with activation "none").  The residual's gradient is ``dy``
+    itself.  16-bit types: ``dy * act'(z)`` is rounded to the type before the
+    two products; ``dbias`` sums it unrounded."""
+    act = _activation_id(activation)
+    z = preact if act else None
+    s = _layer_operands(x, w, "x", dy=dy, preact=z)
+    if act and z is None:
+        raise ValueError("activation %r needs preact, the z that linear kept" % (activation,))
+    n, d_in = x.shape
+    d_out = w.shape[0]
+    dx = torch.empty_like(x) if need_dx else None
+    dw = torch.empty_like(w) if need_dw else None
+    db = torch.empty(d_out, dtype=x.dtype, device=x.device) if bias else None
+    _lib.check(getattr(_lib.load(), "mlrs_linear_grad_" + s)(
+        _ptr(dy), dy.numel(), _ptr(x), x.numel(), n, d_in, _ptr(w), w.numel(), d_out, _ptr(z), _len(z), act, _ptr(dx),
+        _len(dx), _ptr(dw), _len(dw), _ptr(db), _len(db), _stream(x.device)))
+    return dx, dw, db
+
+
+def _check_rows(t, name, dtype, n):
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if t.numel() != n:
+        raise ValueError("%s must hold %d elements, got %d" % (name, n, t.numel()))
+
+
+def softmax_xent(h, w, target, bias=None, ignore_index=-100):
+    """Softmax cross entropy of ``z = h w^T + bias`` (mlrs_softmax_xent_*), the
+    logits never in memory: ``(loss, lse)``, float32 (n,) each.
+
+    ``h`` (n, d), ``w`` (classes, d) and ``bias`` (classes,; -inf leaves a class
+    out) share one dtype; ``target`` (n,) is int64.  ``lse`` is the logarithm of
+    the sum of exponentials, ``loss = lse - z[target]``, 0 where the target is
+    ``ignore_index`` and NaN where it is no class."""
+    s = _layer_operands(h, w, "h", bias=bias)
+    _dev_check(h, target)
+    n, d = h.shape
+    _check_rows(target, "target", torch.int64, n)
+    loss = torch.empty(n, dtype=torch.float32, device=h.device)
+    lse = torch.empty(n, dtype=torch.float32, device=h.device)
+    _lib.check(getattr(_lib.load(), "mlrs_softmax_xent_" + s)(
+        _ptr(h), h.numel(), n, d, _ptr(w), w.numel(), w.shape[0], _ptr(bias), _len(bias), _ptr(target),
+        target.numel(), int(ignore_index), _ptr(loss), _ptr(lse), n, _stream(h.device)))
+    return loss, lse
+
+
+def softmax_xent_grad(h, w, target, lse, grad, bias=None, ignore_index=-100, need_dh=True, need_dw=True):
+    """The gradient of ``sum(grad * loss)`` (mlrs_softmax_xent_grad_*): ``(dh, dw,
+    dbias)``, None in the place of what is not asked for (``dbias`` without a
+    ``bias``).
+
+    ``lse`` is what ``softmax_xent`` returned for the same operands, ``grad``
+    float32 (n,) the gradient of each row's loss (1 / n for their mean).  The
+    logits are computed again, a piece of the vocabulary at a time."""
+    s = _layer_operands(h, w, "h", bias=bias)
+    _dev_check(h, target, lse, grad)
+    n, d = h.shape
+    _check_rows(target, "target", torch.int64, n)
+    _check_rows(lse, "lse", torch.float32, n)
+    _check_rows(grad, "grad", torch.float32, n)
+    dh = torch.empty_like(h) if need_dh else None
+    dw = torch.empty_like(w) if need_dw else None
+    db = torch.empty_like(bias) if bias is not None else None
+    _lib.check(getattr(_lib.load(), "mlrs_softmax_xent_grad_" + s)(
+        _ptr(h), h.numel(), n, d, _ptr(w), w.numel(), w.shape[0], _ptr(bias), _len(bias), _ptr(target),
+        target.numel(), int(ignore_index), _ptr(lse), _ptr(grad), n, _ptr(dh), _len(dh), _ptr(dw), _len(dw),
+        _ptr(db), _len(db), _stream(h.device)))
+    return dh, dw, db
+
+
+def _tensor_list(ts, name, count=None):
+    ts = list(ts)
+    if count is not None and len(ts) != count:
+        raise ValueError("%s must hold a tensor for each of the %d parameters, got %d" % (name, count, len(ts)))
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s must hold tensors, got %s" % (name, type(t).__name__))
+    return ts
+
+
+def clip_scale(grads, max_norm):
+    """``(norm, scale)``, float32 (1,) each on the device: the root of the sum of
+    squares over all ``grads`` and ``min(1, max_norm / norm)``, the factor that
+    clips them (mlrs_grad_clip_scale).  Where the norm is not finite the factor
+    is NaN, with which ``adamw_step`` takes no step.  The norm of no gradients
+    is 0."""
+    grads = _tensor_list(grads, "grads")
+    if not grads:
+        raise ValueError("clip_scale needs at least one gradient")
+    _dev_check(*grads)
+    items = (_lib.GradTensor * len(grads))()
+    for it, g in zip(items, grads):
+        _train_suffix(g)
+        it.grad, it.len, it.dtype = g.data_ptr(), g.numel(), _TRAIN_ID[g.dtype]
+    norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
+    scale = torch.empty_like(norm)
+    _lib.check(_lib.load().mlrs_grad_clip_scale(items, len(grads), float(max_norm), _ptr(norm), _ptr(scale),
+                                                _stream(norm.device)))
+    return norm, scale
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+               masters=None, avg_scales=None, avg_sq_scales=None, scale=None, seed=0):
+    """One AdamW step of every tensor, in place (mlrs_adamw_step).
+
+    Lists with a tensor for each parameter: ``params`` (float32, or float16 /
+    bfloat16 with float32 ``masters``), ``grads``, and the moments.  float32
+    ``exp_avg`` / ``exp_avg_sq`` are the moments themselves; uint8 ones are
+    codes, with float32 ``avg_scales`` / ``avg_sq_scales`` of one scale per
+    ``STATE_BLOCK`` elements (all zero before the first step), and ``seed``
+    decides their rounding: give every step another one.  ``weight_decay`` is
+    one number or one for each tensor; ``scale`` a float32 (1,) device tensor
+    that the gradients are multiplied by first (``clip_scale``'s): where it is
+    not finite nothing changes.  ``step`` counts from 1."""
+    params = _tensor_list(params, "params")
+    count = len(params)
+    grads = _tensor_list(grads, "grads", count)
+    exp_avg = _tensor_list(exp_avg, "exp_avg", count)
+    exp_avg_sq = _tensor_list(exp_avg_sq, "exp_avg_sq", count)
+    masters = None if masters is None else _tensor_list(masters, "masters", count)
+    if count == 0:
+        return
+    bits = 8 if exp_avg[0].dtype == torch.uint8 else 32
+    state = torch.uint8 if bits == 8 else torch.float32
+    if bits == 8:
+        if avg_scales is None or avg_sq_scales is None:
+            raise ValueError("8-bit states need avg_scales and avg_sq_scales")
+        avg_scales = _tensor_list(avg_scales, "avg_scales", count)
+        avg_sq_scales = _tensor_list(avg_sq_scales, "avg_sq_scales", count)
+    elif avg_scales is not None or avg_sq_scales is not None:
+        raise ValueError("avg_scales and avg_sq_scales go with uint8 states")
+    if isinstance(weight_decay, (int, float)):
+        decays = [float(weight_decay)] * count
+    else:
+        decays = [float(d) for d in weight_decay]
+        if len(decays) != count:
+            raise ValueError("weight_decay must hold a number for each of the %d parameters, got %d"
+                             % (count, len(decays)))
+    dev = params[0].device
+    _dev_check(*params, *grads, *exp_avg, *exp_avg_sq, *(masters or []), *(avg_scales or []),
+               *(avg_sq_scales or []))
+    if scale is not None:
+        _check_out(scale, "scale", (torch.float32,), 1, dev)
+    items = (_lib.AdamwTensor * count)()
+    for i, (it, p, g, m, v) in enumerate(zip(items, params, grads, exp_avg, exp_avg_sq)):
+        _train_suffix(p)
+        _train_suffix(g)
+        n = p.numel()
+        if g.numel() != n or m.numel() != n or v.numel() != n:
+            raise ValueError("parameter %d has %d elements, its gradient %d, its moments %d and %d"
+                             % (i, n, g.numel(), m.numel(), v.numel()))
+        if m.dtype != state or v.dtype != state:
+            raise TypeError("the moments must all be %s, got %s and %s" % (state, m.dtype, v.dtype))
+        it.param, it.grad, it.exp_avg, it.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
+        it.len, it.weight_decay = n, decays[i]
+        it.param_dtype, it.grad_dtype = _TRAIN_ID[p.dtype], _TRAIN_ID[g.dtype]
+        if masters is not None:
+            if p.dtype == torch.float32:
+                raise ValueError("masters go with float16 or bfloat16 parameters")
+            _check_out(masters[i], "masters[%d]" % i, (torch.float32,), n, dev)
+            it.master = masters[i].data_ptr()
+        elif p.dtype != torch.float32:
+            raise ValueError("%s parameters need float32 masters" % p.dtype)
+        if bits == 8:
+            blocks = -(-n // STATE_BLOCK)
+            _check_out(avg_scales[i], "avg_scales[%d]" % i, (torch.float32,), blocks, dev)
+            _check_out(avg_sq_scales[i], "avg_sq_scales[%d]" % i, (torch.float32,), blocks, dev)
+            it.avg_scale, it.avg_sq_scale = avg_scales[i].data_ptr(), avg_sq_scales[i].data_ptr()
+    _lib.check(_lib.load().mlrs_adamw_step(items, count, bits, float(lr), float(betas[0]), float(betas[1]),
+                                           float(eps), int(step), _ptr(scale), int(seed) & 0xFFFFFFFF,
+                                           _stream(dev)))
+
+
+def adamw_state_values(codes, scales, which):
+    """The float32 values that an 8-bit state of ``adamw_step`` stands for
+    (mlrs_adamw_state_values): ``which`` "exp_avg", or "exp_avg_sq" for the root
+    of the second moment."""
+    if which not in ("exp_avg", "exp_avg_sq"):
+        raise ValueError("which should be 'exp_avg' or 'exp_avg_sq', got %r" % (which,))
+    _dev_check(codes, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.float32:
+        raise TypeError("codes must be uint8 and scales float32, got %s and %s" % (codes.dtype, scales.dtype))
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    _lib.check(_lib.load().mlrs_adamw_state_values(_ptr(codes), codes.numel(), _ptr(scales), scales.numel(),
+                                                   int(which == "exp_avg_sq"), _ptr(out), out.numel(),
+                                                   _stream(codes.device)))
+    return out

@@ -1,0 +1,556 @@
+"""The training operators on the GPU against their formulas in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import train_reference as ref
+from mlrs_amd import prims
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [F32, F16, BF16]
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+IGNORE = -100
+
+
+def rand(seed, *shape, dtype=F32, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g, dtype=torch.float64) * std).to(dtype)
+
+
+def dev(t, offset=0):
+    """On the GPU; with `offset` elements before it, so that it is aligned to
+    its element size alone."""
+    if t is None:
+        return None
+    if not offset:
+        return t.cuda()
+    flat = torch.empty(t.numel() + offset, dtype=t.dtype, device="cuda")
+    view = flat[offset:].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+def check_linear(n, k, m, dtype, act, bias=True, residual=True, keep=True, offset=0, seed=0):
+    x, w = rand(seed, n, k, dtype=dtype), rand(seed + 1, m, k, dtype=dtype, std=k ** -0.5)
+    b = rand(seed + 2, m, dtype=dtype, std=0.3) if bias else None
+    res = rand(seed + 3, n, m, dtype=dtype) if residual else None
+    got = prims.linear(dev(x, offset), dev(w, offset), bias=dev(b, offset), activation=act,
+                       residual=dev(res, offset), keep_preact=keep)
+    y, z = got if keep else (got, None)
+    want_y, want_z = ref.linear(x, w, b, act, res)
+    what = "linear n=%d k=%d m=%d %s %s" % (n, k, m, dtype, act)
+    ref.assert_near(y, want_y, what + " y")
+    if keep:
+        ref.assert_near(z, want_z, what + " z")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_linear_activations(dtype, act):
+    check_linear(70, 96, 80, dtype, act)
+    check_linear(5, 96, 80, dtype, act)
+
+
+# one row and few rows; one column, one output; sizes around the widths of a
+# fragment, a wave, a tile and a staged width; none a multiple of the next
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [
+    (1, 1, 1), (1, 64, 16), (1, 1000, 33), (3, 17, 5), (15, 63, 31), (16, 64, 32), (17, 65, 33), (32, 128, 48),
+    (33, 129, 47), (63, 40, 100), (64, 512, 64), (65, 1, 65), (66, 64, 64), (127, 100, 129), (128, 256, 128),
+    (129, 31, 257), (257, 257, 130), (300, 72, 520), (1000, 33, 7),
+])
+def test_linear_sizes(dtype, n, k, m):
+    check_linear(n, k, m, dtype, "gelu", seed=n + k + m)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias,residual,keep", [(False, False, False), (True, False, True), (False, True, False)])
+@pytest.mark.parametrize("n", [9, 130])
+def test_linear_options(dtype, bias, residual, keep, n):
+    check_linear(n, 72, 136, dtype, "silu", bias, residual, keep)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [(7, 64, 40), (100, 64, 64), (131, 65, 67)])
+@pytest.mark.parametrize("offset", [1, 3])
+def test_linear_unaligned(dtype, n, k, m, offset):
+    check_linear(n, k, m, dtype, "relu", offset=offset)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_every_tile(dtype):
+    """Sizes that the rule gives the largest tile, the middle one, and parts of
+    a long contraction."""
+    check_linear(2100, 72, 2100, dtype, "gelu_tanh", seed=3)
+    check_linear(1100, 40, 1030, dtype, "none", seed=4)
+    check_linear(130, 8200, 130, dtype, "silu", seed=5)
+
+
+def test_linear_no_rows_and_in_place():
+    w = dev(rand(1, 24, 16))
+    assert prims.linear(torch.empty(0, 16, device="cuda"), w).shape == (0, 24)
+    x, res = rand(2, 90, 16), rand(3, 90, 24)
+    r = dev(res)
+    y = prims.linear(dev(x), w, residual=r, out=r)
+    assert y.data_ptr() == r.data_ptr()
+    ref.assert_near(y, ref.linear(x, w.cpu(), None, "none", res)[0], "residual's buffer")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [4, 100])
+def test_linear_infinities_stay_in_their_rows(dtype, n):
+    x, w = rand(5, n, 40, dtype=dtype), rand(6, 50, 40, dtype=dtype, std=0.1)
+    clean = prims.linear(dev(x), dev(w))
+    x[1, 3] = float("inf")
+    x[2, 7] = float("nan")
+    got = prims.linear(dev(x), dev(w))
+    keep = [i for i in range(n) if i not in (1, 2)]
+    assert torch.equal(got[keep], clean[keep])
+    assert got[2].isnan().all()
+    want = torch.where(w[:, 3].float() > 0, float("inf"), float("-inf"))
+    assert torch.equal(got[1].float().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_tail_of_k_reads_no_neighbours(dtype):
+    """Rows that end inside a staged width: the next row's elements, NaN here,
+    must not reach the sum."""
+    n, k, m = 70, 24, 70
+    x, w = rand(7, n, k, dtype=dtype), rand(8, m, k, dtype=dtype)
+    x[1::2] = float("nan")
+    w[1::2] = float("nan")
+    got = prims.linear(dev(x), dev(w))[::2, ::2]
+    assert not got.isnan().any()
+    ref.assert_near(got, ref.linear(x[::2], w[::2], None, "none", None)[0], "rows between NaN rows")
+
+
+def check_grad(n, k, m, dtype, act, offset=0, seed=0, bias=True):
+    x, w = rand(seed, n, k, dtype=dtype), rand(seed + 1, m, k, dtype=dtype, std=k ** -0.5)
+    dy = rand(seed + 2, n, m, dtype=dtype, std=0.1)
+    z = rand(seed + 3, n, m, dtype=dtype) if act != "none" else None
+    dx, dw, db = prims.linear_grad(dev(dy, offset), dev(x, offset), dev(w, offset), preact=dev(z, offset),
+                                   activation=act, bias=bias)
+    want = ref.linear_grad(dy, x, w, z, act, dtype)
+    what = "linear_grad n=%d k=%d m=%d %s %s " % (n, k, m, dtype, act)
+    ref.assert_near(dx, want[0], what + "dx")
+    ref.assert_near(dw, want[1], what + "dw")
+    if bias:
+        ref.assert_near(db, want[2], what + "db")
+    else:
+        assert db is None
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_linear_grad_activations(dtype, act):
+    check_grad(70, 96, 80, dtype, act)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k,m", [
+    (1, 1, 1), (1, 64, 64), (2, 33, 17), (31, 8, 9), (63, 65, 64), (64, 64, 64), (65, 63, 66), (128, 40, 200),
+    (129, 257, 31), (300, 72, 520), (513, 130, 66),
+])
+def test_linear_grad_sizes(dtype, n, k, m):
+    check_grad(n, k, m, dtype, "silu", seed=n + k + m)
+    check_grad(n, k, m, dtype, "none", seed=n + k + m, bias=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_grad_unaligned_and_every_tile(dtype):
+    check_grad(70, 64, 72, dtype, "gelu", offset=1)
+    check_grad(70, 64, 72, dtype, "none", offset=3)
+    check_grad(2100, 2100, 40, dtype, "relu", seed=1)
+    check_grad(40, 2100, 2100, dtype, "relu", seed=2)
+    check_grad(8300, 72, 66, dtype, "gelu_tanh", seed=3)
+    check_grad(66, 72, 8300, dtype, "none", seed=4)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_grad_no_rows(dtype):
+    x, w = torch.empty(0, 24, device="cuda", dtype=dtype), dev(rand(1, 40, 24, dtype=dtype))
+    dy = torch.empty(0, 40, device="cuda", dtype=dtype)
+    for act, z in (("none", None), ("relu", dy)):
+        dx, dw, db = prims.linear_grad(dy, x, w, preact=z, activation=act)
+        assert dx.shape == (0, 24) and not dw.any() and not db.any()
+        assert dw.shape == (40, 24) and db.shape == (40,)
+
+
+def test_linear_grad_parts_asked_for():
+    n, k, m = 50, 16, 24
+    x, w, dy = (dev(rand(i, *s)) for i, s in enumerate([(n, k), (m, k), (n, m)]))
+    all3 = prims.linear_grad(dy, x, w)
+    for need in range(8):
+        got = prims.linear_grad(dy, x, w, bias=bool(need & 1), need_dx=bool(need & 2), need_dw=bool(need & 4))
+        for part, asked, whole in zip(got, (need & 2, need & 4, need & 1), all3):
+            assert torch.equal(part, whole) if asked else part is None
+
+
+def test_linear_grad_against_differences():
+    """Along random directions, the loss sum(c * y) in 64 bits changes by what
+    the kernel's float32 gradient says."""
+    n, k, m, e = 40, 24, 32, 1e-5
+    x, w, b, c = rand(1, n, k), rand(2, m, k, std=0.2), rand(3, m), rand(4, n, m)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        _, z = prims.linear(dev(x), dev(w), bias=dev(b), activation=act, keep_preact=True)
+        grads = prims.linear_grad(dev(c), dev(x), dev(w), preact=z, activation=act)
+        for i, (t, g) in enumerate(zip((x, w, b), grads)):
+            u = rand(9 + i, *t.shape).double()
+
+            def value(s):
+                a = [q.double() + (s * u if j == i else 0) for j, q in enumerate((x, w, b))]
+                return float((c.double() * ref.act(a[0] @ a[1].t() + a[2], act)[0]).sum())
+
+            slope = (value(e) - value(-e)) / (2 * e)
+            got = float((g.cpu().double() * u).sum())
+            # differences: e^2 of the third derivative and 2^-52 / e of the value;
+            # the gradient: 2^-20 of each of its terms
+            room = 1e-6 * float((g.cpu().double() * u).abs().sum()) + 1e-5
+            assert abs(got - slope) <= room, (act, i, got, slope)
+
+
+def targets(seed, n, v, ignored=0.2):
+    g = torch.Generator().manual_seed(seed)
+    t = torch.randint(0, v, (n,), generator=g)
+    t[torch.rand(n, generator=g) < ignored] = IGNORE
+    return t
+
+
+def check_xent(n, v, k, dtype, bias=True, offset=0, seed=0, spread=1.5, masked=(), grad=None):
+    h, w = rand(seed, n, k, dtype=dtype), rand(seed + 1, v, k, dtype=dtype, std=spread * k ** -0.5)
+    b = rand(seed + 2, v, dtype=dtype, std=0.5) if bias else None
+    t = targets(seed + 3, n, v)
+    for c in masked:
+        b[c] = float("-inf")
+        t[t == c] = IGNORE
+    g = rand(seed + 4, n).abs() / n if grad is None else grad
+    args = [dev(h, offset), dev(w, offset), dev(t)]
+    loss, lse = prims.softmax_xent(*args, bias=dev(b, offset), ignore_index=IGNORE)
+    dh, dw, db = prims.softmax_xent_grad(*args, lse, dev(g), bias=dev(b, offset), ignore_index=IGNORE)
+    want = ref.xent(h, w, b, t, IGNORE, g, dtype)
+    what = "softmax_xent n=%d v=%d k=%d %s " % (n, v, k, dtype)
+    for name, got in (("loss", loss), ("lse", lse), ("dh", dh), ("dw", dw), ("db", db)):
+        if name == "db" and not bias:
+            assert got is None
+        else:
+            ref.assert_near(got, want[name], what + name)
+    gone = (t == IGNORE).cuda()
+    assert not loss[gone].any() and not dh[gone].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,k", [
+    (1, 1, 1), (1, 2, 3), (1, 1000, 64), (2, 63, 8), (31, 64, 33), (32, 65, 64), (33, 127, 65), (64, 128, 128),
+    (65, 129, 17), (100, 257, 40), (129, 1000, 130), (300, 777, 64), (7, 5000, 24),
+])
+def test_xent_sizes(dtype, n, v, k):
+    check_xent(n, v, k, dtype, seed=n + v + k)
+    check_xent(n, v, k, dtype, bias=False, seed=n + v + k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_xent_unaligned_and_every_tile(dtype):
+    check_xent(40, 96, 64, dtype, offset=1)
+    check_xent(2100, 2100, 24, dtype, seed=1)
+    check_xent(1030, 1100, 40, dtype, seed=2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_xent_wide_logits(dtype):
+    """Logits tens apart: one class has nearly all of a row, others nothing."""
+    check_xent(70, 300, 64, dtype, spread=20.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_xent_masked_classes(dtype):
+    """Classes left out by a bias of -inf, whole tiles of them and the first and
+    the last among them, take no part and get no gradient."""
+    n, v, k = 40, 700, 32
+    masked = list(range(0, 260)) + [300] + list(range(690, 700))
+    check_xent(n, v, k, dtype, masked=masked)
+    h, w, t = rand(1, n, k, dtype=dtype), rand(2, v, k, dtype=dtype), targets(3, n, v)
+    b = torch.zeros(v, dtype=dtype)
+    b[masked] = float("-inf")
+    t[torch.isin(t, torch.tensor(masked))] = IGNORE
+    loss, lse = prims.softmax_xent(dev(h), dev(w), dev(t), bias=dev(b))
+    _, dw, db = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, torch.ones(n, device="cuda"), bias=dev(b))
+    assert loss.isfinite().all() and lse.isfinite().all()
+    assert not dw[masked].any() and not db[masked].any()
+
+
+def test_xent_target_that_is_masked_or_no_class():
+    h, w = rand(1, 6, 16), rand(2, 50, 16)
+    b = torch.zeros(50)
+    b[4] = float("-inf")
+    t = torch.tensor([4, 50, -1, 3, IGNORE, 49])
+    loss, lse = prims.softmax_xent(dev(h), dev(w), dev(t), bias=dev(b))
+    assert loss[0] == float("inf") and loss[1].isnan() and loss[2].isnan()
+    assert loss[3:].isfinite().all() and loss[4] == 0 and lse.isfinite().all()
+    dh, _, _ = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, torch.ones(6, device="cuda"), bias=dev(b))
+    assert dh[1].isnan().all() and dh[2].isnan().all() and dh[3].isfinite().all() and not dh[4].any()
+
+
+def test_xent_all_rows_ignored_and_no_rows():
+    for dtype in TYPES:
+        h, w, b = rand(1, 20, 16, dtype=dtype), dev(rand(2, 50, 16, dtype=dtype)), dev(rand(3, 50, dtype=dtype))
+        t = torch.full((20,), IGNORE)
+        loss, lse = prims.softmax_xent(dev(h), w, dev(t), bias=b)
+        assert not loss.any() and lse.isfinite().all()
+        parts = prims.softmax_xent_grad(dev(h), w, dev(t), lse, torch.ones(20, device="cuda"), bias=b)
+        assert not any(p.any() for p in parts)
+        e = torch.empty(0, device="cuda")
+        none = torch.empty(0, dtype=torch.int64, device="cuda")
+        loss, lse = prims.softmax_xent(dev(h)[:0], w, none, bias=b)
+        assert loss.shape == (0,) and lse.shape == (0,)
+        dh, dw, db = prims.softmax_xent_grad(dev(h)[:0], w, none, e, e, bias=b)
+        assert dh.shape == (0, 16) and dw.shape == (50, 16) and not dw.any() and not db.any()
+
+
+def test_xent_rows_with_nan_stay_alone():
+    h, w, t = rand(1, 70, 32), dev(rand(2, 300, 32)), dev(targets(4, 70, 300, 0.0))
+    clean = prims.softmax_xent(dev(h), w, t)
+    h[3, 5] = float("nan")
+    loss, lse = prims.softmax_xent(dev(h), w, t)
+    keep = [i for i in range(70) if i != 3]
+    assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(lse[keep], clean[1][keep])
+    assert loss[3].isnan() and lse[3].isnan()
+
+
+@pytest.mark.parametrize("size", [1e-6, 1.0, 3e4])
+def test_xent_half_precision_gradient_range(size):
+    """Gradients far below and above half precision's range times probabilities
+    of a large vocabulary keep their accuracy; the outputs are what their type
+    can hold."""
+    n, v, k = 64, 3000, 64
+    h, w, t = rand(1, n, k, dtype=F16), rand(2, v, k, dtype=F16, std=0.05), targets(3, n, v)
+    g = torch.full((n,), size)
+    _, lse = prims.softmax_xent(dev(h), dev(w), dev(t))
+    dh, dw, _ = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, dev(g))
+    want = ref.xent(h, w, None, t, IGNORE, g, F16)
+    ref.assert_near(dh, want["dh"], "dh")
+    ref.assert_near(dw, want["dw"], "dw")
+
+
+def test_xent_gradient_against_differences():
+    n, v, k, e = 30, 90, 20, 1e-5
+    h, w, b, t, c = rand(1, n, k), rand(2, v, k, std=0.3), rand(3, v), targets(4, n, v), rand(5, n)
+    _, lse = prims.softmax_xent(dev(h), dev(w), dev(t), bias=dev(b))
+    grads = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, dev(c), bias=dev(b))
+    kept = t != IGNORE
+    for i, (x, g) in enumerate(zip((h, w, b), grads)):
+        u = rand(9 + i, *x.shape).double()
+
+        def value(s):
+            a = [q.double() + (s * u if j == i else 0) for j, q in enumerate((h, w, b))]
+            z = a[0] @ a[1].t() + a[2]
+            rows = torch.logsumexp(z, 1) - z.gather(1, torch.where(kept, t, 0)[:, None])[:, 0]
+            return float((c.double() * rows)[kept].sum())
+
+        slope = (value(e) - value(-e)) / (2 * e)
+        got = float((g.cpu().double() * u).sum())
+        room = 4e-6 * float((g.cpu().double() * u).abs().sum()) + 1e-5
+        assert abs(got - slope) <= room, (i, got, slope)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_same_call_gives_the_same_bits_on_any_stream(dtype):
+    n, v, k = 300, 700, 65
+    h, w, t = dev(rand(1, n, k, dtype=dtype)), dev(rand(2, v, k, dtype=dtype)), dev(targets(3, n, v))
+    g = torch.full((n,), 1.0 / n, device="cuda")
+
+    def both():
+        loss, lse = prims.softmax_xent(h, w, t)
+        dh, dw, _ = prims.softmax_xent_grad(h, w, t, lse, g)
+        y, z = prims.linear(h, w, activation="gelu", keep_preact=True)
+        return [loss, lse, dh, dw, y, z] + list(prims.linear_grad(z, h, w, preact=y, activation="gelu"))
+
+    first = both()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = both()
+    third = both()  # its scratch is the other stream's too: the calls are ordered
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, again, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ---- the optimizer ----
+
+SIZES = [1, 3, 255, 256, 257, 1000, 4096, 4097, 10007]
+
+
+def opt_inputs(sizes, seed, grad_dtype=F32, std=0.01):
+    out = []
+    for i, n in enumerate(sizes):
+        s = seed + 10 * i
+        out.append((rand(s, n, std=0.1), rand(s + 1, n, std=std).to(grad_dtype), rand(s + 2, n, std=std / 3),
+                    rand(s + 3, n, std=std).square()))
+    return out
+
+
+HY = dict(step=7, lr=3e-3, betas=(0.9, 0.995), eps=1e-7)
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("grad_dtype", TYPES)
+def test_adamw_32_bits(grad_dtype, offset):
+    data = opt_inputs(SIZES, 1, grad_dtype)
+    ps, gs, ms, vs = ([dev(d[i], offset) for d in data] for i in range(4))
+    decays = [0.1 * (i % 3) for i in range(len(SIZES))]
+    scale = torch.full((1,), 0.5, device="cuda")
+    prims.adamw_step(ps, gs, ms, vs, weight_decay=decays, scale=scale, **HY)
+    for i, (p, g, m, v) in enumerate(data):
+        want = ref.adamw(p, g.double(), m, v, HY["step"], HY["lr"], HY["betas"], HY["eps"], decays[i], 0.5)
+        size = [np.abs(p.numpy()) + HY["lr"] * 4, np.abs(m.numpy()) + np.abs(g.double().numpy()),
+                np.abs(v.numpy()) + np.abs(g.double().numpy()) ** 2]
+        for got, w, s, name in zip((ps[i], ms[i], vs[i]), want, size, "pmv"):
+            # about eight roundings, each of at most half a unit of the larger term
+            assert np.all(np.abs(got.cpu().numpy() - w) <= 16 * ref.U32 * s), (i, name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_adamw_masters(dtype):
+    data = opt_inputs(SIZES, 2, dtype)
+    masters = [dev(d[0]) for d in data]
+    ps = [m.to(dtype) for m in masters]
+    gs, ms, vs = ([dev(d[i]) for d in data] for i in (1, 2, 3))
+    plain = [t.clone() for t in masters]
+    pm, pv = [t.clone() for t in ms], [t.clone() for t in vs]
+    prims.adamw_step(plain, gs, pm, pv, **HY)
+    prims.adamw_step(ps, gs, ms, vs, masters=masters, **HY)
+    for a, b in zip(plain + pm + pv, masters + ms + vs):
+        assert torch.equal(a, b)
+    for p, m in zip(ps, masters):
+        assert torch.equal(p, m.to(dtype))
+
+
+def test_adamw_more_tensors_than_a_launch():
+    sizes = [(7 * i) % 300 for i in range(130)] + [5000]  # empty ones among them
+    data = opt_inputs(sizes, 3)
+    ps, gs, ms, vs = ([dev(d[i]) for d in data] for i in range(4))
+    prims.adamw_step(ps, gs, ms, vs, **HY)
+    one = [[dev(d[i]) for d in data] for i in range(4)]
+    for p, g, m, v in zip(*one):
+        prims.adamw_step([p], [g], [m], [v], **HY)
+    for got, want in zip((ps, ms, vs), (one[0], one[2], one[3])):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def opt8_inputs(sizes, seed):
+    r = np.random.default_rng(seed)
+    out = []
+    for n in sizes:
+        blocks = -(-n // 256)
+        out.append([r.normal(0, 0.1, n).astype(np.float32), r.normal(0, 0.01, n).astype(np.float32),
+                    r.integers(0, 256, n).astype(np.uint8), r.integers(0, 256, n).astype(np.uint8),
+                    r.uniform(0.001, 0.01, blocks).astype(np.float32), r.uniform(0.001, 0.02, blocks).astype(np.float32)])
+    return out
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+def test_adamw_8_bits_follows_its_definition(offset):
+    """Three steps, codes and scales bit for bit, from states of every code and
+    from the zero state, with blocks whose gradient is zero."""
+    data = opt8_inputs(SIZES, 5)
+    data.append([t.copy() * (0 if i >= 2 else 1) for i, t in enumerate(opt8_inputs([3000], 6)[0])])
+    data[-1][1][256:512] = 0.0
+    dt = [[dev(torch.from_numpy(d[i].copy()), offset) for d in data] for i in range(6)]
+    decays = [0.0 if i % 2 else 0.05 for i in range(len(data))]
+    scale = torch.full((1,), 0.8, device="cuda")
+    for step in (1, 2, 3):
+        prims.adamw_step(dt[0], dt[1], dt[2], dt[3], step=step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+                         weight_decay=decays, avg_scales=dt[4], avg_sq_scales=dt[5], scale=scale, seed=1000 + step)
+        for i, d in enumerate(data):
+            d[0], d[2], d[3], d[4], d[5] = ref.adamw8(*[d[j] for j in (0, 1, 2, 3, 4, 5)], i, step, 1e-3,
+                                                      (0.9, 0.999), 1e-8, decays[i], 1000 + step, np.float32(0.8))
+            for j, name in ((4, "scale m"), (5, "scale root"), (2, "codes m"), (3, "codes root"), (0, "p")):
+                got = dt[j][i].cpu().numpy()
+                assert np.array_equal(got, d[j]), (step, i, name, int((got != d[j]).sum()), len(got))
+    for i, d in enumerate(data):
+        m = prims.adamw_state_values(dt[2][i], dt[4][i], "exp_avg").cpu().numpy()
+        r = prims.adamw_state_values(dt[3][i], dt[5][i], "exp_avg_sq").cpu().numpy()
+        n = len(d[0])
+        vm = ref.code_values(d[2] & 127, 3)
+        assert np.array_equal(m, np.where(d[2] > 127, -vm, vm) * np.repeat(d[4], 256)[:n])
+        assert np.array_equal(r, ref.code_values(d[3], 4) * np.repeat(d[5], 256)[:n])
+
+
+def test_adamw_8_bits_half_parameters():
+    d = opt8_inputs([5000], 8)[0]
+    t = [dev(torch.from_numpy(x.copy())) for x in d]
+    g = t[1].to(BF16)
+    param = t[0].to(BF16)
+    prims.adamw_step([param], [g], [t[2]], [t[3]], step=4, lr=1e-3, masters=[t[0]], avg_scales=[t[4]],
+                     avg_sq_scales=[t[5]], weight_decay=0.1, seed=3)
+    want = ref.adamw8(d[0], g.float().cpu().numpy(), d[2], d[3], d[4], d[5], 0, 4, 1e-3, (0.9, 0.999), 1e-8, 0.1, 3)
+    assert np.array_equal(t[0].cpu().numpy(), want[0]) and np.array_equal(t[2].cpu().numpy(), want[1])
+    assert torch.equal(param, t[0].to(BF16))
+
+
+def test_adamw_8_bits_moves_on_average():
+    """A constant gradient: the second moment's root must approach it although a
+    step is far below half a code, as rounding up by chance lets it."""
+    n = 1 << 16
+    g = torch.full((n,), 0.01, device="cuda")
+    p, m, r = torch.zeros(n, device="cuda"), *(torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ms, rs = (torch.zeros(n // 256, device="cuda") for _ in range(2))
+    m[0::256] = 0
+    # one element of each block has a gradient ten times as large, so that the
+    # others' codes are not the block's largest
+    g[0::256] = 0.1
+    for step in range(1, 201):
+        prims.adamw_step([p], [g], [m], [r], step=step, lr=0.0, betas=(0.9, 0.98), avg_scales=[ms],
+                         avg_sq_scales=[rs], seed=step * 7919)
+    root = prims.adamw_state_values(r, rs, "exp_avg_sq")
+    avg = prims.adamw_state_values(m, ms, "exp_avg")
+    small = torch.ones(n, dtype=torch.bool, device="cuda")
+    small[0::256] = False
+    want = 0.01 * (1 - 0.98 ** 200) ** 0.5
+    # a code is up to 2^-4 of its value; over 65,000 elements the mean of the
+    # random roundings is within a hundredth of that, and squaring a rounded
+    # root adds its variance, under 2^-9, fifty times over: 2^-4 in all
+    assert abs(float(root[small].mean()) / want - 1) < 2.0 ** -4
+    assert abs(float(avg[small].mean()) / 0.01 - 1) < 2.0 ** -6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("factor", [float("nan"), float("inf")])
+def test_adamw_takes_no_step_with_a_factor_that_is_not_finite(bits, factor):
+    d = opt8_inputs([3000], 9)[0]
+    t = [dev(torch.from_numpy(x.copy())) for x in d]
+    if bits == 32:
+        t[2], t[3] = t[2].float(), t[3].float()
+    before = [x.clone() for x in t]
+    more = dict(avg_scales=[t[4]], avg_sq_scales=[t[5]]) if bits == 8 else {}
+    prims.adamw_step([t[0]], [t[1]], [t[2]], [t[3]], step=2, lr=0.1, scale=torch.full((1,), factor, device="cuda"),
+                     **more)
+    for a, b in zip(t, before):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [0, 1])
+def test_clip_scale(dtype, offset):
+    sizes = SIZES + [(11 * i) % 500 for i in range(60)] + [300000]
+    gs = [rand(i, n, dtype=dtype) for i, n in enumerate(sizes)]
+    square = sum(float(g.double().square().sum()) for g in gs)
+    for max_norm in (1.0, 1e6):
+        norm, scale = prims.clip_scale([dev(g, offset) for g in gs], max_norm)
+        assert abs(float(norm) / square ** 0.5 - 1) <= 16 * ref.U32
+        want = min(1.0, max_norm / square ** 0.5)
+        assert abs(float(scale) / want - 1) <= 16 * ref.U32
+
+
+def test_clip_scale_of_nothing_and_of_infinities():
+    norm, scale = prims.clip_scale([torch.empty(0, device="cuda"), torch.zeros(5, device="cuda")], 1.0)
+    assert float(norm) == 0.0 and float(scale) == 1.0
+    for bad in (float("inf"), float("nan")):
+        g = torch.ones(5000, device="cuda")
+        g[4321] = bad
+        norm, scale = prims.clip_scale([torch.ones(3, device="cuda"), g], 1.0)
+        assert not norm.isfinite().any() and scale.isnan().all()
