@@ -32,6 +32,24 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
 }
 
+// The same over a group: one switch for all of it.
+template <int N>
+__device__ __forceinline__ void activate_all(f32x4 (&v)[N], int act) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] = f(v[u][e]);
+    };
+    switch (act) {
+    case kActRelu: each([](float z) { return activate(z, kActRelu); }); break;
+    case kActGelu: each([](float z) { return activate(z, kActGelu); }); break;
+    case kActGeluTanh: each([](float z) { return activate(z, kActGeluTanh); }); break;
+    case kActSilu: each([](float z) { return activate(z, kActSilu); }); break;
+    default: break;
+    }
+}
+
 // d activate / dz
 __device__ __forceinline__ float activate_slope(float z, int act) {
     switch (act) {
@@ -80,20 +98,29 @@ __device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, bool wide
     }
 }
 
-// Hands every element of the wave's part with m < m_end to f(n, m, v): four consecutive m of
-// one n, the lanes along the row, so that a row leaves in whole lines.  The
+// Hands the wave's part with m < m_end to f(n, m, v) in groups: v[u] holds four
+// consecutive m of row n + u * step (which may be past the last row), the lanes
+// along the row, so that a row leaves in whole lines; a lane's m is the same in
+// every call.  Groups, so that what f loads for them is under way at once.  The
 // accumulators (a lane holds four m of one n, lanes run along n) are turned
-// through the wave's own part of LDS, 32 rows at a time; a row's 16-byte
-// chunks are kept at c ^ (n & 7).
+// through the wave's own part of LDS, 32 rows at a time; a row's 16-byte chunks
+// are kept at c ^ (n & 7).
+constexpr int kGroup = 4;
+template <int MB>
+constexpr int row_step() {
+    return 64 / (MB * 8);  // rows that the lanes cover together
+}
 template <int MB, int NB, typename F>
 __device__ __forceinline__ void for_rows(const f32x16 (&acc)[MB][NB], const Place& p, char* lds, int32_t m_end,
                                          F f) {
-    constexpr int kRow = MB * 128;                // bytes
-    constexpr int kLanes = MB * 8;                // of a row
-    constexpr int kStep = 64 / kLanes;            // rows per access
+    constexpr int kRow = MB * 128;      // bytes
+    constexpr int kLanes = MB * 8;      // of a row
+    constexpr int kStep = row_step<MB>();
     char* mine = lds + p.wave * 32 * kRow;
     const int h = p.lane >> 5, r = p.lane & 31;
-    __syncthreads();  // the tiles in LDS are no longer read
+    const int c = p.lane % kLanes;
+    const int32_t m = p.m0 + 4 * c;
+    __syncthreads();  // the panels in LDS are no longer read
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
 #pragma unroll
@@ -107,12 +134,15 @@ __device__ __forceinline__ void for_rows(const f32x16 (&acc)[MB][NB], const Plac
             }
         // the wave's LDS accesses are in order; nothing else touches `mine`
         __builtin_amdgcn_wave_barrier();
-        const int c = p.lane % kLanes;
 #pragma unroll 1
-        for (int t = 0; t < 32; t += kStep) {
-            const int row = t + p.lane / kLanes;
-            const f32x4 v = *reinterpret_cast<const f32x4*>(mine + row * kRow + ((c ^ (row & 7)) << 4));
-            const int32_t n = p.n0 + j * 32 + row, m = p.m0 + 4 * c;
+        for (int t = 0; t < 32; t += kStep * kGroup) {
+            f32x4 v[kGroup];
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) {
+                const int row = t + u * kStep + p.lane / kLanes;
+                v[u] = *reinterpret_cast<const f32x4*>(mine + row * kRow + ((c ^ (row & 7)) << 4));
+            }
+            const int32_t n = p.n0 + j * 32 + t + p.lane / kLanes;
             if (n < p.n && m < m_end) f(n, m, v);
         }
         __builtin_amdgcn_wave_barrier();
@@ -130,17 +160,39 @@ struct LinearEpi {
     int32_t act;
     bool wide;
 
-    __device__ __forceinline__ void point(int64_t n, int64_t m, int64_t end, f32x4 v) const {
-        if (bias) v += load4(bias, m, end, false);
-        if (z) store4(z + n * ld, m, end, wide, v);
+    // rows n, n + step, ... of them those before n_end
+    template <int N>
+    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, f32x4 bv,
+                                         f32x4 (&v)[N]) const {
+        f32x4 res[N] = {};
+        if (residual) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = activate(v[e], act);
-        if (residual) v += load4(residual + n * ld, m, end, wide);
-        store4(y + n * ld, m, end, wide, v);
+            for (int u = 0; u < N; ++u)
+                if (n + u * step < n_end) res[u] = load4(residual + (n + u * step) * ld, m, end, wide);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) v[u] += bv;
+        if (z) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, wide, v[u]);
+        }
+        activate_all(v, act);
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, wide, residual ? v[u] + res[u] : v[u]);
+    }
+    __device__ __forceinline__ f32x4 bias_at(int64_t m, int64_t end) const {
+        f32x4 bv = {};
+        if (bias && m < end) bv = load4(bias, m, end, false);
+        return bv;
     }
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
-        for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 v) { point(n, m, p.m, v); });
+        const f32x4 bv = bias_at(p.m0 + 4 * (p.lane % (MB * 8)), p.m);
+        for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[kGroup]) {
+            rows(n, row_step<MB>(), p.n, m, p.m, bv, v);
+        });
     }
 };
 
@@ -155,22 +207,34 @@ struct StoreEpi {
     int64_t ld, part_ld, part_stride;
     bool wide;
 
-    __device__ __forceinline__ void finish(int64_t n, int64_t m, int64_t end, f32x4 v) const {
-        if (add) v += load4(add + n * part_ld, m, end, true);
-        if (alpha) v *= *alpha;
-        store4(out + n * ld, m, end, wide, v);
+    template <int N>
+    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, int split,
+                                         f32x4 (&v)[N]) const {
+        if (add) {
+            f32x4 old[N] = {};
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, true);
+#pragma unroll
+            for (int u = 0; u < N; ++u) v[u] += old[u];
+        }
+        if (out) {
+            const float by = alpha ? *alpha : 1.0f;
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, wide, v[u] * by);
+        } else {
+            float* to = part + split * part_stride;  // part_ld is a multiple of 4
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, true, v[u]);
+        }
     }
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
-        if (out) {
-            for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 v) { finish(n, m, p.m, v); });
-        } else {
-            float* to = part + p.split * part_stride;
-            for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 v) {
-                if (add) v += load4(add + n * part_ld, m, p.m, true);
-                store4(to + n * part_ld, m, p.m, true, v);  // part_ld is a multiple of 4
-            });
-        }
+        for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[kGroup]) {
+            rows(n, row_step<MB>(), p.n, m, p.m, p.split, v);
+        });
     }
 };
 
@@ -276,25 +340,35 @@ struct LogitGradEpi {
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
         const float scale = up ? *up : 1.0f;
-        for_rows(acc, p, lds, (int32_t)ld, [&](int32_t n, int32_t m, f32x4 v) {
-            const int64_t t = target[n];
-            const bool kept = t != ignore;
-            float g = grad[n] * scale;
-            if (t < 0 || t >= classes) g = __builtin_nanf("");
-            const float l = lse[n];
-            if (bias) v += load4(bias, m, p.m, false);
+        f32x4 bv = {};
+        const int32_t mine = p.m0 + 4 * (p.lane % (MB * 8));
+        if (bias && mine < p.m) bv = load4(bias, mine, p.m, false);
+        for_rows(acc, p, lds, (int32_t)ld, [&](int32_t n, int32_t m, f32x4 (&v)[kGroup]) {
+            constexpr int kStep = row_step<MB>();
+            int64_t t[kGroup];
+            float g[kGroup], l[kGroup];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x = exp_fast(v[e] - l);
-                if (t == first + m + e) x -= 1.0f;
-                v[e] = kept ? x * g : 0.0f;
+            for (int u = 0; u < kGroup; ++u) {
+                const int32_t at = n + u * kStep < p.n ? n + u * kStep : n;
+                t[u] = target[at];
+                g[u] = grad[at];
+                l[u] = lse[at];
             }
-            // the columns up to ld, a multiple of 16 bytes, are read by the
-            // products and must be zero
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (m + e >= p.m) v[e] = 0.0f;
-            store4(out + (int64_t)n * ld, m, ld, true, v);
+            for (int u = 0; u < kGroup; ++u) {
+                if (n + u * kStep >= p.n) break;
+                const bool kept = t[u] != ignore;
+                const float by = t[u] < 0 || t[u] >= classes ? __builtin_nanf("") : g[u] * scale;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = exp_fast(v[u][e] + bv[e] - l[u]);
+                    if (t[u] == first + m + e) x -= 1.0f;
+                    // the columns up to ld, a multiple of 16 bytes, are read by
+                    // the products and must be zero
+                    v[u][e] = kept && m + e < p.m ? x * by : 0.0f;
+                }
+                store4(out + (int64_t)(n + u * kStep) * ld, m, ld, true, v[u]);
+            }
         });
     }
 };

@@ -19,7 +19,8 @@
 // descriptor's bounds check.
 //
 // LDS layout.  K operand: a row's 128 bytes as eight 16-byte chunks, chunk c
-// kept at c ^ (row & 7), so eight rows read at one c touch all banks.  R
+// kept at c ^ ((row >> 1) & 7), so that sixteen rows read at one c (a pass of
+// a 16-byte read: 64 banks) touch all banks.  R
 // operand: the tile's elements of one k back to back, their 16-byte chunks
 // kept at c ^ r_swizzle(k): the four k of a transposing read (16-bit types)
 // and the two halves of a wave (f32) then lie in different banks.  The swizzle
@@ -41,6 +42,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -111,11 +113,32 @@ __device__ __forceinline__ f32x16 mfma_step(typename Elem<T>::Frag a, typename E
     return c;
 }
 
+// K layout: what the chunk index of a row is exclusive-ored with.
+__device__ __forceinline__ int k_swizzle(int row) { return (row >> 1) & 7; }
+
 // R layout: what the chunk index of step k is exclusive-ored with.
 template <typename T, int ROWS>
 __device__ __forceinline__ int r_swizzle(int k) {
     if (sizeof(T) == 4) return (k & 4) << 1;
     return ROWS * 2 >= 256 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+}
+
+// 16 bytes per lane from a buffer straight into LDS, lane i's at lds + 16 i; lds
+// and the descriptor are uniform over the wave.  Counted by vmcnt, which the
+// caller waits for: written as an instruction because the compiler would wait
+// for every copy under way at each transposing LDS read, not knowing that they
+// touch other slots.  It has no result register.
+__device__ __forceinline__ void copy_to_lds(u32x4 rsrc, char* lds, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"((uint32_t)(uintptr_t)(MLRS_LDS void*)lds), "v"(offset), "s"(rsrc)
+                 : "memory");
+#else
+    (void)rsrc;
+    (void)lds;
+    (void)offset;
+#endif
 }
 
 // One operand's copy into LDS: the bytes of ROWS rows (or columns) of one
@@ -128,7 +151,7 @@ struct Stager {
     const char* base;   // the tile's first element at k = 0
     int64_t bytes;      // from base to the operand's end
     int64_t step;       // bytes per element of k
-    int32_t kbytes;     // K layout: 16 * the lane's chunk
+    int32_t chunk[2];   // K layout: 16 * the lane's chunk, of even and of odd copies
     uint32_t off[kInstr];
 
     __device__ __forceinline__ void init(const Operand& o, int32_t row0, int32_t rows, int32_t k, int wave, int lane) {
@@ -140,13 +163,14 @@ struct Stager {
         bytes = total - at;
         step = KC ? es : o.ld * es;
         const uint32_t ldb = (uint32_t)(o.ld * es);
-        kbytes = 0;
+        chunk[0] = chunk[1] = 0;
 #pragma unroll
         for (int i = 0; i < kInstr; ++i) {
             const int q = (wave * kInstr + i) * 64 + lane;
             if constexpr (KC) {
-                const int r = q >> 3, c = (q & 7) ^ (r & 7);
-                kbytes = 16 * c;
+                static_assert(kInstr % 2 == 0, "which chunk a lane copies goes by the copy's parity");
+                const int r = q >> 3, c = (q & 7) ^ k_swizzle(r);
+                chunk[i & 1] = 16 * c;
                 off[i] = (uint32_t)r * ldb + 16u * (uint32_t)c;
             } else {
                 const int kk = q / kChunks;
@@ -156,20 +180,26 @@ struct Stager {
         }
     }
 
-    // Elements k0 .. k0 + the staged width; k is the operand's extent.
+    // Part PART of PARTS of the copies of elements k0 .. k0 + the staged width;
+    // k is the end of the contraction, past which come zeros.
+    template <int PART, int PARTS>
     __device__ __forceinline__ void load(char* lds, int32_t k0, int32_t k, int wave) const {
 #if defined(__HIP_DEVICE_COMPILE__)
         const int64_t skip = (int64_t)k0 * step;
         const int64_t left = bytes - skip;
         const uint32_t records = left < 0x7FFFFFFF ? (left > 0 ? (uint32_t)left : 0u) : 0x7FFFFFFFu;
-        __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + skip), (short)0, (int)records, 0x00027000);
+        const uint64_t at = (uint64_t)(base + skip);
+        u32x4 rsrc;
+        rsrc[0] = (uint32_t)at;
+        rsrc[1] = (uint32_t)(at >> 32) & 0xFFFFu;
+        rsrc[2] = records;
+        rsrc[3] = 0x00027000u;
         // chunks past the end of a row would be the next row's
-        const bool out = KC && kbytes >= (k - k0) * (int)sizeof(T);
+        const bool out[2] = {KC && chunk[0] >= (k - k0) * (int)sizeof(T),
+                             KC && chunk[1] >= (k - k0) * (int)sizeof(T)};
 #pragma unroll
-        for (int i = 0; i < kInstr; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rsrc, (MLRS_LDS void*)(lds + (wave * kInstr + i) * 1024), 16, out ? 0x80000000u : off[i], 0, 0, 0);
+        for (int i = PART * kInstr / PARTS; i < (PART + 1) * kInstr / PARTS; ++i)
+            copy_to_lds(rsrc, lds + (wave * kInstr + i) * 1024, out[i & 1] ? 0x80000000u : off[i]);
 #else
         (void)lds;
         (void)k0;
@@ -189,7 +219,7 @@ struct Reader {
         const int h = lane >> 5, r = lane & 31;
         if constexpr (KC) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = (first + r) * kStageBytes + (((2 * s + h) ^ (r & 7)) << 4);
+            for (int s = 0; s < 4; ++s) at[s] = (first + r) * kStageBytes + (((2 * s + h) ^ k_swizzle(r)) << 4);
         } else if constexpr (sizeof(T) == 2) {
             // lane 4 q + p of sixteen addresses four elements of step q of
             // four; the transposing read hands lane i column i of them
@@ -252,14 +282,22 @@ __device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
     return x * per + (x < extra ? x : extra) + i;
 }
 
+// Waits until at most N of the wave's copies are under way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    static_assert(N < 64, "six bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
 __global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 : 2))) void gemm_kernel(GemmArgs g,
                                                                                                        Epi epi) {
     constexpr int BM = WM * MB * 32, BN = WN * NB * 32, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
     constexpr int BK = stage_elems<T>();
-    static_assert(((kA + kB) & (kA + kB - 1)) == 0, "the buffers are toggled by one bit");
-    __shared__ __attribute__((aligned(1024))) char buf[2 * (kA + kB)];
+    static_assert(kA == kB, "panels of either operand take the same slots");
+    constexpr int kSlots = 5;
+    __shared__ __attribute__((aligned(1024))) char buf[kSlots * kA];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -280,8 +318,8 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 
 
     Stager<T, AKC, BM, WAVES> sa;
     Stager<T, BKC, BN, WAVES> sb;
-    sa.init(g.a, m0, g.m, g.k, wave, lane);
-    sb.init(g.b, n0, g.n, g.k, wave, lane);
+    sa.init(g.a, m0, g.m, k_hi, wave, lane);
+    sb.init(g.b, n0, g.n, k_hi, wave, lane);
     Reader<T, AKC, BM, MB> ra;
     Reader<T, BKC, BN, NB> rb;
     ra.init(wm * MB * 32, lane);
@@ -289,45 +327,78 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 
 
     f32x16 acc[MB][NB] = {};
 
-    auto stage = [&](char* to, int32_t k0) {
-        sa.load(to, k0, g.k, wave);
-        sb.load(to + kA, k0, g.k, wave);
+    // Panels A0 B0 A1 B1 ... go round five slots of LDS.  Fragments are read one
+    // step of sixteen (f32: eight) ahead of the matrix instructions that use
+    // them, across the staged widths too: the barrier that publishes width p + 1
+    // stands before the last step of width p, whose fragments are in registers by
+    // then.  After it nothing reads A_p and B_p any more; B_{p+2} and A_{p+3} are
+    // copied over them, a quarter of the copies in every step, so that neither
+    // the matrix nor the memory pipeline sees a burst.
+    typename Elem<T>::Frag fa[2][MB], fb[2][NB];
+    auto fetch = [&](const char* pa, const char* pb, int s, int set) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i) fa[set][i] = ra.get(pa, s, i);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) fb[set][j] = rb.get(pb, s, j);
     };
-    auto compute = [&](const char* from) {
-        typename Elem<T>::Frag a[2][MB], b[2][NB];
+    auto multiply = [&](int set) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) a[0][i] = ra.get(from, 0, i);
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int j = 0; j < NB; ++j) b[0][j] = rb.get(from + kA, 0, j);
+            for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(fa[set][i], fb[set][j], acc[i][j]);
+    };
+    // one LDS read, one matrix instruction, in turn
+    auto interleave = [&]() {
+        constexpr int kReads = MB * (AKC ? 1 : sizeof(T) == 2 ? 2 : 4) + NB * (BKC ? 1 : sizeof(T) == 2 ? 2 : 4);
+        constexpr int kMath = MB * NB * (sizeof(T) == 4 ? 4 : 1);
+        constexpr int kPer = (kReads + kMath - 1) / kMath;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s + 1 < 4) {
-#pragma unroll
-                for (int i = 0; i < MB; ++i) a[(s + 1) & 1][i] = ra.get(from, s + 1, i);
-#pragma unroll
-                for (int j = 0; j < NB; ++j) b[(s + 1) & 1][j] = rb.get(from + kA, s + 1, j);
-            }
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-#pragma unroll
-                for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(a[s & 1][i], b[s & 1][j], acc[i][j]);
+        for (int i = 0; i < kMath; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
     };
-    // a staged width's copies have landed for every wave, and the other
-    // buffer is no longer read
-    auto publish = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-        __syncthreads();
-    };
+    auto slot = [&](int at) { return buf + (at >= kSlots * kA ? at - kSlots * kA : at); };
+    constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
 
-    int cur = 0;
-    if (k_lo < k_hi) stage(buf, k_lo);
+    sa.template load<0, 1>(buf, k_lo, k_hi, wave);
+    sb.template load<0, 1>(buf + kA, k_lo, k_hi, wave);
+    sa.template load<0, 1>(buf + 2 * kA, k_lo + BK, k_hi, wave);
+    sb.template load<0, 2>(buf + 3 * kA, k_lo + BK, k_hi, wave);
+    wait_copies<IA + IB / 2>();
+    __builtin_amdgcn_s_barrier();
+    fetch(buf, buf + kA, 0, 0);
+    int cur = 0;  // of A_p
     for (int32_t k0 = k_lo; k0 < k_hi; k0 += BK) {
-        publish();
-        if (k0 + BK < k_hi) stage(buf + (cur ^ (kA + kB)), k0 + BK);
-        compute(buf + cur);
-        cur ^= kA + kB;
+        const char *pa = buf + cur, *pb = slot(cur + kA);
+        __builtin_amdgcn_sched_barrier(0);
+        sb.template load<1, 2>(slot(cur + 3 * kA), k0 + BK, k_hi, wave);
+        fetch(pa, pb, 1, 1);
+        multiply(0);
+        interleave();
+        __builtin_amdgcn_sched_barrier(0);
+        sa.template load<0, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
+        fetch(pa, pb, 2, 0);
+        multiply(1);
+        interleave();
+        __builtin_amdgcn_sched_barrier(0);
+        sa.template load<1, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
+        fetch(pa, pb, 3, 1);
+        multiply(0);
+        interleave();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the last fragments of p
+        wait_copies<IA>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        sb.template load<0, 2>(buf + cur, k0 + 2 * BK, k_hi, wave);
+        fetch(slot(cur + 2 * kA), slot(cur + 3 * kA), 0, 0);
+        multiply(1);
+        interleave();
+        cur = cur + 2 * kA >= kSlots * kA ? cur - (kSlots - 2) * kA : cur + 2 * kA;
     }
+    // copies past the end of the contraction may still write their zeros
+    wait_copies<0>();
 
     Place p;
     p.m0 = m0 + wm * MB * 32;

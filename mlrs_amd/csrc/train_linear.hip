@@ -98,18 +98,17 @@ static hipError_t launch_join(const float* part, int splits, int64_t m, int64_t 
 template <typename T>
 struct LinearPoint {
     LinearEpi<T> e;
-    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const { e.point(n, c, m, v); }
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
+        f32x4 g[1] = {v};
+        e.rows(n, 0, n + 1, c, m, e.bias_at(c, m), g);
+    }
 };
 template <typename T>
 struct StorePoint {
     StoreEpi<T> e;
     __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
-        if (e.out) {
-            e.finish(n, c, m, v);
-        } else {
-            if (e.add) v += load4(e.add + n * e.part_ld, c, m, true);
-            store4(e.part + n * e.part_ld, c, m, true, v);
-        }
+        f32x4 g[1] = {v};
+        e.rows(n, 0, n + 1, c, m, 0, g);
     }
 };
 
@@ -226,7 +225,10 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) v += sums[i][b][lane];
         const int32_t row = b * 16 + r, c = m0 + 4 * q;
-        if (row < n && c < m) epi.point(row, c, m, v);
+        if (row < n && c < m) {
+            f32x4 g[1] = {v};
+            epi.rows(row, 0, row + 1, c, m, epi.bias_at(c, m), g);
+        }
     }
 }
 
