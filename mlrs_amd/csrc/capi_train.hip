@@ -212,13 +212,6 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
 }
 
 // ---------------------------------------------------------------------------
-// The tile of a product that is not split.
-template <typename T>
-int tile_for(int64_t m, int64_t n, int cus) {
-    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256), mid = ((m + 127) / 128) * ((n + 127) / 128);
-    return large >= cus ? 0 : mid >= cus ? 1 : 2;
-}
-
 template <typename T>
 int32_t check_xent(int64_t h_len, int64_t n, int64_t d, int64_t w_len, int64_t v, const T* bias, int64_t bias_len,
                    int64_t target_len, int64_t out_len) {
@@ -246,7 +239,7 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         int cus = 0;
         rc = capi::cu_count(&cus);
         if (rc) return rc;
-        const int tile = tile_for<T>(v, n, cus);
+        const int tile = choose_cut((int)sizeof(T), v, n, d, cus, 1).tile;
         const int64_t parts = stats_parts(tile, v);
         Op<T> ho(h, n, d), wo(w, v, d);
         float *top = nullptr, *total = nullptr, *hit = nullptr;
@@ -340,7 +333,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             const int64_t vp = std::min(piece, v - v0);
             const bool last = v0 + vp == v;
             MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
-                                          tile_for<T>(vp, n, cus), s));
+                                          choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile, s));
             const Mat dzm{dz, ld};
             if (db) {
                 MLRS_TRY(launch_column_sums<T>(dzm, n, vp, sums, parts, s));

@@ -25,7 +25,7 @@ struct Cut {
         return splits > 1 ? (size_t)splits * (size_t)n * (size_t)((m + 3) & ~(int64_t)3) * 4 : 0;
     }
 };
-Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus);
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
 
 // dst (rows x ld, ld >= cols) := src (rows x cols), zeros behind each row.
 template <typename T>

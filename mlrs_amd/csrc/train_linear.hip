@@ -10,28 +10,36 @@ namespace train {
 // ---------------------------------------------------------------------------
 // how a product is cut
 // ---------------------------------------------------------------------------
-// Cycles of a staged width (128 bytes of k) of a tile with its resident
-// neighbours on the CU, and how many those are.
-Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus) {
-    const double stage[3] = {elem_bytes == 2 ? 3000.0 : 18000.0, elem_bytes == 2 ? 2000.0 : 9500.0,
-                             elem_bytes == 2 ? 1800.0 : 5500.0};
-    const int resident[3] = {1, 2, 4};
+// The time of each choice, in microseconds, from measurements on this chip:
+// a staged width (128 bytes of k) of the one, two, ... tiles that a CU holds at
+// a time, and what a round of tiles costs besides (its first copies, its
+// epilogue).  16-bit tiles are bound by LDS and copies, so a CU that holds one
+// of the smaller tiles is far from twice as fast as one that holds two; f32
+// tiles are bound by the matrix cores, and only the count matters.  Measured at
+// 2048 x 1024 x 4096 in bf16: 32.1 us in 256 x 256 tiles, 24.8 in 128 x 128,
+// 33.8 in 64 x 64; at 16384 x 4096 x 4096: 433, 513, -.
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits) {
+    static const double stage16[3][4] = {{1.6}, {0.62, 0.98}, {0.45, 0.55, 0.8, 1.0}};
+    static const double stage32[3][4] = {{7.4}, {2.0, 4.0}, {0.7, 1.05, 1.55, 2.05}};
+    static const double round_us[3] = {6.0, 4.5, 4.0};
+    static const int resident[3] = {1, 2, 4};
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
     Cut best{0, 1, 0};
     double best_cost = 1e300;
     for (int t = 0; t < 3; ++t) {
+        const double* stage = elem_bytes == 2 ? stage16[t] : stage32[t];
         const int rows = kTileRows[t];
         const int64_t tiles = ((m + rows - 1) / rows) * ((n + rows - 1) / rows);
-        for (int64_t sp = 1; sp <= 64 && sp <= stages; sp = sp < 4 ? sp + 1 : sp * 2) {
+        for (int64_t sp = 1; sp <= max_splits && sp <= stages; sp = sp < 4 ? sp + 1 : sp * 2) {
             const int64_t each = (stages + sp - 1) / sp;
-            if (sp > 1 && (each < 4 || (sp - 1) * each >= stages)) continue;
-            const int64_t wgs = tiles * sp;
-            const double rounds = std::ceil((double)wgs / (double)(cus * resident[t]));
-            // a CU that holds fewer than its neighbours runs them faster
-            const double fill = std::min(1.0, std::max(0.4, (double)wgs / (double)(cus * resident[t])));
-            double cost = rounds * (each * stage[t] * (rounds > 1 ? 1.0 : fill) + 6000.0);
-            if (sp > 1) cost += 8000.0 + (double)sp * (double)m * (double)n * 8.0 / 2000.0;
+            if (sp > 1 && (each < 3 || (sp - 1) * each >= stages)) continue;
+            const int64_t on_cu = (tiles * sp + cus - 1) / cus;  // tiles that the busiest CU computes
+            const int64_t rounds = on_cu / resident[t], rest = on_cu % resident[t];
+            double cost = (double)rounds * ((double)each * stage[resident[t] - 1] + round_us[t]);
+            if (rest) cost += (double)each * stage[rest - 1] + round_us[t];
+            // joining the parts: a launch, and their bytes twice
+            if (sp > 1) cost += 5.0 + (double)sp * (double)m * (double)n * 8.0 / 4.5e6;
             if (cost < best_cost) {
                 best_cost = cost;
                 best.tile = t;
@@ -321,13 +329,22 @@ hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, float* sums, int part
     return act_grad<T>((const T*)a.p, a.ld, nullptr, kActNone, n, m, nullptr, 0, sums, parts, s);
 }
 
+// A workgroup joins the parts of 16 columns: sixteen threads take every
+// sixteenth part of a column, then one of them joins the sixteen in order.
 template <typename T>
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ sums, int parts, int64_t m,
                                                         const float* __restrict__ alpha, T* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= m) return;
+    __shared__ float join[16][16];
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
+    const int64_t c = (int64_t)blockIdx.x * 16 + col;
     float v = 0.0f;
-    for (int p = 0; p < parts; ++p) v += sums[(int64_t)p * m + c];
+    if (c < m)
+        for (int p = slice; p < parts; p += 16) v += sums[(int64_t)p * m + c];
+    join[slice][col] = v;
+    __syncthreads();
+    if (slice != 0 || c >= m) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) v += join[i][col];
     if (alpha) v *= *alpha;
     out[c] = (T)v;
 }
@@ -335,7 +352,7 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
 template <typename T>
 hipError_t launch_sum_parts(const float* sums, int parts, int64_t m, const float* alpha, T* out, hipStream_t s) {
     if (m == 0) return hipSuccess;
-    sum_parts_kernel<T><<<dim3((unsigned)((m + 255) / 256)), 256, 0, s>>>(sums, parts, m, alpha, out);
+    sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(sums, parts, m, alpha, out);
     return hipGetLastError();
 }
 

@@ -22,34 +22,50 @@ hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target,
     return launch_gemm<T, true, true>(tile, w, h, classes, n, k, 1, 0, e, s);
 }
 
-// A workgroup joins the parts of 32 rows: eight threads take every eighth part
-// of a row, then one of them joins the eight.  Fixed order, so a row's loss
-// does not depend on the others.
+// A workgroup joins the parts of 16 rows: sixteen threads take every sixteenth
+// part of a row, four at a time, with a running largest and sum; then one of
+// them joins the sixteen.  Fixed order, so a row's loss does not depend on the
+// others.
 __global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict__ top, const float* __restrict__ total,
                                                         int64_t parts, const float* __restrict__ hit,
                                                         const int64_t* __restrict__ target, int64_t n,
                                                         int64_t classes, int64_t ignore, float* __restrict__ loss,
                                                         float* __restrict__ lse) {
-    __shared__ float tops[8][32], sums[8][32];
-    const int c = threadIdx.x & 31, p0 = threadIdx.x >> 5;
-    const int64_t i = (int64_t)blockIdx.x * 32 + c;
+    constexpr int kRows = 16, kSlices = 16, kAtOnce = 4;
+    __shared__ float tops[kSlices][kRows], sums[kSlices][kRows];
+    const int c = threadIdx.x % kRows, p0 = threadIdx.x / kRows;
+    const int64_t i = (int64_t)blockIdx.x * kRows + c;
     const float none = -__builtin_huge_valf();
     float mx = none, sum = 0.0f;
     if (i < n) {
-        for (int64_t p = p0; p < parts; p += 8) mx = fmaxf(mx, top[p * n + i]);
-        const float base = mx == none ? 0.0f : mx;
-        for (int64_t p = p0; p < parts; p += 8) sum += total[p * n + i] * exp_fast(top[p * n + i] - base);
+        for (int64_t p = p0; p < parts; p += kSlices * kAtOnce) {
+            float t[kAtOnce], s[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int64_t at = p + u * kSlices;
+                t[u] = at < parts ? top[at * n + i] : none;
+                s[u] = at < parts ? total[at * n + i] : 0.0f;
+            }
+            float most = mx;
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) most = fmaxf(most, t[u]);
+            const float base = most == none ? 0.0f : most;
+            sum *= exp_fast(mx - base);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) sum += s[u] * exp_fast(t[u] - base);
+            mx = most;
+        }
     }
     tops[p0][c] = mx;
     sums[p0][c] = sum;
     __syncthreads();
     if (p0 != 0 || i >= n) return;
 #pragma unroll
-    for (int p = 1; p < 8; ++p) mx = fmaxf(mx, tops[p][c]);
+    for (int p = 1; p < kSlices; ++p) mx = fmaxf(mx, tops[p][c]);
     const float base = mx == none ? 0.0f : mx;
     sum = 0.0f;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) sum += sums[p][c] * exp_fast(tops[p][c] - base);
+    for (int p = 0; p < kSlices; ++p) sum += sums[p][c] * exp_fast(tops[p][c] - base);
     const float l = base + logf(sum);
     lse[i] = l;
     const int64_t t = target[i];
@@ -61,7 +77,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict_
 hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
                             const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
                             hipStream_t s) {
-    xent_join_kernel<<<dim3((unsigned)((n + 31) / 32)), 256, 0, s>>>(top, total, parts, hit, target, n, classes,
+    xent_join_kernel<<<dim3((unsigned)((n + 15) / 16)), 256, 0, s>>>(top, total, parts, hit, target, n, classes,
                                                                     ignore, loss, lse);
     return hipGetLastError();
 }

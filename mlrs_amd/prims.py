@@ -36,6 +36,7 @@ it takes float32, float16 and bfloat16 tensors:
 | ``adamw_state_values``   | the values that an 8-bit state stands for                  |
 """
 import ctypes
+import struct
 
 import torch
 
@@ -58,7 +59,9 @@ def _ptr(t):
 
 
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the raw handle of torch.cuda.current_stream(dev), without the objects
+    # around it (a microsecond of a small call)
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _metric_id(metric):
@@ -76,10 +79,15 @@ def _dev_check(*ts):
             raise ValueError("mlrs_amd prims take device tensors (got a %s tensor)" % t.device)
         if not t.is_contiguous():
             raise ValueError("mlrs_amd prims take contiguous row-major tensors")
-    if any(t.device != ts[0].device for t in ts[1:]):
-        raise ValueError("mlrs_amd prims take operands on one device (got %s)" % sorted({str(t.device) for t in ts}))
+    if not ts:
+        return
+    index = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != index:
+            raise ValueError("mlrs_amd prims take operands on one device (got %s)"
+                             % sorted({str(t.device) for t in ts}))
     # the library works on the current HIP device
-    if ts and ts[0].device.index != torch.cuda.current_device():
+    if index != torch.cuda.current_device():
         raise ValueError("operands are on %s but the current device is cuda:%d (use torch.cuda.device(...))"
                          % (ts[0].device, torch.cuda.current_device()))
 
@@ -436,6 +444,10 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 STATE_BLOCK = 256  # elements of a tensor that share a scale of an 8-bit state
 _TRAIN_DT = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
 _TRAIN_ID = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+# mlrs_grad_tensor and mlrs_adamw_tensor
+_GRAD_ITEM = struct.Struct("@Qqi4x")
+_ADAMW_ITEM = struct.Struct("@7Qqdii")
+assert _GRAD_ITEM.size == ctypes.sizeof(_lib.GradTensor) and _ADAMW_ITEM.size == ctypes.sizeof(_lib.AdamwTensor)
 
 
 def _train_suffix(t):
@@ -452,15 +464,19 @@ def _activation_id(name):
         raise ValueError("unknown activation %r (expected one of %s)" % (name, sorted(ACTIVATIONS)))
 
 
-def _layer_operands(a, w, a_name, **others):
+def _layer_operands(a, w, a_name, *others):
     """The checks a layer and a loss share: device, contiguity, one element
-    type, two dimensions.  The C ABI checks the sizes."""
-    given = [t for t in others.values() if t is not None]
+    type, two dimensions.  The C ABI checks the sizes.  `others`: (tensor or
+    None, name) pairs."""
+    given = [t for t, _ in others if t is not None]
     _dev_check(a, w, *given)
     s = _train_suffix(a)
-    for name, t in dict(w=w, **others).items():
-        if t is not None and t.dtype != a.dtype:
-            raise TypeError("%s and %s dtypes differ (%s, %s)" % (a_name, name, a.dtype, t.dtype))
+    dtype = a.dtype
+    if w.dtype != dtype:
+        raise TypeError("%s and w dtypes differ (%s, %s)" % (a_name, dtype, w.dtype))
+    for t, name in others:
+        if t is not None and t.dtype != dtype:
+            raise TypeError("%s and %s dtypes differ (%s, %s)" % (a_name, name, dtype, t.dtype))
     if a.dim() != 2 or w.dim() != 2:
         raise ValueError("%s and w must have two dimensions, got %s and %s"
                          % (a_name, tuple(a.shape), tuple(w.shape)))
@@ -482,7 +498,7 @@ def linear(x, w, bias=None, activation="none", residual=None, keep_preact=False,
     "gelu" (the erf form), "gelu_tanh" or "silu".  Returns ``y`` (n, d_out), or
     ``(y, z)`` with ``keep_preact``: z = x w^T + bias, what ``linear_grad``
     takes.  ``out`` receives y (it may be ``residual`` itself)."""
-    s = _layer_operands(x, w, "x", bias=bias, residual=residual)
+    s = _layer_operands(x, w, "x", (bias, "bias"), (residual, "residual"))
     act = _activation_id(activation)
     n, d_in = x.shape
     d_out = w.shape[0]
@@ -508,7 +524,7 @@ def linear_grad(dy, x, w, preact=None, activation="none", bias=True, need_dx=Tru
     two products; ``dbias`` sums it unrounded."""
     act = _activation_id(activation)
     z = preact if act else None
-    s = _layer_operands(x, w, "x", dy=dy, preact=z)
+    s = _layer_operands(x, w, "x", (dy, "dy"), (z, "preact"))
     if act and z is None:
         raise ValueError("activation %r needs preact, the z that linear kept" % (activation,))
     n, d_in = x.shape
@@ -537,7 +553,7 @@ def softmax_xent(h, w, target, bias=None, ignore_index=-100):
     out) share one dtype; ``target`` (n,) is int64.  ``lse`` is the logarithm of
     the sum of exponentials, ``loss = lse - z[target]``, 0 where the target is
     ``ignore_index`` and NaN where it is no class."""
-    s = _layer_operands(h, w, "h", bias=bias)
+    s = _layer_operands(h, w, "h", (bias, "bias"))
     _dev_check(h, target)
     n, d = h.shape
     _check_rows(target, "target", torch.int64, n)
@@ -557,7 +573,7 @@ def softmax_xent_grad(h, w, target, lse, grad, bias=None, ignore_index=-100, nee
     ``lse`` is what ``softmax_xent`` returned for the same operands, ``grad``
     float32 (n,) the gradient of each row's loss (1 / n for their mean).  The
     logits are computed again, a piece of the vocabulary at a time."""
-    s = _layer_operands(h, w, "h", bias=bias)
+    s = _layer_operands(h, w, "h", (bias, "bias"))
     _dev_check(h, target, lse, grad)
     n, d = h.shape
     _check_rows(target, "target", torch.int64, n)
@@ -593,13 +609,16 @@ def clip_scale(grads, max_norm):
     if not grads:
         raise ValueError("clip_scale needs at least one gradient")
     _dev_check(*grads)
-    items = (_lib.GradTensor * len(grads))()
-    for it, g in zip(items, grads):
+    items = bytearray(_GRAD_ITEM.size * len(grads))
+    at = 0
+    for g in grads:
         _train_suffix(g)
-        it.grad, it.len, it.dtype = g.data_ptr(), g.numel(), _TRAIN_ID[g.dtype]
+        _GRAD_ITEM.pack_into(items, at, g.data_ptr(), g.numel(), _TRAIN_ID[g.dtype])
+        at += _GRAD_ITEM.size
+    table = (_lib.GradTensor * len(grads)).from_buffer(items)
     norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
     scale = torch.empty_like(norm)
-    _lib.check(_lib.load().mlrs_grad_clip_scale(items, len(grads), float(max_norm), _ptr(norm), _ptr(scale),
+    _lib.check(_lib.load().mlrs_grad_clip_scale(table, len(grads), float(max_norm), _ptr(norm), _ptr(scale),
                                                 _stream(norm.device)))
     return norm, scale
 
@@ -642,36 +661,41 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
             raise ValueError("weight_decay must hold a number for each of the %d parameters, got %d"
                              % (count, len(decays)))
     dev = params[0].device
-    _dev_check(*params, *grads, *exp_avg, *exp_avg_sq, *(masters or []), *(avg_scales or []),
-               *(avg_sq_scales or []))
+    _dev_check(*params, *grads, *exp_avg, *exp_avg_sq, *(masters or ()), *(avg_scales or ()), *(avg_sq_scales or ()))
     if scale is not None:
         _check_out(scale, "scale", (torch.float32,), 1, dev)
-    items = (_lib.AdamwTensor * count)()
-    for i, (it, p, g, m, v) in enumerate(zip(items, params, grads, exp_avg, exp_avg_sq)):
-        _train_suffix(p)
-        _train_suffix(g)
-        n = p.numel()
+    items = bytearray(_ADAMW_ITEM.size * count)
+    put, at = _ADAMW_ITEM.pack_into, 0
+    ids = _TRAIN_ID
+    master = avg_scale = sq_scale = 0
+    for i in range(count):
+        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
+        n, pd, gd = p.numel(), p.dtype, g.dtype
+        if pd not in ids or gd not in ids:
+            _train_suffix(p)
+            _train_suffix(g)
         if g.numel() != n or m.numel() != n or v.numel() != n:
             raise ValueError("parameter %d has %d elements, its gradient %d, its moments %d and %d"
                              % (i, n, g.numel(), m.numel(), v.numel()))
         if m.dtype != state or v.dtype != state:
             raise TypeError("the moments must all be %s, got %s and %s" % (state, m.dtype, v.dtype))
-        it.param, it.grad, it.exp_avg, it.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
-        it.len, it.weight_decay = n, decays[i]
-        it.param_dtype, it.grad_dtype = _TRAIN_ID[p.dtype], _TRAIN_ID[g.dtype]
         if masters is not None:
-            if p.dtype == torch.float32:
+            if pd == torch.float32:
                 raise ValueError("masters go with float16 or bfloat16 parameters")
             _check_out(masters[i], "masters[%d]" % i, (torch.float32,), n, dev)
-            it.master = masters[i].data_ptr()
-        elif p.dtype != torch.float32:
-            raise ValueError("%s parameters need float32 masters" % p.dtype)
+            master = masters[i].data_ptr()
+        elif pd != torch.float32:
+            raise ValueError("%s parameters need float32 masters" % pd)
         if bits == 8:
             blocks = -(-n // STATE_BLOCK)
             _check_out(avg_scales[i], "avg_scales[%d]" % i, (torch.float32,), blocks, dev)
             _check_out(avg_sq_scales[i], "avg_sq_scales[%d]" % i, (torch.float32,), blocks, dev)
-            it.avg_scale, it.avg_sq_scale = avg_scales[i].data_ptr(), avg_sq_scales[i].data_ptr()
-    _lib.check(_lib.load().mlrs_adamw_step(items, count, bits, float(lr), float(betas[0]), float(betas[1]),
+            avg_scale, sq_scale = avg_scales[i].data_ptr(), avg_sq_scales[i].data_ptr()
+        put(items, at, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), master, avg_scale, sq_scale, n,
+            decays[i], ids[pd], ids[gd])
+        at += _ADAMW_ITEM.size
+    table = (_lib.AdamwTensor * count).from_buffer(items)
+    _lib.check(_lib.load().mlrs_adamw_step(table, count, bits, float(lr), float(betas[0]), float(betas[1]),
                                            float(eps), int(step), _ptr(scale), int(seed) & 0xFFFFFFFF,
                                            _stream(dev)))
 
