@@ -368,39 +368,110 @@ struct LogitGradEpi {
     int32_t first;    // the piece's first class
     int32_t classes;  // of the whole vocabulary
 
+    // A lane's accumulators belong to one row of the batch for each block of
+    // columns, so the row's target, lse and gradient are three registers; the
+    // result is turned through LDS in its own type, and leaves in 16-byte pieces.
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
+        constexpr int kEach = 16 / (int)sizeof(T);             // elements of a piece
+        constexpr int kRow = MB * 32 * (int)sizeof(T);         // bytes of a row
+        constexpr int kPieces = kRow / 16;
+        constexpr int kStep = 64 / kPieces;                    // rows that the lanes cover together
+        constexpr int kSwap = kPieces < 16 ? kPieces - 1 : 15;  // piece c of row n lies at c ^ (n & kSwap)
+        const int h = p.lane >> 5, r = p.lane & 31;
         const float scale = up ? *up : 1.0f;
-        f32x4 bv = {};
-        const int32_t mine = p.m0 + 4 * (p.lane % (MB * 8));
-        if (bias && mine < p.m) bv = load4(bias, mine, p.m, false);
-        for_rows(acc, p, lds, (int32_t)ld, [&](int32_t n, int32_t m, f32x4 (&v)[row_group<MB>()]) {
-            constexpr int kStep = row_step<MB>(), kGroup = row_group<MB>();
-            int64_t t[kGroup];
-            float g[kGroup], l[kGroup];
+        float l[NB], by[NB];
+        int32_t hot[NB];    // the target's place among the wave's classes
+        uint32_t keep[NB];  // all ones, or none in an ignored row
 #pragma unroll
-            for (int u = 0; u < kGroup; ++u) {
-                const int32_t at = n + u * kStep < p.n ? n + u * kStep : n;
-                t[u] = target[at];
-                g[u] = grad[at];
-                l[u] = lse[at];
-            }
+        for (int j = 0; j < NB; ++j) {
+            const int32_t n = p.n0 + j * 32 + r;
+            const int32_t at = n < p.n ? n : p.n - 1;
+            const int64_t t = target[at];
+            const bool valid = t >= 0 && t < classes;
+            l[j] = sizeof(T) == 2 ? lse[at] * kLog2E : lse[at];
+            keep[j] = t != ignore ? 0xFFFFFFFFu : 0u;
+            by[j] = valid ? grad[at] * scale : __builtin_nanf("");
+            hot[j] = valid ? (int32_t)t - first - p.m0 : -1;
+        }
+        if (bias) {
 #pragma unroll
-            for (int u = 0; u < kGroup; ++u) {
-                if (n + u * kStep >= p.n) break;
-                const bool kept = t[u] != ignore;
-                const float by = t[u] < 0 || t[u] >= classes ? __builtin_nanf("") : g[u] * scale;
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = exp_fast(v[u][e] + bv[e] - l[u]);
-                    if (t[u] == first + m + e) x -= 1.0f;
-                    // the columns up to ld, a multiple of 16 bytes, are read by
-                    // the products and must be zero
-                    v[u][e] = kept && m + e < p.m ? x * by : 0.0f;
+                for (int q = 0; q < 4; ++q) {
+                    const int32_t m = p.m0 + i * 32 + 8 * q + 4 * h;
+                    const f32x4 bv = m < p.m ? load4(bias, m, p.m, false) : f32x4{};
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += bv[e];
                 }
-                store4(out + (int64_t)(n + u * kStep) * ld, m, ld, true, v[u]);
+        }
+        // Three vector operations and an exponential for an element where no
+        // lane holds its row's target and the wave's classes are whole (the
+        // rest of a piece): vector work is what this epilogue costs.  16-bit
+        // types fold the subtraction into the multiplication by log2(e), which
+        // costs |lse| 2^-24 of a probability that is then rounded to 2^-8 or 2^-11.
+        auto element = [&](int i, int j, int q, int e) {
+            const float z = acc[i][j][4 * q + e];
+            return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2E, -l[j])) : exp_fast(z - l[j]);
+        };
+        auto mask = [&](typename Elem<T>::Vec4 v, uint32_t by_row) {
+            typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+            Words w = __builtin_bit_cast(Words, v);
+            w &= by_row;
+            return __builtin_bit_cast(typename Elem<T>::Vec4, w);
+        };
+        char* mine = lds + p.wave * 32 * kRow;
+        __syncthreads();  // the panels in LDS are no longer read
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            auto place = [&](int i, int q) {
+                const int at = (i * 32 + 8 * q + 4 * h) * (int)sizeof(T);
+                return reinterpret_cast<typename Elem<T>::Vec4*>(mine + r * kRow +
+                                                                 (((at >> 4) ^ (r & kSwap)) << 4) + (at & 15));
+            };
+            const bool odd = p.m0 + MB * 32 > p.m || __any(hot[j] >= 0 && hot[j] < MB * 32);
+            if (!odd) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        typename Elem<T>::Vec4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = (T)(element(i, j, q, e) * by[j]);
+                        *place(i, q) = mask(v, keep[j]);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int32_t m = i * 32 + 8 * q + 4 * h;  // of the wave's classes
+                        typename Elem<T>::Vec4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = element(i, j, q, e) - (hot[j] == m + e ? 1.0f : 0.0f);
+                            // the columns up to ld, a multiple of 16 bytes, are
+                            // read by the products and must be zero
+                            v[e] = (T)(p.m0 + m + e < p.m ? x * by[j] : 0.0f);
+                        }
+                        *place(i, q) = mask(v, keep[j]);
+                    }
             }
-        });
+            // the wave's LDS accesses are in order; nothing else touches `mine`
+            __builtin_amdgcn_wave_barrier();
+            const int c = p.lane % kPieces;
+#pragma unroll
+            for (int t = 0; t < 32; t += kStep) {
+                const int row = t + p.lane / kPieces;
+                const typename Elem<T>::Frag v = *reinterpret_cast<const typename Elem<T>::Frag*>(
+                    mine + row * kRow + ((c ^ (row & kSwap)) << 4));
+                const int32_t n = p.n0 + j * 32 + row, m = p.m0 + kEach * c;
+                if (n < p.n && m < ld) *reinterpret_cast<typename Elem<T>::Frag*>(out + (int64_t)n * ld + m) = v;
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 };
 
