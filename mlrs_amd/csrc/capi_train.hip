@@ -57,9 +57,7 @@ struct Op {
     void plan(Scratch& sc) {
         if (!in_place()) packed = sc.take<T>((size_t)(rows * padded<T>(cols)));
     }
-    hipError_t pack(hipStream_t s) const {
-        return in_place() ? hipSuccess : launch_pack<T>(src, rows, cols, packed, padded<T>(cols), s);
-    }
+    PackJob job() const { return PackJob{src, packed, in_place() ? 0 : rows, cols, padded<T>(cols)}; }
     Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, padded<T>(cols)}; }
 };
 
@@ -131,8 +129,7 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
                 sc.used = 0;
             }
         }
-        MLRS_TRY(xo.pack(s));
-        MLRS_TRY(wo.pack(s));
+        MLRS_TRY(launch_pack<T>(xo.job(), wo.job(), s));
         capi::Timed timed(s, "linear");
         MLRS_TRY(launch_linear<T>(xo.mat(), wo.mat(), n, m, k, o, cut, part, s));
         return MLRS_OK;
@@ -193,17 +190,18 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         }
         if (make_dz || db)
             MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, padded<T>(m),
-                                        db ? sums : nullptr, parts, s));
-        if (db) MLRS_TRY(launch_sum_parts<T>(sums, parts, m, nullptr, db, s));
+                                        ColumnSums<T>{db, sums, parts, nullptr}, s));
         const Mat dzm = make_dz ? Mat{dz, padded<T>(m)} : Mat{dy, m};
+        PackJob xj = xo.job(), wj = wo.job();
+        if (!dw) xj.rows = 0;
+        if (!dx) wj.rows = 0;
+        MLRS_TRY(launch_pack<T>(xj, wj, s));
         capi::Timed timed(s, "linear_grad");
         if (dx && n > 0) {
-            MLRS_TRY(wo.pack(s));
             const StoreTo o{dx, k, nullptr, nullptr, 0, nullptr};
             MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, o, cx, part, s));
         }
         if (dw) {
-            MLRS_TRY(xo.pack(s));
             const StoreTo o{dw, k, nullptr, nullptr, 0, nullptr};
             MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, o, cw, part, s));
         }
@@ -256,8 +254,7 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
                 sc.used = 0;
             }
         }
-        MLRS_TRY(ho.pack(s));
-        MLRS_TRY(wo.pack(s));
+        MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), s));
         capi::Timed timed(s, "softmax_xent");
         MLRS_TRY(launch_xent_stats<T>(ho.mat(), wo.mat(), bias, target, n, v, d, tile, top, total, hit, s));
         MLRS_TRY(launch_xent_join(top, total, parts, hit, target, n, v, ignore, loss, lse, s));
@@ -292,7 +289,8 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 MLRS_TRY(launch_product<T>(Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, false, d, v, 0, o,
                                            Cut{2, 1, 0}, nullptr, s));
             }
-            if (db) MLRS_TRY(launch_sum_parts<T>(nullptr, 0, v, nullptr, db, s));
+            if (db)
+                MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
             return MLRS_OK;
         }
         // classes of a piece: a multiple of 256, at least one tile
@@ -323,8 +321,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 sc.used = 0;
             }
         }
-        MLRS_TRY(ho.pack(s));
-        MLRS_TRY(wo.pack(s));
+        MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), s));
         if (scaled) MLRS_TRY(launch_grad_scale(grad, target, n, ignore, up, s));
         const float* down = scaled ? up + 1 : nullptr;
         const Mat hm = ho.mat(), wm = wo.mat();
@@ -336,8 +333,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                                           choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile, s));
             const Mat dzm{dz, ld};
             if (db) {
-                MLRS_TRY(launch_column_sums<T>(dzm, n, vp, sums, parts, s));
-                MLRS_TRY(launch_sum_parts<T>(sums, parts, vp, down, db + v0, s));
+                MLRS_TRY(launch_column_sums<T>(dzm, n, vp, ColumnSums<T>{db + v0, sums, parts, down}, s));
             }
             if (dw) {
                 const StoreTo o{dw + v0 * d, d, nullptr, nullptr, 0, down};

@@ -97,14 +97,20 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
 }
 
 // Four consecutive elements of a row from m on, those at or past `end` left
-// out.  `wide`: the row's start and m are aligned for one access.
+// out.  `width`: how many of them one access may hold, 4, 2 or 1, by the
+// alignment of the rows (m is a multiple of 4).
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, bool wide) {
+__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, int width) {
+    typedef typename Elem<T>::Vec4 Vec4;
+    typedef T Vec2 __attribute__((ext_vector_type(2)));
     f32x4 v;
-    if (wide && m + 4 <= end) {
-        const typename Elem<T>::Vec4 t = *reinterpret_cast<const typename Elem<T>::Vec4*>(row + m);
+    if (width == 4 && m + 4 <= end) {
+        const Vec4 t = *reinterpret_cast<const Vec4*>(row + m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+    } else if (width == 2 && m + 4 <= end) {
+        const Vec2 lo = *reinterpret_cast<const Vec2*>(row + m), hi = *reinterpret_cast<const Vec2*>(row + m + 2);
+        v = f32x4{(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]};
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = m + e < end ? (float)row[m + e] : 0.0f;
@@ -113,12 +119,17 @@ __device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, boo
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, bool wide, f32x4 v) {
-    if (wide && m + 4 <= end) {
-        typename Elem<T>::Vec4 t;
+__device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, int width, f32x4 v) {
+    typedef typename Elem<T>::Vec4 Vec4;
+    typedef T Vec2 __attribute__((ext_vector_type(2)));
+    if (width == 4 && m + 4 <= end) {
+        Vec4 t;
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = (T)v[e];
-        *reinterpret_cast<typename Elem<T>::Vec4*>(row + m) = t;
+        *reinterpret_cast<Vec4*>(row + m) = t;
+    } else if (width == 2 && m + 4 <= end) {
+        *reinterpret_cast<Vec2*>(row + m) = Vec2{(T)v[0], (T)v[1]};
+        *reinterpret_cast<Vec2*>(row + m + 2) = Vec2{(T)v[2], (T)v[3]};
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -189,7 +200,7 @@ struct LinearEpi {
     T* z;
     int64_t ld;  // of residual, y and z
     int32_t act;
-    bool wide;
+    int32_t width;  // of the rows' accesses
 
     // rows n, n + step, ... of them those before n_end
     template <int N>
@@ -199,23 +210,23 @@ struct LinearEpi {
         if (residual) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) res[u] = load4(residual + (n + u * step) * ld, m, end, wide);
+                if (n + u * step < n_end) res[u] = load4(residual + (n + u * step) * ld, m, end, width);
         }
 #pragma unroll
         for (int u = 0; u < N; ++u) v[u] += bv;
         if (z) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, wide, v[u]);
+                if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, width, v[u]);
         }
         activate_all(v, act);
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, wide, residual ? v[u] + res[u] : v[u]);
+            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, width, residual ? v[u] + res[u] : v[u]);
     }
     __device__ __forceinline__ f32x4 bias_at(int64_t m, int64_t end) const {
         f32x4 bv = {};
-        if (bias && m < end) bv = load4(bias, m, end, false);
+        if (bias && m < end) bv = load4(bias, m, end, 1);
         return bv;
     }
     template <int WM, int WN, int MB, int NB>
@@ -236,7 +247,7 @@ struct StoreEpi {
     const float* add;    // may be null
     const float* alpha;  // device scalar; may be null
     int64_t ld, part_ld, part_stride;
-    bool wide;
+    int32_t width;  // of the rows' accesses
 
     template <int N>
     __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, int split,
@@ -245,7 +256,7 @@ struct StoreEpi {
             f32x4 old[N] = {};
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, true);
+                if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, 4);
 #pragma unroll
             for (int u = 0; u < N; ++u) v[u] += old[u];
         }
@@ -253,12 +264,12 @@ struct StoreEpi {
             const float by = alpha ? *alpha : 1.0f;
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, wide, v[u] * by);
+                if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, width, v[u] * by);
         } else {
             float* to = part + split * part_stride;  // part_ld is a multiple of 4
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, true, v[u]);
+                if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, 4, v[u]);
         }
     }
     template <int WM, int WN, int MB, int NB>
@@ -290,7 +301,7 @@ struct StatsEpi {
             for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const f32x4 bv = load4(bias, p.m0 + i * 32 + 8 * q + 4 * h, p.m, false);
+                    const f32x4 bv = load4(bias, p.m0 + i * 32 + 8 * q + 4 * h, p.m, 1);
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -400,7 +411,7 @@ struct LogitGradEpi {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int32_t m = p.m0 + i * 32 + 8 * q + 4 * h;
-                    const f32x4 bv = m < p.m ? load4(bias, m, p.m, false) : f32x4{};
+                    const f32x4 bv = m < p.m ? load4(bias, m, p.m, 1) : f32x4{};
 #pragma unroll
                     for (int j = 0; j < NB; ++j)
 #pragma unroll

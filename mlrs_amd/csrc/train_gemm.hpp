@@ -282,6 +282,12 @@ __device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
     return x * per + (x < extra ? x : extra) + i;
 }
 
+// A number as a type: which of two sets of fragments.
+template <int V>
+struct Set {
+    static constexpr int v = V;
+};
+
 // Waits until at most N of the wave's copies are under way.
 template <int N>
 __device__ __forceinline__ void wait_copies() {
@@ -290,13 +296,15 @@ __device__ __forceinline__ void wait_copies() {
 }
 
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
-__global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 : 2))) void gemm_kernel(GemmArgs g,
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
                                                                                                        Epi epi) {
     constexpr int BM = WM * MB * 32, BN = WN * NB * 32, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
     constexpr int BK = stage_elems<T>();
     static_assert(kA == kB, "panels of either operand take the same slots");
-    constexpr int kSlots = 5;
+    constexpr bool kSmall = MB * NB == 1;
+    constexpr int kAhead = 3;  // staged widths under way, of a small tile
+    constexpr int kSlots = kSmall ? 2 * kAhead : 5;
     __shared__ __attribute__((aligned(1024))) char buf[kSlots * kA];
 
     const int lane = threadIdx.x & 63;
@@ -327,78 +335,133 @@ __global__ __launch_bounds__(WM* WN * 64, (WM * WN >= 8 ? 2 : (MB * NB <= 1 ? 4 
 
     f32x16 acc[MB][NB] = {};
 
-    // Panels A0 B0 A1 B1 ... go round five slots of LDS.  Fragments are read one
-    // step of sixteen (f32: eight) ahead of the matrix instructions that use
-    // them, across the staged widths too: the barrier that publishes width p + 1
-    // stands before the last step of width p, whose fragments are in registers by
-    // then.  After it nothing reads A_p and B_p any more; B_{p+2} and A_{p+3} are
-    // copied over them, a quarter of the copies in every step, so that neither
-    // the matrix nor the memory pipeline sees a burst.
-    typename Elem<T>::Frag fa[2][MB], fb[2][NB];
-    auto fetch = [&](const char* pa, const char* pb, int s, int set) {
+    if constexpr (kSmall) {
+        // A small tile has too little to multiply in a step to hide an LDS read
+        // behind: the fragments of a whole staged width are read while those of
+        // the one before are multiplied.  At the barrier of width p its fragments
+        // are in registers, width p + 1 is published, and width p + kAhead goes
+        // where p was.  4096 x 256 x 4096 in bf16: 33.1 us a step at a time with
+        // five slots, 20.2 so.
+        typename Elem<T>::Frag fa[2][4][MB], fb[2][4][NB];
+        constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
+        auto fetch = [&](const char* from, auto set) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fa[set][i] = ra.get(pa, s, i);
+            for (int s = 0; s < 4; ++s) {
 #pragma unroll
-        for (int j = 0; j < NB; ++j) fb[set][j] = rb.get(pb, s, j);
-    };
-    auto multiply = [&](int set) {
+                for (int i = 0; i < MB; ++i) fa[set.v][s][i] = ra.get(from, s, i);
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
+                for (int j = 0; j < NB; ++j) fb[set.v][s][j] = rb.get(from + kA, s, j);
+            }
+        };
+        int cur = 0;
+        auto next = [&](int at) { return at + 2 * kA >= kAhead * 2 * kA ? 0 : at + 2 * kA; };
+        auto width = [&](int32_t k0, auto set, auto other) {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+            wait_copies<(kAhead - 2) * (IA + IB)>();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            sa.template load<0, 1>(buf + cur, k0 + kAhead * BK, k_hi, wave);
+            sb.template load<0, 1>(buf + cur + kA, k0 + kAhead * BK, k_hi, wave);
+            cur = next(cur);
+            fetch(buf + cur, other);
 #pragma unroll
-            for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(fa[set][i], fb[set][j], acc[i][j]);
-    };
-    // one LDS read, one matrix instruction, in turn
-    auto interleave = [&]() {
-        constexpr int kReads = MB * (AKC ? 1 : sizeof(T) == 2 ? 2 : 4) + NB * (BKC ? 1 : sizeof(T) == 2 ? 2 : 4);
-        constexpr int kMath = MB * NB * (sizeof(T) == 4 ? 4 : 1);
-        constexpr int kPer = (kReads + kMath - 1) / kMath;
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int i = 0; i < kMath; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int i = 0; i < MB; ++i)
+                        acc[i][j] = mfma_step<T>(fa[set.v][s][i], fb[set.v][s][j], acc[i][j]);
+        };
+#pragma unroll
+        for (int p = 0; p < kAhead; ++p) {
+            sa.template load<0, 1>(buf + 2 * p * kA, k_lo + p * BK, k_hi, wave);
+            sb.template load<0, 1>(buf + (2 * p + 1) * kA, k_lo + p * BK, k_hi, wave);
         }
-    };
-    auto slot = [&](int at) { return buf + (at >= kSlots * kA ? at - kSlots * kA : at); };
-    constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
-
-    sa.template load<0, 1>(buf, k_lo, k_hi, wave);
-    sb.template load<0, 1>(buf + kA, k_lo, k_hi, wave);
-    sa.template load<0, 1>(buf + 2 * kA, k_lo + BK, k_hi, wave);
-    sb.template load<0, 2>(buf + 3 * kA, k_lo + BK, k_hi, wave);
-    wait_copies<IA + IB / 2>();
-    __builtin_amdgcn_s_barrier();
-    fetch(buf, buf + kA, 0, 0);
-    int cur = 0;  // of A_p
-    for (int32_t k0 = k_lo; k0 < k_hi; k0 += BK) {
-        const char *pa = buf + cur, *pb = slot(cur + kA);
-        __builtin_amdgcn_sched_barrier(0);
-        sb.template load<1, 2>(slot(cur + 3 * kA), k0 + BK, k_hi, wave);
-        fetch(pa, pb, 1, 1);
-        multiply(0);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        sa.template load<0, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
-        fetch(pa, pb, 2, 0);
-        multiply(1);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        sa.template load<1, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
-        fetch(pa, pb, 3, 1);
-        multiply(0);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the last fragments of p
-        wait_copies<IA>();
+        wait_copies<(kAhead - 1) * (IA + IB)>();
         __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        sb.template load<0, 2>(buf + cur, k0 + 2 * BK, k_hi, wave);
-        fetch(slot(cur + 2 * kA), slot(cur + 3 * kA), 0, 0);
-        multiply(1);
-        interleave();
-        cur = cur + 2 * kA >= kSlots * kA ? cur - (kSlots - 2) * kA : cur + 2 * kA;
+        fetch(buf, Set<0>{});
+        // an even number of widths: past the end come zeros
+        for (int32_t k0 = k_lo; k0 < k_hi; k0 += 2 * BK) {
+            width(k0, Set<0>{}, Set<1>{});
+            width(k0 + BK, Set<1>{}, Set<0>{});
+        }
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        wait_copies<0>();
+    } else {
+        // Panels A0 B0 A1 B1 ... go round five slots of LDS.  Fragments are read one
+        // step of sixteen (f32: eight) ahead of the matrix instructions that use
+        // them, across the staged widths too: the barrier that publishes width p + 1
+        // stands before the last step of width p, whose fragments are in registers by
+        // then.  After it nothing reads A_p and B_p any more; B_{p+2} and A_{p+3} are
+        // copied over them, a quarter of the copies in every step, so that neither
+        // the matrix nor the memory pipeline sees a burst.
+        typename Elem<T>::Frag fa[2][MB], fb[2][NB];
+        auto fetch = [&](const char* pa, const char* pb, int s, int set) {
+#pragma unroll
+            for (int i = 0; i < MB; ++i) fa[set][i] = ra.get(pa, s, i);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[set][j] = rb.get(pb, s, j);
+        };
+        auto multiply = [&](int set) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(fa[set][i], fb[set][j], acc[i][j]);
+        };
+        // one LDS read, one matrix instruction, in turn
+        auto interleave = [&]() {
+            constexpr int kReads = MB * (AKC ? 1 : sizeof(T) == 2 ? 2 : 4) + NB * (BKC ? 1 : sizeof(T) == 2 ? 2 : 4);
+            constexpr int kMath = MB * NB * (sizeof(T) == 4 ? 4 : 1);
+            constexpr int kPer = (kReads + kMath - 1) / kMath;
+#pragma unroll
+            for (int i = 0; i < kMath; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            }
+        };
+        auto slot = [&](int at) { return buf + (at >= kSlots * kA ? at - kSlots * kA : at); };
+        constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
+
+        sa.template load<0, 1>(buf, k_lo, k_hi, wave);
+        sb.template load<0, 1>(buf + kA, k_lo, k_hi, wave);
+        sa.template load<0, 1>(buf + 2 * kA, k_lo + BK, k_hi, wave);
+        sb.template load<0, 2>(buf + 3 * kA, k_lo + BK, k_hi, wave);
+        wait_copies<IA + IB / 2>();
+        __builtin_amdgcn_s_barrier();
+        fetch(buf, buf + kA, 0, 0);
+        int cur = 0;  // of A_p
+        for (int32_t k0 = k_lo; k0 < k_hi; k0 += BK) {
+            const char *pa = buf + cur, *pb = slot(cur + kA);
+            __builtin_amdgcn_sched_barrier(0);
+            sb.template load<1, 2>(slot(cur + 3 * kA), k0 + BK, k_hi, wave);
+            fetch(pa, pb, 1, 1);
+            multiply(0);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+            sa.template load<0, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
+            fetch(pa, pb, 2, 0);
+            multiply(1);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+            sa.template load<1, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
+            fetch(pa, pb, 3, 1);
+            multiply(0);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the last fragments of p
+            wait_copies<IA>();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            sb.template load<0, 2>(buf + cur, k0 + 2 * BK, k_hi, wave);
+            fetch(slot(cur + 2 * kA), slot(cur + 3 * kA), 0, 0);
+            multiply(1);
+            interleave();
+            cur = cur + 2 * kA >= kSlots * kA ? cur - (kSlots - 2) * kA : cur + 2 * kA;
+        }
+        // copies past the end of the contraction may still write their zeros
+        wait_copies<0>();
     }
-    // copies past the end of the contraction may still write their zeros
-    wait_copies<0>();
 
     Place p;
     p.m0 = m0 + wm * MB * 32;

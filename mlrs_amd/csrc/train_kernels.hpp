@@ -27,9 +27,15 @@ struct Cut {
 };
 Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
 
-// dst (rows x ld, ld >= cols) := src (rows x cols), zeros behind each row.
+// dst (rows x ld, ld >= cols) := src (rows x cols), zeros behind each row; no
+// rows: nothing to do.
+struct PackJob {
+    const void* src;
+    void* dst;
+    int64_t rows, cols, ld;
+};
 template <typename T>
-hipError_t launch_pack(const T* src, int64_t rows, int64_t cols, T* dst, int64_t ld, hipStream_t s);
+hipError_t launch_pack(const PackJob& a, const PackJob& b, hipStream_t s);
 
 // y (n x m) = act(x w^T + bias) + residual; z, where not null, x w^T + bias.
 struct LinearOut {
@@ -48,18 +54,24 @@ template <typename T>
 hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                              hipStream_t s);
 
-// dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and the
-// column sums of it in parts (sums may be null): parts x m floats.
+// Column sums: out (null: none wanted) := alpha * the sums, made in `parts` runs
+// of rows, parts x m floats of scratch.
+template <typename T>
+struct ColumnSums {
+    T* out;
+    float* sums;
+    int parts;
+    const float* alpha;  // device scalar; may be null
+};
 int column_parts(int64_t n, int64_t m, int cus);
+// dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and its
+// column sums.
 template <typename T>
-hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld, float* sums,
-                           int parts, hipStream_t s);
-// The column sums of a packed matrix, in parts.
+hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
+                           const ColumnSums<T>& to, hipStream_t s);
+// The column sums of a packed matrix.
 template <typename T>
-hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, float* sums, int parts, hipStream_t s);
-// out := alpha * (sum of the parts), in order.
-template <typename T>
-hipError_t launch_sum_parts(const float* sums, int parts, int64_t m, const float* alpha, T* out, hipStream_t s);
+hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& to, hipStream_t s);
 
 // Stores of a product P (m x n, element (i, j) at out[j * ld + i]): a (rows m)
 // with its row index contiguous, b (rows n) with k contiguous (b_k) or not.

@@ -41,10 +41,11 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
     return hipGetLastError();
 }
 
-// Whether rows `ld` elements apart from p on can be read four at a time.
+// How many elements of rows `ld` elements apart from p on an access may hold.
 template <typename T>
-inline bool wide_rows(const void* p, int64_t ld) {
-    return ((uintptr_t)p % (4 * sizeof(T))) == 0 && ld % 4 == 0;
+inline int row_width(const void* p, int64_t ld) {
+    if ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0) return 4;
+    return (uintptr_t)p % (2 * sizeof(T)) == 0 && ld % 2 == 0 ? 2 : 1;
 }
 
 }  // namespace train

@@ -19,10 +19,10 @@ namespace train {
 // 2048 x 1024 x 4096 in bf16: 32.1 us in 256 x 256 tiles, 24.8 in 128 x 128,
 // 33.8 in 64 x 64; at 16384 x 4096 x 4096: 433, 513, -.
 Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits) {
-    static const double stage16[3][4] = {{1.6}, {0.62, 0.98}, {0.45, 0.55, 0.8, 1.0}};
-    static const double stage32[3][4] = {{7.4}, {2.0, 4.0}, {0.7, 1.05, 1.55, 2.05}};
+    static const double stage16[3][3] = {{1.6}, {0.62, 0.98}, {0.27, 0.5, 0.75}};
+    static const double stage32[3][3] = {{7.4}, {2.0, 4.0}, {0.68, 1.05, 1.55}};
     static const double round_us[3] = {6.0, 4.5, 4.0};
-    static const int resident[3] = {1, 2, 4};
+    static const int resident[3] = {1, 2, 3};
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
     Cut best{0, 1, 0};
@@ -39,7 +39,7 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
             double cost = (double)rounds * ((double)each * stage[resident[t] - 1] + round_us[t]);
             if (rest) cost += (double)each * stage[rest - 1] + round_us[t];
             // joining the parts: a launch, and their bytes twice
-            if (sp > 1) cost += 5.0 + (double)sp * (double)m * (double)n * 8.0 / 4.5e6;
+            if (sp > 1) cost += 7.0 + (double)sp * (double)m * (double)n * 8.0 / 4.5e6;
             if (cost < best_cost) {
                 best_cost = cost;
                 best.tile = t;
@@ -54,27 +54,29 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
 // ---------------------------------------------------------------------------
 // packing
 // ---------------------------------------------------------------------------
+// Two matrices in a launch: both operands of a product are usually packed.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
-                                                   T* __restrict__ dst, int64_t ld) {
+__global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b) {
     constexpr int E = 16 / (int)sizeof(T);
-    const int64_t chunks = ld / E, total = rows * chunks;
+    const int64_t total_a = a.rows * (a.ld / E), total = total_a + b.rows * (b.ld / E);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / chunks, c = (i - r * chunks) * E;
-        const T* from = src + r * cols;
+        const PackJob& j = i < total_a ? a : b;
+        const int64_t at = i < total_a ? i : i - total_a;
+        const int64_t chunks = j.ld / E, r = at / chunks, c = (at - r * chunks) * E;
+        const T* from = (const T*)j.src + r * j.cols;
         typename Elem<T>::Frag v;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = c + e < cols ? from[c + e] : (T)0.0f;
-        *reinterpret_cast<typename Elem<T>::Frag*>(dst + r * ld + c) = v;
+        for (int e = 0; e < E; ++e) v[e] = c + e < j.cols ? from[c + e] : (T)0.0f;
+        *reinterpret_cast<typename Elem<T>::Frag*>((T*)j.dst + r * j.ld + c) = v;
     }
 }
 
 template <typename T>
-hipError_t launch_pack(const T* src, int64_t rows, int64_t cols, T* dst, int64_t ld, hipStream_t s) {
-    const int64_t total = rows * (ld / (16 / (int64_t)sizeof(T)));
+hipError_t launch_pack(const PackJob& a, const PackJob& b, hipStream_t s) {
+    const int64_t total = (a.rows * a.ld + b.rows * b.ld) / (16 / (int64_t)sizeof(T));
     if (total == 0) return hipSuccess;
     const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
-    pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, s>>>(src, rows, cols, dst, ld);
+    pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, s>>>(a, b);
     return hipGetLastError();
 }
 
@@ -126,7 +128,7 @@ static StoreEpi<T> parts_epi(float* part, int64_t m, int64_t n) {
     e.part = part;
     e.part_ld = (m + 3) & ~(int64_t)3;
     e.part_stride = n * e.part_ld;
-    e.wide = true;
+    e.width = 4;
     return e;
 }
 
@@ -142,7 +144,9 @@ static LinearEpi<T> linear_epi(const LinearOut& o, int64_t m) {
     e.z = (T*)o.z;
     e.ld = m;
     e.act = o.act;
-    e.wide = wide_rows<T>(o.y, m) && (!o.z || wide_rows<T>(o.z, m)) && (!o.residual || wide_rows<T>(o.residual, m));
+    e.width = row_width<T>(o.y, m);
+    if (o.z) e.width = std::min(e.width, row_width<T>(o.z, m));
+    if (o.residual) e.width = std::min(e.width, row_width<T>(o.residual, m));
     return e;
 }
 
@@ -261,40 +265,53 @@ hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64
 // ---------------------------------------------------------------------------
 // backwards
 // ---------------------------------------------------------------------------
-// A workgroup takes 256 columns (four per lane) and every parts-th run of
-// rows; its four waves take rows in turn and their sums are joined in order.
+// A workgroup takes 256 columns (four per lane) and a run of rows, at least 32
+// where there are as many; its four waves take rows in turn and their sums are
+// joined in order.  A single run is the column sum itself: it goes out at once.
 int column_parts(int64_t n, int64_t m, int cus) {
     const int64_t across = std::max<int64_t>(1, (m + 255) / 256);
     const int64_t want = std::max<int64_t>(1, (int64_t)cus * 8 / across);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 15) / 16));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 31) / 32));
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, int64_t dy_ld,
                                                        const T* __restrict__ z, int act, int64_t n, int64_t m,
                                                        T* __restrict__ dz, int64_t ld, float* __restrict__ sums,
-                                                       int64_t rows_per, bool wide) {
+                                                       T* __restrict__ out, const float* __restrict__ alpha,
+                                                       int64_t rows_per, int width) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per;
     const int64_t r1 = r0 + rows_per < n ? r0 + rows_per : n;
     f32x4 sum = {};
     if (c < (dz ? ld : m)) {
-        for (int64_t r = r0 + wave; r < r1; r += 4) {
-            f32x4 v = load4(dy + r * dy_ld, c, m, wide);
-            if (z) {
-                const f32x4 zz = load4(z + r * m, c, m, wide);
+        constexpr int kRows = 2;  // of a wave, under way at once
+        for (int64_t r = r0 + wave; r < r1; r += 4 * kRows) {
+            f32x4 v[kRows] = {}, zz[kRows] = {};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= activate_slope(zz[e], act);
+            for (int u = 0; u < kRows; ++u)
+                if (r + 4 * u < r1) v[u] = load4(dy + (r + 4 * u) * dy_ld, c, m, width);
+            if (z) {
+#pragma unroll
+                for (int u = 0; u < kRows; ++u)
+                    if (r + 4 * u < r1) zz[u] = load4(z + (r + 4 * u) * m, c, m, width);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e >= m) v[e] = 0.0f;
-            sum += v;
-            if (dz) store4(dz + r * ld, c, ld, true, v);
+            for (int u = 0; u < kRows; ++u) {
+                if (z) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[u][e] *= activate_slope(zz[u][e], act);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e >= m || r + 4 * u >= r1) v[u][e] = 0.0f;
+                sum += v[u];
+                if (dz && r + 4 * u < r1) store4(dz + (r + 4 * u) * ld, c, ld, 4, v[u]);
+            }
         }
     }
-    if (!sums) return;
+    if (!out) return;
     __shared__ f32x4 join[4][64];
     join[wave][lane] = sum;
     __syncthreads();
@@ -302,31 +319,11 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
         f32x4 v = join[0][lane];
 #pragma unroll
         for (int i = 1; i < 4; ++i) v += join[i][lane];
-        store4(sums + (int64_t)blockIdx.y * m, c, m, false, v);
+        if (gridDim.y == 1)
+            store4(out, c, m, 1, alpha ? v * *alpha : v);
+        else
+            store4(sums + (int64_t)blockIdx.y * m, c, m, 1, v);
     }
-}
-
-template <typename T>
-static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
-                           float* sums, int parts, hipStream_t s) {
-    const int64_t across = ((dz ? ld : m) + 255) / 256;
-    if (across == 0 || (n == 0 && !sums)) return hipSuccess;
-    const int64_t rows_per = (n + parts - 1) / parts;
-    const bool wide = wide_rows<T>(dy, dy_ld) && (!z || wide_rows<T>(z, m));
-    act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)parts), 256, 0, s>>>(dy, dy_ld, z, act, n, m, dz, ld, sums,
-                                                                             rows_per, wide);
-    return hipGetLastError();
-}
-
-template <typename T>
-hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld, float* sums,
-                           int parts, hipStream_t s) {
-    return act_grad<T>(dy, m, z, act, n, m, dz, ld, sums, parts, s);
-}
-
-template <typename T>
-hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, float* sums, int parts, hipStream_t s) {
-    return act_grad<T>((const T*)a.p, a.ld, nullptr, kActNone, n, m, nullptr, 0, sums, parts, s);
 }
 
 // A workgroup joins the parts of 16 columns: sixteen threads take every
@@ -350,10 +347,29 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
 }
 
 template <typename T>
-hipError_t launch_sum_parts(const float* sums, int parts, int64_t m, const float* alpha, T* out, hipStream_t s) {
-    if (m == 0) return hipSuccess;
-    sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(sums, parts, m, alpha, out);
+static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
+                           const ColumnSums<T>& to, hipStream_t s) {
+    const int64_t across = ((dz ? ld : m) + 255) / 256;
+    if (across == 0 || (n == 0 && !to.out)) return hipSuccess;
+    const int64_t rows_per = (n + to.parts - 1) / to.parts;
+    const int width = z ? std::min(row_width<T>(dy, dy_ld), row_width<T>(z, m)) : row_width<T>(dy, dy_ld);
+    act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)to.parts), 256, 0, s>>>(
+        dy, dy_ld, z, act, n, m, dz, ld, to.sums, to.out, to.alpha, rows_per, width);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !to.out || to.parts == 1) return e;
+    sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(to.sums, to.parts, m, to.alpha, to.out);
     return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
+                           const ColumnSums<T>& to, hipStream_t s) {
+    return act_grad<T>(dy, m, z, act, n, m, dz, ld, to, s);
+}
+
+template <typename T>
+hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& to, hipStream_t s) {
+    return act_grad<T>((const T*)a.p, a.ld, nullptr, kActNone, n, m, nullptr, 0, to, s);
 }
 
 template <typename T>
@@ -367,7 +383,7 @@ hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t 
     e.ld = o.ld;
     e.part_ld = o.acc_ld;
     e.part_stride = 0;
-    e.wide = o.out && wide_rows<T>(o.out, o.ld);
+    e.width = o.out ? row_width<T>(o.out, o.ld) : 4;
     if (cut.splits == 1)
         return b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, 1, 0, e, s)
                    : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, 1, 0, e, s);
@@ -379,15 +395,14 @@ hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t 
 }
 
 #define MLRS_INST(T)                                                                                               \
-    template hipError_t launch_pack<T>(const T*, int64_t, int64_t, T*, int64_t, hipStream_t);                      \
+    template hipError_t launch_pack<T>(const PackJob&, const PackJob&, hipStream_t);                               \
     template hipError_t launch_linear<T>(Mat, Mat, int64_t, int64_t, int64_t, const LinearOut&, const Cut&, float*, \
                                          hipStream_t);                                                             \
     template hipError_t launch_linear_few<T>(const T*, const T*, int64_t, int64_t, int64_t, const LinearOut&,      \
                                              hipStream_t);                                                         \
-    template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t, float*, int,    \
-                                           hipStream_t);                                                           \
-    template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, float*, int, hipStream_t);                    \
-    template hipError_t launch_sum_parts<T>(const float*, int, int64_t, const float*, T*, hipStream_t);            \
+    template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t,                 \
+                                           const ColumnSums<T>&, hipStream_t);                                     \
+    template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, const ColumnSums<T>&, hipStream_t);           \
     template hipError_t launch_product<T>(Mat, Mat, bool, int64_t, int64_t, int64_t, const StoreTo&, const Cut&,   \
                                           float*, hipStream_t);
 MLRS_INST(float)

@@ -36,6 +36,7 @@ it takes float32, float16 and bfloat16 tensors:
 | ``adamw_state_values``   | the values that an 8-bit state stands for                  |
 """
 import ctypes
+import itertools
 import struct
 
 import torch
@@ -589,14 +590,56 @@ def softmax_xent_grad(h, w, target, lse, grad, bias=None, ignore_index=-100, nee
     return dh, dw, db
 
 
+# Tensor attributes as functions, so that a list of hundreds of tensors is
+# checked by map() and not by as many lines of Python.
+_data_ptr, _numel, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_is_contiguous, _dtype_of = torch.Tensor.is_contiguous, torch.Tensor.dtype.__get__
+_TENSOR_TYPES = {torch.Tensor, torch.nn.Parameter}
+
+
 def _tensor_list(ts, name, count=None):
     ts = list(ts)
     if count is not None and len(ts) != count:
         raise ValueError("%s must hold a tensor for each of the %d parameters, got %d" % (name, count, len(ts)))
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError("%s must hold tensors, got %s" % (name, type(t).__name__))
+    if not set(map(type, ts)) <= _TENSOR_TYPES:
+        for t in ts:
+            if not isinstance(t, torch.Tensor):
+                raise TypeError("%s must hold tensors, got %s" % (name, type(t).__name__))
     return ts
+
+
+def _check_lists(*lists):
+    """_dev_check of every tensor of the lists."""
+    index = lists[0][0].get_device()
+    if index < 0 or index != torch.cuda.current_device() or any(
+            set(map(_get_device, ts)) != {index} or not all(map(_is_contiguous, ts)) for ts in lists):
+        _dev_check(*(t for ts in lists for t in ts))
+
+
+def _train_ids(ts):
+    """The element types of a list of tensors, as the C ABI numbers them."""
+    dtypes = list(map(_dtype_of, ts))
+    if not set(dtypes) <= _TRAIN_ID.keys():
+        _train_suffix(next(t for t in ts if t.dtype not in _TRAIN_ID))
+    return list(map(_TRAIN_ID.__getitem__, dtypes))
+
+
+def _table(item, fields, count):
+    """`count` packed structures of the columns in `fields`."""
+    return bytearray(struct.pack("@" + item.format[1:] * count, *itertools.chain.from_iterable(zip(*fields))))
+
+
+def _check_counts(counts, ts, name):
+    got = list(map(_numel, ts))
+    if got != counts:
+        i = next(i for i, (a, b) in enumerate(zip(got, counts)) if a != b)
+        raise ValueError("%s[%d] must hold %d elements, got %d" % (name, i, counts[i], got[i]))
+
+
+def _check_dtype(dtype, ts, name):
+    if set(map(_dtype_of, ts)) != {dtype}:
+        i = next(i for i, t in enumerate(ts) if t.dtype != dtype)
+        raise TypeError("%s[%d] must be %s, got %s" % (name, i, dtype, ts[i].dtype))
 
 
 def clip_scale(grads, max_norm):
@@ -608,17 +651,14 @@ def clip_scale(grads, max_norm):
     grads = _tensor_list(grads, "grads")
     if not grads:
         raise ValueError("clip_scale needs at least one gradient")
-    _dev_check(*grads)
-    items = bytearray(_GRAD_ITEM.size * len(grads))
-    at = 0
-    for g in grads:
-        _train_suffix(g)
-        _GRAD_ITEM.pack_into(items, at, g.data_ptr(), g.numel(), _TRAIN_ID[g.dtype])
-        at += _GRAD_ITEM.size
-    table = (_lib.GradTensor * len(grads)).from_buffer(items)
+    _check_lists(grads)
+    ids = _train_ids(grads)
+    count = len(grads)
+    table = (_lib.GradTensor * count).from_buffer(
+        _table(_GRAD_ITEM, (map(_data_ptr, grads), map(_numel, grads), ids), count))
     norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
     scale = torch.empty_like(norm)
-    _lib.check(_lib.load().mlrs_grad_clip_scale(table, len(grads), float(max_norm), _ptr(norm), _ptr(scale),
+    _lib.check(_lib.load().mlrs_grad_clip_scale(table, count, float(max_norm), _ptr(norm), _ptr(scale),
                                                 _stream(norm.device)))
     return norm, scale
 
@@ -645,56 +685,52 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999),
     if count == 0:
         return
     bits = 8 if exp_avg[0].dtype == torch.uint8 else 32
-    state = torch.uint8 if bits == 8 else torch.float32
+    lists = [params, grads, exp_avg, exp_avg_sq]
+    if masters is not None:
+        lists.append(masters)
     if bits == 8:
         if avg_scales is None or avg_sq_scales is None:
             raise ValueError("8-bit states need avg_scales and avg_sq_scales")
         avg_scales = _tensor_list(avg_scales, "avg_scales", count)
         avg_sq_scales = _tensor_list(avg_sq_scales, "avg_sq_scales", count)
+        lists += [avg_scales, avg_sq_scales]
     elif avg_scales is not None or avg_sq_scales is not None:
         raise ValueError("avg_scales and avg_sq_scales go with uint8 states")
     if isinstance(weight_decay, (int, float)):
         decays = [float(weight_decay)] * count
     else:
-        decays = [float(d) for d in weight_decay]
+        decays = list(map(float, weight_decay))
         if len(decays) != count:
             raise ValueError("weight_decay must hold a number for each of the %d parameters, got %d"
                              % (count, len(decays)))
+    _check_lists(*lists)
     dev = params[0].device
-    _dev_check(*params, *grads, *exp_avg, *exp_avg_sq, *(masters or ()), *(avg_scales or ()), *(avg_sq_scales or ()))
     if scale is not None:
         _check_out(scale, "scale", (torch.float32,), 1, dev)
-    items = bytearray(_ADAMW_ITEM.size * count)
-    put, at = _ADAMW_ITEM.pack_into, 0
-    ids = _TRAIN_ID
-    master = avg_scale = sq_scale = 0
-    for i in range(count):
-        p, g, m, v = params[i], grads[i], exp_avg[i], exp_avg_sq[i]
-        n, pd, gd = p.numel(), p.dtype, g.dtype
-        if pd not in ids or gd not in ids:
-            _train_suffix(p)
-            _train_suffix(g)
-        if g.numel() != n or m.numel() != n or v.numel() != n:
-            raise ValueError("parameter %d has %d elements, its gradient %d, its moments %d and %d"
-                             % (i, n, g.numel(), m.numel(), v.numel()))
-        if m.dtype != state or v.dtype != state:
-            raise TypeError("the moments must all be %s, got %s and %s" % (state, m.dtype, v.dtype))
-        if masters is not None:
-            if pd == torch.float32:
-                raise ValueError("masters go with float16 or bfloat16 parameters")
-            _check_out(masters[i], "masters[%d]" % i, (torch.float32,), n, dev)
-            master = masters[i].data_ptr()
-        elif pd != torch.float32:
-            raise ValueError("%s parameters need float32 masters" % pd)
-        if bits == 8:
-            blocks = -(-n // STATE_BLOCK)
-            _check_out(avg_scales[i], "avg_scales[%d]" % i, (torch.float32,), blocks, dev)
-            _check_out(avg_sq_scales[i], "avg_sq_scales[%d]" % i, (torch.float32,), blocks, dev)
-            avg_scale, sq_scale = avg_scales[i].data_ptr(), avg_sq_scales[i].data_ptr()
-        put(items, at, p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), master, avg_scale, sq_scale, n,
-            decays[i], ids[pd], ids[gd])
-        at += _ADAMW_ITEM.size
-    table = (_lib.AdamwTensor * count).from_buffer(items)
+    param_ids, grad_ids = _train_ids(params), _train_ids(grads)
+    counts = list(map(_numel, params))
+    _check_counts(counts, grads, "grads")
+    state = torch.uint8 if bits == 8 else torch.float32
+    for name, ts in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):
+        _check_dtype(state, ts, name)
+        _check_counts(counts, ts, name)
+    nothing = [0] * count
+    if masters is not None:
+        if 0 in param_ids:
+            raise ValueError("masters go with float16 or bfloat16 parameters")
+        _check_dtype(torch.float32, masters, "masters")
+        _check_counts(counts, masters, "masters")
+    elif any(param_ids):
+        raise ValueError("float16 and bfloat16 parameters need float32 masters")
+    if bits == 8:
+        blocks = [-(-n // STATE_BLOCK) for n in counts]
+        for name, ts in (("avg_scales", avg_scales), ("avg_sq_scales", avg_sq_scales)):
+            _check_dtype(torch.float32, ts, name)
+            _check_counts(blocks, ts, name)
+    pointers = [map(_data_ptr, ts) if ts is not None else nothing for ts in
+                (params, grads, exp_avg, exp_avg_sq, masters, avg_scales, avg_sq_scales)]
+    table = (_lib.AdamwTensor * count).from_buffer(
+        _table(_ADAMW_ITEM, (*pointers, counts, decays, param_ids, grad_ids), count))
     _lib.check(_lib.load().mlrs_adamw_step(table, count, bits, float(lr), float(betas[0]), float(betas[1]),
                                            float(eps), int(step), _ptr(scale), int(seed) & 0xFFFFFFFF,
                                            _stream(dev)))
