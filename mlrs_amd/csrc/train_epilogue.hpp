@@ -141,38 +141,42 @@ __device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, int width
 // consecutive m of row n + u * step (which may be past the last row), the lanes
 // along the row, so that a row leaves in whole lines; a lane's m is the same in
 // every call.  Groups, so that what f loads for them is under way at once.  The
-// accumulators (a lane holds four m of one n, lanes run along n) are turned
-// through the wave's own part of LDS, 32 rows at a time; a row's 16-byte chunks
-// are kept at c ^ (n & 7).
+// accumulators (a lane holds four m of one n, sixteen lanes run along n) are
+// turned through the wave's own part of LDS, 32 rows at a time.
 template <int MB>
 constexpr int row_step() {
-    return 64 / (MB * 8);  // rows that the lanes cover together
+    return 64 / (MB * 4);  // rows that the lanes cover together
 }
 template <int MB>
 constexpr int row_group() {
-    return MB == 1 ? 4 : 8;
+    return MB == 2 ? 4 : 8;
+}
+// Rows of BYTES bytes in LDS: piece c (16 bytes) of row r lies at c ^ this, and
+// sixteen rows read or written at one c touch all banks.
+template <int BYTES>
+__device__ __forceinline__ int turn_swizzle(int r) {
+    return BYTES >= 256 ? r & 15 : BYTES == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 template <int MB, int NB, typename F>
-__device__ __forceinline__ void for_rows(const f32x16 (&acc)[MB][NB], const Place& p, char* lds, int32_t m_end,
+__device__ __forceinline__ void for_rows(const f32x4 (&acc)[MB][NB], const Place& p, char* lds, int32_t m_end,
                                          F f) {
-    constexpr int kRow = MB * 128;      // bytes
-    constexpr int kLanes = MB * 8;      // of a row
+    constexpr int kRow = MB * 64;       // bytes
+    constexpr int kLanes = MB * 4;      // of a row
     constexpr int kStep = row_step<MB>(), kGroup = row_group<MB>();
     char* mine = lds + p.wave * 32 * kRow;
-    const int h = p.lane >> 5, r = p.lane & 31;
+    const int g = p.lane >> 4, r = p.lane & 15;
     const int c = p.lane % kLanes;
     const int32_t m = p.m0 + 4 * c;
     __syncthreads();  // the panels in LDS are no longer read
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
+    for (int j = 0; j < NB; j += 2) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
+        for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-                *reinterpret_cast<f32x4*>(mine + r * kRow + (((8 * i + 2 * q + h) ^ (r & 7)) << 4)) = v;
+            for (int i = 0; i < MB; ++i) {
+                const int row = 16 * jj + r;
+                *reinterpret_cast<f32x4*>(mine + row * kRow + (((4 * i + g) ^ turn_swizzle<kRow>(row)) << 4)) =
+                    acc[i][j + jj];
             }
         // the wave's LDS accesses are in order; nothing else touches `mine`
         __builtin_amdgcn_wave_barrier();
@@ -182,9 +186,9 @@ __device__ __forceinline__ void for_rows(const f32x16 (&acc)[MB][NB], const Plac
 #pragma unroll
             for (int u = 0; u < kGroup; ++u) {
                 const int row = t + u * kStep + p.lane / kLanes;
-                v[u] = *reinterpret_cast<const f32x4*>(mine + row * kRow + ((c ^ (row & 7)) << 4));
+                v[u] = *reinterpret_cast<const f32x4*>(mine + row * kRow + ((c ^ turn_swizzle<kRow>(row)) << 4));
             }
-            const int32_t n = p.n0 + j * 32 + t + p.lane / kLanes;
+            const int32_t n = p.n0 + j * 16 + t + p.lane / kLanes;
             if (n < p.n && m < m_end) f(n, m, v);
         }
         __builtin_amdgcn_wave_barrier();
@@ -230,8 +234,8 @@ struct LinearEpi {
         return bv;
     }
     template <int WM, int WN, int MB, int NB>
-    __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
-        const f32x4 bv = bias_at(p.m0 + 4 * (p.lane % (MB * 8)), p.m);
+    __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char* lds) const {
+        const f32x4 bv = bias_at(p.m0 + 4 * (p.lane % (MB * 4)), p.m);
         for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[row_group<MB>()]) {
             rows(n, row_step<MB>(), p.n, m, p.m, bv, v);
         });
@@ -273,12 +277,25 @@ struct StoreEpi {
         }
     }
     template <int WM, int WN, int MB, int NB>
-    __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
+    __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char* lds) const {
         for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[row_group<MB>()]) {
             rows(n, row_step<MB>(), p.n, m, p.m, p.split, v);
         });
     }
 };
+
+// acc += bias, along m.
+template <typename T, int MB, int NB>
+__device__ __forceinline__ void add_bias(f32x4 (&acc)[MB][NB], const T* bias, const Place& p) {
+    if (!bias) return;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int32_t m = p.m0 + i * 16 + 4 * (p.lane >> 4);
+        const f32x4 bv = m < p.m ? load4(bias, m, p.m, 1) : f32x4{};
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] += bv;
+    }
+}
 
 // The statistics of a tile of logits z = P + bias (rows: classes, columns:
 // rows of the batch): the largest and the sum of e^(z - largest) over the
@@ -293,39 +310,29 @@ struct StatsEpi {
     float* hit;      // n
 
     template <int WM, int WN, int MB, int NB>
-    __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char*) const {
-        const int h = p.lane >> 5, r = p.lane & 31;
+    __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char*) const {
+        const int g = p.lane >> 4, r = p.lane & 15;
         const int64_t at = ((int64_t)p.tile_m * WM + p.wm) * p.n;
-        if (bias) {
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 bv = load4(bias, p.m0 + i * 32 + 8 * q + 4 * h, p.m, 1);
-#pragma unroll
-                    for (int j = 0; j < NB; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += bv[e];
-                }
-        }
+        add_bias(acc, bias, p);
         const float none = -__builtin_huge_valf();
-        if (p.m0 + MB * 32 > p.m) {  // classes past the end
+        if (p.m0 + MB * 16 > p.m) {  // classes past the end
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q)
-                    if (p.m0 + i * 32 + 8 * (q >> 2) + 4 * h + (q & 3) >= p.m)
+                for (int e = 0; e < 4; ++e)
+                    if (p.m0 + i * 16 + 4 * g + e >= p.m)
 #pragma unroll
-                        for (int j = 0; j < NB; ++j) acc[i][j][q] = none;
+                        for (int j = 0; j < NB; ++j) acc[i][j][e] = none;
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int32_t n = p.n0 + j * 32 + r;
+            const int32_t n = p.n0 + j * 16 + r;
             float mx = none;
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) mx = fmaxf(mx, acc[i][j][q]);
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[i][j][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             // the sum is relative to a finite value where there is one to be
             // had: a NaN logit reaches it, and +inf - +inf is NaN
@@ -334,26 +341,25 @@ struct StatsEpi {
 #pragma unroll
             for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) sum += exp_fast(acc[i][j][q] - base);
+                for (int e = 0; e < 4; ++e) sum += exp_fast(acc[i][j][e] - base);
+            sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (n < p.n) {
-                if (h == 0) {
+                if (g == 0) {
                     top[at + n] = mx;
                     total[at + n] = sum;
                 }
                 const int64_t t = target[n] - p.m0;
-                if (t >= 0 && t < MB * 32 && t < p.m - p.m0) {
-                    float v = 0.0f;
-                    bool found = false;
+                if (t >= 0 && t < MB * 16 && t < p.m - p.m0) {
+                    const int32_t place = (int32_t)t;
+                    if (((place >> 2) & 3) == g) {  // this lane has it
+                        float v = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < MB; ++i)
+                        for (int i = 0; i < MB; ++i)
 #pragma unroll
-                        for (int q = 0; q < 16; ++q)
-                            if (t == i * 32 + 8 * (q >> 2) + 4 * h + (q & 3)) {
-                                v = acc[i][j][q];
-                                found = true;
-                            }
-                    if (found) hit[n] = v;
+                            for (int e = 0; e < 4; ++e) v = place == i * 16 + 4 * g + e ? acc[i][j][e] : v;
+                        hit[n] = v;
+                    }
                 }
             }
         }
@@ -383,20 +389,19 @@ struct LogitGradEpi {
     // columns, so the row's target, lse and gradient are three registers; the
     // result is turned through LDS in its own type, and leaves in 16-byte pieces.
     template <int WM, int WN, int MB, int NB>
-    __device__ __forceinline__ void run(f32x16 (&acc)[MB][NB], const Place& p, char* lds) const {
-        constexpr int kEach = 16 / (int)sizeof(T);             // elements of a piece
-        constexpr int kRow = MB * 32 * (int)sizeof(T);         // bytes of a row
+    __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char* lds) const {
+        constexpr int kEach = 16 / (int)sizeof(T);      // elements of a piece
+        constexpr int kRow = MB * 16 * (int)sizeof(T);  // bytes of a row
         constexpr int kPieces = kRow / 16;
-        constexpr int kStep = 64 / kPieces;                    // rows that the lanes cover together
-        constexpr int kSwap = kPieces < 16 ? kPieces - 1 : 15;  // piece c of row n lies at c ^ (n & kSwap)
-        const int h = p.lane >> 5, r = p.lane & 31;
+        constexpr int kStep = 64 / kPieces;             // rows that the lanes cover together
+        const int g = p.lane >> 4, r = p.lane & 15;
         const float scale = up ? *up : 1.0f;
         float l[NB], by[NB];
         int32_t hot[NB];    // the target's place among the wave's classes
         uint32_t keep[NB];  // all ones, or none in an ignored row
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int32_t n = p.n0 + j * 32 + r;
+            const int32_t n = p.n0 + j * 16 + r;
             const int32_t at = n < p.n ? n : p.n - 1;
             const int64_t t = target[at];
             const bool valid = t >= 0 && t < classes;
@@ -405,26 +410,14 @@ struct LogitGradEpi {
             by[j] = valid ? grad[at] * scale : __builtin_nanf("");
             hot[j] = valid ? (int32_t)t - first - p.m0 : -1;
         }
-        if (bias) {
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int32_t m = p.m0 + i * 32 + 8 * q + 4 * h;
-                    const f32x4 bv = m < p.m ? load4(bias, m, p.m, 1) : f32x4{};
-#pragma unroll
-                    for (int j = 0; j < NB; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += bv[e];
-                }
-        }
+        add_bias(acc, bias, p);
         // Three vector operations and an exponential for an element where no
         // lane holds its row's target and the wave's classes are whole (the
         // rest of a piece): vector work is what this epilogue costs.  16-bit
         // types fold the subtraction into the multiplication by log2(e), which
         // costs |lse| 2^-24 of a probability that is then rounded to 2^-8 or 2^-11.
-        auto element = [&](int i, int j, int q, int e) {
-            const float z = acc[i][j][4 * q + e];
+        auto element = [&](int i, int j, int e) {
+            const float z = acc[i][j][e];
             return sizeof(T) == 2 ? __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2E, -l[j])) : exp_fast(z - l[j]);
         };
         auto mask = [&](typename Elem<T>::Vec4 v, uint32_t by_row) {
@@ -436,39 +429,39 @@ struct LogitGradEpi {
         char* mine = lds + p.wave * 32 * kRow;
         __syncthreads();  // the panels in LDS are no longer read
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            auto place = [&](int i, int q) {
-                const int at = (i * 32 + 8 * q + 4 * h) * (int)sizeof(T);
-                return reinterpret_cast<typename Elem<T>::Vec4*>(mine + r * kRow +
-                                                                 (((at >> 4) ^ (r & kSwap)) << 4) + (at & 15));
+        for (int j0 = 0; j0 < NB; j0 += 2) {
+            auto place = [&](int i, int jj) {
+                const int row = 16 * jj + r, at = (i * 16 + 4 * g) * (int)sizeof(T);
+                return reinterpret_cast<typename Elem<T>::Vec4*>(
+                    mine + row * kRow + (((at >> 4) ^ turn_swizzle<kRow>(row)) << 4) + (at & 15));
             };
-            const bool odd = p.m0 + MB * 32 > p.m || __any(hot[j] >= 0 && hot[j] < MB * 32);
-            if (!odd) {
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
+            for (int jj = 0; jj < 2; ++jj) {
+                const int j = j0 + jj;
+                const bool odd = p.m0 + MB * 16 > p.m || __any(hot[j] >= 0 && hot[j] < MB * 16);
+                if (!odd) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int i = 0; i < MB; ++i) {
                         typename Elem<T>::Vec4 v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = (T)(element(i, j, q, e) * by[j]);
-                        *place(i, q) = mask(v, keep[j]);
+                        for (int e = 0; e < 4; ++e) v[e] = (T)(element(i, j, e) * by[j]);
+                        *place(i, jj) = mask(v, keep[j]);
                     }
-            } else {
+                } else {
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int32_t m = i * 32 + 8 * q + 4 * h;  // of the wave's classes
+                    for (int i = 0; i < MB; ++i) {
+                        const int32_t m = i * 16 + 4 * g;  // of the wave's classes
                         typename Elem<T>::Vec4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float x = element(i, j, q, e) - (hot[j] == m + e ? 1.0f : 0.0f);
+                            const float x = element(i, j, e) - (hot[j] == m + e ? 1.0f : 0.0f);
                             // the columns up to ld, a multiple of 16 bytes, are
                             // read by the products and must be zero
                             v[e] = (T)(p.m0 + m + e < p.m ? x * by[j] : 0.0f);
                         }
-                        *place(i, q) = mask(v, keep[j]);
+                        *place(i, jj) = mask(v, keep[j]);
                     }
+                }
             }
             // the wave's LDS accesses are in order; nothing else touches `mine`
             __builtin_amdgcn_wave_barrier();
@@ -477,8 +470,8 @@ struct LogitGradEpi {
             for (int t = 0; t < 32; t += kStep) {
                 const int row = t + p.lane / kPieces;
                 const typename Elem<T>::Frag v = *reinterpret_cast<const typename Elem<T>::Frag*>(
-                    mine + row * kRow + ((c ^ (row & kSwap)) << 4));
-                const int32_t n = p.n0 + j * 32 + row, m = p.m0 + kEach * c;
+                    mine + row * kRow + ((c ^ turn_swizzle<kRow>(row)) << 4));
+                const int32_t n = p.n0 + j0 * 16 + row, m = p.m0 + kEach * c;
                 if (n < p.n && m < ld) *reinterpret_cast<typename Elem<T>::Frag*>(out + (int64_t)n * ld + m) = v;
             }
             __builtin_amdgcn_wave_barrier();

@@ -9,21 +9,23 @@
 // are 16-byte aligned and ld is a multiple of 16 bytes; the host packs what is
 // not.
 //
-// Tile.  A workgroup computes BM x BN of P, its waves a WM x WN grid of
-// 32 x 32 blocks (v_mfma_f32_32x32x16 for 16-bit types, four
-// v_mfma_f32_32x32x2 for f32).  A is the operand whose index runs along the
-// output's rows in memory: a lane then holds four consecutive elements of one
-// output row.  128 bytes of the contraction axis are staged at a time,
-// straight from HBM into one of two LDS buffers, the other one being read
-// meanwhile; out-of-range elements come back as zeros from the buffer
-// descriptor's bounds check.
+// Tile.  A workgroup computes BM x BN of P, its waves a WM x WN grid of parts
+// of MB x NB blocks of 16 x 16 (v_mfma_f32_16x16x32 for 16-bit types, four
+// v_mfma_f32_16x16x4 for f32).  A large product is bound by the chip's power,
+// and register-only chains of the 16 x 16 instruction reach 2,080 TFLOP/s where
+// those of 32 x 32 x 16 reach 1,830.  A is the operand whose index runs along
+// the output's rows in memory: a lane then holds four consecutive elements of
+// one output row.  128 bytes of the contraction axis are staged at a time,
+// straight from HBM into a ring of LDS slots; out-of-range elements come back as
+// zeros from the buffer descriptor's bounds check.
 //
 // LDS layout.  K operand: a row's 128 bytes as eight 16-byte chunks, chunk c
 // kept at c ^ ((row >> 1) & 7), so that sixteen rows read at one c (a pass of
 // a 16-byte read: 64 banks) touch all banks.  R
 // operand: the tile's elements of one k back to back, their 16-byte chunks
-// kept at c ^ r_swizzle(k): the four k of a transposing read (16-bit types)
-// and the two halves of a wave (f32) then lie in different banks.  The swizzle
+// kept at c ^ r_swizzle(k): the eight k of half a wave's transposing read
+// (16-bit types) and the four of a wave's read (f32) then lie in different
+// banks.  The swizzle
 // is applied to the global address of each lane, as the copy into LDS is
 // linear.
 #pragma once
@@ -37,7 +39,6 @@ namespace mlrs {
 namespace train {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -94,17 +95,15 @@ __host__ __device__ constexpr int stage_elems() {
 #endif
 
 template <typename T>
-__device__ __forceinline__ f32x16 mfma_step(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x16 c) {
+__device__ __forceinline__ f32x4 mfma_step(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x4 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
     if constexpr (sizeof(T) == 4) {
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[0], b[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[1], b[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[2], b[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[3], b[3], c, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
     } else if constexpr (__is_same(T, _Float16)) {
-        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     } else {
-        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
 #else
     (void)a;
@@ -119,8 +118,8 @@ __device__ __forceinline__ int k_swizzle(int row) { return (row >> 1) & 7; }
 // R layout: what the chunk index of step k is exclusive-ored with.
 template <typename T, int ROWS>
 __device__ __forceinline__ int r_swizzle(int k) {
-    if (sizeof(T) == 4) return (k & 4) << 1;
-    return ROWS * 2 >= 256 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+    if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+    return (ROWS * 2 >= 256 ? (k & 3) << 2 : ((k >> 1) & 1) << 2) ^ (((k >> 3) & 1) << 1);
 }
 
 // 16 bytes per lane from a buffer straight into LDS, lane i's at lds + 16 i; lds
@@ -209,31 +208,32 @@ struct Stager {
     }
 };
 
-// One operand's fragments out of LDS: BLOCKS blocks of 32 rows from row
-// `first`; step s of the four in a staged width.
+// One operand's fragments out of LDS: BLOCKS blocks of 16 rows from row
+// `first`; step s of the two in a staged width.  Lane l holds sixteen bytes of
+// row l % 16 along k, the (l / 16)-th of the step.
 template <typename T, bool KC, int ROWS, int BLOCKS>
 struct Reader {
-    int at[KC ? 4 : BLOCKS];
+    int at[KC ? 2 : BLOCKS];
 
     __device__ __forceinline__ void init(int first, int lane) {
-        const int h = lane >> 5, r = lane & 31;
+        const int g = lane >> 4, r = lane & 15;
         if constexpr (KC) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = (first + r) * kStageBytes + (((2 * s + h) ^ k_swizzle(r)) << 4);
+            for (int s = 0; s < 2; ++s) at[s] = (first + r) * kStageBytes + (((4 * s + g) ^ k_swizzle(r)) << 4);
         } else if constexpr (sizeof(T) == 2) {
             // lane 4 q + p of sixteen addresses four elements of step q of
             // four; the transposing read hands lane i column i of them
-            const int q = (lane & 15) >> 2, p = lane & 3, side = (lane >> 4) & 1;
+            const int q = r >> 2, p = lane & 3;
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
-                const int c = ((first >> 5) + b) * 4 + side * 2 + (p >> 1);
-                at[b] = (8 * h + q) * (ROWS * 2) + ((c ^ r_swizzle<T, ROWS>(q)) << 4) + (p & 1) * 8;
+                const int c = ((first >> 4) + b) * 2 + (p >> 1);
+                at[b] = (8 * g + q) * (ROWS * 2) + ((c ^ r_swizzle<T, ROWS>(8 * g + q)) << 4) + (p & 1) * 8;
             }
         } else {
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
-                const int c = ((first >> 5) + b) * 8 + (r >> 2);
-                at[b] = 4 * h * (ROWS * 4) + ((c ^ r_swizzle<T, ROWS>(4 * h)) << 4) + (r & 3) * 4;
+                const int c = ((first >> 4) + b) * 4 + (r >> 2);
+                at[b] = 4 * g * (ROWS * 4) + ((c ^ r_swizzle<T, ROWS>(4 * g)) << 4) + (r & 3) * 4;
             }
         }
     }
@@ -242,14 +242,15 @@ struct Reader {
         typedef typename Elem<T>::Frag Frag;
 #if defined(__HIP_DEVICE_COMPILE__)
         if constexpr (KC) {
-            return *reinterpret_cast<const Frag*>(lds + at[s] + b * 32 * kStageBytes);
+            return *reinterpret_cast<const Frag*>(lds + at[s] + b * 16 * kStageBytes);
         } else if constexpr (sizeof(T) == 2) {
-            const char* q = lds + at[b] + s * 16 * (ROWS * 2);
+            // the swizzle of k + 4 and of k + 32 is that of k
+            const char* q = lds + at[b] + s * 32 * (ROWS * 2);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLRS_LDS s16x4*)q);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLRS_LDS s16x4*)(q + 4 * (ROWS * 2)));
             return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const char* q = lds + at[b] + s * 8 * (ROWS * 4);
+            const char* q = lds + at[b] + s * 16 * (ROWS * 4);
             Frag f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const float*>(q + i * (ROWS * 4));
@@ -298,11 +299,11 @@ __device__ __forceinline__ void wait_copies() {
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
                                                                                                        Epi epi) {
-    constexpr int BM = WM * MB * 32, BN = WN * NB * 32, WAVES = WM * WN;
+    constexpr int BM = WM * MB * 16, BN = WN * NB * 16, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
     constexpr int BK = stage_elems<T>();
     static_assert(kA == kB, "panels of either operand take the same slots");
-    constexpr bool kSmall = MB * NB == 1;
+    constexpr bool kSmall = MB * NB == 4;
     constexpr int kAhead = 3;  // staged widths under way, of a small tile
     constexpr int kSlots = kSmall ? 2 * kAhead : 5;
     __shared__ __attribute__((aligned(1024))) char buf[kSlots * kA];
@@ -330,10 +331,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
     sb.init(g.b, n0, g.n, k_hi, wave, lane);
     Reader<T, AKC, BM, MB> ra;
     Reader<T, BKC, BN, NB> rb;
-    ra.init(wm * MB * 32, lane);
-    rb.init(wn * NB * 32, lane);
+    ra.init(wm * MB * 16, lane);
+    rb.init(wn * NB * 16, lane);
 
-    f32x16 acc[MB][NB] = {};
+    f32x4 acc[MB][NB] = {};
 
     if constexpr (kSmall) {
         // A small tile has too little to multiply in a step to hide an LDS read
@@ -342,11 +343,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
         // are in registers, width p + 1 is published, and width p + kAhead goes
         // where p was.  4096 x 256 x 4096 in bf16: 33.1 us a step at a time with
         // five slots, 20.2 so.
-        typename Elem<T>::Frag fa[2][4][MB], fb[2][4][NB];
+        typename Elem<T>::Frag fa[2][2][MB], fb[2][2][NB];
         constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
         auto fetch = [&](const char* from, auto set) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < 2; ++s) {
 #pragma unroll
                 for (int i = 0; i < MB; ++i) fa[set.v][s][i] = ra.get(from, s, i);
 #pragma unroll
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
             cur = next(cur);
             fetch(buf + cur, other);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -389,38 +390,48 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
         __builtin_amdgcn_s_waitcnt(0xC07F);
         wait_copies<0>();
     } else {
-        // Panels A0 B0 A1 B1 ... go round five slots of LDS.  Fragments are read one
-        // step of sixteen (f32: eight) ahead of the matrix instructions that use
-        // them, across the staged widths too: the barrier that publishes width p + 1
-        // stands before the last step of width p, whose fragments are in registers by
-        // then.  After it nothing reads A_p and B_p any more; B_{p+2} and A_{p+3} are
-        // copied over them, a quarter of the copies in every step, so that neither
-        // the matrix nor the memory pipeline sees a burst.
-        typename Elem<T>::Frag fa[2][MB], fb[2][NB];
-        auto fetch = [&](const char* pa, const char* pb, int s, int set) {
+        // Panels A0 B0 A1 B1 ... go round five slots of LDS.  A staged width is
+        // multiplied in four parts, the lower and the upper half of the wave's rows
+        // in each of its two steps, and fragments are read a part ahead, across the
+        // widths too: the barrier that publishes width p + 1 stands before the last
+        // part of width p, whose fragments are in registers by then.  After it
+        // nothing reads A_p and B_p any more; B_{p+2} and A_{p+3} are copied over
+        // them, a quarter of the copies in every part, so that neither the matrix
+        // nor the memory pipeline sees a burst.
+        constexpr int HB = MB / 2;
+        typename Elem<T>::Frag fa[2][HB], fb[2][NB];
+        auto fetch_a = [&](const char* from, int s, int half) {
 #pragma unroll
-            for (int i = 0; i < MB; ++i) fa[set][i] = ra.get(pa, s, i);
-#pragma unroll
-            for (int j = 0; j < NB; ++j) fb[set][j] = rb.get(pb, s, j);
+            for (int i = 0; i < HB; ++i) fa[half][i] = ra.get(from, s, half * HB + i);
         };
-        auto multiply = [&](int set) {
+        auto fetch_b = [&](const char* from, int s) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) fb[s][j] = rb.get(from, s, j);
+        };
+        auto multiply = [&](int half, int s) {
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
-                for (int i = 0; i < MB; ++i) acc[i][j] = mfma_step<T>(fa[set][i], fb[set][j], acc[i][j]);
+                for (int i = 0; i < HB; ++i)
+                    acc[half * HB + i][j] = mfma_step<T>(fa[half][i], fb[s][j], acc[half * HB + i][j]);
         };
-        // one LDS read, one matrix instruction, in turn
-        auto interleave = [&]() {
-            constexpr int kReads = MB * (AKC ? 1 : sizeof(T) == 2 ? 2 : 4) + NB * (BKC ? 1 : sizeof(T) == 2 ? 2 : 4);
-            constexpr int kMath = MB * NB * (sizeof(T) == 4 ? 4 : 1);
-            constexpr int kPer = (kReads + kMath - 1) / kMath;
+        // LDS reads and matrix instructions in turn
+        auto interleave = [&](auto with_b) {
+            constexpr int kA1 = AKC ? 1 : sizeof(T) == 2 ? 2 : 4, kB1 = BKC ? 1 : sizeof(T) == 2 ? 2 : 4;
+            constexpr int kReads = HB * kA1 + (decltype(with_b)::v ? NB * kB1 : 0);
+            constexpr int kMath = HB * NB * (sizeof(T) == 4 ? 4 : 1);
+            constexpr int kPer = (kReads + kMath - 1) / kMath, kEvery = kMath / kReads > 1 ? kMath / kReads : 1;
 #pragma unroll
-            for (int i = 0; i < kMath; ++i) {
+            for (int i = 0; i < kMath / kEvery; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, kEvery, 0);
             }
         };
-        auto slot = [&](int at) { return buf + (at >= kSlots * kA ? at - kSlots * kA : at); };
+        // `ahead` slots past the one at `at`
+        auto slot = [&](int at, int ahead) {
+            const int to = at + ahead * kA;
+            return buf + (to >= kSlots * kA ? to - kSlots * kA : to);
+        };
         constexpr int IA = decltype(sa)::kInstr, IB = decltype(sb)::kInstr;
 
         sa.template load<0, 1>(buf, k_lo, k_hi, wave);
@@ -429,34 +440,37 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
         sb.template load<0, 2>(buf + 3 * kA, k_lo + BK, k_hi, wave);
         wait_copies<IA + IB / 2>();
         __builtin_amdgcn_s_barrier();
-        fetch(buf, buf + kA, 0, 0);
+        fetch_a(buf, 0, 0);
+        fetch_b(buf + kA, 0);
         int cur = 0;  // of A_p
         for (int32_t k0 = k_lo; k0 < k_hi; k0 += BK) {
-            const char *pa = buf + cur, *pb = slot(cur + kA);
+            const char *pa = buf + cur, *pb = slot(cur, 1);
             __builtin_amdgcn_sched_barrier(0);
-            sb.template load<1, 2>(slot(cur + 3 * kA), k0 + BK, k_hi, wave);
-            fetch(pa, pb, 1, 1);
-            multiply(0);
-            interleave();
+            sb.template load<1, 2>(slot(cur, 3), k0 + BK, k_hi, wave);
+            fetch_a(pa, 0, 1);
+            multiply(0, 0);
+            interleave(Set<0>{});
             __builtin_amdgcn_sched_barrier(0);
-            sa.template load<0, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
-            fetch(pa, pb, 2, 0);
-            multiply(1);
-            interleave();
+            sa.template load<0, 2>(slot(cur, 4), k0 + 2 * BK, k_hi, wave);
+            fetch_a(pa, 1, 0);
+            fetch_b(pb, 1);
+            multiply(1, 0);
+            interleave(Set<1>{});
             __builtin_amdgcn_sched_barrier(0);
-            sa.template load<1, 2>(slot(cur + 4 * kA), k0 + 2 * BK, k_hi, wave);
-            fetch(pa, pb, 3, 1);
-            multiply(0);
-            interleave();
+            sa.template load<1, 2>(slot(cur, 4), k0 + 2 * BK, k_hi, wave);
+            fetch_a(pa, 1, 1);
+            multiply(0, 1);
+            interleave(Set<0>{});
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the last fragments of p
             wait_copies<IA>();
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             sb.template load<0, 2>(buf + cur, k0 + 2 * BK, k_hi, wave);
-            fetch(slot(cur + 2 * kA), slot(cur + 3 * kA), 0, 0);
-            multiply(1);
-            interleave();
+            fetch_a(slot(cur, 2), 0, 0);
+            fetch_b(slot(cur, 3), 0);
+            multiply(1, 1);
+            interleave(Set<1>{});
             cur = cur + 2 * kA >= kSlots * kA ? cur - (kSlots - 2) * kA : cur + 2 * kA;
         }
         // copies past the end of the contraction may still write their zeros
@@ -464,8 +478,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
     }
 
     Place p;
-    p.m0 = m0 + wm * MB * 32;
-    p.n0 = n0 + wn * NB * 32;
+    p.m0 = m0 + wm * MB * 16;
+    p.n0 = n0 + wn * NB * 16;
     p.m = g.m;
     p.n = g.n;
     p.split = split;

@@ -33,11 +33,11 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
     if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
     const dim3 grid((unsigned)blocks);
     if (tile == 0)
-        gemm_kernel<T, AKC, BKC, 2, 4, 4, 2, Epi><<<grid, 512, 0, s>>>(g, epi);
+        gemm_kernel<T, AKC, BKC, 2, 4, 8, 4, Epi><<<grid, 512, 0, s>>>(g, epi);
     else if (tile == 1)
-        gemm_kernel<T, AKC, BKC, 2, 2, 2, 2, Epi><<<grid, 256, 0, s>>>(g, epi);
+        gemm_kernel<T, AKC, BKC, 2, 2, 4, 4, Epi><<<grid, 256, 0, s>>>(g, epi);
     else
-        gemm_kernel<T, AKC, BKC, 2, 2, 1, 1, Epi><<<grid, 256, 0, s>>>(g, epi);
+        gemm_kernel<T, AKC, BKC, 2, 2, 2, 2, Epi><<<grid, 256, 0, s>>>(g, epi);
     return hipGetLastError();
 }
 

@@ -162,27 +162,9 @@ hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const Li
 }
 
 // A few rows: the weights are read once, straight into registers as the
-// fragments of v_mfma_f32_16x16x32 (f32: 16x16x4).  A workgroup computes
+// fragments of the matrix instructions.  A workgroup computes
 // sixteen outputs of every row; its waves take the contraction axis in turn
 // and their sums are joined in LDS, in the order of the waves.
-template <typename T>
-__device__ __forceinline__ f32x4 mfma16_step(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x4 c) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    } else if constexpr (__is_same(T, _Float16)) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    } else {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-#else
-    (void)a;
-    (void)b;
-#endif
-    return c;
-}
-
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ typename Elem<T>::Frag chunk_at(const T* row, int64_t c, int64_t k) {
     constexpr int E = 16 / (int)sizeof(T);
@@ -226,7 +208,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int u = 0; u < U; ++u) acc[b] = mfma16_step<T>(a[u], bx[b][u], acc[b]);
+            for (int u = 0; u < U; ++u) acc[b] = mfma_step<T>(a[u], bx[b][u], acc[b]);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) sums[wave][b][lane] = acc[b];
