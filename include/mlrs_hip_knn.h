@@ -546,8 +546,9 @@ int32_t mlrs_softmax_xent_bf16(const uint16_t *h, int64_t h_len, int64_t n, int6
  * The gradient of sum_i grad_i loss_i: with dz_iv = grad_i (e^(z_iv - lse_i) -
  * [v = target(i)]), zero in ignored rows, dh = dz w (n x d), dw = dz^T h
  * (classes x d) and dbias = the column sums of dz.  lse is mlrs_softmax_xent's
- * of the same operands; z is computed again, in pieces of the vocabulary whose
- * dz takes at most MLRS_XENT_PIECE_BYTES of workspace.  Any of dh, dw and dbias
+ * of the same operands; z is computed again, in pieces of the vocabulary (256
+ * classes at least) whose dz takes at most MLRS_XENT_PIECE_BYTES of workspace;
+ * of several pieces, dh is added up in f32.  Any of dh, dw and dbias
  * may be NULL (length 0).  16-bit types: dz is rounded to the type before the
  * products (f16: scaled by a power of two first, by the largest |grad|).
  * n = 0 gives dw = 0 and dbias = 0.

@@ -17,6 +17,8 @@ namespace {
 constexpr int64_t kMaxCount = 0x7FFFFFFF - 512;  // a tile past it must not overflow
 constexpr int64_t kMaxRowBytes = (int64_t)1 << 22;  // 256 rows of a tile within a buffer descriptor's 2^31
 
+constexpr int64_t kStatsBytes = (int64_t)256 << 20;  // of a loss's partial statistics
+
 int32_t null_error(const char* operand) {
     return capi::error(MLRS_ERR_NULL_POINTER, operand, 0, 0, 0, "null pointer");
 }
@@ -238,16 +240,18 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         rc = capi::cu_count(&cus);
         if (rc) return rc;
         const int tile = choose_cut((int)sizeof(T), v, n, d, cus, 1).tile;
+        // the statistics of as many rows at a time as their parts have room for
         const int64_t parts = stats_parts(tile, v);
+        const int64_t rows = std::min(n, std::max<int64_t>(256, kStatsBytes / (8 * parts) / 256 * 256));
         Op<T> ho(h, n, d), wo(w, v, d);
         float *top = nullptr, *total = nullptr, *hit = nullptr;
         Scratch sc;
         for (int pass = 0; pass < 2; ++pass) {
             ho.plan(sc);
             wo.plan(sc);
-            top = sc.take<float>((size_t)(parts * n));
-            total = sc.take<float>((size_t)(parts * n));
-            hit = sc.take<float>((size_t)n);
+            top = sc.take<float>((size_t)(parts * rows));
+            total = sc.take<float>((size_t)(parts * rows));
+            hit = sc.take<float>((size_t)rows);
             if (pass == 0) {
                 rc = capi::scratch(sc.used, s, &sc.base, &cus);
                 if (rc) return rc;
@@ -255,9 +259,14 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
             }
         }
         MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), s));
+        const Mat hm = ho.mat();
         capi::Timed timed(s, "softmax_xent");
-        MLRS_TRY(launch_xent_stats<T>(ho.mat(), wo.mat(), bias, target, n, v, d, tile, top, total, hit, s));
-        MLRS_TRY(launch_xent_join(top, total, parts, hit, target, n, v, ignore, loss, lse, s));
+        for (int64_t r0 = 0; r0 < n; r0 += rows) {
+            const int64_t r = std::min(rows, n - r0);
+            MLRS_TRY(launch_xent_stats<T>(Mat{(const T*)hm.p + r0 * hm.ld, hm.ld}, wo.mat(), bias, target + r0, r, v,
+                                          d, tile, top, total, hit, s));
+            MLRS_TRY(launch_xent_join(top, total, parts, hit, target + r0, r, v, ignore, loss + r0, lse + r0, s));
+        }
         return MLRS_OK;
     });
 }
@@ -293,8 +302,10 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
             return MLRS_OK;
         }
-        // classes of a piece: a multiple of 256, at least one tile
-        const int64_t fit = MLRS_XENT_PIECE_BYTES / ((int64_t)sizeof(T) * n) / 256 * 256;
+        // classes of a piece: a multiple of 256, at least one tile, and a row of
+        // them within the kernels' limit
+        const int64_t fit = std::min<int64_t>(MLRS_XENT_PIECE_BYTES / ((int64_t)sizeof(T) * n),
+                                              kMaxRowBytes / (int64_t)sizeof(T)) / 256 * 256;
         const int64_t pieces = (v + std::max<int64_t>(fit, 256) - 1) / std::max<int64_t>(fit, 256);
         const int64_t piece = pieces == 1 ? v : ((v + pieces - 1) / pieces + 255) / 256 * 256;
         const int64_t ld = padded<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;

@@ -280,6 +280,46 @@ def test_xent_masked_classes(dtype):
     assert not dw[masked].any() and not db[masked].any()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_xent_many_rows_in_pieces(dtype):
+    """More rows than the statistics have room for at a time, and a gradient of
+    the logits of several pieces, the last of them short and odd.  The 64-bit
+    reference is computed on the GPU (its products are float64)."""
+    n, v, k = 56000, 20011, 16
+    h, w, b = rand(1, n, k, dtype=dtype).cuda(), rand(2, v, k, dtype=dtype, std=0.4).cuda(), rand(3, v, dtype=dtype).cuda()
+    t = targets(4, n, v).cuda()
+    g = torch.full((n,), 1.0 / n, device="cuda")
+    loss, lse = prims.softmax_xent(h, w, t, bias=b)
+    dh, dw, db = prims.softmax_xent_grad(h, w, t, lse, g, bias=b)
+    hd, wd = h.double(), w.double()
+    want_dw, want_db = torch.zeros_like(wd), torch.zeros(v, dtype=torch.float64, device="cuda")
+    for a in range(0, n, 14000):
+        part = slice(a, a + 14000)
+        z = hd[part] @ wd.t() + b.double()
+        l = torch.logsumexp(z, 1)
+        kept = t[part] != IGNORE
+        at = torch.where(kept, t[part], 0)[:, None]
+        # the logits are sums of 17 terms of size up to about ten, the sum of
+        # exponentials one of 20,011: 2^-19 covers both
+        assert (lse[part] - l).abs().max() < 2.0 ** -19 * 16
+        want = torch.where(kept, l - z.gather(1, at)[:, 0], 0.0)
+        assert (loss[part] - want).abs().max() < 2.0 ** -19 * 16
+        d = torch.exp(z - l[:, None])
+        d.scatter_add_(1, at, torch.full_like(l, -1.0)[:, None])
+        d *= (kept / n)[:, None]
+        want = d @ wd
+        # each term is rounded once to the type, and the result
+        unit = ref.UNIT[dtype]
+        room = 2 * unit * (d.abs() @ wd.abs()) + unit * want.abs() + 2.0 ** -18 * (d.abs() @ wd.abs())
+        assert bool(((dh[part].double() - want).abs() <= room).all())
+        want_dw += d.t() @ hd[part]
+        want_db += d.sum(0)
+        del z, d
+    size = want_dw.abs().max()
+    assert (dw.double() - want_dw).abs().max() <= (4 * ref.UNIT[dtype] + 2.0 ** -16) * size
+    assert (db.double() - want_db).abs().max() <= (4 * ref.UNIT[dtype] + 2.0 ** -16) * want_db.abs().max()
+
+
 def test_xent_target_that_is_masked_or_no_class():
     h, w = rand(1, 6, 16), rand(2, 50, 16)
     b = torch.zeros(50)
