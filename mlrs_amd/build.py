@@ -21,7 +21,8 @@ SOURCES = ["capi.hip", "knn_exact.hip", "knn_gram_f32.hip", "knn_gram_f64.hip", 
            "knn_consumers.hip", "knn_radius.hip", "knn_radius_gram.hip", "knn_graph.hip",
            "kmeans_loop.hip", "probe.hip", "knn_k1_resident.hip", "knn_groupmin.hip",
            "knn_groupmin_scan.hip", "knn_groupmin_metric.hip", "knn_groupmin_precise.hip",
-           "capi_train.hip", "train_linear.hip", "train_xent.hip", "train_adamw.hip"]
+           "capi_train.hip", "train_linear.hip", "train_xent.hip", "train_split.hip",
+           "train_adamw.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

@@ -63,6 +63,28 @@ struct Op {
     Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, padded<T>(cols)}; }
 };
 
+// f32 products may run on the bf16 matrix cores, in three parts of each operand
+// (train_split.hpp).  What packing `elements` of them costs, in microseconds: 10
+// bytes each at 5.5 TB/s, its launch, and the launches of the
+// f32 kernels that take over where an element is not finite.
+double split_us(double elements) { return elements * 10.0 / 5.5e6 + 9.0; }
+
+// A mark that no earlier call has left behind.
+uint32_t next_mark() {
+    static uint32_t mark = 0;  // under the call lock
+    return ++mark;
+}
+
+// The split kernels of a call and the f32 ones that stand in for them.
+struct Sides {
+    uint32_t* flag = nullptr;
+    uint32_t mark = 0;
+    Only split() const { return Only{flag, mark, false}; }
+    Only plain() const { return Only{flag, mark, true}; }
+};
+
+constexpr Cut kPlainCut{0, 1, 0, 0.0};  // of the kernels that stand in
+
 // Sizes that both layers of operators share: a (n x d) and w (m x d).
 template <typename T>
 int32_t check_sizes(const char* a_name, int64_t a_len, int64_t n, int64_t d, int64_t w_len, int64_t m) {
@@ -116,14 +138,27 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
         int cus = 0;
         rc = capi::cu_count(&cus);
         if (rc) return rc;
-        const Cut cut = choose_cut((int)sizeof(T), m, n, k, cus);
+        Cut cut = choose_cut((int)sizeof(T), m, n, k, cus);
+        bool split = false;
+        if constexpr (std::is_same<T, float>::value) {
+            const Cut other = choose_cut_split(m, n, k, cus);
+            split = other.us + split_us((double)(n + m) * (double)k) < cut.us;
+            if (split) cut = other;
+        }
         Op<T> xo(x, n, k), wo(w, m, k);
         float* part = nullptr;
+        char *xs = nullptr, *ws = nullptr;
+        Sides sides;
         Scratch sc;
         for (int pass = 0; pass < 2; ++pass) {
             xo.plan(sc);
             wo.plan(sc);
             part = sc.take<float>(cut.part_bytes(m, n) / 4);
+            if (split) {
+                xs = sc.take<char>(split_bytes(n, k));
+                ws = sc.take<char>(split_bytes(m, k));
+                sides.flag = sc.take<uint32_t>(1);
+            }
             if (sc.used == 0) break;
             if (pass == 0) {
                 rc = capi::scratch(sc.used, s, &sc.base, &cus);
@@ -131,9 +166,22 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
                 sc.used = 0;
             }
         }
-        MLRS_TRY(launch_pack<T>(xo.job(), wo.job(), s));
+        if constexpr (std::is_same<T, float>::value) {
+            if (split) {
+                sides.mark = next_mark();
+                MLRS_TRY(launch_pack_split(split_job(x, k, n, k, xs, false), split_job(w, k, m, k, ws, false),
+                                           sides.flag, sides.mark, s));
+                capi::Timed timed(s, "linear");
+                MLRS_TRY(launch_linear_split(split_mat(xs, k, false), split_mat(ws, k, false), n, m, k, o, cut, part,
+                                             sides.split(), s));
+                MLRS_TRY(launch_pack<T>(xo.job(), wo.job(), sides.plain(), s));
+                MLRS_TRY(launch_linear<T>(xo.mat(), wo.mat(), n, m, k, o, kPlainCut, nullptr, sides.plain(), s));
+                return MLRS_OK;
+            }
+        }
+        MLRS_TRY(launch_pack<T>(xo.job(), wo.job(), Only{}, s));
         capi::Timed timed(s, "linear");
-        MLRS_TRY(launch_linear<T>(xo.mat(), wo.mat(), n, m, k, o, cut, part, s));
+        MLRS_TRY(launch_linear<T>(xo.mat(), wo.mat(), n, m, k, o, cut, part, Only{}, s));
         return MLRS_OK;
     });
 }
@@ -171,8 +219,18 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         const bool products = (dx && n > 0) || dw;
         // dy itself serves as dz where there is no slope and its rows can be read
         const bool make_dz = products && n > 0 && (act != MLRS_ACT_NONE || !readable(dy, m));
-        const Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
+        Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
+        bool split_x = false, split_w = false;
+        if constexpr (std::is_same<T, float>::value) {
+            const Cut ox = choose_cut_split(k, n, m, cus), ow = choose_cut_split(k, m, n, cus);
+            split_x = dx && n > 0 && ox.us + split_us((double)(n + k) * (double)m) < cx.us;
+            split_w = dw && n > 0 && ow.us + split_us((double)(m + k) * (double)n) < cw.us;
+            if (split_x) cx = ox;
+            if (split_w) cw = ow;
+        }
         const int parts = column_parts(n, m, cus);
+        char *w_r = nullptr, *dz_k = nullptr, *x_r = nullptr, *dz_r = nullptr;
+        Sides sides;
         Op<T> xo(x, n, k), wo(w, m, k);
         T* dz = nullptr;
         float *part = nullptr, *sums = nullptr;
@@ -183,6 +241,15 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
             if (make_dz) dz = sc.take<T>((size_t)(n * padded<T>(m)));
             if (db) sums = sc.take<float>((size_t)parts * (size_t)m);
             part = sc.take<float>(std::max(dx ? cx.part_bytes(k, n) : 0, dw ? cw.part_bytes(k, m) : 0) / 4);
+            if (split_x) {
+                w_r = sc.take<char>(split_bytes(m, k));
+                dz_k = sc.take<char>(split_bytes(n, m));
+            }
+            if (split_w) {
+                x_r = sc.take<char>(split_bytes(n, k));
+                dz_r = sc.take<char>(split_bytes(n, m));
+            }
+            if (split_x || split_w) sides.flag = sc.take<uint32_t>(1);
             if (sc.used == 0) break;
             if (pass == 0) {
                 rc = capi::scratch(sc.used, s, &sc.base, &cus);
@@ -195,18 +262,41 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
                                         ColumnSums<T>{db, sums, parts, nullptr}, s));
         const Mat dzm = make_dz ? Mat{dz, padded<T>(m)} : Mat{dy, m};
         PackJob xj = xo.job(), wj = wo.job();
-        if (!dw) xj.rows = 0;
-        if (!dx) wj.rows = 0;
-        MLRS_TRY(launch_pack<T>(xj, wj, s));
+        if (!dw || split_w) xj.rows = 0;
+        if (!dx || split_x) wj.rows = 0;
+        MLRS_TRY(launch_pack<T>(xj, wj, Only{}, s));
         capi::Timed timed(s, "linear_grad");
-        if (dx && n > 0) {
-            const StoreTo o{dx, k, nullptr, nullptr, 0, nullptr};
-            MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, o, cx, part, s));
+        const StoreTo to_x{dx, k, nullptr, nullptr, 0, nullptr}, to_w{dw, k, nullptr, nullptr, 0, nullptr};
+        if constexpr (std::is_same<T, float>::value) {
+            if (split_x || split_w) {
+                sides.mark = next_mark();
+                const float* z32 = (const float*)dzm.p;
+                if (split_x) {
+                    MLRS_TRY(launch_pack_split(split_job(w, k, m, k, w_r, true),
+                                               split_job(z32, dzm.ld, n, m, dz_k, false), sides.flag, sides.mark, s));
+                    MLRS_TRY(launch_product_split(split_mat(w_r, k, true), split_mat(dz_k, m, false), true, k, n, m,
+                                                  to_x, cx, part, sides.split(), s));
+                }
+                if (split_w) {
+                    MLRS_TRY(launch_pack_split(split_job(x, k, n, k, x_r, true),
+                                               split_job(z32, dzm.ld, n, m, dz_r, true), sides.flag, sides.mark, s));
+                    MLRS_TRY(launch_product_split(split_mat(x_r, k, true), split_mat(dz_r, m, true), false, k, m, n,
+                                                  to_w, cw, part, sides.split(), s));
+                }
+                // what dw's packing marked is marked for dx as well, whose
+                // product the f32 kernel then computes again, to the same values
+                PackJob xp = xo.job(), wp = wo.job();
+                if (!split_w) xp.rows = 0;
+                if (!split_x) wp.rows = 0;
+                MLRS_TRY(launch_pack<T>(xp, wp, sides.plain(), s));
+                if (split_x)
+                    MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, to_x, kPlainCut, nullptr, sides.plain(), s));
+                if (split_w)
+                    MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, to_w, kPlainCut, nullptr, sides.plain(), s));
+            }
         }
-        if (dw) {
-            const StoreTo o{dw, k, nullptr, nullptr, 0, nullptr};
-            MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, o, cw, part, s));
-        }
+        if (dx && n > 0 && !split_x) MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, to_x, cx, part, Only{}, s));
+        if (dw && !split_w) MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, to_w, cw, part, Only{}, s));
         return MLRS_OK;
     });
 }
@@ -239,33 +329,69 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         int cus = 0;
         rc = capi::cu_count(&cus);
         if (rc) return rc;
-        const int tile = choose_cut((int)sizeof(T), v, n, d, cus, 1).tile;
+        const Cut cut = choose_cut((int)sizeof(T), v, n, d, cus, 1);
+        int tile = cut.tile;
+        int64_t parts = stats_parts(tile, v), parts_s = 0;
+        bool split = false;
+        if constexpr (std::is_same<T, float>::value) {
+            split = choose_cut_split(v, n, d, cus, 1).us + split_us((double)(n + v) * (double)d) < cut.us;
+            if (split) {
+                tile = kPlainCut.tile;
+                parts = stats_parts(tile, v);
+                parts_s = stats_parts_split(v);
+            }
+        }
         // the statistics of as many rows at a time as their parts have room for
-        const int64_t parts = stats_parts(tile, v);
-        const int64_t rows = std::min(n, std::max<int64_t>(256, kStatsBytes / (8 * parts) / 256 * 256));
+        const int64_t room = std::max(parts, parts_s);
+        const int64_t rows = std::min(n, std::max<int64_t>(256, kStatsBytes / (8 * room) / 256 * 256));
         Op<T> ho(h, n, d), wo(w, v, d);
         float *top = nullptr, *total = nullptr, *hit = nullptr;
+        char *hs = nullptr, *ws = nullptr;
+        Sides sides;
         Scratch sc;
         for (int pass = 0; pass < 2; ++pass) {
             ho.plan(sc);
             wo.plan(sc);
-            top = sc.take<float>((size_t)(parts * rows));
-            total = sc.take<float>((size_t)(parts * rows));
+            top = sc.take<float>((size_t)(room * rows));
+            total = sc.take<float>((size_t)(room * rows));
             hit = sc.take<float>((size_t)rows);
+            if (split) {
+                hs = sc.take<char>(split_bytes(n, d));
+                ws = sc.take<char>(split_bytes(v, d));
+                sides.flag = sc.take<uint32_t>(1);
+            }
             if (pass == 0) {
                 rc = capi::scratch(sc.used, s, &sc.base, &cus);
                 if (rc) return rc;
                 sc.used = 0;
             }
         }
-        MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), s));
+        if constexpr (std::is_same<T, float>::value) {
+            if (split) {
+                sides.mark = next_mark();
+                MLRS_TRY(launch_pack_split(split_job(h, d, n, d, hs, false), split_job(w, d, v, d, ws, false),
+                                           sides.flag, sides.mark, s));
+            }
+        }
+        const Only plain = split ? sides.plain() : Only{};
+        MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), plain, s));
         const Mat hm = ho.mat();
         capi::Timed timed(s, "softmax_xent");
         for (int64_t r0 = 0; r0 < n; r0 += rows) {
             const int64_t r = std::min(rows, n - r0);
+            if constexpr (std::is_same<T, float>::value) {
+                if (split) {
+                    MLRS_TRY(launch_xent_stats_split(split_mat(hs + split_bytes(r0, d), d, false),
+                                                     split_mat(ws, d, false), bias, target + r0, r, v, d, top, total,
+                                                     hit, sides.split(), s));
+                    MLRS_TRY(launch_xent_join(top, total, parts_s, hit, target + r0, r, v, ignore, loss + r0, lse + r0,
+                                              sides.split(), s));
+                }
+            }
             MLRS_TRY(launch_xent_stats<T>(Mat{(const T*)hm.p + r0 * hm.ld, hm.ld}, wo.mat(), bias, target + r0, r, v,
-                                          d, tile, top, total, hit, s));
-            MLRS_TRY(launch_xent_join(top, total, parts, hit, target + r0, r, v, ignore, loss + r0, lse + r0, s));
+                                          d, tile, top, total, hit, plain, s));
+            MLRS_TRY(launch_xent_join(top, total, parts, hit, target + r0, r, v, ignore, loss + r0, lse + r0, plain,
+                                      s));
         }
         return MLRS_OK;
     });
@@ -296,7 +422,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             if (dw) {
                 const StoreTo o{dw, d, nullptr, nullptr, 0, nullptr};
                 MLRS_TRY(launch_product<T>(Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, false, d, v, 0, o,
-                                           Cut{2, 1, 0}, nullptr, s));
+                                           Cut{2, 1, 0, 0.0}, nullptr, Only{}, s));
             }
             if (db)
                 MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
@@ -310,60 +436,129 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
         const int64_t piece = pieces == 1 ? v : ((v + pieces - 1) / pieces + 255) / 256 * 256;
         const int64_t ld = padded<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;
         const bool scaled = sizeof(T) == 2 && std::is_same<T, _Float16>::value;
-        const Cut ch = choose_cut((int)sizeof(T), d, n, std::min(piece, v), cus);
-        const Cut cw = choose_cut((int)sizeof(T), d, std::min(piece, v), n, cus);
-        const int parts = column_parts(n, std::min(piece, v), cus);
+        const int64_t most = std::min(piece, v);  // classes of the largest piece
+        const Cut ch = choose_cut((int)sizeof(T), d, n, most, cus), cw = choose_cut((int)sizeof(T), d, most, n, cus);
+        // f32: which of a piece's three products run in parts; the gradient of the
+        // logits is packed for each of the two that take it
+        Cut sh{}, sw{};
+        bool split_z = false, split_h = false, split_w = false;
+        if constexpr (std::is_same<T, float>::value) {
+            const double nv = (double)n * (double)most, nd = (double)n * (double)d, vd = (double)most * (double)d;
+            sh = choose_cut_split(d, n, most, cus);
+            sw = choose_cut_split(d, most, n, cus);
+            split_z = choose_cut_split(most, n, d, cus, 1).us + split_us(nd + vd) <
+                      choose_cut((int)sizeof(T), most, n, d, cus, 1).us;
+            split_h = dh && sh.us + split_us(nv + vd) < ch.us;
+            split_w = dw && sw.us + split_us(nv + nd) < cw.us;
+        }
+        const bool split = split_z || split_h || split_w;
+        const int parts = column_parts(n, most, cus);
         Op<T> ho(h, n, d), wo(w, v, d);
         T* dz = nullptr;
         float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr;
+        char *h_k = nullptr, *w_k = nullptr, *h_r = nullptr, *w_r = nullptr, *dz_k = nullptr, *dz_r = nullptr;
+        Sides sides;
         Scratch sc;
         for (int pass = 0; pass < 2; ++pass) {
             ho.plan(sc);
             wo.plan(sc);
             dz = sc.take<T>((size_t)(n * ld));
             if (dh && pieces > 1) acc = sc.take<float>((size_t)(n * dh_ld));
-            if (db) sums = sc.take<float>((size_t)parts * (size_t)std::min(piece, v));
+            if (db) sums = sc.take<float>((size_t)parts * (size_t)most);
             if (scaled) up = sc.take<float>(2);
-            part = sc.take<float>(
-                std::max(dh ? ch.part_bytes(d, n) : 0, dw ? cw.part_bytes(d, std::min(piece, v)) : 0) / 4);
+            size_t bytes = std::max(dh ? ch.part_bytes(d, n) : 0, dw ? cw.part_bytes(d, most) : 0);
+            if (split_h) bytes = std::max(bytes, sh.part_bytes(d, n));
+            if (split_w) bytes = std::max(bytes, sw.part_bytes(d, most));
+            part = sc.take<float>(bytes / 4);
+            if (split_z) {
+                h_k = sc.take<char>(split_bytes(n, d));
+                w_k = sc.take<char>(split_bytes(most, d));
+            }
+            if (split_w) {
+                h_r = sc.take<char>(split_bytes(n, d));
+                dz_r = sc.take<char>(split_bytes(n, most));
+            }
+            if (split_h) {
+                w_r = sc.take<char>(split_bytes(most, d));
+                dz_k = sc.take<char>(split_bytes(n, most));
+            }
+            if (split) sides.flag = sc.take<uint32_t>(1);
             if (pass == 0) {
                 rc = capi::scratch(sc.used, s, &sc.base, &cus);
                 if (rc) return rc;
                 sc.used = 0;
             }
         }
-        MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), s));
+        if (split) sides.mark = next_mark();
+        // f32 operands that every product has in parts are needed only where the
+        // plain kernels stand in
+        const Only plain = split ? sides.plain() : Only{};
+        const bool all_split = split_z && (!dh || split_h) && (!dw || split_w);
         if (scaled) MLRS_TRY(launch_grad_scale(grad, target, n, ignore, up, s));
         const float* down = scaled ? up + 1 : nullptr;
         const Mat hm = ho.mat(), wm = wo.mat();
         capi::Timed timed(s, "softmax_xent_grad");
+        if constexpr (std::is_same<T, float>::value) {
+            SplitJob hk = split_job(h, d, n, d, h_k, false), hr = split_job(h, d, n, d, h_r, true);
+            if (!split_z) hk.rows = 0;
+            if (!split_w) hr.rows = 0;
+            if (split) MLRS_TRY(launch_pack_split(hk, hr, sides.flag, sides.mark, s));
+        }
+        if (!all_split) MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), Only{}, s));
         for (int64_t v0 = 0; v0 < v; v0 += piece) {
             const int64_t vp = std::min(piece, v - v0);
             const bool last = v0 + vp == v;
-            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
-                                          choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile, s));
             const Mat dzm{dz, ld};
-            if (db) {
-                MLRS_TRY(launch_column_sums<T>(dzm, n, vp, ColumnSums<T>{db + v0, sums, parts, down}, s));
+            if constexpr (std::is_same<T, float>::value) {
+                const float* wp = w + v0 * d;
+                SplitJob wk = split_job(wp, d, vp, d, w_k, false), wr = split_job(wp, d, vp, d, w_r, true);
+                if (!split_z) wk.rows = 0;
+                if (!split_h) wr.rows = 0;
+                if (split) MLRS_TRY(launch_pack_split(wk, wr, sides.flag, sides.mark, s));
+                if (all_split) MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), plain, s));
+                if (split_z)
+                    MLRS_TRY(launch_logit_grad_split(split_mat(h_k, d, false), split_mat(w_k, d, false), bias, target,
+                                                     lse, grad, n, v0, vp, v, d, ignore, dz, ld, sides.split(), s));
             }
-            if (dw) {
-                const StoreTo o{dw + v0 * d, d, nullptr, nullptr, 0, down};
-                MLRS_TRY(launch_product<T>(hm, dzm, false, d, vp, n, o, cw, part, s));
+            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
+                                          split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile,
+                                          split_z ? plain : Only{}, s));
+            if (db) MLRS_TRY(launch_column_sums<T>(dzm, n, vp, ColumnSums<T>{db + v0, sums, parts, down}, s));
+            const StoreTo to_w{dw ? dw + v0 * d : nullptr, d, nullptr, nullptr, 0, down};
+            StoreTo to_h{};
+            to_h.ld = d;
+            to_h.acc = acc;
+            to_h.acc_ld = dh_ld;
+            to_h.add = v0 > 0 ? acc : nullptr;
+            if (last) {
+                to_h.out = dh;
+                to_h.alpha = down;
             }
+            if constexpr (std::is_same<T, float>::value) {
+                SplitJob zk = split_job(dz, ld, n, vp, dz_k, false), zr = split_job(dz, ld, n, vp, dz_r, true);
+                if (!split_h) zk.rows = 0;
+                if (!split_w) zr.rows = 0;
+                if (split_h || split_w) MLRS_TRY(launch_pack_split(zk, zr, sides.flag, sides.mark, s));
+                if (all_split) MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), plain, s));
+                if (split_w)
+                    MLRS_TRY(launch_product_split(split_mat(h_r, d, true), split_mat(dz_r, vp, true), false, d, vp, n,
+                                                  to_w, sw, part, sides.split(), s));
+                // a last piece's parts of the contraction may be empty ones
+                Cut c = sh;
+                if (vp < most) c = Cut{0, 1, 0, 0.0};
+                if (split_h)
+                    MLRS_TRY(launch_product_split(split_mat(w_r, d, true), split_mat(dz_k, vp, false), true, d, n, vp,
+                                                  to_h, c, part, sides.split(), s));
+            }
+            if (dw)
+                MLRS_TRY(launch_product<T>(hm, dzm, false, d, vp, n, to_w, split_w ? kPlainCut : cw, part,
+                                           split_w ? plain : Only{}, s));
             if (dh) {
-                StoreTo o{};
-                o.ld = d;
-                o.acc = acc;
-                o.acc_ld = dh_ld;
-                o.add = v0 > 0 ? acc : nullptr;
-                if (last) {
-                    o.out = dh;
-                    o.alpha = down;
-                }
-                Cut c = ch;
-                if (vp < piece) c = choose_cut((int)sizeof(T), d, n, vp, cus);
-                if (c.part_bytes(d, n) > ch.part_bytes(d, n)) c = Cut{c.tile, 1, 0};
-                MLRS_TRY(launch_product<T>(Mat{(const T*)wm.p + v0 * wm.ld, wm.ld}, dzm, true, d, n, vp, o, c, part, s));
+                Cut c = split_h ? kPlainCut : ch;
+                if (!split_h && vp < most) c = choose_cut((int)sizeof(T), d, n, vp, cus);
+                if (c.part_bytes(d, n) > ch.part_bytes(d, n)) c = Cut{c.tile, 1, 0, 0.0};
+                MLRS_TRY(launch_product<T>(Mat{(const T*)wm.p + v0 * wm.ld, wm.ld}, dzm, true, d, n, vp, to_h, c, part,
+                                           split_h ? plain : Only{}, s));
             }
         }
         return MLRS_OK;

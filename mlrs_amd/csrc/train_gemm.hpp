@@ -79,7 +79,16 @@ struct GemmArgs {
     int32_t splits;        // parts of the contraction axis, a grid's worth of tiles each
     int32_t k_split;       // elements of k in a part (a multiple of the staged width)
     int32_t band;          // tiles of m that are walked together (L2 reuse)
+    const uint32_t* flag;  // null, or: run only where (*flag == mark) == wanted
+    uint32_t mark;
+    bool wanted;
 };
+
+// Whether another kernel does this launch's work.
+__device__ __forceinline__ bool skipped(const uint32_t* flag, uint32_t mark, bool wanted) {
+    return flag && (*flag == mark) != wanted;
+}
+__device__ __forceinline__ bool skipped(const GemmArgs& g) { return skipped(g.flag, g.mark, g.wanted); }
 
 constexpr int kStageBytes = 128;  // of the contraction axis, per buffer
 
@@ -283,6 +292,23 @@ __device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
     return x * per + (x < extra ? x : extra) + i;
 }
 
+// The tile of a workgroup: bands of `band` tiles of m, walked along n.
+struct TilePlace {
+    int32_t tm, tn, split;
+};
+__device__ __forceinline__ TilePlace tile_place(const GemmArgs& g) {
+    const int32_t tiles = g.tiles_m * g.tiles_n;
+    TilePlace p;
+    p.split = blockIdx.x / tiles;
+    const int32_t t = xcd_tile(blockIdx.x - p.split * tiles, tiles);
+    const int32_t per_band = g.band * g.tiles_n;
+    const int32_t bnd = t / per_band, in = t - bnd * per_band;
+    const int32_t width = g.tiles_m - bnd * g.band < g.band ? g.tiles_m - bnd * g.band : g.band;
+    p.tm = bnd * g.band + in % width;
+    p.tn = in / width;
+    return p;
+}
+
 // A number as a type: which of two sets of fragments.
 template <int V>
 struct Set {
@@ -307,22 +333,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
     constexpr int kAhead = 3;  // staged widths under way, of a small tile
     constexpr int kSlots = kSmall ? 2 * kAhead : 5;
     __shared__ __attribute__((aligned(1024))) char buf[kSlots * kA];
+    if (skipped(g)) return;
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    const int32_t tiles = g.tiles_m * g.tiles_n;
-    const int32_t split = blockIdx.x / tiles;
-    const int32_t t = xcd_tile(blockIdx.x - split * tiles, tiles);
-    // bands of `band` tiles of m, walked along n
-    const int32_t per_band = g.band * g.tiles_n;
-    const int32_t bnd = t / per_band, in = t - bnd * per_band;
-    const int32_t width = g.tiles_m - bnd * g.band < g.band ? g.tiles_m - bnd * g.band : g.band;
-    const int32_t tm = bnd * g.band + in % width, tn = in / width;
-    const int32_t m0 = tm * BM, n0 = tn * BN;
-
-    const int32_t k_lo = split * g.k_split;
+    const TilePlace t = tile_place(g);
+    const int32_t m0 = t.tm * BM, n0 = t.tn * BN;
+    const int32_t k_lo = t.split * g.k_split;
     const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;
 
     Stager<T, AKC, BM, WAVES> sa;
@@ -482,8 +501,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
     p.n0 = n0 + wn * NB * 16;
     p.m = g.m;
     p.n = g.n;
-    p.split = split;
-    p.tile_m = tm;
+    p.split = t.split;
+    p.tile_m = t.tm;
     p.lane = lane;
     p.wave = wave;
     p.wm = wm;

@@ -21,11 +21,19 @@ struct Cut {
     int tile;         // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
     int splits;
     int32_t k_split;
+    double us;        // the estimate it was chosen by
     size_t part_bytes(int64_t m, int64_t n) const {
         return splits > 1 ? (size_t)splits * (size_t)n * (size_t)((m + 3) & ~(int64_t)3) * 4 : 0;
     }
 };
 Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
+
+// A launch that runs only where (*flag == mark) == wanted (flag null: always).
+struct Only {
+    const uint32_t* flag = nullptr;
+    uint32_t mark = 0;
+    bool wanted = true;
+};
 
 // dst (rows x ld, ld >= cols) := src (rows x cols), zeros behind each row; no
 // rows: nothing to do.
@@ -35,7 +43,7 @@ struct PackJob {
     int64_t rows, cols, ld;
 };
 template <typename T>
-hipError_t launch_pack(const PackJob& a, const PackJob& b, hipStream_t s);
+hipError_t launch_pack(const PackJob& a, const PackJob& b, const Only& only, hipStream_t s);
 
 // y (n x m) = act(x w^T + bias) + residual; z, where not null, x w^T + bias.
 struct LinearOut {
@@ -47,7 +55,7 @@ struct LinearOut {
 };
 template <typename T>
 hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
-                         float* part, hipStream_t s);
+                         float* part, const Only& only, hipStream_t s);
 // The same for a few rows, straight from the caller's unpacked operands.
 constexpr int kFewRows = 64;
 template <typename T>
@@ -85,23 +93,56 @@ struct StoreTo {
 };
 template <typename T>
 hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
-                          float* part, hipStream_t s);
+                          float* part, const Only& only, hipStream_t s);
 
 // Softmax cross entropy: the statistics of every wave's classes, joined into
 // lse and loss; the scale of a half-precision gradient; a piece's gradient.
 int64_t stats_parts(int tile, int64_t classes);
 template <typename T>
 hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target, int64_t n, int64_t classes, int64_t k,
-                             int tile, float* top, float* total, float* hit, hipStream_t s);
+                             int tile, float* top, float* total, float* hit, const Only& only, hipStream_t s);
 hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
                             const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
-                            hipStream_t s);
+                            const Only& only, hipStream_t s);
 hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n, int64_t ignore, float* up_down,
                              hipStream_t s);
 template <typename T>
 hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
                              const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
-                             int64_t ignore, T* out, int64_t ld, int tile, hipStream_t s);
+                             int64_t ignore, T* out, int64_t ld, int tile, const Only& only, hipStream_t s);
+
+// f32 products on the bf16 matrix cores (train_split.hpp).  K layout: ld is
+// bytes, split_row_bytes of the columns; R layout: ld is elements, a multiple of
+// 8, of the three rows of one k.
+struct SplitJob {
+    const float* src;
+    int64_t src_ld;
+    void* dst;
+    int64_t rows, cols;
+    int width;
+    bool r_layout;
+};
+SplitJob split_job(const float* src, int64_t src_ld, int64_t rows, int64_t cols, void* dst, bool r_layout);
+inline int64_t split_row_bytes(int64_t cols) { return (cols + 7) / 8 * 48; }
+inline size_t split_bytes(int64_t rows, int64_t cols) { return (size_t)rows * (size_t)split_row_bytes(cols); }
+inline Mat split_mat(const void* p, int64_t cols, bool r_layout) {
+    return Mat{p, r_layout ? (cols + 7) / 8 * 8 : split_row_bytes(cols)};
+}
+Cut choose_cut_split(int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
+// *flag := mark where an element is not finite.
+hipError_t launch_pack_split(const SplitJob& a, const SplitJob& b, uint32_t* flag, uint32_t mark, hipStream_t s);
+hipError_t launch_linear_split(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
+                               float* part, const Only& only, hipStream_t s);
+hipError_t launch_product_split(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o,
+                                const Cut& cut, float* part, const Only& only, hipStream_t s);
+int64_t stats_parts_split(int64_t classes);
+hipError_t launch_xent_stats_split(Mat h, Mat w, const float* bias, const int64_t* target, int64_t n, int64_t classes,
+                                   int64_t k, float* top, float* total, float* hit, const Only& only, hipStream_t s);
+// w: the piece's classes; bias: the whole vocabulary's.
+hipError_t launch_logit_grad_split(Mat h, Mat w, const float* bias, const int64_t* target, const float* lse,
+                                   const float* grad, int64_t n, int64_t first, int64_t piece, int64_t classes,
+                                   int64_t k, int64_t ignore, float* out, int64_t ld, const Only& only,
+                                   hipStream_t s);
 
 // Optimizer.
 int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);

@@ -16,7 +16,7 @@ inline int32_t band_of(int tile, int32_t tiles_m) { return std::min<int32_t>(til
 
 template <typename T, bool AKC, bool BKC, typename Epi>
 hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, int splits, int32_t k_split,
-                       const Epi& epi, hipStream_t s) {
+                       const Only& only, const Epi& epi, hipStream_t s) {
     const int rows = kTileRows[tile];
     GemmArgs g;
     g.a = Operand{a.p, a.ld};
@@ -29,6 +29,9 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
     g.splits = splits;
     g.k_split = splits > 1 ? k_split : (int32_t)std::max<int64_t>(k, 1);
     g.band = band_of(tile, g.tiles_m);
+    g.flag = only.flag;
+    g.mark = only.mark;
+    g.wanted = only.wanted;
     const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * splits;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
     const dim3 grid((unsigned)blocks);
@@ -46,6 +49,88 @@ template <typename T>
 inline int row_width(const void* p, int64_t ld) {
     if ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0) return 4;
     return (uintptr_t)p % (2 * sizeof(T)) == 0 && ld % 2 == 0 ? 2 : 1;
+}
+
+// The parts of a split contraction, joined in order.
+template <typename Point>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t stride,
+                                                   int64_t part_ld, int64_t m, int64_t n, Point point, Only only) {
+    if (skipped(only.flag, only.mark, only.wanted)) return;
+    const int64_t quads = part_ld / 4, total = quads * n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / quads, c = (i - r * quads) * 4;
+        const float* at = part + r * part_ld + c;
+        f32x4 v = *reinterpret_cast<const f32x4*>(at);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(at + s * stride);
+        point(r, c, m, v);
+    }
+}
+
+template <typename Point>
+hipError_t launch_join(const float* part, int splits, int64_t m, int64_t n, const Point& point, const Only& only,
+                       hipStream_t s) {
+    const int64_t part_ld = (m + 3) & ~(int64_t)3;
+    const int64_t total = part_ld / 4 * n;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
+    join_kernel<Point><<<dim3((unsigned)blocks), 256, 0, s>>>(part, splits, n * part_ld, part_ld, m, n, point,
+                                                               only);
+    return hipGetLastError();
+}
+
+template <typename T>
+struct LinearPoint {
+    LinearEpi<T> e;
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
+        f32x4 g[1] = {v};
+        e.rows(n, 0, n + 1, c, m, e.bias_at(c, m), g);
+    }
+};
+template <typename T>
+struct StorePoint {
+    StoreEpi<T> e;
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
+        f32x4 g[1] = {v};
+        e.rows(n, 0, n + 1, c, m, 0, g);
+    }
+};
+
+template <typename T>
+inline StoreEpi<T> parts_epi(float* part, int64_t m, int64_t n) {
+    StoreEpi<T> e{};
+    e.part = part;
+    e.part_ld = (m + 3) & ~(int64_t)3;
+    e.part_stride = n * e.part_ld;
+    e.width = 4;
+    return e;
+}
+
+template <typename T>
+inline LinearEpi<T> linear_epi(const LinearOut& o, int64_t m) {
+    LinearEpi<T> e;
+    e.bias = (const T*)o.bias;
+    e.residual = (const T*)o.residual;
+    e.y = (T*)o.y;
+    e.z = (T*)o.z;
+    e.ld = m;
+    e.act = o.act;
+    e.width = row_width<T>(o.y, m);
+    if (o.z) e.width = std::min(e.width, row_width<T>(o.z, m));
+    if (o.residual) e.width = std::min(e.width, row_width<T>(o.residual, m));
+    return e;
+}
+
+template <typename T>
+inline StoreEpi<T> store_epi(const StoreTo& o) {
+    StoreEpi<T> e{};
+    e.out = (T*)o.out;
+    e.part = o.acc;
+    e.add = o.add;
+    e.alpha = o.alpha;
+    e.ld = o.ld;
+    e.part_ld = o.acc_ld;
+    e.part_stride = 0;
+    e.width = o.out ? row_width<T>(o.out, o.ld) : 4;
+    return e;
 }
 
 }  // namespace train

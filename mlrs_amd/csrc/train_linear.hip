@@ -25,8 +25,7 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
     static const int resident[3] = {1, 2, 3};
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
-    Cut best{0, 1, 0};
-    double best_cost = 1e300;
+    Cut best{0, 1, 0, 1e300};
     for (int t = 0; t < 3; ++t) {
         const double* stage = elem_bytes == 2 ? stage16[t] : stage32[t];
         const int rows = kTileRows[t];
@@ -40,12 +39,7 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
             if (rest) cost += (double)each * stage[rest - 1] + round_us[t];
             // joining the parts: a launch, and their bytes twice
             if (sp > 1) cost += 7.0 + (double)sp * (double)m * (double)n * 8.0 / 4.5e6;
-            if (cost < best_cost) {
-                best_cost = cost;
-                best.tile = t;
-                best.splits = (int)sp;
-                best.k_split = (int32_t)(each * per);
-            }
+            if (cost < best.us) best = Cut{t, (int)sp, (int32_t)(each * per), cost};
         }
     }
     return best;
@@ -56,7 +50,8 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
 // ---------------------------------------------------------------------------
 // Two matrices in a launch: both operands of a product are usually packed.
 template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b) {
+__global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b, Only only) {
+    if (skipped(only.flag, only.mark, only.wanted)) return;
     constexpr int E = 16 / (int)sizeof(T);
     const int64_t total_a = a.rows * (a.ld / E), total = total_a + b.rows * (b.ld / E);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -72,93 +67,26 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b) {
 }
 
 template <typename T>
-hipError_t launch_pack(const PackJob& a, const PackJob& b, hipStream_t s) {
+hipError_t launch_pack(const PackJob& a, const PackJob& b, const Only& only, hipStream_t s) {
     const int64_t total = (a.rows * a.ld + b.rows * b.ld) / (16 / (int64_t)sizeof(T));
     if (total == 0) return hipSuccess;
     const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
-    pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, s>>>(a, b);
+    pack_kernel<T><<<dim3((unsigned)blocks), 256, 0, s>>>(a, b, only);
     return hipGetLastError();
-}
-
-// ---------------------------------------------------------------------------
-// the parts of a split contraction, joined in order
-// ---------------------------------------------------------------------------
-template <typename Point>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t stride,
-                                                   int64_t part_ld, int64_t m, int64_t n, Point point) {
-    const int64_t quads = part_ld / 4, total = quads * n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / quads, c = (i - r * quads) * 4;
-        const float* at = part + r * part_ld + c;
-        f32x4 v = *reinterpret_cast<const f32x4*>(at);
-        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(at + s * stride);
-        point(r, c, m, v);
-    }
-}
-
-template <typename Point>
-static hipError_t launch_join(const float* part, int splits, int64_t m, int64_t n, const Point& point, hipStream_t s) {
-    const int64_t part_ld = (m + 3) & ~(int64_t)3;
-    const int64_t total = part_ld / 4 * n;
-    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
-    join_kernel<Point><<<dim3((unsigned)blocks), 256, 0, s>>>(part, splits, n * part_ld, part_ld, m, n, point);
-    return hipGetLastError();
-}
-
-template <typename T>
-struct LinearPoint {
-    LinearEpi<T> e;
-    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
-        f32x4 g[1] = {v};
-        e.rows(n, 0, n + 1, c, m, e.bias_at(c, m), g);
-    }
-};
-template <typename T>
-struct StorePoint {
-    StoreEpi<T> e;
-    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
-        f32x4 g[1] = {v};
-        e.rows(n, 0, n + 1, c, m, 0, g);
-    }
-};
-
-template <typename T>
-static StoreEpi<T> parts_epi(float* part, int64_t m, int64_t n) {
-    StoreEpi<T> e{};
-    e.part = part;
-    e.part_ld = (m + 3) & ~(int64_t)3;
-    e.part_stride = n * e.part_ld;
-    e.width = 4;
-    return e;
 }
 
 // ---------------------------------------------------------------------------
 // forwards
 // ---------------------------------------------------------------------------
 template <typename T>
-static LinearEpi<T> linear_epi(const LinearOut& o, int64_t m) {
-    LinearEpi<T> e;
-    e.bias = (const T*)o.bias;
-    e.residual = (const T*)o.residual;
-    e.y = (T*)o.y;
-    e.z = (T*)o.z;
-    e.ld = m;
-    e.act = o.act;
-    e.width = row_width<T>(o.y, m);
-    if (o.z) e.width = std::min(e.width, row_width<T>(o.z, m));
-    if (o.residual) e.width = std::min(e.width, row_width<T>(o.residual, m));
-    return e;
-}
-
-template <typename T>
 hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
-                         float* part, hipStream_t s) {
+                         float* part, const Only& only, hipStream_t s) {
     const LinearEpi<T> e = linear_epi<T>(o, m);
-    if (cut.splits == 1) return launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, 1, 0, e, s);
-    const hipError_t r = launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, cut.splits, cut.k_split,
+    if (cut.splits == 1) return launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, 1, 0, only, e, s);
+    const hipError_t r = launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, cut.splits, cut.k_split, only,
                                                     parts_epi<T>(part, m, n), s);
     if (r != hipSuccess) return r;
-    return launch_join(part, cut.splits, m, n, LinearPoint<T>{e}, s);
+    return launch_join(part, cut.splits, m, n, LinearPoint<T>{e}, only, s);
 }
 
 // A few rows: the weights are read once, straight into registers as the
@@ -356,37 +284,29 @@ hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& 
 
 template <typename T>
 hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
-                          float* part, hipStream_t s) {
-    StoreEpi<T> e{};
-    e.out = (T*)o.out;
-    e.part = o.acc;
-    e.add = o.add;
-    e.alpha = o.alpha;
-    e.ld = o.ld;
-    e.part_ld = o.acc_ld;
-    e.part_stride = 0;
-    e.width = o.out ? row_width<T>(o.out, o.ld) : 4;
+                          float* part, const Only& only, hipStream_t s) {
+    const StoreEpi<T> e = store_epi<T>(o);
     if (cut.splits == 1)
-        return b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, 1, 0, e, s)
-                   : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, 1, 0, e, s);
+        return b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, 1, 0, only, e, s)
+                   : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, 1, 0, only, e, s);
     const StoreEpi<T> pe = parts_epi<T>(part, m, n);
-    const hipError_t r = b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, pe, s)
-                             : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, pe, s);
+    const hipError_t r = b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, only, pe, s)
+                             : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, only, pe, s);
     if (r != hipSuccess) return r;
-    return launch_join(part, cut.splits, m, n, StorePoint<T>{e}, s);
+    return launch_join(part, cut.splits, m, n, StorePoint<T>{e}, only, s);
 }
 
 #define MLRS_INST(T)                                                                                               \
-    template hipError_t launch_pack<T>(const PackJob&, const PackJob&, hipStream_t);                               \
+    template hipError_t launch_pack<T>(const PackJob&, const PackJob&, const Only&, hipStream_t);                  \
     template hipError_t launch_linear<T>(Mat, Mat, int64_t, int64_t, int64_t, const LinearOut&, const Cut&, float*, \
-                                         hipStream_t);                                                             \
+                                         const Only&, hipStream_t);                                                \
     template hipError_t launch_linear_few<T>(const T*, const T*, int64_t, int64_t, int64_t, const LinearOut&,      \
                                              hipStream_t);                                                         \
     template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t,                 \
                                            const ColumnSums<T>&, hipStream_t);                                     \
     template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, const ColumnSums<T>&, hipStream_t);           \
     template hipError_t launch_product<T>(Mat, Mat, bool, int64_t, int64_t, int64_t, const StoreTo&, const Cut&,   \
-                                          float*, hipStream_t);
+                                          float*, const Only&, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)

@@ -17,9 +17,9 @@ int64_t stats_parts(int tile, int64_t classes) {
 
 template <typename T>
 hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target, int64_t n, int64_t classes, int64_t k,
-                             int tile, float* top, float* total, float* hit, hipStream_t s) {
+                             int tile, float* top, float* total, float* hit, const Only& only, hipStream_t s) {
     const StatsEpi<T> e{bias, target, top, total, hit};
-    return launch_gemm<T, true, true>(tile, w, h, classes, n, k, 1, 0, e, s);
+    return launch_gemm<T, true, true>(tile, w, h, classes, n, k, 1, 0, only, e, s);
 }
 
 // A workgroup joins the parts of 16 rows: sixteen threads take every sixteenth
@@ -30,7 +30,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict_
                                                         int64_t parts, const float* __restrict__ hit,
                                                         const int64_t* __restrict__ target, int64_t n,
                                                         int64_t classes, int64_t ignore, float* __restrict__ loss,
-                                                        float* __restrict__ lse) {
+                                                        float* __restrict__ lse, Only only) {
+    if (skipped(only.flag, only.mark, only.wanted)) return;
     constexpr int kRows = 16, kSlices = 16, kAtOnce = 4;
     __shared__ float tops[kSlices][kRows], sums[kSlices][kRows];
     const int c = threadIdx.x % kRows, p0 = threadIdx.x / kRows;
@@ -76,9 +77,9 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict_
 
 hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
                             const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
-                            hipStream_t s) {
+                            const Only& only, hipStream_t s) {
     xent_join_kernel<<<dim3((unsigned)((n + 15) / 16)), 256, 0, s>>>(top, total, parts, hit, target, n, classes,
-                                                                    ignore, loss, lse);
+                                                                    ignore, loss, lse, only);
     return hipGetLastError();
 }
 
@@ -116,19 +117,19 @@ hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n
 template <typename T>
 hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
                              const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
-                             int64_t ignore, T* out, int64_t ld, int tile, hipStream_t s) {
+                             int64_t ignore, T* out, int64_t ld, int tile, const Only& only, hipStream_t s) {
     const LogitGradEpi<T> e{bias ? bias + first : nullptr, target, lse, grad, up, out, ld, ignore, (int32_t)first,
                             (int32_t)classes};
     const Mat wp{(const T*)w.p + first * w.ld, w.ld};
-    return launch_gemm<T, true, true>(tile, wp, h, piece, n, k, 1, 0, e, s);
+    return launch_gemm<T, true, true>(tile, wp, h, piece, n, k, 1, 0, only, e, s);
 }
 
 #define MLRS_INST(T)                                                                                              \
     template hipError_t launch_xent_stats<T>(Mat, Mat, const T*, const int64_t*, int64_t, int64_t, int64_t, int,  \
-                                             float*, float*, float*, hipStream_t);                                \
+                                             float*, float*, float*, const Only&, hipStream_t);                   \
     template hipError_t launch_logit_grad<T>(Mat, Mat, const T*, const int64_t*, const float*, const float*,      \
                                              const float*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,  \
-                                             T*, int64_t, int, hipStream_t);
+                                             T*, int64_t, int, const Only&, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)

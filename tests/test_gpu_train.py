@@ -418,6 +418,86 @@ def test_the_same_call_gives_the_same_bits_on_any_stream(dtype):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+# f32 products large enough to run in three bf16 parts: whole and ragged sizes,
+# parts of the contraction (the gradients), rows aligned to four bytes alone
+@pytest.mark.parametrize("n,k,m,offset", [(4100, 1040, 4096, 0), (4100, 1031, 4100, 0), (4099, 1040, 4101, 1)])
+def test_large_f32_layers(n, k, m, offset):
+    check_linear(n, k, m, F32, "gelu", offset=offset, seed=n + k)
+
+
+@pytest.mark.parametrize("n,k,m,offset", [(2600, 2048, 2496, 0), (2050, 1031, 2101, 0), (2051, 1040, 2100, 1)])
+def test_large_f32_layer_gradients(n, k, m, offset):
+    check_grad(n, k, m, F32, "silu", offset=offset, seed=n + k)
+    check_grad(n, k, m, F32, "none", offset=offset, seed=n + k, bias=False)
+
+
+@pytest.mark.parametrize("n,v,k,offset", [(2048, 3080, 1024, 0), (2051, 3001, 1031, 1)])
+def test_large_f32_losses(n, v, k, offset):
+    check_xent(n, v, k, F32, offset=offset, seed=v)
+    check_xent(n, v, k, F32, offset=offset, seed=v, bias=False)
+
+
+def test_large_f32_products_keep_every_scale():
+    """Columns of very different size, whose weights make up for it: each term
+    has f32's relative accuracy, whatever the others of its row are."""
+    n, k, m = 4100, 1040, 4100
+    x, w = rand(1, n, k), rand(2, m, k)
+    size = 10.0 ** torch.linspace(-18, 18, k)
+    x, w = x * size, w / size
+    got = prims.linear(dev(x), dev(w))
+    ref.assert_near(got, ref.linear(x, w, None, "none", None)[0], "scaled columns")
+
+
+def test_large_f32_infinities_and_nan():
+    """Elements that have no bf16 parts: infinities, NaN, and floats that round
+    to an infinity in bf16, in either operand, give what f32 arithmetic gives."""
+    n, k, m = 4100, 1040, 4100
+    x, w = rand(1, n, k), rand(2, m, k, std=0.03)
+    big = torch.finfo(F32).max
+    for where in ("x", "w"):
+        xs, ws = x.clone(), w.clone()
+        a = xs if where == "x" else ws
+        a[5, 3], a[6, 4], a[7, 8] = float("inf"), float("nan"), big
+        got = prims.linear(dev(xs), dev(ws))
+        lines = got if where == "x" else got.t()
+        other = ws if where == "x" else xs
+        assert torch.equal(lines[5].cpu(), torch.where(other[:, 3] > 0, float("inf"), float("-inf")))
+        assert lines[6].isnan().all()
+        keep = [i for i in range(4100) if i not in (5, 6, 7)]
+        y, off = ref.linear(x, w, None, "none", None)[0]
+        y, off = (y, off) if where == "x" else (y.t(), off.t())
+        ref.assert_near(lines[keep], (y[keep], off[keep]), "rows beside them")
+        one = big * other[:, 8].double()
+        rest = (ref.U32 * 4 * one.abs() + 1e30)
+        fits = one.abs() < big * 0.99
+        assert bool(((lines[7].cpu().double() - one).abs() <= rest)[fits].all())
+    dy = rand(3, 2600, 2496)
+    x, w = rand(4, 2600, 2048), rand(5, 2496, 2048, std=0.03)
+    clean = prims.linear_grad(dev(dy), dev(x), dev(w))
+    x[9, 2] = float("inf")  # a column of dw; dx does not read x
+    dx, dw, db = prims.linear_grad(dev(dy), dev(x), dev(w))
+    assert torch.equal(db, clean[2])
+    assert (dx - clean[0]).abs().max() <= 1e-5 * clean[0].abs().max()
+    assert torch.equal(dw[:, 2].cpu(), torch.where(dy[9] > 0, float("inf"), float("-inf")))
+    keep = [i for i in range(2048) if i != 2]
+    assert (dw[:, keep] - clean[1][:, keep]).abs().max() <= 1e-5 * clean[1].abs().max()
+
+
+def test_large_f32_loss_of_a_row_with_nan():
+    n, v, k = 2051, 3001, 1031
+    h, w, t = rand(1, n, k), dev(rand(2, v, k, std=0.05)), dev(targets(3, n, v, 0.0))
+    g = torch.full((n,), 1.0 / n, device="cuda")
+    loss, lse = prims.softmax_xent(dev(h), w, t)
+    dh, _, _ = prims.softmax_xent_grad(dev(h), w, t, lse, g)
+    h[17, 4] = float("nan")
+    loss2, lse2 = prims.softmax_xent(dev(h), w, t)
+    dh2, dw2, _ = prims.softmax_xent_grad(dev(h), w, t, lse2, g)
+    keep = [i for i in range(n) if i != 17]
+    assert loss2[17].isnan() and dh2[17].isnan().all() and dw2.isnan().all()
+    assert (loss2 - loss)[keep].abs().max() <= 1e-5 * loss.abs().max()
+    assert (dh2 - dh)[keep].abs().max() <= 1e-5 * dh.abs().max()
+
+
 # ---- the optimizer ----
 
 SIZES = [1, 3, 255, 256, 257, 1000, 4096, 4097, 10007]
