@@ -100,22 +100,30 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
 // out.  `width`: how many of them one access may hold, 4, 2 or 1, by the
 // alignment of the rows (m is a multiple of 4).
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, int width) {
+__device__ __forceinline__ typename Elem<T>::Vec4 load_raw4(const T* row, int64_t m, int64_t end, int width) {
     typedef typename Elem<T>::Vec4 Vec4;
     typedef T Vec2 __attribute__((ext_vector_type(2)));
-    f32x4 v;
+    Vec4 v;
     if (width == 4 && m + 4 <= end) {
-        const Vec4 t = *reinterpret_cast<const Vec4*>(row + m);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+        v = *reinterpret_cast<const Vec4*>(row + m);
     } else if (width == 2 && m + 4 <= end) {
         const Vec2 lo = *reinterpret_cast<const Vec2*>(row + m), hi = *reinterpret_cast<const Vec2*>(row + m + 2);
-        v = f32x4{(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]};
+        v = Vec4{lo[0], lo[1], hi[0], hi[1]};
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = m + e < end ? (float)row[m + e] : 0.0f;
+        for (int e = 0; e < 4; ++e) v[e] = m + e < end ? row[m + e] : (T)0.0f;
     }
     return v;
+}
+
+template <typename V>
+__device__ __forceinline__ f32x4 widen(V v) {
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, int width) {
+    return widen(load_raw4(row, m, end, width));
 }
 
 template <typename T>
@@ -137,12 +145,15 @@ __device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, int width
     }
 }
 
-// Hands the wave's part with m < m_end to f(n, m, v) in groups: v[u] holds four
-// consecutive m of row n + u * step (which may be past the last row), the lanes
-// along the row, so that a row leaves in whole lines; a lane's m is the same in
-// every call.  Groups, so that what f loads for them is under way at once.  The
-// accumulators (a lane holds four m of one n, sixteen lanes run along n) are
-// turned through the wave's own part of LDS, 32 rows at a time.
+// Hands the wave's part with m < m_end to f(n, m, v, with) in groups: v[u] holds
+// four consecutive m of row n + u * step (which may be past the last row), the
+// lanes along the row, so that a row leaves in whole lines; a lane's m is the
+// same in every call.  `with` is what load(n, m, with) read for the same rows, a
+// group ahead: a group's loads are under way at once and while the group before
+// is worked on (a residual of 16384 x 4096 bf16 beside a product costs 75 us when
+// a group loads its own, 26 so).  The accumulators (a lane holds four m of one n,
+// sixteen lanes run along n) are turned through the wave's own part of LDS, 32
+// rows at a time.
 template <int MB>
 constexpr int row_step() {
     return 64 / (MB * 4);  // rows that the lanes cover together
@@ -157,16 +168,18 @@ template <int BYTES>
 __device__ __forceinline__ int turn_swizzle(int r) {
     return BYTES >= 256 ? r & 15 : BYTES == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
-template <int MB, int NB, typename F>
-__device__ __forceinline__ void for_rows(const f32x4 (&acc)[MB][NB], const Place& p, char* lds, int32_t m_end,
+template <typename With, int MB, int NB, typename L, typename F>
+__device__ __forceinline__ void for_rows(const f32x4 (&acc)[MB][NB], const Place& p, char* lds, int32_t m_end, L load,
                                          F f) {
     constexpr int kRow = MB * 64;       // bytes
     constexpr int kLanes = MB * 4;      // of a row
-    constexpr int kStep = row_step<MB>(), kGroup = row_group<MB>();
+    constexpr int kStep = row_step<MB>(), kGroup = row_group<MB>(), kRows = kStep * kGroup;
     char* mine = lds + p.wave * 32 * kRow;
     const int g = p.lane >> 4, r = p.lane & 15;
     const int c = p.lane % kLanes;
-    const int32_t m = p.m0 + 4 * c;
+    const int32_t m = p.m0 + 4 * c, n_first = p.n0 + p.lane / kLanes;
+    With with[kGroup], next[kGroup];
+    if (n_first < p.n && m < m_end) load(n_first, m, with);
     __syncthreads();  // the panels in LDS are no longer read
 #pragma unroll
     for (int j = 0; j < NB; j += 2) {
@@ -181,15 +194,18 @@ __device__ __forceinline__ void for_rows(const f32x4 (&acc)[MB][NB], const Place
         // the wave's LDS accesses are in order; nothing else touches `mine`
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-        for (int t = 0; t < 32; t += kStep * kGroup) {
+        for (int t = 0; t < 32; t += kRows) {
+            const int32_t n = n_first + j * 16 + t;
+            if (j * 16 + t + kRows < NB * 16 && n + kRows < p.n && m < m_end) load(n + kRows, m, next);
             f32x4 v[kGroup];
 #pragma unroll
             for (int u = 0; u < kGroup; ++u) {
                 const int row = t + u * kStep + p.lane / kLanes;
                 v[u] = *reinterpret_cast<const f32x4*>(mine + row * kRow + ((c ^ turn_swizzle<kRow>(row)) << 4));
             }
-            const int32_t n = p.n0 + j * 16 + t + p.lane / kLanes;
-            if (n < p.n && m < m_end) f(n, m, v);
+            if (n < p.n && m < m_end) f(n, m, v, with);
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) with[u] = next[u];
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -206,16 +222,19 @@ struct LinearEpi {
     int32_t act;
     int32_t width;  // of the rows' accesses
 
+    typedef typename Elem<T>::Vec4 Vec4;
     // rows n, n + step, ... of them those before n_end
     template <int N>
-    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, f32x4 bv,
-                                         f32x4 (&v)[N]) const {
-        f32x4 res[N] = {};
-        if (residual) {
+    __device__ __forceinline__ void load(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end,
+                                         Vec4 (&res)[N]) const {
+        if (!residual) return;
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) res[u] = load4(residual + (n + u * step) * ld, m, end, width);
-        }
+        for (int u = 0; u < N; ++u)
+            if (n + u * step < n_end) res[u] = load_raw4(residual + (n + u * step) * ld, m, end, width);
+    }
+    template <int N>
+    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, f32x4 bv,
+                                         f32x4 (&v)[N], const Vec4 (&res)[N]) const {
 #pragma unroll
         for (int u = 0; u < N; ++u) v[u] += bv;
         if (z) {
@@ -224,9 +243,20 @@ struct LinearEpi {
                 if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, width, v[u]);
         }
         activate_all(v, act);
+        if (residual) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) v[u] += widen(res[u]);
+        }
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, width, residual ? v[u] + res[u] : v[u]);
+            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, width, v[u]);
+    }
+    // one group of four elements
+    __device__ __forceinline__ void point(int64_t n, int64_t m, int64_t end, f32x4 v) const {
+        f32x4 one[1] = {v};
+        Vec4 res[1] = {};
+        load(n, 0, n + 1, m, end, res);
+        rows(n, 0, n + 1, m, end, bias_at(m, end), one, res);
     }
     __device__ __forceinline__ f32x4 bias_at(int64_t m, int64_t end) const {
         f32x4 bv = {};
@@ -236,9 +266,13 @@ struct LinearEpi {
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char* lds) const {
         const f32x4 bv = bias_at(p.m0 + 4 * (p.lane % (MB * 4)), p.m);
-        for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[row_group<MB>()]) {
-            rows(n, row_step<MB>(), p.n, m, p.m, bv, v);
-        });
+        constexpr int kGroup = row_group<MB>(), kStep = row_step<MB>();
+        for_rows<Vec4>(
+            acc, p, lds, p.m,
+            [&](int32_t n, int32_t m, Vec4 (&res)[kGroup]) { load(n, kStep, p.n, m, p.m, res); },
+            [&](int32_t n, int32_t m, f32x4 (&v)[kGroup], const Vec4 (&res)[kGroup]) {
+                rows(n, kStep, p.n, m, p.m, bv, v, res);
+            });
     }
 };
 
@@ -254,13 +288,17 @@ struct StoreEpi {
     int32_t width;  // of the rows' accesses
 
     template <int N>
-    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, int split,
-                                         f32x4 (&v)[N]) const {
-        if (add) {
-            f32x4 old[N] = {};
+    __device__ __forceinline__ void load(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end,
+                                         f32x4 (&old)[N]) const {
+        if (!add) return;
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, 4);
+        for (int u = 0; u < N; ++u)
+            if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, 4);
+    }
+    template <int N>
+    __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, int split,
+                                         f32x4 (&v)[N], const f32x4 (&old)[N]) const {
+        if (add) {
 #pragma unroll
             for (int u = 0; u < N; ++u) v[u] += old[u];
         }
@@ -276,11 +314,20 @@ struct StoreEpi {
                 if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, 4, v[u]);
         }
     }
+    __device__ __forceinline__ void point(int64_t n, int64_t m, int64_t end, f32x4 v) const {
+        f32x4 one[1] = {v}, old[1] = {};
+        load(n, 0, n + 1, m, end, old);
+        rows(n, 0, n + 1, m, end, 0, one, old);
+    }
     template <int WM, int WN, int MB, int NB>
     __device__ __forceinline__ void run(f32x4 (&acc)[MB][NB], const Place& p, char* lds) const {
-        for_rows(acc, p, lds, p.m, [&](int32_t n, int32_t m, f32x4 (&v)[row_group<MB>()]) {
-            rows(n, row_step<MB>(), p.n, m, p.m, p.split, v);
-        });
+        constexpr int kGroup = row_group<MB>(), kStep = row_step<MB>();
+        for_rows<f32x4>(
+            acc, p, lds, p.m,
+            [&](int32_t n, int32_t m, f32x4 (&old)[kGroup]) { load(n, kStep, p.n, m, p.m, old); },
+            [&](int32_t n, int32_t m, f32x4 (&v)[kGroup], const f32x4 (&old)[kGroup]) {
+                rows(n, kStep, p.n, m, p.m, p.split, v, old);
+            });
     }
 };
 

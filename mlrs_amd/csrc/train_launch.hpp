@@ -80,18 +80,12 @@ hipError_t launch_join(const float* part, int splits, int64_t m, int64_t n, cons
 template <typename T>
 struct LinearPoint {
     LinearEpi<T> e;
-    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
-        f32x4 g[1] = {v};
-        e.rows(n, 0, n + 1, c, m, e.bias_at(c, m), g);
-    }
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const { e.point(n, c, m, v); }
 };
 template <typename T>
 struct StorePoint {
     StoreEpi<T> e;
-    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const {
-        f32x4 g[1] = {v};
-        e.rows(n, 0, n + 1, c, m, 0, g);
-    }
+    __device__ __forceinline__ void operator()(int64_t n, int64_t c, int64_t m, f32x4 v) const { e.point(n, c, m, v); }
 };
 
 template <typename T>

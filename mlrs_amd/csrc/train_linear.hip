@@ -147,10 +147,7 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) v += sums[i][b][lane];
         const int32_t row = b * 16 + r, c = m0 + 4 * q;
-        if (row < n && c < m) {
-            f32x4 g[1] = {v};
-            epi.rows(row, 0, row + 1, c, m, epi.bias_at(c, m), g);
-        }
+        if (row < n && c < m) epi.point(row, c, m, v);
     }
 }
 
