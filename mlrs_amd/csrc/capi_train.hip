@@ -130,15 +130,15 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
         if (!grid_fits(m, n)) return grid_error(m, n);
         const hipStream_t s = (hipStream_t)stream;
         const LinearOut o{bias, residual, y, z, act};
-        if (n <= kFewRows) {
-            capi::Timed timed(s, "linear_few");
-            MLRS_TRY(launch_linear_few<T>(x, w, n, m, k, o, s));
-            return MLRS_OK;
-        }
         int cus = 0;
         rc = capi::cu_count(&cus);
         if (rc) return rc;
         Cut cut = choose_cut((int)sizeof(T), m, n, k, cus);
+        if (few_rows((int)sizeof(T), n, m, k, cut)) {
+            capi::Timed timed(s, "linear_few");
+            MLRS_TRY(launch_linear_few<T>(x, w, n, m, k, o, s));
+            return MLRS_OK;
+        }
         bool split = false;
         if constexpr (std::is_same<T, float>::value) {
             const Cut other = choose_cut_split(m, n, k, cus);

@@ -56,8 +56,9 @@ struct LinearOut {
 template <typename T>
 hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
                          float* part, const Only& only, hipStream_t s);
-// The same for a few rows, straight from the caller's unpacked operands.
-constexpr int kFewRows = 64;
+// The same for at most 32 rows, straight from the caller's unpacked operands, and
+// whether that is the faster way.
+bool few_rows(int elem_bytes, int64_t n, int64_t m, int64_t k, const Cut& cut);
 template <typename T>
 hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                              hipStream_t s);

@@ -164,9 +164,19 @@ hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64
                              hipStream_t s) {
     const LinearEpi<T> e = linear_epi<T>(o, m);
     const bool al = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && (k * (int64_t)sizeof(T)) % 16 == 0;
-    if (n <= 16) return al ? launch_few_nb<T, true, 1>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 1>(x, w, n, m, k, e, s);
-    if (n <= 32) return al ? launch_few_nb<T, true, 2>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 2>(x, w, n, m, k, e, s);
-    return al ? launch_few_nb<T, true, 4>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 4>(x, w, n, m, k, e, s);
+    if (n <= 16)
+        return al ? launch_few_nb<T, true, 1>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 1>(x, w, n, m, k, e, s);
+    return al ? launch_few_nb<T, true, 2>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 2>(x, w, n, m, k, e, s);
+}
+
+// Sixteen rows are bound by reading the weights (8192 x 8192 bf16: 29 us at one
+// row, 35 at sixteen, of a floor of 28; in 64 x 64 tiles 35 from the first row
+// on); thirty-two read twice as many fragments of x from the caches for them (47
+// us), and the tiles are as fast or faster where there are weights enough.
+bool few_rows(int elem_bytes, int64_t n, int64_t m, int64_t k, const Cut& cut) {
+    if (n <= 16) return true;
+    if (n > 32) return false;
+    return 4.0 + 1.6 * (double)elem_bytes * (double)m * (double)k / 4.75e6 < cut.us;
 }
 
 // ---------------------------------------------------------------------------
