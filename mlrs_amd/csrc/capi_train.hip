@@ -69,10 +69,13 @@ struct Op {
 // f32 kernels that take over where an element is not finite.
 double split_us(double elements) { return elements * 10.0 / 5.5e6 + 9.0; }
 
-// A mark that no earlier call has left behind.
+// A mark that no earlier call has left behind, and that what else lies in the
+// workspace (indices, counts) does not look like; were it there all the same, the
+// f32 kernels would compute the call.
 uint32_t next_mark() {
     static uint32_t mark = 0;  // under the call lock
-    return ++mark;
+    mark += 0x9E3779B1u;
+    return mark;
 }
 
 // The split kernels of a call and the f32 ones that stand in for them.

@@ -135,10 +135,11 @@ __device__ __forceinline__ int r_swizzle(int k) {
 // and the descriptor are uniform over the wave.  Counted by vmcnt, which the
 // caller waits for: written as an instruction because the compiler would wait
 // for every copy under way at each transposing LDS read, not knowing that they
-// touch other slots.  It has no result register.
+// touch other slots.  It has no result register; the wait state between writing
+// M0 and the copy is written too, as the compiler does not look into the block.
 __device__ __forceinline__ void copy_to_lds(u32x4 rsrc, char* lds, uint32_t offset) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"((uint32_t)(uintptr_t)(MLRS_LDS void*)lds), "v"(offset), "s"(rsrc)
                  : "memory");
