@@ -126,6 +126,27 @@ def test_linear_tail_of_k_reads_no_neighbours(dtype):
     ref.assert_near(got, ref.linear(x[::2], w[::2], None, "none", None)[0], "rows between NaN rows")
 
 
+def test_layer_of_more_elements_than_32_bits_count():
+    """70,000 x 65,536 outputs: the last rows and columns are where they belong."""
+    n, k, m = 70000, 32, 65536
+    x, w = rand(1, n, k, dtype=BF16), rand(2, m, k, dtype=BF16, std=0.2)
+    xd, wd = dev(x), dev(w)
+    y = prims.linear(xd, wd, activation="relu")
+    for r in (slice(0, 3), slice(32767, 32770), slice(65534, 65538), slice(n - 3, n)):
+        ref.assert_near(y[r], ref.linear(x[r], w, None, "relu", None)[0], "rows %s" % r)
+    dx, dw, db = prims.linear_grad(y, xd, wd)
+    ones = torch.ones(n, dtype=torch.float64, device="cuda")
+    for r in (slice(0, 2), slice(65535, 65537), slice(n - 2, n)):
+        want = ref.linear_grad(y[r].cpu(), x[r], w, None, "none", BF16)
+        ref.assert_near(dx[r], want[0], "dx rows %s" % r)
+    for c in (slice(0, 64), slice(m - 64, m)):
+        part = y[:, c].double()
+        size = part.t().abs() @ xd.double().abs()
+        room = (ref.dot_bound(n) + ref.UNIT[BF16]) * size
+        assert bool(((dw[c].double() - part.t() @ xd.double()).abs() <= room).all())
+        assert bool(((db[c].double() - ones @ part).abs() <= (ref.dot_bound(n) + ref.UNIT[BF16]) * (ones @ part.abs())).all())
+
+
 def check_grad(n, k, m, dtype, act, offset=0, seed=0, bias=True):
     x, w = rand(seed, n, k, dtype=dtype), rand(seed + 1, m, k, dtype=dtype, std=k ** -0.5)
     dy = rand(seed + 2, n, m, dtype=dtype, std=0.1)
@@ -598,6 +619,27 @@ def test_adamw_8_bits_follows_its_definition(offset):
         vm = ref.code_values(d[2] & 127, 3)
         assert np.array_equal(m, np.where(d[2] > 127, -vm, vm) * np.repeat(d[4], 256)[:n])
         assert np.array_equal(r, ref.code_values(d[3], 4) * np.repeat(d[5], 256)[:n])
+
+
+def test_adamw_8_bits_past_32_bits():
+    """A tensor of 2^32 + 5000 elements: its last blocks, whose elements' numbers
+    have a thirty-third bit."""
+    n, tail = 2 ** 32 + 5000, 5000 + 512
+    first = n - tail
+    first -= first % 256
+    d = opt8_inputs([n - first], 11)[0]
+    t = [torch.zeros(n, device="cuda"), torch.zeros(n, dtype=BF16, device="cuda"),
+         torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda"),
+         torch.zeros(-(-n // 256), device="cuda"), torch.zeros(-(-n // 256), device="cuda")]
+    for i, x in enumerate(d):
+        t[i][-len(x):] = dev(torch.from_numpy(x))
+    g = t[1][first:].float().cpu().numpy()
+    prims.adamw_step([t[0]], [t[1]], [t[2]], [t[3]], step=4, lr=1e-3, avg_scales=[t[4]], avg_sq_scales=[t[5]],
+                     weight_decay=0.1, seed=3)
+    want = ref.adamw8(d[0], g, *d[2:], 0, 4, 1e-3, (0.9, 0.999), 1e-8, 0.1, 3, first=first)
+    for i, w in zip((0, 2, 3, 4, 5), want):
+        assert np.array_equal(t[i][-len(w):].cpu().numpy(), w)
+    assert not t[2][:first].any() and not t[0][:first].any()
 
 
 def test_adamw_8_bits_half_parameters():

@@ -174,9 +174,10 @@ def codes_of(y, r16, mant):
     return np.minimum(np.where(normal, big, small), (16 << mant) - 1)
 
 
-def adamw8(p, g, codes_m, codes_r, scale_m, scale_r, ordinal, step, lr, betas, eps, decay, seed, scale=1.0):
-    """New (p, codes_m, codes_r, scale_m, scale_r) of one tensor by the float32
-    steps of the definition, each rounded by itself."""
+def adamw8(p, g, codes_m, codes_r, scale_m, scale_r, ordinal, step, lr, betas, eps, decay, seed, scale=1.0, first=0):
+    """New (p, codes_m, codes_r, scale_m, scale_r) of one tensor, or of its
+    elements from `first` (a multiple of 256) on, by the float32 steps of the
+    definition, each rounded by itself."""
     f = np.float32
     n, block = len(p), 256
     sm, sr = (np.repeat(s, block)[:n] for s in (scale_m, scale_r))
@@ -195,7 +196,9 @@ def adamw8(p, g, codes_m, codes_r, scale_m, scale_r, ordinal, step, lr, betas, e
     new_sm = np.pad(np.abs(m), (0, pad)).reshape(-1, block).max(1) / f(1.875)
     new_sr = np.pad(r, (0, pad)).reshape(-1, block).max(1) / f(1.9375)
     key = mix32((seed + ordinal * 0x9E3779B1) & 0xFFFFFFFF)
-    u = mix32(np.arange(n, dtype=np.uint64) ^ key)
+    index = np.arange(first, first + n, dtype=np.uint64)
+    low, high = index & np.uint64(0xFFFFFFFF), index >> np.uint64(32)
+    u = mix32(((low ^ key) + high * np.uint64(0x9E3779B1)) & np.uint64(0xFFFFFFFF))
     sm, sr = (np.repeat(s, block)[:n] for s in (new_sm, new_sr))
     with np.errstate(divide="ignore", invalid="ignore"):
         ym = np.where(sm > 0, np.abs(m) / sm, f(0))
