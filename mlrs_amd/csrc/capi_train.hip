@@ -87,6 +87,7 @@ struct Sides {
 };
 
 constexpr Cut kPlainCut{0, 1, 0, 0.0};  // of the kernels that stand in
+constexpr PairCut kPlainPair{kPlainCut, kPlainCut, true};
 
 // Sizes that both layers of operators share: a (n x d) and w (m x d).
 template <typename T>
@@ -222,15 +223,19 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         const bool products = (dx && n > 0) || dw;
         // dy itself serves as dz where there is no slope and its rows can be read
         const bool make_dz = products && n > 0 && (act != MLRS_ACT_NONE || !readable(dy, m));
-        Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
+        const bool want_x = dx && n > 0;
+        PairCut cut = choose_pair((int)sizeof(T), k, n, m, k, m, n, cus);
+        Cut sx{}, sw{};  // of those that run in parts
         bool split_x = false, split_w = false;
         if constexpr (std::is_same<T, float>::value) {
-            const Cut ox = choose_cut_split(k, n, m, cus), ow = choose_cut_split(k, m, n, cus);
-            split_x = dx && n > 0 && ox.us + split_us((double)(n + k) * (double)m) < cx.us;
-            split_w = dw && n > 0 && ow.us + split_us((double)(m + k) * (double)n) < cw.us;
-            if (split_x) cx = ox;
-            if (split_w) cw = ow;
+            const Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
+            sx = choose_cut_split(k, n, m, cus);
+            sw = choose_cut_split(k, m, n, cus);
+            split_x = want_x && sx.us + split_us((double)(n + k) * (double)m) < cx.us;
+            split_w = dw && n > 0 && sw.us + split_us((double)(m + k) * (double)n) < cw.us;
+            if (split_x || split_w) cut = PairCut{cx, cw, false};
         }
+        if (!want_x || !dw) cut = PairCut{choose_cut((int)sizeof(T), k, n, m, cus), choose_cut((int)sizeof(T), k, m, n, cus), false};
         const int parts = column_parts(n, m, cus);
         char *w_r = nullptr, *dz_k = nullptr, *x_r = nullptr, *dz_r = nullptr;
         Sides sides;
@@ -243,7 +248,8 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
             if (dx) wo.plan(sc);
             if (make_dz) dz = sc.take<T>((size_t)(n * padded<T>(m)));
             if (db) sums = sc.take<float>((size_t)parts * (size_t)m);
-            part = sc.take<float>(std::max(dx ? cx.part_bytes(k, n) : 0, dw ? cw.part_bytes(k, m) : 0) / 4);
+            part = sc.take<float>(std::max(cut.part_bytes(k, n, k, m),
+                                           std::max(split_x ? sx.part_bytes(k, n) : 0, split_w ? sw.part_bytes(k, m) : 0)) / 4);
             if (split_x) {
                 w_r = sc.take<char>(split_bytes(m, k));
                 dz_k = sc.take<char>(split_bytes(n, m));
@@ -260,9 +266,9 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
                 sc.used = 0;
             }
         }
+        const ColumnSums<T> col{db, sums, parts, nullptr};
         if (make_dz || db)
-            MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, padded<T>(m),
-                                        ColumnSums<T>{db, sums, parts, nullptr}, s));
+            MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, padded<T>(m), col, s));
         const Mat dzm = make_dz ? Mat{dz, padded<T>(m)} : Mat{dy, m};
         PackJob xj = xo.job(), wj = wo.job();
         if (!dw || split_w) xj.rows = 0;
@@ -270,6 +276,7 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         MLRS_TRY(launch_pack<T>(xj, wj, Only{}, s));
         capi::Timed timed(s, "linear_grad");
         const StoreTo to_x{dx, k, nullptr, nullptr, 0, nullptr}, to_w{dw, k, nullptr, nullptr, 0, nullptr};
+        Product px{wo.mat(), dzm, k, n, m, to_x}, pw{xo.mat(), dzm, k, m, n, to_w};
         if constexpr (std::is_same<T, float>::value) {
             if (split_x || split_w) {
                 sides.mark = next_mark();
@@ -278,13 +285,13 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
                     MLRS_TRY(launch_pack_split(split_job(w, k, m, k, w_r, true),
                                                split_job(z32, dzm.ld, n, m, dz_k, false), sides.flag, sides.mark, s));
                     MLRS_TRY(launch_product_split(split_mat(w_r, k, true), split_mat(dz_k, m, false), true, k, n, m,
-                                                  to_x, cx, part, sides.split(), s));
+                                                  to_x, sx, part, sides.split(), s));
                 }
                 if (split_w) {
                     MLRS_TRY(launch_pack_split(split_job(x, k, n, k, x_r, true),
                                                split_job(z32, dzm.ld, n, m, dz_r, true), sides.flag, sides.mark, s));
                     MLRS_TRY(launch_product_split(split_mat(x_r, k, true), split_mat(dz_r, m, true), false, k, m, n,
-                                                  to_w, cw, part, sides.split(), s));
+                                                  to_w, sw, part, sides.split(), s));
                 }
                 // what dw's packing marked is marked for dx as well, whose
                 // product the f32 kernel then computes again, to the same values
@@ -292,14 +299,16 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
                 if (!split_w) xp.rows = 0;
                 if (!split_x) wp.rows = 0;
                 MLRS_TRY(launch_pack<T>(xp, wp, sides.plain(), s));
-                if (split_x)
-                    MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, to_x, kPlainCut, nullptr, sides.plain(), s));
-                if (split_w)
-                    MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, to_w, kPlainCut, nullptr, sides.plain(), s));
+                MLRS_TRY(launch_products<T>(split_x ? px : Product{}, split_w ? pw : Product{}, kPlainPair, nullptr,
+                                            ColumnSums<T>{}, 0, sides.plain(), s));
             }
         }
-        if (dx && n > 0 && !split_x) MLRS_TRY(launch_product<T>(wo.mat(), dzm, true, k, n, m, to_x, cx, part, Only{}, s));
-        if (dw && !split_w) MLRS_TRY(launch_product<T>(xo.mat(), dzm, false, k, m, n, to_w, cw, part, Only{}, s));
+        if (!want_x || split_x) px.m = 0;
+        if (!dw || split_w) pw.m = 0;
+        if (px.m || pw.m)
+            MLRS_TRY(launch_products<T>(px, pw, cut, part, col, m, Only{}, s));
+        else
+            MLRS_TRY(launch_sum_parts<T>(col, m, s));
         return MLRS_OK;
     });
 }
@@ -424,8 +433,9 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             // no rows: the products over them are empty sums
             if (dw) {
                 const StoreTo o{dw, d, nullptr, nullptr, 0, nullptr};
-                MLRS_TRY(launch_product<T>(Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, false, d, v, 0, o,
-                                           Cut{2, 1, 0, 0.0}, nullptr, Only{}, s));
+                const Product p{Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, d, v, 0, o};
+                const Cut c{2, 1, 0, 0.0};
+                MLRS_TRY(launch_products<T>(Product{}, p, PairCut{c, c, false}, nullptr, ColumnSums<T>{}, 0, Only{}, s));
             }
             if (db)
                 MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
@@ -440,20 +450,23 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
         const int64_t ld = padded<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;
         const bool scaled = sizeof(T) == 2 && std::is_same<T, _Float16>::value;
         const int64_t most = std::min(piece, v);  // classes of the largest piece
-        const Cut ch = choose_cut((int)sizeof(T), d, n, most, cus), cw = choose_cut((int)sizeof(T), d, most, n, cus);
+        PairCut cut = choose_pair((int)sizeof(T), d, n, most, d, most, n, cus);
         // f32: which of a piece's three products run in parts; the gradient of the
         // logits is packed for each of the two that take it
         Cut sh{}, sw{};
         bool split_z = false, split_h = false, split_w = false;
         if constexpr (std::is_same<T, float>::value) {
             const double nv = (double)n * (double)most, nd = (double)n * (double)d, vd = (double)most * (double)d;
+            const Cut ch = choose_cut((int)sizeof(T), d, n, most, cus), cw = choose_cut((int)sizeof(T), d, most, n, cus);
             sh = choose_cut_split(d, n, most, cus);
             sw = choose_cut_split(d, most, n, cus);
             split_z = choose_cut_split(most, n, d, cus, 1).us + split_us(nd + vd) <
                       choose_cut((int)sizeof(T), most, n, d, cus, 1).us;
             split_h = dh && sh.us + split_us(nv + vd) < ch.us;
             split_w = dw && sw.us + split_us(nv + nd) < cw.us;
+            if (split_h || split_w) cut = PairCut{ch, cw, false};
         }
+        if (!dh || !dw) cut = PairCut{choose_cut((int)sizeof(T), d, n, most, cus), choose_cut((int)sizeof(T), d, most, n, cus), false};
         const bool split = split_z || split_h || split_w;
         const int parts = column_parts(n, most, cus);
         Op<T> ho(h, n, d), wo(w, v, d);
@@ -469,7 +482,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             if (dh && pieces > 1) acc = sc.take<float>((size_t)(n * dh_ld));
             if (db) sums = sc.take<float>((size_t)parts * (size_t)most);
             if (scaled) up = sc.take<float>(2);
-            size_t bytes = std::max(dh ? ch.part_bytes(d, n) : 0, dw ? cw.part_bytes(d, most) : 0);
+            size_t bytes = cut.part_bytes(d, n, d, most);
             if (split_h) bytes = std::max(bytes, sh.part_bytes(d, n));
             if (split_w) bytes = std::max(bytes, sw.part_bytes(d, most));
             part = sc.take<float>(bytes / 4);
@@ -526,7 +539,8 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
                                           split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile,
                                           split_z ? plain : Only{}, s));
-            if (db) MLRS_TRY(launch_column_sums<T>(dzm, n, vp, ColumnSums<T>{db + v0, sums, parts, down}, s));
+            const ColumnSums<T> col{db ? db + v0 : nullptr, sums, parts, down};
+            if (db) MLRS_TRY(launch_column_sums<T>(dzm, n, vp, col, s));
             const StoreTo to_w{dw ? dw + v0 * d : nullptr, d, nullptr, nullptr, 0, down};
             StoreTo to_h{};
             to_h.ld = d;
@@ -553,16 +567,18 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                     MLRS_TRY(launch_product_split(split_mat(w_r, d, true), split_mat(dz_k, vp, false), true, d, n, vp,
                                                   to_h, c, part, sides.split(), s));
             }
-            if (dw)
-                MLRS_TRY(launch_product<T>(hm, dzm, false, d, vp, n, to_w, split_w ? kPlainCut : cw, part,
-                                           split_w ? plain : Only{}, s));
-            if (dh) {
-                Cut c = split_h ? kPlainCut : ch;
-                if (!split_h && vp < most) c = choose_cut((int)sizeof(T), d, n, vp, cus);
-                if (c.part_bytes(d, n) > ch.part_bytes(d, n)) c = Cut{c.tile, 1, 0, 0.0};
-                MLRS_TRY(launch_product<T>(Mat{(const T*)wm.p + v0 * wm.ld, wm.ld}, dzm, true, d, n, vp, to_h, c, part,
-                                           split_h ? plain : Only{}, s));
-            }
+            Product ph{Mat{(const T*)wm.p + v0 * wm.ld, wm.ld}, dzm, d, n, vp, to_h}, pw{hm, dzm, d, vp, n, to_w};
+            if (split_h || split_w)
+                MLRS_TRY(launch_products<T>(split_h ? ph : Product{}, split_w ? pw : Product{}, kPlainPair, nullptr,
+                                            ColumnSums<T>{}, 0, plain, s));
+            if (!dh || split_h) ph.m = 0;
+            if (!dw || split_w) pw.m = 0;
+            PairCut c = cut;  // a last piece's contraction may have fewer parts
+            if (c.x.splits > 1) c.x.splits = (int)((vp + c.x.k_split - 1) / c.x.k_split);
+            if (ph.m || pw.m)
+                MLRS_TRY(launch_products<T>(ph, pw, c, part, col, vp, Only{}, s));
+            else
+                MLRS_TRY(launch_sum_parts<T>(col, vp, s));
         }
         return MLRS_OK;
     });

@@ -297,11 +297,11 @@ __device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
 struct TilePlace {
     int32_t tm, tn, split;
 };
-__device__ __forceinline__ TilePlace tile_place(const GemmArgs& g) {
+__device__ __forceinline__ TilePlace tile_place(const GemmArgs& g, int32_t wg) {
     const int32_t tiles = g.tiles_m * g.tiles_n;
     TilePlace p;
-    p.split = blockIdx.x / tiles;
-    const int32_t t = xcd_tile(blockIdx.x - p.split * tiles, tiles);
+    p.split = wg / tiles;
+    const int32_t t = xcd_tile(wg - p.split * tiles, tiles);
     const int32_t per_band = g.band * g.tiles_n;
     const int32_t bnd = t / per_band, in = t - bnd * per_band;
     const int32_t width = g.tiles_m - bnd * g.band < g.band ? g.tiles_m - bnd * g.band : g.band;
@@ -323,7 +323,7 @@ __device__ __forceinline__ void wait_copies() {
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// The kernel of every product.  8192 x 8192 x 8192 in bf16: 729 us forwards (K x
+// A workgroup of every product.  8192 x 8192 x 8192 in bf16: 729 us forwards (K x
 // K), 764 for dx (R x K), 740 for dw (R x R), 1508, 1439 and 1486 TFLOP/s, where
 // the matrix instructions alone would do 2080 at the clock that the chip's power
 // allows; with the copies left out it was 1576 in 32 x 32 blocks.  In 256 x 256
@@ -331,24 +331,31 @@ __device__ __forceinline__ void wait_copies() {
 // cycles of matrix work a staged width, the LDS being busy for as long; one
 // workgroup fills a CU.  Four waves of 128 x 128 read a third less and are no
 // faster (756 us), as a wave alone on its SIMD waits for itself.
+// buf: gemm_lds bytes, the kernel's only LDS.
+template <int MB, int NB>
+__host__ __device__ constexpr int gemm_slots() {
+    return MB * NB == 4 ? 6 : 5;
+}
+template <int WM, int MB, int NB>
+__host__ __device__ constexpr int gemm_lds() {
+    return gemm_slots<MB, NB>() * WM * MB * 16 * kStageBytes;
+}
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
-__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
-                                                                                                       Epi epi) {
+__device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi, int32_t wg, char* buf) {
     constexpr int BM = WM * MB * 16, BN = WN * NB * 16, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
     constexpr int BK = stage_elems<T>();
     static_assert(kA == kB, "panels of either operand take the same slots");
     constexpr bool kSmall = MB * NB == 4;
     constexpr int kAhead = 3;  // staged widths under way, of a small tile
-    constexpr int kSlots = kSmall ? 2 * kAhead : 5;
-    __shared__ __attribute__((aligned(1024))) char buf[kSlots * kA];
-    if (skipped(g)) return;
+    constexpr int kSlots = gemm_slots<MB, NB>();
+    static_assert(!kSmall || kSlots == 2 * kAhead, "two panels a width");
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    const TilePlace t = tile_place(g);
+    const TilePlace t = tile_place(g, wg);
     const int32_t m0 = t.tm * BM, n0 = t.tn * BN;
     const int32_t k_lo = t.split * g.k_split;
     const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;
@@ -517,6 +524,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g,
     p.wm = wm;
     p.wn = wn;
     epi.template run<WM, WN, MB, NB>(acc, p, buf);
+}
+
+// A product of operands in K layout.
+template <typename T, int WM, int WN, int MB, int NB, typename Epi>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g, Epi epi) {
+    __shared__ __attribute__((aligned(1024))) char buf[gemm_lds<WM, MB, NB>()];
+    if (skipped(g)) return;
+    gemm_workgroup<T, true, true, WM, WN, MB, NB, Epi>(g, epi, blockIdx.x, buf);
 }
 
 }  // namespace train

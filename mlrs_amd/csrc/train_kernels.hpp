@@ -74,13 +74,15 @@ struct ColumnSums {
 };
 int column_parts(int64_t n, int64_t m, int cus);
 // dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and its
-// column sums.
+// column sums: done with one part, else for launch_products or launch_sum_parts.
 template <typename T>
 hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
                            const ColumnSums<T>& to, hipStream_t s);
-// The column sums of a packed matrix.
+// The same of a packed matrix's column sums alone.
 template <typename T>
 hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& to, hipStream_t s);
+template <typename T>
+hipError_t launch_sum_parts(const ColumnSums<T>& to, int64_t m, hipStream_t s);
 
 // Stores of a product P (m x n, element (i, j) at out[j * ld + i]): a (rows m)
 // with its row index contiguous, b (rows n) with k contiguous (b_k) or not.
@@ -92,9 +94,25 @@ struct StoreTo {
     int64_t acc_ld;      // a multiple of 4
     const float* alpha;  // device scalar; may be null
 };
+// The two products of a gradient: x (dz w: b with k contiguous) and w (dz^T x: b
+// with its row index contiguous); one of m = 0 is not wanted.
+struct Product {
+    Mat a, b;
+    int64_t m, n, k;
+    StoreTo to;
+};
+struct PairCut {
+    Cut x, w;
+    bool together;  // in one grid
+    size_t part_bytes(int64_t xm, int64_t xn, int64_t wm, int64_t wn) const {
+        return x.part_bytes(xm, xn) + w.part_bytes(wm, wn);
+    }
+};
+PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus);
+// sums: of `columns` columns, still to be joined (parts < 2: none).
 template <typename T>
-hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
-                          float* part, const Only& only, hipStream_t s);
+hipError_t launch_products(const Product& x, const Product& w, const PairCut& cut, float* part,
+                           const ColumnSums<T>& sums, int64_t columns, const Only& only, hipStream_t s);
 
 // Softmax cross entropy: the statistics of every wave's classes, joined into
 // lse and loss; the scale of a half-precision gradient; a piece's gradient.

@@ -14,11 +14,10 @@ constexpr int kTileRows[3] = {256, 128, 64};
 // XCD (32 CUs) then share about as many panels of either operand.
 inline int32_t band_of(int tile, int32_t tiles_m) { return std::min<int32_t>(tiles_m, tile == 0 ? 4 : 8); }
 
-template <typename T, bool AKC, bool BKC, typename Epi>
-hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, int splits, int32_t k_split,
-                       const Only& only, const Epi& epi, hipStream_t s) {
+// The arguments of a product in tiles of `rows` on a side, and its workgroups.
+inline int64_t gemm_args(GemmArgs& g, int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, int splits,
+                         int32_t k_split, const Only& only) {
     const int rows = kTileRows[tile];
-    GemmArgs g;
     g.a = Operand{a.p, a.ld};
     g.b = Operand{b.p, b.ld};
     g.m = (int32_t)m;
@@ -32,15 +31,22 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
     g.flag = only.flag;
     g.mark = only.mark;
     g.wanted = only.wanted;
-    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * splits;
+    return (int64_t)g.tiles_m * g.tiles_n * splits;
+}
+
+template <typename T, typename Epi>
+hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, int splits, int32_t k_split,
+                       const Only& only, const Epi& epi, hipStream_t s) {
+    GemmArgs g;
+    const int64_t blocks = gemm_args(g, tile, a, b, m, n, k, splits, k_split, only);
     if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
     const dim3 grid((unsigned)blocks);
     if (tile == 0)
-        gemm_kernel<T, AKC, BKC, 2, 4, 8, 4, Epi><<<grid, 512, 0, s>>>(g, epi);
+        gemm_kernel<T, 2, 4, 8, 4, Epi><<<grid, 512, 0, s>>>(g, epi);
     else if (tile == 1)
-        gemm_kernel<T, AKC, BKC, 2, 2, 4, 4, Epi><<<grid, 256, 0, s>>>(g, epi);
+        gemm_kernel<T, 2, 2, 4, 4, Epi><<<grid, 256, 0, s>>>(g, epi);
     else
-        gemm_kernel<T, AKC, BKC, 2, 2, 2, 2, Epi><<<grid, 256, 0, s>>>(g, epi);
+        gemm_kernel<T, 2, 2, 2, 2, Epi><<<grid, 256, 0, s>>>(g, epi);
     return hipGetLastError();
 }
 
@@ -51,30 +57,44 @@ inline int row_width(const void* p, int64_t ld) {
     return (uintptr_t)p % (2 * sizeof(T)) == 0 && ld % 2 == 0 ? 2 : 1;
 }
 
-// The parts of a split contraction, joined in order.
+// The parts of split contractions, joined in order: of one product or of two.
 template <typename Point>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, int splits, int64_t stride,
-                                                   int64_t part_ld, int64_t m, int64_t n, Point point, Only only) {
+struct JoinJob {
+    const float* part;
+    int32_t splits;  // none: nothing to do
+    int64_t m, n;
+    Point point;
+    __host__ __device__ int64_t quads() const { return (m + 3) / 4; }  // of a row
+    __host__ __device__ int64_t total() const { return splits ? quads() * n : 0; }
+};
+
+template <typename Point>
+__global__ __launch_bounds__(256) void join_kernel(JoinJob<Point> x, JoinJob<Point> w, Only only) {
     if (skipped(only.flag, only.mark, only.wanted)) return;
-    const int64_t quads = part_ld / 4, total = quads * n;
+    const int64_t first = x.total(), total = first + w.total();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / quads, c = (i - r * quads) * 4;
-        const float* at = part + r * part_ld + c;
-        f32x4 v = *reinterpret_cast<const f32x4*>(at);
-        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(at + s * stride);
-        point(r, c, m, v);
+        const JoinJob<Point>& j = i < first ? x : w;
+        const int64_t at = i < first ? i : i - first, quads = j.quads();
+        const int64_t r = at / quads, c = (at - r * quads) * 4;
+        const float* from = j.part + at * 4;
+        f32x4 v = *reinterpret_cast<const f32x4*>(from);
+        for (int s = 1; s < j.splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * quads * 4 * j.n);
+        j.point(r, c, j.m, v);
     }
 }
 
 template <typename Point>
+hipError_t launch_join(const JoinJob<Point>& x, const JoinJob<Point>& w, const Only& only, hipStream_t s) {
+    const int64_t total = x.total() + w.total();
+    if (total == 0) return hipSuccess;
+    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
+    join_kernel<Point><<<dim3((unsigned)blocks), 256, 0, s>>>(x, w, only);
+    return hipGetLastError();
+}
+template <typename Point>
 hipError_t launch_join(const float* part, int splits, int64_t m, int64_t n, const Point& point, const Only& only,
                        hipStream_t s) {
-    const int64_t part_ld = (m + 3) & ~(int64_t)3;
-    const int64_t total = part_ld / 4 * n;
-    const int64_t blocks = std::min<int64_t>((total + 255) / 256, 16384);
-    join_kernel<Point><<<dim3((unsigned)blocks), 256, 0, s>>>(part, splits, n * part_ld, part_ld, m, n, point,
-                                                               only);
-    return hipGetLastError();
+    return launch_join(JoinJob<Point>{part, splits, m, n, point}, JoinJob<Point>{nullptr, 0, 0, 0, point}, only, s);
 }
 
 template <typename T>

@@ -18,28 +18,100 @@ namespace train {
 // tiles are bound by the matrix cores, and only the count matters.  Measured at
 // 2048 x 1024 x 4096 in bf16: 32.1 us in 256 x 256 tiles, 24.8 in 128 x 128,
 // 33.8 in 64 x 64; at 16384 x 4096 x 4096: 433, 513, -.
+static const double kStage16[3][3] = {{1.6}, {0.62, 0.98}, {0.27, 0.5, 0.75}};
+static const double kStage32[3][3] = {{7.4}, {2.0, 4.0}, {0.68, 1.05, 1.55}};
+static const double kRoundUs[3] = {6.0, 4.5, 4.0};
+static const int kResident[3] = {1, 2, 3};
+
+// Joining parts: a launch, and their bytes twice.
+static double join_us(int64_t elements) { return elements ? 10.0 + (double)elements * 8.0 / 4.5e6 : 0.0; }
+
 Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits) {
-    static const double stage16[3][3] = {{1.6}, {0.62, 0.98}, {0.27, 0.5, 0.75}};
-    static const double stage32[3][3] = {{7.4}, {2.0, 4.0}, {0.68, 1.05, 1.55}};
-    static const double round_us[3] = {6.0, 4.5, 4.0};
-    static const int resident[3] = {1, 2, 3};
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
     Cut best{0, 1, 0, 1e300};
     for (int t = 0; t < 3; ++t) {
-        const double* stage = elem_bytes == 2 ? stage16[t] : stage32[t];
+        const double* stage = elem_bytes == 2 ? kStage16[t] : kStage32[t];
         const int rows = kTileRows[t];
         const int64_t tiles = ((m + rows - 1) / rows) * ((n + rows - 1) / rows);
         for (int64_t sp = 1; sp <= max_splits && sp <= stages; sp = sp < 4 ? sp + 1 : sp * 2) {
             const int64_t each = (stages + sp - 1) / sp;
             if (sp > 1 && (each < 3 || (sp - 1) * each >= stages)) continue;
             const int64_t on_cu = (tiles * sp + cus - 1) / cus;  // tiles that the busiest CU computes
-            const int64_t rounds = on_cu / resident[t], rest = on_cu % resident[t];
-            double cost = (double)rounds * ((double)each * stage[resident[t] - 1] + round_us[t]);
-            if (rest) cost += (double)each * stage[rest - 1] + round_us[t];
-            // joining the parts: a launch, and their bytes twice
-            if (sp > 1) cost += 7.0 + (double)sp * (double)m * (double)n * 8.0 / 4.5e6;
+            const int64_t rounds = on_cu / kResident[t], rest = on_cu % kResident[t];
+            double cost = (double)rounds * ((double)each * stage[kResident[t] - 1] + kRoundUs[t]);
+            if (rest) cost += (double)each * stage[rest - 1] + kRoundUs[t];
+            if (sp > 1) cost += join_us(sp * m * n);
             if (cost < best.us) best = Cut{t, (int)sp, (int32_t)(each * per), cost};
+        }
+    }
+    return best;
+}
+
+// When the last of two kinds of workgroups is done, `first` of which go to `slots`
+// places before `then` of the other: places that fall free together are taken
+// together.
+static double last_done(int64_t first, double first_us, int64_t then, double then_us, int64_t slots) {
+    struct Group {
+        double at;
+        int64_t size;
+    } g[3] = {{(double)(first / slots) * first_us, slots - first % slots},
+              {(double)(first / slots + 1) * first_us, first % slots},
+              {0.0, 0}};
+    const int64_t rounds = std::max<int64_t>(0, then / slots - 8);  // of many, all but a few at once
+    then -= rounds * slots;
+    for (Group& o : g) o.at += (double)rounds * then_us;
+    while (then > 0) {
+        Group& o = g[1].size && g[1].at < g[0].at ? g[1] : g[0];
+        const int64_t n = std::min(then, o.size);
+        if (n < o.size) g[2] = Group{o.at + then_us, n};
+        else o.at += then_us;
+        then -= n;
+    }
+    double end = 0.0;
+    for (const Group& o : g)
+        if (o.size) end = std::max(end, o.at);
+    return end;
+}
+
+// Two products in one grid: what the places of a full CU need for both, and of
+// what its last workgroups need beyond that a part, as a CU that is left to few of
+// them is faster for each; no less than the longest workgroup alone.  Over thirty
+// layers in bf16 and f32 of 64 to 30,000 rows and 96 to 10,000 columns the choice
+// was 2% slower than the best of some sixty cuts each, 13% at most, and in bf16 a
+// fifth to a third faster than the best two launches below 100 us: 4099 x 2056 by
+// 1000 takes 55 us, 66 in two; 2048^3 36 and 53; 16020 x 960 by 2816 174 and 202.
+PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus) {
+    PairCut best{choose_cut(elem_bytes, xm, xn, xk, cus), choose_cut(elem_bytes, wm, wn, wk, cus), false};
+    double least = best.x.us + best.w.us + 3.0;  // another launch
+    const int64_t per = kStageBytes / elem_bytes;
+    const int64_t xs = std::max<int64_t>(1, (xk + per - 1) / per), ws = std::max<int64_t>(1, (wk + per - 1) / per);
+    auto next = [](int64_t sp) { return sp < 4 ? sp + 1 : sp * 2; };
+    for (int t = 0; t < 3; ++t) {
+        const double* stage = elem_bytes == 2 ? kStage16[t] : kStage32[t];
+        const int rows = kTileRows[t];
+        const int64_t xt = ((xm + rows - 1) / rows) * ((xn + rows - 1) / rows);
+        const int64_t wt = ((wm + rows - 1) / rows) * ((wn + rows - 1) / rows);
+        for (int64_t sx = 1; sx <= 64; sx = next(sx)) {
+            const int64_t ex = (xs + sx - 1) / sx;
+            if (sx > 1 && (ex < 3 || (sx - 1) * ex >= xs || xt * sx > 8 * cus)) continue;
+            for (int64_t sw = 1; sw <= 64; sw = next(sw)) {
+                const int64_t ew = (ws + sw - 1) / sw;
+                if (sw > 1 && (ew < 3 || (sw - 1) * ew >= ws || wt * sw > 8 * cus)) continue;
+                const int64_t count = xt * sx + wt * sw;
+                const int64_t full = std::min<int64_t>(kResident[t], (count + cus - 1) / cus), slots = full * cus;
+                const double ux = (double)ex * stage[full - 1] + kRoundUs[t], uw = (double)ew * stage[full - 1] + kRoundUs[t];
+                const double all = ((double)(xt * sx) * ux + (double)(wt * sw) * uw) / (double)slots;
+                const double end = ex >= ew ? last_done(xt * sx, ux, wt * sw, uw, slots)
+                                            : last_done(wt * sw, uw, xt * sx, ux, slots);
+                double cost = std::max(all + 0.6 * (end - all) * stage[0] / stage[full - 1],
+                                       (double)std::max(ex, ew) * stage[0] + kRoundUs[t]);
+                cost += join_us((sx > 1 ? sx * xm * xn : 0) + (sw > 1 ? sw * wm * wn : 0));
+                if (cost < least) {
+                    least = cost;
+                    best = PairCut{Cut{t, (int)sx, (int32_t)(ex * per), cost}, Cut{t, (int)sw, (int32_t)(ew * per), cost}, true};
+                }
+            }
         }
     }
     return best;
@@ -82,8 +154,8 @@ template <typename T>
 hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const LinearOut& o, const Cut& cut,
                          float* part, const Only& only, hipStream_t s) {
     const LinearEpi<T> e = linear_epi<T>(o, m);
-    if (cut.splits == 1) return launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, 1, 0, only, e, s);
-    const hipError_t r = launch_gemm<T, true, true>(cut.tile, w, x, m, n, k, cut.splits, cut.k_split, only,
+    if (cut.splits == 1) return launch_gemm<T>(cut.tile, w, x, m, n, k, 1, 0, only, e, s);
+    const hipError_t r = launch_gemm<T>(cut.tile, w, x, m, n, k, cut.splits, cut.k_split, only,
                                                     parts_epi<T>(part, m, n), s);
     if (r != hipSuccess) return r;
     return launch_join(part, cut.splits, m, n, LinearPoint<T>{e}, only, s);
@@ -183,11 +255,12 @@ bool few_rows(int elem_bytes, int64_t n, int64_t m, int64_t k, const Cut& cut) {
 // backwards
 // ---------------------------------------------------------------------------
 // A workgroup takes 256 columns (four per lane) and a run of rows, at least 32
-// where there are as many; its four waves take rows in turn and their sums are
+// where there are more than 64; its four waves take rows in turn and their sums are
 // joined in order.  A single run is the column sum itself: it goes out at once.
 int column_parts(int64_t n, int64_t m, int cus) {
     const int64_t across = std::max<int64_t>(1, (m + 255) / 256);
     const int64_t want = std::max<int64_t>(1, (int64_t)cus * 8 / across);
+    if (n <= 64) return 1;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 31) / 32));
 }
 
@@ -243,24 +316,28 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
     }
 }
 
-// A workgroup joins the parts of 16 columns: sixteen threads take every
-// sixteenth part of a column, then one of them joins the sixteen in order.
-template <typename T>
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ sums, int parts, int64_t m,
-                                                        const float* __restrict__ alpha, T* __restrict__ out) {
-    __shared__ float join[16][16];
+// A workgroup joins the parts of 16 columns: a sixteenth of its threads each
+// takes every so-manieth part of a column, then one of them joins theirs in order.
+template <typename T, int THREADS>
+__device__ __forceinline__ void sum_parts(const ColumnSums<T>& to, int64_t m, int32_t wg, float* join) {
+    constexpr int kSlices = THREADS / 16;
     const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const int64_t c = (int64_t)blockIdx.x * 16 + col;
+    const int64_t c = (int64_t)wg * 16 + col;
     float v = 0.0f;
     if (c < m)
-        for (int p = slice; p < parts; p += 16) v += sums[(int64_t)p * m + c];
-    join[slice][col] = v;
+        for (int p = slice; p < to.parts; p += kSlices) v += to.sums[(int64_t)p * m + c];
+    join[threadIdx.x] = v;
     __syncthreads();
     if (slice != 0 || c >= m) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += join[i][col];
-    if (alpha) v *= *alpha;
-    out[c] = (T)v;
+    for (int i = 1; i < kSlices; ++i) v += join[i * 16 + col];
+    if (to.alpha) v *= *to.alpha;
+    to.out[c] = (T)v;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(ColumnSums<T> to, int64_t m) {
+    __shared__ float join[256];
+    sum_parts<T, 256>(to, m, blockIdx.x, join);
 }
 
 template <typename T>
@@ -272,9 +349,6 @@ static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int6
     const int width = z ? std::min(row_width<T>(dy, dy_ld), row_width<T>(z, m)) : row_width<T>(dy, dy_ld);
     act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)to.parts), 256, 0, s>>>(
         dy, dy_ld, z, act, n, m, dz, ld, to.sums, to.out, to.alpha, rows_per, width);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !to.out || to.parts == 1) return e;
-    sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(to.sums, to.parts, m, to.alpha, to.out);
     return hipGetLastError();
 }
 
@@ -290,17 +364,83 @@ hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& 
 }
 
 template <typename T>
-hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t k, const StoreTo& o, const Cut& cut,
-                          float* part, const Only& only, hipStream_t s) {
-    const StoreEpi<T> e = store_epi<T>(o);
-    if (cut.splits == 1)
-        return b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, 1, 0, only, e, s)
-                   : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, 1, 0, only, e, s);
-    const StoreEpi<T> pe = parts_epi<T>(part, m, n);
-    const hipError_t r = b_k ? launch_gemm<T, false, true>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, only, pe, s)
-                             : launch_gemm<T, false, false>(cut.tile, a, b, m, n, k, cut.splits, cut.k_split, only, pe, s);
-    if (r != hipSuccess) return r;
-    return launch_join(part, cut.splits, m, n, StorePoint<T>{e}, only, s);
+hipError_t launch_sum_parts(const ColumnSums<T>& to, int64_t m, hipStream_t s) {
+    if (!to.out || to.parts < 2) return hipSuccess;
+    sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(to, m);
+    return hipGetLastError();
+}
+
+// Both products of a gradient in one grid, and the column sums' join: none needs
+// another's results, and the workgroups of one fill the CUs that the last ones
+// of the other leave.
+template <typename T>
+struct PairArgs {
+    GemmArgs x, w;
+    StoreEpi<T> to_x, to_w;
+    int32_t x_wgs, w_wgs;
+    bool x_first;  // the one with the longer workgroups
+    ColumnSums<T> sums;
+    int64_t columns;
+};
+template <typename T, int WM, int WN, int MB, int NB>
+__global__ __launch_bounds__(WM* WN * 64, 2) void pair_kernel(PairArgs<T> q) {
+    __shared__ __attribute__((aligned(1024))) char buf[gemm_lds<WM, MB, NB>()];
+    if (skipped(q.x)) return;  // both have the same flag
+    int32_t wg = blockIdx.x;
+    const int32_t lead = q.x_first ? q.x_wgs : q.w_wgs;
+    if (wg >= q.x_wgs + q.w_wgs) {
+        sum_parts<T, WM * WN * 64>(q.sums, q.columns, wg - q.x_wgs - q.w_wgs, reinterpret_cast<float*>(buf));
+        return;
+    }
+    const bool second = wg >= lead;
+    if (second) wg -= lead;
+    if (second != q.x_first)
+        gemm_workgroup<T, false, true, WM, WN, MB, NB, StoreEpi<T>>(q.x, q.to_x, wg, buf);
+    else
+        gemm_workgroup<T, false, false, WM, WN, MB, NB, StoreEpi<T>>(q.w, q.to_w, wg, buf);
+}
+
+template <typename T>
+static hipError_t launch_pair(const Product& x, const Product& w, const Cut& cx, const Cut& cw, float* part,
+                              const ColumnSums<T>& sums, int64_t columns, const Only& only, hipStream_t s) {
+    PairArgs<T> q;
+    const int tile = x.m ? cx.tile : cw.tile;
+    int64_t wgs[2];
+    float* parts[2] = {part, part + (x.m ? cx.part_bytes(x.m, x.n) / 4 : 0)};
+    const StoreEpi<T> to[2] = {store_epi<T>(x.to), store_epi<T>(w.to)};
+    wgs[0] = gemm_args(q.x, tile, x.a, x.b, x.m, x.n, x.k, cx.splits, cx.k_split, only);
+    wgs[1] = gemm_args(q.w, tile, w.a, w.b, w.m, w.n, w.k, cw.splits, cw.k_split, only);
+    q.to_x = cx.splits > 1 ? parts_epi<T>(parts[0], x.m, x.n) : to[0];
+    q.to_w = cw.splits > 1 ? parts_epi<T>(parts[1], w.m, w.n) : to[1];
+    q.x_wgs = (int32_t)wgs[0];
+    q.w_wgs = (int32_t)wgs[1];
+    q.x_first = q.x.k_split >= q.w.k_split;
+    q.sums = sums;
+    q.columns = columns;
+    const int64_t blocks = wgs[0] + wgs[1] + (sums.out && sums.parts > 1 ? (columns + 15) / 16 : 0);
+    if (blocks == 0) return hipSuccess;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
+    const dim3 grid((unsigned)blocks);
+    if (tile == 0)
+        pair_kernel<T, 2, 4, 8, 4><<<grid, 512, 0, s>>>(q);
+    else if (tile == 1)
+        pair_kernel<T, 2, 2, 4, 4><<<grid, 256, 0, s>>>(q);
+    else
+        pair_kernel<T, 2, 2, 2, 2><<<grid, 256, 0, s>>>(q);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    typedef JoinJob<StorePoint<T>> Job;
+    return launch_join(Job{parts[0], x.m && cx.splits > 1 ? cx.splits : 0, x.m, x.n, StorePoint<T>{to[0]}},
+                       Job{parts[1], w.m && cw.splits > 1 ? cw.splits : 0, w.m, w.n, StorePoint<T>{to[1]}}, only, s);
+}
+
+template <typename T>
+hipError_t launch_products(const Product& x, const Product& w, const PairCut& cut, float* part,
+                           const ColumnSums<T>& sums, int64_t columns, const Only& only, hipStream_t s) {
+    if (cut.together || !x.m || !w.m) return launch_pair<T>(x, w, cut.x, cut.w, part, sums, columns, only, s);
+    const hipError_t e = launch_pair<T>(x, Product{}, cut.x, Cut{}, part, sums, columns, only, s);
+    if (e != hipSuccess) return e;
+    return launch_pair<T>(Product{}, w, Cut{}, cut.w, part, ColumnSums<T>{}, 0, only, s);
 }
 
 #define MLRS_INST(T)                                                                                               \
@@ -312,8 +452,9 @@ hipError_t launch_product(Mat a, Mat b, bool b_k, int64_t m, int64_t n, int64_t 
     template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t,                 \
                                            const ColumnSums<T>&, hipStream_t);                                     \
     template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, const ColumnSums<T>&, hipStream_t);           \
-    template hipError_t launch_product<T>(Mat, Mat, bool, int64_t, int64_t, int64_t, const StoreTo&, const Cut&,   \
-                                          float*, const Only&, hipStream_t);
+    template hipError_t launch_sum_parts<T>(const ColumnSums<T>&, int64_t, hipStream_t);                           \
+    template hipError_t launch_products<T>(const Product&, const Product&, const PairCut&, float*,                 \
+                                           const ColumnSums<T>&, int64_t, const Only&, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)

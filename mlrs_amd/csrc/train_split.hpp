@@ -134,7 +134,7 @@ __global__ __launch_bounds__(512, 2) void gemm_split_kernel(GemmArgs g, Epi epi)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const TilePlace t = tile_place(g);
+    const TilePlace t = tile_place(g, blockIdx.x);
     const int32_t m0 = t.tm * BM, n0 = t.tn * BN;
     const int32_t k_lo = t.split * g.k_split;
     const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;

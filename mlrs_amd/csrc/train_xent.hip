@@ -19,7 +19,7 @@ template <typename T>
 hipError_t launch_xent_stats(Mat h, Mat w, const T* bias, const int64_t* target, int64_t n, int64_t classes, int64_t k,
                              int tile, float* top, float* total, float* hit, const Only& only, hipStream_t s) {
     const StatsEpi<T> e{bias, target, top, total, hit};
-    return launch_gemm<T, true, true>(tile, w, h, classes, n, k, 1, 0, only, e, s);
+    return launch_gemm<T>(tile, w, h, classes, n, k, 1, 0, only, e, s);
 }
 
 // A workgroup joins the parts of 16 rows: sixteen threads take every sixteenth
@@ -121,7 +121,7 @@ hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target,
     const LogitGradEpi<T> e{bias ? bias + first : nullptr, target, lse, grad, up, out, ld, ignore, (int32_t)first,
                             (int32_t)classes};
     const Mat wp{(const T*)w.p + first * w.ld, w.ld};
-    return launch_gemm<T, true, true>(tile, wp, h, piece, n, k, 1, 0, only, e, s);
+    return launch_gemm<T>(tile, wp, h, piece, n, k, 1, 0, only, e, s);
 }
 
 #define MLRS_INST(T)                                                                                              \
