@@ -254,14 +254,14 @@ bool few_rows(int elem_bytes, int64_t n, int64_t m, int64_t k, const Cut& cut) {
 // ---------------------------------------------------------------------------
 // backwards
 // ---------------------------------------------------------------------------
-// A workgroup takes 256 columns (four per lane) and a run of rows, at least 32
-// where there are more than 64; its four waves take rows in turn and their sums are
-// joined in order.  A single run is the column sum itself: it goes out at once.
+// A workgroup takes 256 columns (four per lane) and a run of rows, at least eight
+// where there are more; its four waves take rows in turn and their sums are joined
+// in order.  A single run is the column sum itself: it goes out at once; the grid
+// of the products joins several, so that they cost no launch.
 int column_parts(int64_t n, int64_t m, int cus) {
     const int64_t across = std::max<int64_t>(1, (m + 255) / 256);
     const int64_t want = std::max<int64_t>(1, (int64_t)cus * 8 / across);
-    if (n <= 64) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 31) / 32));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 7) / 8));
 }
 
 template <typename T>
