@@ -48,6 +48,14 @@ bool readable(const T* p, int64_t cols) {
     return (uintptr_t)p % 16 == 0 && padded<T>(cols) == cols;
 }
 
+// Where the rows of a packed matrix lie: a cache line apart or a multiple of it,
+// from a few lines on.
+template <typename T>
+int64_t spaced(int64_t cols) {
+    constexpr int64_t L = 128 / (int64_t)sizeof(T);
+    return cols < 4 * L ? padded<T>(cols) : (cols + L - 1) / L * L;
+}
+
 // An operand as the kernels read it: in place, or packed.
 template <typename T>
 struct Op {
@@ -57,10 +65,10 @@ struct Op {
     Op(const T* p, int64_t r, int64_t c) : src(p), rows(r), cols(c) {}
     bool in_place() const { return readable(src, cols); }
     void plan(Scratch& sc) {
-        if (!in_place()) packed = sc.take<T>((size_t)(rows * padded<T>(cols)));
+        if (!in_place()) packed = sc.take<T>((size_t)(rows * spaced<T>(cols)));
     }
-    PackJob job() const { return PackJob{src, packed, in_place() ? 0 : rows, cols, padded<T>(cols)}; }
-    Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, padded<T>(cols)}; }
+    PackJob job() const { return PackJob{src, packed, in_place() ? 0 : rows, cols, spaced<T>(cols)}; }
+    Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, spaced<T>(cols)}; }
 };
 
 // f32 products may run on the bf16 matrix cores, in three parts of each operand
@@ -246,7 +254,7 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         for (int pass = 0; pass < 2; ++pass) {
             if (dw) xo.plan(sc);
             if (dx) wo.plan(sc);
-            if (make_dz) dz = sc.take<T>((size_t)(n * padded<T>(m)));
+            if (make_dz) dz = sc.take<T>((size_t)(n * spaced<T>(m)));
             if (db) sums = sc.take<float>((size_t)parts * (size_t)m);
             part = sc.take<float>(std::max(cut.part_bytes(k, n, k, m),
                                            std::max(split_x ? sx.part_bytes(k, n) : 0, split_w ? sw.part_bytes(k, m) : 0)) / 4);
@@ -268,8 +276,8 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         }
         const ColumnSums<T> col{db, sums, parts, nullptr};
         if (make_dz || db)
-            MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, padded<T>(m), col, s));
-        const Mat dzm = make_dz ? Mat{dz, padded<T>(m)} : Mat{dy, m};
+            MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, spaced<T>(m), col, s));
+        const Mat dzm = make_dz ? Mat{dz, spaced<T>(m)} : Mat{dy, m};
         PackJob xj = xo.job(), wj = wo.job();
         if (!dw || split_w) xj.rows = 0;
         if (!dx || split_x) wj.rows = 0;
@@ -447,7 +455,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                                               kMaxRowBytes / (int64_t)sizeof(T)) / 256 * 256;
         const int64_t pieces = (v + std::max<int64_t>(fit, 256) - 1) / std::max<int64_t>(fit, 256);
         const int64_t piece = pieces == 1 ? v : ((v + pieces - 1) / pieces + 255) / 256 * 256;
-        const int64_t ld = padded<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;
+        const int64_t ld = spaced<T>(std::min(piece, v)), dh_ld = (d + 3) / 4 * 4;
         const bool scaled = sizeof(T) == 2 && std::is_same<T, _Float16>::value;
         const int64_t most = std::min(piece, v);  // classes of the largest piece
         PairCut cut = choose_pair((int)sizeof(T), d, n, most, d, most, n, cus);
