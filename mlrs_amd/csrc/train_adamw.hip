@@ -41,24 +41,21 @@ __device__ __forceinline__ int find_item(const Batch<Item>& b, int32_t run) {
 }
 
 // Four elements from i on as floats; those at or past `end` are 0.
-__device__ __forceinline__ f32x4 load_any(const void* p, int dtype, int64_t i, int64_t end, int width) {
+__device__ __forceinline__ f32x4 load_any(const void* p, int dtype, int64_t i, int64_t end) {
     switch (dtype) {
-    case kF32: return load4((const float*)p, i, end, width);
-    case kF16: return load4((const _Float16*)p, i, end, width);
-    default: return load4((const __bf16*)p, i, end, width);
+    case kF32: return load4((const float*)p, i, end);
+    case kF16: return load4((const _Float16*)p, i, end);
+    default: return load4((const __bf16*)p, i, end);
     }
 }
-__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, int64_t end, int width, f32x4 v) {
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, int64_t end, f32x4 v) {
     switch (dtype) {
-    case kF32: store4((float*)p, i, end, width, v); break;
-    case kF16: store4((_Float16*)p, i, end, width, v); break;
-    default: store4((__bf16*)p, i, end, width, v); break;
+    case kF32: store4((float*)p, i, end, v); break;
+    case kF16: store4((_Float16*)p, i, end, v); break;
+    default: store4((__bf16*)p, i, end, v); break;
     }
 }
 
-static int bytes_of(int dtype) { return dtype == kF32 ? 4 : 2; }
-// whether four elements can be accessed at once, as load4's width
-static int access_width(const void* p, int elem) { return (uintptr_t)p % (4u * (unsigned)elem) == 0 ? 4 : 1; }
 
 // ---------------------------------------------------------------------------
 // the norm of all gradients
@@ -67,7 +64,6 @@ struct NormItem {
     const void* g;
     int64_t len;
     int32_t dtype;
-    int32_t width;
 };
 
 // A workgroup's sum of squares.  Each thread adds its sixteen in f32 (their
@@ -82,7 +78,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Batch<NormItem> b, double* __
     for (int u = 0; u < kRun / 1024; ++u) {
         const int64_t i = at + u * 1024 + threadIdx.x * 4;
         if (i >= it.len) continue;
-        const f32x4 v = load_any(it.g, it.dtype, i, it.len, it.width);
+        const f32x4 v = load_any(it.g, it.dtype, i, it.len);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum += v[e] * v[e];
     }
@@ -159,7 +155,6 @@ hipError_t launch_clip_scale(const mlrs_grad_tensor* t, int64_t count, double ma
             it.g = t[i].grad;
             it.len = t[i].len;
             it.dtype = t[i].dtype;
-            it.width = access_width(t[i].grad, bytes_of(t[i].dtype));
         },
         [&](const Batch<NormItem>& b, int64_t runs) {
             norm_kernel<<<dim3((unsigned)runs), 256, 0, s>>>(b, parts + at);
@@ -185,7 +180,7 @@ struct AdamwItem {
     int64_t len;
     float decay;   // 1 - lr * weight_decay
     uint32_t key;  // of the roundings
-    uint8_t param_dtype, grad_dtype, width;
+    uint8_t param_dtype, grad_dtype;
 };
 
 // 8-bit states.  The first moment is a sign and seven bits, four of exponent
@@ -261,7 +256,6 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyp
     const int64_t at = (int64_t)((int32_t)blockIdx.x - b.first[t]) * kRun;
     const float scale = scale_p ? *scale_p : 1.0f;
     if (!(fabsf(scale) < __builtin_huge_valf())) return;  // gradients that are not finite: no step
-    const int width = it.width;
 #pragma unroll
     for (int u = 0; u < kRun / 1024; ++u) {
         const int64_t i = at + u * 1024 + threadIdx.x * 4;
@@ -270,18 +264,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyp
         f32x4 p = {}, g = {}, m = {}, r = {}, v = {};
         float* master = it.master;
         if (i < end) {
-            p = master ? load4(master, i, end, width) : load_any(it.param, it.param_dtype, i, end, width);
-            g = load_any(it.grad, it.grad_dtype, i, end, width);
+            p = master ? load4(master, i, end) : load_any(it.param, it.param_dtype, i, end);
+            g = load_any(it.grad, it.grad_dtype, i, end);
             if (scale_p) g *= scale;
             if constexpr (BITS == 32) {
-                m = load4((const float*)it.avg, i, end, width);
-                v = load4((const float*)it.sq, i, end, width);
+                m = load4((const float*)it.avg, i, end);
+                v = load4((const float*)it.sq, i, end);
             } else {
                 const float ms = it.avg_scale[i / kBlock], rs = it.sq_scale[i / kBlock];
                 uint32_t mc = 0, rc = 0;
-                if (width == 4 && i + 4 <= end) {
-                    mc = *reinterpret_cast<const uint32_t*>((const uint8_t*)it.avg + i);
-                    rc = *reinterpret_cast<const uint32_t*>((const uint8_t*)it.sq + i);
+                if (i + 4 <= end) {
+                    __builtin_memcpy(&mc, (const uint8_t*)it.avg + i, 4);
+                    __builtin_memcpy(&rc, (const uint8_t*)it.sq + i, 4);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -308,13 +302,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyp
                 if (i + e >= end) m[e] = r[e] = 0.0f;  // no part of the block
         }
         if (i < end) {
-            if (master) store4(master, i, end, width, p);
-            store_any(it.param, it.param_dtype, i, end, width, p);
+            if (master) store4(master, i, end, p);
+            store_any(it.param, it.param_dtype, i, end, p);
         }
         if constexpr (BITS == 32) {
             if (i < end) {
-                store4((float*)it.avg, i, end, width, m);
-                store4((float*)it.sq, i, end, width, v);
+                store4((float*)it.avg, i, end, m);
+                store4((float*)it.sq, i, end, v);
             }
         } else {
             const float ms = wave_most(most4(m)) / 1.875f, rs = wave_most(most4(r)) / 1.9375f;
@@ -332,9 +326,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyp
                 rc |= c << (8 * e);
             }
             if (i < end) {
-                if (width == 4 && i + 4 <= end) {
-                    *reinterpret_cast<uint32_t*>((uint8_t*)it.avg + i) = mc;
-                    *reinterpret_cast<uint32_t*>((uint8_t*)it.sq + i) = rc;
+                if (i + 4 <= end) {
+                    __builtin_memcpy((uint8_t*)it.avg + i, &mc, 4);
+                    __builtin_memcpy((uint8_t*)it.sq + i, &rc, 4);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -370,10 +364,6 @@ hipError_t launch_adamw(const mlrs_adamw_tensor* t, int64_t count, int bits, con
             it.key = mix32(hy.seed + (uint32_t)i * 0x9E3779B1u);
             it.param_dtype = (uint8_t)x.param_dtype;
             it.grad_dtype = (uint8_t)x.grad_dtype;
-            const int se = bits == 32 ? 4 : 1;
-            it.width = (uint8_t)std::min(std::min(access_width(x.param, bytes_of(x.param_dtype)), access_width(x.grad, bytes_of(x.grad_dtype))),
-                                        std::min(access_width(x.exp_avg, se), access_width(x.exp_avg_sq, se)));
-            if (x.master) it.width = (uint8_t)std::min<int>(it.width, access_width(x.master, 4));
         },
         [&](const Batch<AdamwItem>& b, int64_t runs) {
             if (bits == 32)
@@ -387,12 +377,12 @@ hipError_t launch_adamw(const mlrs_adamw_tensor* t, int64_t count, int bits, con
 // The values that 8-bit codes stand for.
 template <bool ROOT>
 __global__ __launch_bounds__(256) void state_values_kernel(const uint8_t* __restrict__ codes,
-                                                           const float* __restrict__ scales, int64_t len, int width,
+                                                           const float* __restrict__ scales, int64_t len,
                                                            float* __restrict__ out) {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < len; i += (int64_t)gridDim.x * 1024) {
         uint32_t c = 0;
-        if (width == 4 && i + 4 <= len) {
-            c = *reinterpret_cast<const uint32_t*>(codes + i);
+        if (i + 4 <= len) {
+            __builtin_memcpy(&c, codes + i, 4);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -405,18 +395,17 @@ __global__ __launch_bounds__(256) void state_values_kernel(const uint8_t* __rest
             const uint32_t x = (c >> (8 * e)) & 255u;
             v[e] = (ROOT ? code_value<4>(x) : avg_value(x)) * sc;
         }
-        store4(out, i, len, width, v);
+        store4(out, i, len, v);
     }
 }
 
 hipError_t launch_state_values(const uint8_t* codes, const float* scales, int64_t len, int which, float* out,
                                hipStream_t s) {
     const int64_t blocks = std::min<int64_t>((len + 1023) / 1024, 65536);
-    const int width = std::min(access_width(codes, 1), access_width(out, 4));
     if (which == 0)
-        state_values_kernel<false><<<dim3((unsigned)blocks), 256, 0, s>>>(codes, scales, len, width, out);
+        state_values_kernel<false><<<dim3((unsigned)blocks), 256, 0, s>>>(codes, scales, len, out);
     else
-        state_values_kernel<true><<<dim3((unsigned)blocks), 256, 0, s>>>(codes, scales, len, width, out);
+        state_values_kernel<true><<<dim3((unsigned)blocks), 256, 0, s>>>(codes, scales, len, out);
     return hipGetLastError();
 }
 

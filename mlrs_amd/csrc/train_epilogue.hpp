@@ -97,18 +97,13 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
 }
 
 // Four consecutive elements of a row from m on, those at or past `end` left
-// out.  `width`: how many of them one access may hold, 4, 2 or 1, by the
-// alignment of the rows (m is a multiple of 4).
+// out.  Global accesses need no more than their elements' alignment, so rows of
+// any length are read and written four elements at a time.
 template <typename T>
-__device__ __forceinline__ typename Elem<T>::Vec4 load_raw4(const T* row, int64_t m, int64_t end, int width) {
-    typedef typename Elem<T>::Vec4 Vec4;
-    typedef T Vec2 __attribute__((ext_vector_type(2)));
-    Vec4 v;
-    if (width == 4 && m + 4 <= end) {
-        v = *reinterpret_cast<const Vec4*>(row + m);
-    } else if (width == 2 && m + 4 <= end) {
-        const Vec2 lo = *reinterpret_cast<const Vec2*>(row + m), hi = *reinterpret_cast<const Vec2*>(row + m + 2);
-        v = Vec4{lo[0], lo[1], hi[0], hi[1]};
+__device__ __forceinline__ typename Elem<T>::Vec4 load_raw4(const T* row, int64_t m, int64_t end) {
+    typename Elem<T>::Vec4 v;
+    if (m + 4 <= end) {
+        __builtin_memcpy(&v, row + m, sizeof v);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = m + e < end ? row[m + e] : (T)0.0f;
@@ -122,22 +117,17 @@ __device__ __forceinline__ f32x4 widen(V v) {
 }
 
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end, int width) {
-    return widen(load_raw4(row, m, end, width));
+__device__ __forceinline__ f32x4 load4(const T* row, int64_t m, int64_t end) {
+    return widen(load_raw4(row, m, end));
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, int width, f32x4 v) {
-    typedef typename Elem<T>::Vec4 Vec4;
-    typedef T Vec2 __attribute__((ext_vector_type(2)));
-    if (width == 4 && m + 4 <= end) {
-        Vec4 t;
+__device__ __forceinline__ void store4(T* row, int64_t m, int64_t end, f32x4 v) {
+    if (m + 4 <= end) {
+        typename Elem<T>::Vec4 t;
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = (T)v[e];
-        *reinterpret_cast<Vec4*>(row + m) = t;
-    } else if (width == 2 && m + 4 <= end) {
-        *reinterpret_cast<Vec2*>(row + m) = Vec2{(T)v[0], (T)v[1]};
-        *reinterpret_cast<Vec2*>(row + m + 2) = Vec2{(T)v[2], (T)v[3]};
+        __builtin_memcpy(row + m, &t, sizeof t);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -220,7 +210,6 @@ struct LinearEpi {
     T* z;
     int64_t ld;  // of residual, y and z
     int32_t act;
-    int32_t width;  // of the rows' accesses
 
     typedef typename Elem<T>::Vec4 Vec4;
     // rows n, n + step, ... of them those before n_end
@@ -230,7 +219,7 @@ struct LinearEpi {
         if (!residual) return;
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (n + u * step < n_end) res[u] = load_raw4(residual + (n + u * step) * ld, m, end, width);
+            if (n + u * step < n_end) res[u] = load_raw4(residual + (n + u * step) * ld, m, end);
     }
     template <int N>
     __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, f32x4 bv,
@@ -240,7 +229,7 @@ struct LinearEpi {
         if (z) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, width, v[u]);
+                if (n + u * step < n_end) store4(z + (n + u * step) * ld, m, end, v[u]);
         }
         activate_all(v, act);
         if (residual) {
@@ -249,7 +238,7 @@ struct LinearEpi {
         }
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, width, v[u]);
+            if (n + u * step < n_end) store4(y + (n + u * step) * ld, m, end, v[u]);
     }
     // one group of four elements
     __device__ __forceinline__ void point(int64_t n, int64_t m, int64_t end, f32x4 v) const {
@@ -260,7 +249,7 @@ struct LinearEpi {
     }
     __device__ __forceinline__ f32x4 bias_at(int64_t m, int64_t end) const {
         f32x4 bv = {};
-        if (bias && m < end) bv = load4(bias, m, end, 1);
+        if (bias && m < end) bv = load4(bias, m, end);
         return bv;
     }
     template <int WM, int WN, int MB, int NB>
@@ -285,7 +274,6 @@ struct StoreEpi {
     const float* add;    // may be null
     const float* alpha;  // device scalar; may be null
     int64_t ld, part_ld, part_stride;
-    int32_t width;  // of the rows' accesses
 
     template <int N>
     __device__ __forceinline__ void load(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end,
@@ -293,7 +281,7 @@ struct StoreEpi {
         if (!add) return;
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end, 4);
+            if (n + u * step < n_end) old[u] = load4(add + (n + u * step) * part_ld, m, end);
     }
     template <int N>
     __device__ __forceinline__ void rows(int64_t n, int64_t step, int64_t n_end, int64_t m, int64_t end, int split,
@@ -306,12 +294,12 @@ struct StoreEpi {
             const float by = alpha ? *alpha : 1.0f;
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, width, v[u] * by);
+                if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, v[u] * by);
         } else {
             float* to = part + split * part_stride;  // part_ld is a multiple of 4
 #pragma unroll
             for (int u = 0; u < N; ++u)
-                if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, 4, v[u]);
+                if (n + u * step < n_end) store4(to + (n + u * step) * part_ld, m, end, v[u]);
         }
     }
     __device__ __forceinline__ void point(int64_t n, int64_t m, int64_t end, f32x4 v) const {
@@ -338,7 +326,7 @@ __device__ __forceinline__ void add_bias(f32x4 (&acc)[MB][NB], const T* bias, co
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         const int32_t m = p.m0 + i * 16 + 4 * (p.lane >> 4);
-        const f32x4 bv = m < p.m ? load4(bias, m, p.m, 1) : f32x4{};
+        const f32x4 bv = m < p.m ? load4(bias, m, p.m) : f32x4{};
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] += bv;
     }

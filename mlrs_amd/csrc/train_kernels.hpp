@@ -138,7 +138,6 @@ struct SplitJob {
     int64_t src_ld;
     void* dst;
     int64_t rows, cols;
-    int width;
     bool r_layout;
 };
 SplitJob split_job(const float* src, int64_t src_ld, int64_t rows, int64_t cols, void* dst, bool r_layout);

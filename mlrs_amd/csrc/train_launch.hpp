@@ -50,13 +50,6 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
     return hipGetLastError();
 }
 
-// How many elements of rows `ld` elements apart from p on an access may hold.
-template <typename T>
-inline int row_width(const void* p, int64_t ld) {
-    if ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0) return 4;
-    return (uintptr_t)p % (2 * sizeof(T)) == 0 && ld % 2 == 0 ? 2 : 1;
-}
-
 // The parts of split contractions, joined in order: of one product or of two.
 template <typename Point>
 struct JoinJob {
@@ -114,7 +107,6 @@ inline StoreEpi<T> parts_epi(float* part, int64_t m, int64_t n) {
     e.part = part;
     e.part_ld = (m + 3) & ~(int64_t)3;
     e.part_stride = n * e.part_ld;
-    e.width = 4;
     return e;
 }
 
@@ -127,9 +119,6 @@ inline LinearEpi<T> linear_epi(const LinearOut& o, int64_t m) {
     e.z = (T*)o.z;
     e.ld = m;
     e.act = o.act;
-    e.width = row_width<T>(o.y, m);
-    if (o.z) e.width = std::min(e.width, row_width<T>(o.z, m));
-    if (o.residual) e.width = std::min(e.width, row_width<T>(o.residual, m));
     return e;
 }
 
@@ -143,7 +132,6 @@ inline StoreEpi<T> store_epi(const StoreTo& o) {
     e.ld = o.ld;
     e.part_ld = o.acc_ld;
     e.part_stride = 0;
-    e.width = o.out ? row_width<T>(o.out, o.ld) : 4;
     return e;
 }
 

@@ -132,8 +132,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackJob a, PackJob b, Only on
         const int64_t chunks = j.ld / E, r = at / chunks, c = (at - r * chunks) * E;
         const T* from = (const T*)j.src + r * j.cols;
         typename Elem<T>::Frag v;
+        if (c + E <= j.cols) {
+            __builtin_memcpy(&v, from + c, sizeof v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = c + e < j.cols ? from[c + e] : (T)0.0f;
+            for (int e = 0; e < E; ++e) v[e] = c + e < j.cols ? from[c + e] : (T)0.0f;
+        }
         *reinterpret_cast<typename Elem<T>::Frag*>((T*)j.dst + r * j.ld + c) = v;
     }
 }
@@ -165,16 +169,12 @@ hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const Li
 // fragments of the matrix instructions.  A workgroup computes
 // sixteen outputs of every row; its waves take the contraction axis in turn
 // and their sums are joined in LDS, in the order of the waves.
-template <typename T, bool ALIGNED>
+template <typename T>
 __device__ __forceinline__ typename Elem<T>::Frag chunk_at(const T* row, int64_t c, int64_t k) {
     constexpr int E = 16 / (int)sizeof(T);
     typename Elem<T>::Frag f;
-    if constexpr (ALIGNED) {  // k is a multiple of E
-        if (c < k)
-            f = *reinterpret_cast<const typename Elem<T>::Frag*>(row + c);
-        else
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = (T)0.0f;
+    if (c + E <= k) {
+        __builtin_memcpy(&f, row + c, sizeof f);
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = c + e < k ? row[c + e] : (T)0.0f;
@@ -182,7 +182,7 @@ __device__ __forceinline__ typename Elem<T>::Frag chunk_at(const T* row, int64_t
     return f;
 }
 
-template <typename T, bool ALIGNED, int NB, int WAVES>
+template <typename T, int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restrict__ x, const T* __restrict__ w,
                                                                 int32_t n, int32_t m, int64_t k, LinearEpi<T> epi) {
     constexpr int E = 16 / (int)sizeof(T);
@@ -200,11 +200,11 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
     for (int64_t k0 = (int64_t)wave * (U * STEP); k0 < k; k0 += (int64_t)WAVES * (U * STEP)) {
         typename Elem<T>::Frag a[U], bx[NB][U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u] = chunk_at<T, ALIGNED>(wr, k0 + u * STEP + q * E, k);
+        for (int u = 0; u < U; ++u) a[u] = chunk_at<T>(wr, k0 + u * STEP + q * E, k);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int u = 0; u < U; ++u) bx[b][u] = chunk_at<T, ALIGNED>(xr[b], k0 + u * STEP + q * E, k);
+            for (int u = 0; u < U; ++u) bx[b][u] = chunk_at<T>(xr[b], k0 + u * STEP + q * E, k);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -223,10 +223,10 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
     }
 }
 
-template <typename T, bool ALIGNED, int NB>
+template <typename T, int NB>
 static hipError_t launch_few_nb(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearEpi<T>& e,
                                 hipStream_t s) {
-    linear_few_kernel<T, ALIGNED, NB, 8>
+    linear_few_kernel<T, NB, 8>
         <<<dim3((unsigned)((m + 15) / 16)), 512, 0, s>>>(x, w, (int32_t)n, (int32_t)m, k, e);
     return hipGetLastError();
 }
@@ -235,10 +235,7 @@ template <typename T>
 hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                              hipStream_t s) {
     const LinearEpi<T> e = linear_epi<T>(o, m);
-    const bool al = (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && (k * (int64_t)sizeof(T)) % 16 == 0;
-    if (n <= 16)
-        return al ? launch_few_nb<T, true, 1>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 1>(x, w, n, m, k, e, s);
-    return al ? launch_few_nb<T, true, 2>(x, w, n, m, k, e, s) : launch_few_nb<T, false, 2>(x, w, n, m, k, e, s);
+    return n <= 16 ? launch_few_nb<T, 1>(x, w, n, m, k, e, s) : launch_few_nb<T, 2>(x, w, n, m, k, e, s);
 }
 
 // Sixteen rows are bound by reading the weights (8192 x 8192 bf16: 29 us at one
@@ -269,7 +266,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
                                                        const T* __restrict__ z, int act, int64_t n, int64_t m,
                                                        T* __restrict__ dz, int64_t ld, float* __restrict__ sums,
                                                        T* __restrict__ out, const float* __restrict__ alpha,
-                                                       int64_t rows_per, int width) {
+                                                       int64_t rows_per) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per;
@@ -281,11 +278,11 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
             f32x4 v[kRows] = {}, zz[kRows] = {};
 #pragma unroll
             for (int u = 0; u < kRows; ++u)
-                if (r + 4 * u < r1) v[u] = load4(dy + (r + 4 * u) * dy_ld, c, m, width);
+                if (r + 4 * u < r1) v[u] = load4(dy + (r + 4 * u) * dy_ld, c, m);
             if (z) {
 #pragma unroll
                 for (int u = 0; u < kRows; ++u)
-                    if (r + 4 * u < r1) zz[u] = load4(z + (r + 4 * u) * m, c, m, width);
+                    if (r + 4 * u < r1) zz[u] = load4(z + (r + 4 * u) * m, c, m);
             }
 #pragma unroll
             for (int u = 0; u < kRows; ++u) {
@@ -297,7 +294,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
                 for (int e = 0; e < 4; ++e)
                     if (c + e >= m || r + 4 * u >= r1) v[u][e] = 0.0f;
                 sum += v[u];
-                if (dz && r + 4 * u < r1) store4(dz + (r + 4 * u) * ld, c, ld, 4, v[u]);
+                if (dz && r + 4 * u < r1) store4(dz + (r + 4 * u) * ld, c, ld, v[u]);
             }
         }
     }
@@ -310,9 +307,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
 #pragma unroll
         for (int i = 1; i < 4; ++i) v += join[i][lane];
         if (gridDim.y == 1)
-            store4(out, c, m, 1, alpha ? v * *alpha : v);
+            store4(out, c, m, alpha ? v * *alpha : v);
         else
-            store4(sums + (int64_t)blockIdx.y * m, c, m, 1, v);
+            store4(sums + (int64_t)blockIdx.y * m, c, m, v);
     }
 }
 
@@ -346,9 +343,8 @@ static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int6
     const int64_t across = ((dz ? ld : m) + 255) / 256;
     if (across == 0 || (n == 0 && !to.out)) return hipSuccess;
     const int64_t rows_per = (n + to.parts - 1) / to.parts;
-    const int width = z ? std::min(row_width<T>(dy, dy_ld), row_width<T>(z, m)) : row_width<T>(dy, dy_ld);
     act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)to.parts), 256, 0, s>>>(
-        dy, dy_ld, z, act, n, m, dz, ld, to.sums, to.out, to.alpha, rows_per, width);
+        dy, dy_ld, z, act, n, m, dz, ld, to.sums, to.out, to.alpha, rows_per);
     return hipGetLastError();
 }
 

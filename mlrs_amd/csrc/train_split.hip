@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void pack_split_kernel(SplitJob a, SplitJob b,
         const int64_t at = i < total_a ? i : i - total_a;
         const int64_t groups = (j.cols + 7) / 8, r = at / groups, c = at - r * groups;
         const float* from = j.src + r * j.src_ld;
-        const f32x4 lo = load4(from, 8 * c, j.cols, j.width), hi = load4(from, 8 * c + 4, j.cols, j.width);
+        const f32x4 lo = load4(from, 8 * c, j.cols), hi = load4(from, 8 * c + 4, j.cols);
         bf16x8 p0, p1, p2;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void pack_split_kernel(SplitJob a, SplitJob b,
 }
 
 SplitJob split_job(const float* src, int64_t src_ld, int64_t rows, int64_t cols, void* dst, bool r_layout) {
-    return SplitJob{src, src_ld, dst, rows, cols, row_width<float>(src, src_ld), r_layout};
+    return SplitJob{src, src_ld, dst, rows, cols, r_layout};
 }
 
 hipError_t launch_pack_split(const SplitJob& a, const SplitJob& b, uint32_t* flag, uint32_t mark, hipStream_t s) {
