@@ -297,7 +297,7 @@ __device__ __forceinline__ int32_t xcd_tile(int32_t wg, int32_t total) {
 struct TilePlace {
     int32_t tm, tn, split;
 };
-__device__ __forceinline__ TilePlace tile_place(const GemmArgs& g, int32_t wg) {
+__device__ __forceinline__ TilePlace tile_place(const GemmArgs& g, uint32_t wg) {
     const int32_t tiles = g.tiles_m * g.tiles_n;
     TilePlace p;
     p.split = wg / tiles;
@@ -341,7 +341,7 @@ __host__ __device__ constexpr int gemm_lds() {
     return gemm_slots<MB, NB>() * WM * MB * 16 * kStageBytes;
 }
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
-__device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi, int32_t wg, char* buf) {
+__device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi, uint32_t wg, char* buf) {
     constexpr int BM = WM * MB * 16, BN = WN * NB * 16, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
     constexpr int BK = stage_elems<T>();

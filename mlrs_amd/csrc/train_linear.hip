@@ -434,9 +434,9 @@ template <typename T>
 hipError_t launch_products(const Product& x, const Product& w, const PairCut& cut, float* part,
                            const ColumnSums<T>& sums, int64_t columns, const Only& only, hipStream_t s) {
     if (cut.together || !x.m || !w.m) return launch_pair<T>(x, w, cut.x, cut.w, part, sums, columns, only, s);
-    const hipError_t e = launch_pair<T>(x, Product{}, cut.x, Cut{}, part, sums, columns, only, s);
+    const hipError_t e = launch_pair<T>(Product{}, w, Cut{}, cut.w, part, sums, columns, only, s);
     if (e != hipSuccess) return e;
-    return launch_pair<T>(Product{}, w, Cut{}, cut.w, part, ColumnSums<T>{}, 0, only, s);
+    return launch_pair<T>(x, Product{}, cut.x, Cut{}, part, ColumnSums<T>{}, 0, only, s);
 }
 
 #define MLRS_INST(T)                                                                                               \
