@@ -56,20 +56,31 @@ int64_t spaced(int64_t cols) {
     return cols < 4 * L ? padded<T>(cols) : (cols + L - 1) / L * L;
 }
 
-// An operand as the kernels read it: in place, or packed.
+// An operand as the kernels read it: in place (f32 of any rows, word by word), or
+// packed.
 template <typename T>
 struct Op {
     const T* src;
     int64_t rows, cols;
+    bool words;
     T* packed = nullptr;
-    Op(const T* p, int64_t r, int64_t c) : src(p), rows(r), cols(c) {}
-    bool in_place() const { return readable(src, cols); }
+    Op(const T* p, int64_t r, int64_t c, bool by_words) : src(p), rows(r), cols(c), words(by_words) {}
+    bool in_place() const { return words || readable(src, cols); }
     void plan(Scratch& sc) {
         if (!in_place()) packed = sc.take<T>((size_t)(rows * spaced<T>(cols)));
     }
     PackJob job() const { return PackJob{src, packed, in_place() ? 0 : rows, cols, spaced<T>(cols)}; }
     Mat mat() const { return in_place() ? Mat{src, cols} : Mat{packed, spaced<T>(cols)}; }
 };
+
+// f32 operands whose rows are no multiple of 16 bytes: whether their products (`us`
+// by words, `packed_us` else) copy them word by word, which makes a product about
+// 6% slower (3001 x 10007 by 250 backwards: 372 us, 358 packed), or `elements` of
+// them are packed: a launch, and their bytes twice (300 x 7001 by 501 forwards: 36
+// us by words, 49 packed).
+bool by_words(double us, double packed_us, double elements) {
+    return 1.06 * us < packed_us + 4.5 + elements * 8.0 / 4.5e6;
+}
 
 // f32 products may run on the bf16 matrix cores, in three parts of each operand
 // (train_split.hpp).  What packing `elements` of them costs, in microseconds: 10
@@ -95,7 +106,7 @@ struct Sides {
 };
 
 constexpr Cut kPlainCut{0, 1, 0, 0.0};  // of the kernels that stand in
-constexpr PairCut kPlainPair{kPlainCut, kPlainCut, true};
+constexpr PairCut kPlainPair{kPlainCut, kPlainCut, true, 0.0};
 
 // Sizes that both layers of operators share: a (n x d) and w (m x d).
 template <typename T>
@@ -151,13 +162,17 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
             MLRS_TRY(launch_linear_few<T>(x, w, n, m, k, o, s));
             return MLRS_OK;
         }
-        bool split = false;
+        bool split = false, words = false;
         if constexpr (std::is_same<T, float>::value) {
             const Cut other = choose_cut_split(m, n, k, cus);
             split = other.us + split_us((double)(n + m) * (double)k) < cut.us;
             if (split) cut = other;
+            const bool rx = readable(x, k), rw = readable(w, k);
+            const Cut by = choose_cut((int)sizeof(T), m, n, k, cus, 64, true);
+            words = !split && !(rx && rw) && by_words(by.us, cut.us, (double)((rx ? 0 : n) + (rw ? 0 : m)) * (double)k);
+            if (words) cut = by;
         }
-        Op<T> xo(x, n, k), wo(w, m, k);
+        Op<T> xo(x, n, k, words), wo(w, m, k, words);
         float* part = nullptr;
         char *xs = nullptr, *ws = nullptr;
         Sides sides;
@@ -231,6 +246,7 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         const bool products = (dx && n > 0) || dw;
         // dy itself serves as dz where there is no slope and its rows can be read
         const bool make_dz = products && n > 0 && (act != MLRS_ACT_NONE || !readable(dy, m));
+        bool words = false;
         const bool want_x = dx && n > 0;
         PairCut cut = choose_pair((int)sizeof(T), k, n, m, k, m, n, cus);
         Cut sx{}, sw{};  // of those that run in parts
@@ -241,13 +257,20 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
             sw = choose_cut_split(k, m, n, cus);
             split_x = want_x && sx.us + split_us((double)(n + k) * (double)m) < cx.us;
             split_w = dw && n > 0 && sw.us + split_us((double)(m + k) * (double)n) < cw.us;
-            if (split_x || split_w) cut = PairCut{cx, cw, false};
+            if (split_x || split_w) cut = PairCut{cx, cw, false, 0.0};
+            const bool rw = !want_x || readable(w, k), rx = !dw || readable(x, k);
+            const PairCut by = choose_pair((int)sizeof(T), k, n, m, k, m, n, cus, true);
+            words = !split_x && !split_w && !(rx && rw) &&
+                    by_words(by.us, cut.us, (double)((rx ? 0 : n) + (rw ? 0 : m)) * (double)k);
+            if (words) cut = by;
         }
-        if (!want_x || !dw) cut = PairCut{choose_cut((int)sizeof(T), k, n, m, cus), choose_cut((int)sizeof(T), k, m, n, cus), false};
+        if (!want_x || !dw)
+            cut = PairCut{choose_cut((int)sizeof(T), k, n, m, cus, 64, words),
+                          choose_cut((int)sizeof(T), k, m, n, cus, 64, words), false, 0.0};
         const int parts = column_parts(n, m, cus);
         char *w_r = nullptr, *dz_k = nullptr, *x_r = nullptr, *dz_r = nullptr;
         Sides sides;
-        Op<T> xo(x, n, k), wo(w, m, k);
+        Op<T> xo(x, n, k, words), wo(w, m, k, words);
         T* dz = nullptr;
         float *part = nullptr, *sums = nullptr;
         Scratch sc;
@@ -352,7 +375,7 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         const Cut cut = choose_cut((int)sizeof(T), v, n, d, cus, 1);
         int tile = cut.tile;
         int64_t parts = stats_parts(tile, v), parts_s = 0;
-        bool split = false;
+        bool split = false, words = false;
         if constexpr (std::is_same<T, float>::value) {
             split = choose_cut_split(v, n, d, cus, 1).us + split_us((double)(n + v) * (double)d) < cut.us;
             if (split) {
@@ -360,11 +383,18 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
                 parts = stats_parts(tile, v);
                 parts_s = stats_parts_split(v);
             }
+            const bool rh = readable(h, d), rw = readable(w, d);
+            const Cut by = choose_cut((int)sizeof(T), v, n, d, cus, 1, true);
+            words = !split && !(rh && rw) && by_words(by.us, cut.us, (double)((rh ? 0 : n) + (rw ? 0 : v)) * (double)d);
+            if (words) {
+                tile = by.tile;
+                parts = stats_parts(tile, v);
+            }
         }
         // the statistics of as many rows at a time as their parts have room for
         const int64_t room = std::max(parts, parts_s);
         const int64_t rows = std::min(n, std::max<int64_t>(256, kStatsBytes / (8 * room) / 256 * 256));
-        Op<T> ho(h, n, d), wo(w, v, d);
+        Op<T> ho(h, n, d, words), wo(w, v, d, words);
         float *top = nullptr, *total = nullptr, *hit = nullptr;
         char *hs = nullptr, *ws = nullptr;
         Sides sides;
@@ -443,7 +473,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 const StoreTo o{dw, d, nullptr, nullptr, 0, nullptr};
                 const Product p{Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, d, v, 0, o};
                 const Cut c{2, 1, 0, 0.0};
-                MLRS_TRY(launch_products<T>(Product{}, p, PairCut{c, c, false}, nullptr, ColumnSums<T>{}, 0, Only{}, s));
+                MLRS_TRY(launch_products<T>(Product{}, p, PairCut{c, c, false, 0.0}, nullptr, ColumnSums<T>{}, 0, Only{}, s));
             }
             if (db)
                 MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
@@ -472,12 +502,24 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                       choose_cut((int)sizeof(T), most, n, d, cus, 1).us;
             split_h = dh && sh.us + split_us(nv + vd) < ch.us;
             split_w = dw && sw.us + split_us(nv + nd) < cw.us;
-            if (split_h || split_w) cut = PairCut{ch, cw, false};
+            if (split_h || split_w) cut = PairCut{ch, cw, false, 0.0};
         }
-        if (!dh || !dw) cut = PairCut{choose_cut((int)sizeof(T), d, n, most, cus), choose_cut((int)sizeof(T), d, most, n, cus), false};
         const bool split = split_z || split_h || split_w;
+        bool words = false;
+        if constexpr (std::is_same<T, float>::value) {
+            const bool rh = readable(h, d), rw = readable(w, d);
+            const PairCut by = choose_pair((int)sizeof(T), d, n, most, d, most, n, cus, true);
+            const double z = choose_cut((int)sizeof(T), most, n, d, cus, 1).us * (double)pieces;
+            words = !split && !(rh && rw) &&
+                    by_words(by.us * (double)pieces + z, cut.us * (double)pieces + z,
+                             (double)((rh ? 0 : n) + (rw ? 0 : v)) * (double)d);
+            if (words) cut = by;
+        }
+        if (!dh || !dw)
+            cut = PairCut{choose_cut((int)sizeof(T), d, n, most, cus, 64, words),
+                          choose_cut((int)sizeof(T), d, most, n, cus, 64, words), false, 0.0};
         const int parts = column_parts(n, most, cus);
-        Op<T> ho(h, n, d), wo(w, v, d);
+        Op<T> ho(h, n, d, words), wo(w, v, d, words);
         T* dz = nullptr;
         float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr;
         char *h_k = nullptr, *w_k = nullptr, *h_r = nullptr, *w_r = nullptr, *dz_k = nullptr, *dz_r = nullptr;
@@ -545,7 +587,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                                                      lse, grad, n, v0, vp, v, d, ignore, dz, ld, sides.split(), s));
             }
             MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
-                                          split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), vp, n, d, cus, 1).tile,
+                                          split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), vp, n, d, cus, 1, words).tile,
                                           split_z ? plain : Only{}, s));
             const ColumnSums<T> col{db ? db + v0 : nullptr, sums, parts, down};
             if (db) MLRS_TRY(launch_column_sums<T>(dzm, n, vp, col, s));

@@ -6,8 +6,9 @@
 // ("K layout", ptr[row * ld + k]) or with its row index contiguous ("R
 // layout", ptr[k * ld + row]), so the three products of a layer need no
 // transposed copies: x w^T is K x K, dz w is R x K, dz^T x is R x R.  Pointers
-// are 16-byte aligned and ld is a multiple of 16 bytes; the host packs what is
-// not.
+// are 16-byte aligned and ld is a multiple of 16 bytes; what is not the host
+// packs, or f32 operands are copied word by word (BYTES 4, 64 x 64 tiles: their
+// matrix instructions take longer than four times as many copies).
 //
 // Tile.  A workgroup computes BM x BN of P, its waves a WM x WN grid of parts
 // of MB x NB blocks of 16 x 16 (v_mfma_f32_16x16x32 for 16-bit types, four
@@ -150,41 +151,59 @@ __device__ __forceinline__ void copy_to_lds(u32x4 rsrc, char* lds, uint32_t offs
 #endif
 }
 
+// The same with four bytes per lane, for f32 operands in place whose rows are no
+// multiple of 16 bytes: lane i's are at lds + 4 i.
+__device__ __forceinline__ void copy_word_to_lds(u32x4 rsrc, char* lds, uint32_t offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"((uint32_t)(uintptr_t)(MLRS_LDS void*)lds), "v"(offset), "s"(rsrc)
+                 : "memory");
+#else
+    (void)rsrc;
+    (void)lds;
+    (void)offset;
+#endif
+}
+
 // One operand's copy into LDS: the bytes of ROWS rows (or columns) of one
-// staged width, 1,024 per wave and instruction.
-template <typename T, bool KC, int ROWS, int WAVES>
+// staged width, 64 BYTES per wave and instruction.
+template <typename T, bool KC, int ROWS, int WAVES, int BYTES = 16>
 struct Stager {
-    static constexpr int kInstr = ROWS * kStageBytes / 1024 / WAVES;
+    static constexpr int kInstr = ROWS * kStageBytes / (64 * BYTES) / WAVES;
+    static constexpr int kPlaces = BYTES == 16 ? 2 : 8;  // of a lane in a row, K layout: by the copy
     static constexpr int kChunks = ROWS * (int)sizeof(T) / 16;  // of one k (R layout)
     static_assert(kInstr >= 1, "a wave copies at least one kilobyte");
     const char* base;   // the tile's first element at k = 0
     int64_t bytes;      // from base to the operand's end
     int64_t step;       // bytes per element of k
-    int32_t chunk[2];   // K layout: 16 * the lane's chunk, of even and of odd copies
+    int32_t chunk[kPlaces];  // K layout: where in the row the lane's bytes are
     uint32_t off[kInstr];
 
     __device__ __forceinline__ void init(const Operand& o, int32_t row0, int32_t rows, int32_t k, int wave, int lane) {
         const int64_t es = (int64_t)sizeof(T);
-        // whole rows: the bounds check works by 16-byte chunks, which end at ld
+        // whole rows: the bounds check works by the lanes' bytes, which end at ld
         const int64_t total = (KC ? (int64_t)rows : (int64_t)k) * o.ld * es;
         const int64_t at = KC ? (int64_t)row0 * o.ld * es : (int64_t)row0 * es;
         base = reinterpret_cast<const char*>(o.p) + at;
         bytes = total - at;
         step = KC ? es : o.ld * es;
         const uint32_t ldb = (uint32_t)(o.ld * es);
-        chunk[0] = chunk[1] = 0;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) chunk[i] = 0;
 #pragma unroll
         for (int i = 0; i < kInstr; ++i) {
-            const int q = (wave * kInstr + i) * 64 + lane;
+            const int q = ((wave * kInstr + i) * 64 + lane) / (16 / BYTES);  // the chunk's place in LDS
+            const uint32_t in = BYTES == 16 ? 0u : 4u * (uint32_t)(lane & 3);
             if constexpr (KC) {
-                static_assert(kInstr % 2 == 0, "which chunk a lane copies goes by the copy's parity");
+                static_assert(kInstr % kPlaces == 0, "which chunk a lane copies goes by the copy");
                 const int r = q >> 3, c = (q & 7) ^ k_swizzle(r);
-                chunk[i & 1] = 16 * c;
-                off[i] = (uint32_t)r * ldb + 16u * (uint32_t)c;
+                chunk[i % kPlaces] = 16 * c + (int)in;
+                off[i] = (uint32_t)r * ldb + 16u * (uint32_t)c + in;
             } else {
                 const int kk = q / kChunks;
                 const int c = (q % kChunks) ^ r_swizzle<T, ROWS>(kk);
-                off[i] = (uint32_t)kk * ldb + 16u * (uint32_t)c;
+                off[i] = (uint32_t)kk * ldb + 16u * (uint32_t)c + in;
             }
         }
     }
@@ -204,11 +223,17 @@ struct Stager {
         rsrc[2] = records;
         rsrc[3] = 0x00027000u;
         // chunks past the end of a row would be the next row's
-        const bool out[2] = {KC && chunk[0] >= (k - k0) * (int)sizeof(T),
-                             KC && chunk[1] >= (k - k0) * (int)sizeof(T)};
+        bool out[kPlaces];
 #pragma unroll
-        for (int i = PART * kInstr / PARTS; i < (PART + 1) * kInstr / PARTS; ++i)
-            copy_to_lds(rsrc, lds + (wave * kInstr + i) * 1024, out[i & 1] ? 0x80000000u : off[i]);
+        for (int i = 0; i < kPlaces; ++i) out[i] = KC && chunk[i] >= (k - k0) * (int)sizeof(T);
+#pragma unroll
+        for (int i = PART * kInstr / PARTS; i < (PART + 1) * kInstr / PARTS; ++i) {
+            const uint32_t from = out[i % kPlaces] ? 0x80000000u : off[i];
+            if constexpr (BYTES == 16)
+                copy_to_lds(rsrc, lds + (wave * kInstr + i) * 1024, from);
+            else
+                copy_word_to_lds(rsrc, lds + (wave * kInstr + i) * 256, from);
+        }
 #else
         (void)lds;
         (void)k0;
@@ -340,7 +365,7 @@ template <int WM, int MB, int NB>
 __host__ __device__ constexpr int gemm_lds() {
     return gemm_slots<MB, NB>() * WM * MB * 16 * kStageBytes;
 }
-template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi>
+template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi, int BYTES = 16>
 __device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi, uint32_t wg, char* buf) {
     constexpr int BM = WM * MB * 16, BN = WN * NB * 16, WAVES = WM * WN;
     constexpr int kA = BM * kStageBytes, kB = BN * kStageBytes;
@@ -360,8 +385,8 @@ __device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi
     const int32_t k_lo = t.split * g.k_split;
     const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;
 
-    Stager<T, AKC, BM, WAVES> sa;
-    Stager<T, BKC, BN, WAVES> sb;
+    Stager<T, AKC, BM, WAVES, BYTES> sa;
+    Stager<T, BKC, BN, WAVES, BYTES> sb;
     sa.init(g.a, m0, g.m, k_hi, wave, lane);
     sb.init(g.b, n0, g.n, k_hi, wave, lane);
     Reader<T, AKC, BM, MB> ra;
@@ -527,11 +552,11 @@ __device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi
 }
 
 // A product of operands in K layout.
-template <typename T, int WM, int WN, int MB, int NB, typename Epi>
+template <typename T, int WM, int WN, int MB, int NB, typename Epi, int BYTES = 16>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(GemmArgs g, Epi epi) {
     __shared__ __attribute__((aligned(1024))) char buf[gemm_lds<WM, MB, NB>()];
     if (skipped(g)) return;
-    gemm_workgroup<T, true, true, WM, WN, MB, NB, Epi>(g, epi, blockIdx.x, buf);
+    gemm_workgroup<T, true, true, WM, WN, MB, NB, Epi, BYTES>(g, epi, blockIdx.x, buf);
 }
 
 }  // namespace train

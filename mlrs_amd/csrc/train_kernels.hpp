@@ -10,7 +10,7 @@ namespace mlrs {
 namespace train {
 
 // A row-major matrix the matrix-core kernels can read: 16-byte aligned, rows
-// a multiple of 16 bytes apart.
+// a multiple of 16 bytes apart (of f32 in tiles copied by words, any).
 struct Mat {
     const void* p;
     int64_t ld;
@@ -18,7 +18,7 @@ struct Mat {
 
 // How a product is cut: the tile, and the parts of its contraction axis.
 struct Cut {
-    int tile;         // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
+    int tile;         // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64, 3: the same, f32 copied by words
     int splits;
     int32_t k_split;
     double us;        // the estimate it was chosen by
@@ -26,7 +26,7 @@ struct Cut {
         return splits > 1 ? (size_t)splits * (size_t)n * (size_t)((m + 3) & ~(int64_t)3) * 4 : 0;
     }
 };
-Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64, bool words = false);
 
 // A launch that runs only where (*flag == mark) == wanted (flag null: always).
 struct Only {
@@ -104,11 +104,13 @@ struct Product {
 struct PairCut {
     Cut x, w;
     bool together;  // in one grid
+    double us;      // the estimate, of both
     size_t part_bytes(int64_t xm, int64_t xn, int64_t wm, int64_t wn) const {
         return x.part_bytes(xm, xn) + w.part_bytes(wm, wn);
     }
 };
-PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus);
+PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus,
+                    bool words = false);
 // sums: of `columns` columns, still to be joined (parts < 2: none).
 template <typename T>
 hipError_t launch_products(const Product& x, const Product& w, const PairCut& cut, float* part,

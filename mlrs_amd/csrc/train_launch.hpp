@@ -8,7 +8,7 @@
 namespace mlrs {
 namespace train {
 
-constexpr int kTileRows[3] = {256, 128, 64};
+constexpr int kTileRows[4] = {256, 128, 64, 64};
 
 // Tiles of m walked together along n.  The workgroups that run at once on an
 // XCD (32 CUs) then share about as many panels of either operand.
@@ -45,8 +45,12 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
         gemm_kernel<T, 2, 4, 8, 4, Epi><<<grid, 512, 0, s>>>(g, epi);
     else if (tile == 1)
         gemm_kernel<T, 2, 2, 4, 4, Epi><<<grid, 256, 0, s>>>(g, epi);
-    else
+    else if (tile == 2)
         gemm_kernel<T, 2, 2, 2, 2, Epi><<<grid, 256, 0, s>>>(g, epi);
+    else if constexpr (sizeof(T) == 4)
+        gemm_kernel<T, 2, 2, 2, 2, Epi, 4><<<grid, 256, 0, s>>>(g, epi);
+    else
+        return hipErrorInvalidValue;
     return hipGetLastError();
 }
 

@@ -26,11 +26,11 @@ static const int kResident[3] = {1, 2, 3};
 // Joining parts: a launch, and their bytes twice.
 static double join_us(int64_t elements) { return elements ? 10.0 + (double)elements * 8.0 / 4.5e6 : 0.0; }
 
-Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits) {
+Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits, bool words) {
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t stages = std::max<int64_t>(1, (k + per - 1) / per);
     Cut best{0, 1, 0, 1e300};
-    for (int t = 0; t < 3; ++t) {
+    for (int t = words ? 2 : 0; t < 3; ++t) {
         const double* stage = elem_bytes == 2 ? kStage16[t] : kStage32[t];
         const int rows = kTileRows[t];
         const int64_t tiles = ((m + rows - 1) / rows) * ((n + rows - 1) / rows);
@@ -42,7 +42,7 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
             double cost = (double)rounds * ((double)each * stage[kResident[t] - 1] + kRoundUs[t]);
             if (rest) cost += (double)each * stage[rest - 1] + kRoundUs[t];
             if (sp > 1) cost += join_us(sp * m * n);
-            if (cost < best.us) best = Cut{t, (int)sp, (int32_t)(each * per), cost};
+            if (cost < best.us) best = Cut{words ? 3 : t, (int)sp, (int32_t)(each * per), cost};
         }
     }
     return best;
@@ -81,13 +81,15 @@ static double last_done(int64_t first, double first_us, int64_t then, double the
 // was 2% slower than the best of some sixty cuts each, 13% at most, and in bf16 a
 // fifth to a third faster than the best two launches below 100 us: 4099 x 2056 by
 // 1000 takes 55 us, 66 in two; 2048^3 36 and 53; 16020 x 960 by 2816 174 and 202.
-PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus) {
-    PairCut best{choose_cut(elem_bytes, xm, xn, xk, cus), choose_cut(elem_bytes, wm, wn, wk, cus), false};
-    double least = best.x.us + best.w.us + 3.0;  // another launch
+PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus,
+                    bool words) {
+    PairCut best{choose_cut(elem_bytes, xm, xn, xk, cus, 64, words), choose_cut(elem_bytes, wm, wn, wk, cus, 64, words),
+                 false, 0.0};
+    best.us = best.x.us + best.w.us + 3.0;  // another launch
     const int64_t per = kStageBytes / elem_bytes;
     const int64_t xs = std::max<int64_t>(1, (xk + per - 1) / per), ws = std::max<int64_t>(1, (wk + per - 1) / per);
     auto next = [](int64_t sp) { return sp < 4 ? sp + 1 : sp * 2; };
-    for (int t = 0; t < 3; ++t) {
+    for (int t = words ? 2 : 0; t < 3; ++t) {
         const double* stage = elem_bytes == 2 ? kStage16[t] : kStage32[t];
         const int rows = kTileRows[t];
         const int64_t xt = ((xm + rows - 1) / rows) * ((xn + rows - 1) / rows);
@@ -107,9 +109,10 @@ PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t 
                 double cost = std::max(all + 0.6 * (end - all) * stage[0] / stage[full - 1],
                                        (double)std::max(ex, ew) * stage[0] + kRoundUs[t]);
                 cost += join_us((sx > 1 ? sx * xm * xn : 0) + (sw > 1 ? sw * wm * wn : 0));
-                if (cost < least) {
-                    least = cost;
-                    best = PairCut{Cut{t, (int)sx, (int32_t)(ex * per), cost}, Cut{t, (int)sw, (int32_t)(ew * per), cost}, true};
+                if (cost < best.us) {
+                    const int tile = words ? 3 : t;
+                    best = PairCut{Cut{tile, (int)sx, (int32_t)(ex * per), cost},
+                                   Cut{tile, (int)sw, (int32_t)(ew * per), cost}, true, cost};
                 }
             }
         }
@@ -378,7 +381,7 @@ struct PairArgs {
     ColumnSums<T> sums;
     int64_t columns;
 };
-template <typename T, int WM, int WN, int MB, int NB>
+template <typename T, int WM, int WN, int MB, int NB, int BYTES = 16>
 __global__ __launch_bounds__(WM* WN * 64, 2) void pair_kernel(PairArgs<T> q) {
     __shared__ __attribute__((aligned(1024))) char buf[gemm_lds<WM, MB, NB>()];
     if (skipped(q.x)) return;  // both have the same flag
@@ -391,9 +394,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void pair_kernel(PairArgs<T> q) {
     const bool second = wg >= lead;
     if (second) wg -= lead;
     if (second != q.x_first)
-        gemm_workgroup<T, false, true, WM, WN, MB, NB, StoreEpi<T>>(q.x, q.to_x, wg, buf);
+        gemm_workgroup<T, false, true, WM, WN, MB, NB, StoreEpi<T>, BYTES>(q.x, q.to_x, wg, buf);
     else
-        gemm_workgroup<T, false, false, WM, WN, MB, NB, StoreEpi<T>>(q.w, q.to_w, wg, buf);
+        gemm_workgroup<T, false, false, WM, WN, MB, NB, StoreEpi<T>, BYTES>(q.w, q.to_w, wg, buf);
 }
 
 template <typename T>
@@ -421,8 +424,12 @@ static hipError_t launch_pair(const Product& x, const Product& w, const Cut& cx,
         pair_kernel<T, 2, 4, 8, 4><<<grid, 512, 0, s>>>(q);
     else if (tile == 1)
         pair_kernel<T, 2, 2, 4, 4><<<grid, 256, 0, s>>>(q);
-    else
+    else if (tile == 2)
         pair_kernel<T, 2, 2, 2, 2><<<grid, 256, 0, s>>>(q);
+    else if constexpr (sizeof(T) == 4)
+        pair_kernel<T, 2, 2, 2, 2, 4><<<grid, 256, 0, s>>>(q);
+    else
+        return hipErrorInvalidValue;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     typedef JoinJob<StorePoint<T>> Job;

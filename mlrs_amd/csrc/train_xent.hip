@@ -8,7 +8,7 @@
 namespace mlrs {
 namespace train {
 
-static const int kWaveRows[3] = {128, 64, 32};  // classes of a wave, by tile
+static const int kWaveRows[4] = {128, 64, 32, 32};  // classes of a wave, by tile
 
 int64_t stats_parts(int tile, int64_t classes) {
     const int rows = kTileRows[tile];
