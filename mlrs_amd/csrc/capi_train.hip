@@ -297,9 +297,10 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
                 sc.used = 0;
             }
         }
-        const ColumnSums<T> col{db, sums, parts, nullptr};
+        ColumnSums<T> col{db, sums, parts, nullptr};
         if (make_dz || db)
             MLRS_TRY(launch_act_grad<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, spaced<T>(m), col, s));
+        if (parts == 1) col.out = nullptr;  // done
         const Mat dzm = make_dz ? Mat{dz, spaced<T>(m)} : Mat{dy, m};
         PackJob xj = xo.job(), wj = wo.job();
         if (!dw || split_w) xj.rows = 0;
@@ -476,7 +477,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 MLRS_TRY(launch_products<T>(Product{}, p, PairCut{c, c, false, 0.0}, nullptr, ColumnSums<T>{}, 0, Only{}, s));
             }
             if (db)
-                MLRS_TRY(launch_column_sums<T>(Mat{nullptr, padded<T>(v)}, 0, v, ColumnSums<T>{db, nullptr, 1, nullptr}, s));
+                MLRS_TRY(launch_sum_parts<T>(ColumnSums<T>{db, nullptr, 0, nullptr}, v, s));
             return MLRS_OK;
         }
         // classes of a piece: a multiple of 256, at least one tile, and a row of
@@ -518,7 +519,9 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
         if (!dh || !dw)
             cut = PairCut{choose_cut((int)sizeof(T), d, n, most, cus, 64, words),
                           choose_cut((int)sizeof(T), d, most, n, cus, 64, words), false, 0.0};
-        const int parts = column_parts(n, most, cus);
+        // one tile for every piece: its column sums are of as many parts
+        const int z_tile = split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), most, n, d, cus, 1, words).tile;
+        const int parts = (int)logit_grad_parts(z_tile, n);
         Op<T> ho(h, n, d, words), wo(w, v, d, words);
         T* dz = nullptr;
         float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr;
@@ -575,6 +578,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             const int64_t vp = std::min(piece, v - v0);
             const bool last = v0 + vp == v;
             const Mat dzm{dz, ld};
+            const ColumnSums<T> col{db ? db + v0 : nullptr, sums, parts, down};
             if constexpr (std::is_same<T, float>::value) {
                 const float* wp = w + v0 * d;
                 SplitJob wk = split_job(wp, d, vp, d, w_k, false), wr = split_job(wp, d, vp, d, w_r, true);
@@ -584,13 +588,11 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                 if (all_split) MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), plain, s));
                 if (split_z)
                     MLRS_TRY(launch_logit_grad_split(split_mat(h_k, d, false), split_mat(w_k, d, false), bias, target,
-                                                     lse, grad, n, v0, vp, v, d, ignore, dz, ld, sides.split(), s));
+                                                     lse, grad, n, v0, vp, v, d, ignore, dz, ld, sums, sides.split(), s));
             }
-            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld,
-                                          split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), vp, n, d, cus, 1, words).tile,
+            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld, sums,
+                                          z_tile,
                                           split_z ? plain : Only{}, s));
-            const ColumnSums<T> col{db ? db + v0 : nullptr, sums, parts, down};
-            if (db) MLRS_TRY(launch_column_sums<T>(dzm, n, vp, col, s));
             const StoreTo to_w{dw ? dw + v0 * d : nullptr, d, nullptr, nullptr, 0, down};
             StoreTo to_h{};
             to_h.ld = d;

@@ -415,6 +415,7 @@ struct LogitGradEpi {
     const float* grad;
     const float* up;  // device scalar; may be null
     T* out;
+    float* sums;  // null, or the column sums of every wave's rows, piece by piece of NB * 16 rows
     int64_t ld;
     int64_t ignore;
     int32_t first;    // the piece's first class
@@ -462,6 +463,7 @@ struct LogitGradEpi {
             return __builtin_bit_cast(typename Elem<T>::Vec4, w);
         };
         char* mine = lds + p.wave * 32 * kRow;
+        float col[kEach] = {};
         __syncthreads();  // the panels in LDS are no longer read
 #pragma unroll
         for (int j0 = 0; j0 < NB; j0 += 2) {
@@ -507,10 +509,26 @@ struct LogitGradEpi {
                 const typename Elem<T>::Frag v = *reinterpret_cast<const typename Elem<T>::Frag*>(
                     mine + row * kRow + ((c ^ turn_swizzle<kRow>(row)) << 4));
                 const int32_t n = p.n0 + j0 * 16 + row, m = p.m0 + kEach * c;
-                if (n < p.n && m < ld) *reinterpret_cast<typename Elem<T>::Frag*>(out + (int64_t)n * ld + m) = v;
+                if (n < p.n && m < ld) {
+                    *reinterpret_cast<typename Elem<T>::Frag*>(out + (int64_t)n * ld + m) = v;
+                    if (sums) {
+#pragma unroll
+                        for (int e = 0; e < kEach; ++e) col[e] += (float)v[e];
+                    }
+                }
             }
             __builtin_amdgcn_wave_barrier();
         }
+        if (!sums || p.n0 >= p.n) return;
+#pragma unroll
+        for (int s = kPieces; s < 64; s <<= 1)
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) col[e] += __shfl_xor(col[e], s);
+        if (p.lane >= kPieces) return;
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4)
+            store4(sums + (int64_t)(p.n0 / (NB * 16)) * p.m, p.m0 + kEach * p.lane + e, p.m,
+                   f32x4{col[e], col[e + 1], col[e + 2], col[e + 3]});
     }
 };
 

@@ -63,8 +63,8 @@ template <typename T>
 hipError_t launch_linear_few(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                              hipStream_t s);
 
-// Column sums: out (null: none wanted) := alpha * the sums, made in `parts` runs
-// of rows, parts x m floats of scratch.
+// Column sums that are still to be joined: out (null: none) := alpha * the sum of
+// `parts` runs of rows, parts x columns floats.
 template <typename T>
 struct ColumnSums {
     T* out;
@@ -73,14 +73,12 @@ struct ColumnSums {
     const float* alpha;  // device scalar; may be null
 };
 int column_parts(int64_t n, int64_t m, int cus);
-// dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and its
-// column sums: done with one part, else for launch_products or launch_sum_parts.
+// dz (n x ld) := dy * act'(z), zeros behind each row (dz may be null), and where
+// sums.out its column sums: done with one part, else for launch_products or
+// launch_sum_parts.
 template <typename T>
 hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
-                           const ColumnSums<T>& to, hipStream_t s);
-// The same of a packed matrix's column sums alone.
-template <typename T>
-hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& to, hipStream_t s);
+                           const ColumnSums<T>& sums, hipStream_t s);
 template <typename T>
 hipError_t launch_sum_parts(const ColumnSums<T>& to, int64_t m, hipStream_t s);
 
@@ -111,7 +109,7 @@ struct PairCut {
 };
 PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus,
                     bool words = false);
-// sums: of `columns` columns, still to be joined (parts < 2: none).
+// sums: of `columns` columns.
 template <typename T>
 hipError_t launch_products(const Product& x, const Product& w, const PairCut& cut, float* part,
                            const ColumnSums<T>& sums, int64_t columns, const Only& only, hipStream_t s);
@@ -127,10 +125,14 @@ hipError_t launch_xent_join(const float* top, const float* total, int64_t parts,
                             const Only& only, hipStream_t s);
 hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n, int64_t ignore, float* up_down,
                              hipStream_t s);
+// sums: null, or logit_grad_parts(tile, n) runs of rows' column sums (f32's split
+// kernels: as of tile 0).
+int64_t logit_grad_parts(int tile, int64_t n);
 template <typename T>
 hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
                              const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
-                             int64_t ignore, T* out, int64_t ld, int tile, const Only& only, hipStream_t s);
+                             int64_t ignore, T* out, int64_t ld, float* sums, int tile, const Only& only,
+                             hipStream_t s);
 
 // f32 products on the bf16 matrix cores (train_split.hpp).  K layout: ld is
 // bytes, split_row_bytes of the columns; R layout: ld is elements, a multiple of
@@ -161,8 +163,8 @@ hipError_t launch_xent_stats_split(Mat h, Mat w, const float* bias, const int64_
 // w: the piece's classes; bias: the whole vocabulary's.
 hipError_t launch_logit_grad_split(Mat h, Mat w, const float* bias, const int64_t* target, const float* lse,
                                    const float* grad, int64_t n, int64_t first, int64_t piece, int64_t classes,
-                                   int64_t k, int64_t ignore, float* out, int64_t ld, const Only& only,
-                                   hipStream_t s);
+                                   int64_t k, int64_t ignore, float* out, int64_t ld, float* sums,
+                                   const Only& only, hipStream_t s);
 
 // Optimizer.
 int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);

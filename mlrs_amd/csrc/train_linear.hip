@@ -265,11 +265,9 @@ int column_parts(int64_t n, int64_t m, int cus) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, int64_t dy_ld,
-                                                       const T* __restrict__ z, int act, int64_t n, int64_t m,
-                                                       T* __restrict__ dz, int64_t ld, float* __restrict__ sums,
-                                                       T* __restrict__ out, const float* __restrict__ alpha,
-                                                       int64_t rows_per) {
+__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, const T* __restrict__ z, int act,
+                                                       int64_t n, int64_t m, T* __restrict__ dz, int64_t ld,
+                                                       ColumnSums<T> sums, int64_t rows_per) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per;
@@ -281,7 +279,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
             f32x4 v[kRows] = {}, zz[kRows] = {};
 #pragma unroll
             for (int u = 0; u < kRows; ++u)
-                if (r + 4 * u < r1) v[u] = load4(dy + (r + 4 * u) * dy_ld, c, m);
+                if (r + 4 * u < r1) v[u] = load4(dy + (r + 4 * u) * m, c, m);
             if (z) {
 #pragma unroll
                 for (int u = 0; u < kRows; ++u)
@@ -301,7 +299,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
             }
         }
     }
-    if (!out) return;
+    if (!sums.out) return;
     __shared__ f32x4 join[4][64];
     join[wave][lane] = sum;
     __syncthreads();
@@ -310,9 +308,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
 #pragma unroll
         for (int i = 1; i < 4; ++i) v += join[i][lane];
         if (gridDim.y == 1)
-            store4(out, c, m, alpha ? v * *alpha : v);
+            store4(sums.out, c, m, v);
         else
-            store4(sums + (int64_t)blockIdx.y * m, c, m, v);
+            store4(sums.sums + (int64_t)blockIdx.y * m, c, m, v);
     }
 }
 
@@ -341,30 +339,19 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(ColumnSums<T> to, int64_
 }
 
 template <typename T>
-static hipError_t act_grad(const T* dy, int64_t dy_ld, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
-                           const ColumnSums<T>& to, hipStream_t s) {
+hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
+                           const ColumnSums<T>& sums, hipStream_t s) {
     const int64_t across = ((dz ? ld : m) + 255) / 256;
-    if (across == 0 || (n == 0 && !to.out)) return hipSuccess;
-    const int64_t rows_per = (n + to.parts - 1) / to.parts;
-    act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)to.parts), 256, 0, s>>>(
-        dy, dy_ld, z, act, n, m, dz, ld, to.sums, to.out, to.alpha, rows_per);
+    if (across == 0 || (n == 0 && !sums.out)) return hipSuccess;
+    const int64_t rows_per = (n + sums.parts - 1) / sums.parts;
+    act_grad_kernel<T><<<dim3((unsigned)across, (unsigned)sums.parts), 256, 0, s>>>(dy, z, act, n, m, dz, ld, sums,
+                                                                                   rows_per);
     return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t m, T* dz, int64_t ld,
-                           const ColumnSums<T>& to, hipStream_t s) {
-    return act_grad<T>(dy, m, z, act, n, m, dz, ld, to, s);
-}
-
-template <typename T>
-hipError_t launch_column_sums(Mat a, int64_t n, int64_t m, const ColumnSums<T>& to, hipStream_t s) {
-    return act_grad<T>((const T*)a.p, a.ld, nullptr, kActNone, n, m, nullptr, 0, to, s);
-}
-
-template <typename T>
 hipError_t launch_sum_parts(const ColumnSums<T>& to, int64_t m, hipStream_t s) {
-    if (!to.out || to.parts < 2) return hipSuccess;
+    if (!to.out) return hipSuccess;
     sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(to, m);
     return hipGetLastError();
 }
@@ -416,7 +403,7 @@ static hipError_t launch_pair(const Product& x, const Product& w, const Cut& cx,
     q.x_first = q.x.k_split >= q.w.k_split;
     q.sums = sums;
     q.columns = columns;
-    const int64_t blocks = wgs[0] + wgs[1] + (sums.out && sums.parts > 1 ? (columns + 15) / 16 : 0);
+    const int64_t blocks = wgs[0] + wgs[1] + (sums.out ? (columns + 15) / 16 : 0);
     if (blocks == 0) return hipSuccess;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
     const dim3 grid((unsigned)blocks);
@@ -454,7 +441,6 @@ hipError_t launch_products(const Product& x, const Product& w, const PairCut& cu
                                              hipStream_t);                                                         \
     template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t,                 \
                                            const ColumnSums<T>&, hipStream_t);                                     \
-    template hipError_t launch_column_sums<T>(Mat, int64_t, int64_t, const ColumnSums<T>&, hipStream_t);           \
     template hipError_t launch_sum_parts<T>(const ColumnSums<T>&, int64_t, hipStream_t);                           \
     template hipError_t launch_products<T>(const Product&, const Product&, const PairCut&, float*,                 \
                                            const ColumnSums<T>&, int64_t, const Only&, hipStream_t);

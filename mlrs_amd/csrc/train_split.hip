@@ -130,9 +130,9 @@ hipError_t launch_xent_stats_split(Mat h, Mat w, const float* bias, const int64_
 
 hipError_t launch_logit_grad_split(Mat h, Mat w, const float* bias, const int64_t* target, const float* lse,
                                    const float* grad, int64_t n, int64_t first, int64_t piece, int64_t classes,
-                                   int64_t k, int64_t ignore, float* out, int64_t ld, const Only& only,
-                                   hipStream_t s) {
-    const LogitGradEpi<float> e{bias ? bias + first : nullptr, target, lse, grad, nullptr, out, ld, ignore,
+                                   int64_t k, int64_t ignore, float* out, int64_t ld, float* sums,
+                                   const Only& only, hipStream_t s) {
+    const LogitGradEpi<float> e{bias ? bias + first : nullptr, target, lse, grad, nullptr, out, sums, ld, ignore,
                                 (int32_t)first, (int32_t)classes};
     return launch_split<true, true>(w, h, piece, n, k, Cut{0, 1, 0, 0.0}, only, e, s);
 }

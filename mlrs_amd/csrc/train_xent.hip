@@ -114,11 +114,14 @@ hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n
     return hipGetLastError();
 }
 
+int64_t logit_grad_parts(int tile, int64_t n) { return tile < 2 ? (n + 63) / 64 : (n + 31) / 32; }
+
 template <typename T>
 hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target, const float* lse, const float* grad,
                              const float* up, int64_t n, int64_t first, int64_t piece, int64_t classes, int64_t k,
-                             int64_t ignore, T* out, int64_t ld, int tile, const Only& only, hipStream_t s) {
-    const LogitGradEpi<T> e{bias ? bias + first : nullptr, target, lse, grad, up, out, ld, ignore, (int32_t)first,
+                             int64_t ignore, T* out, int64_t ld, float* sums, int tile, const Only& only,
+                             hipStream_t s) {
+    const LogitGradEpi<T> e{bias ? bias + first : nullptr, target, lse, grad, up, out, sums, ld, ignore, (int32_t)first,
                             (int32_t)classes};
     const Mat wp{(const T*)w.p + first * w.ld, w.ld};
     return launch_gemm<T>(tile, wp, h, piece, n, k, 1, 0, only, e, s);
@@ -129,7 +132,7 @@ hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target,
                                              float*, float*, float*, const Only&, hipStream_t);                   \
     template hipError_t launch_logit_grad<T>(Mat, Mat, const T*, const int64_t*, const float*, const float*,      \
                                              const float*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,  \
-                                             T*, int64_t, int, const Only&, hipStream_t);
+                                             T*, int64_t, float*, int, const Only&, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)
