@@ -504,11 +504,11 @@ def linear(x, w, bias=None, activation="none", residual=None, keep_preact=False,
     n, d_in = x.shape
     d_out = w.shape[0]
     if out is None:
-        y = torch.empty((n, d_out), dtype=x.dtype, device=x.device)
+        y = x.new_empty((n, d_out))
     else:
         _check_out(out, "out", (x.dtype,), n * d_out, x.device)
         y = out
-    z = torch.empty((n, d_out), dtype=x.dtype, device=x.device) if keep_preact else None
+    z = x.new_empty((n, d_out)) if keep_preact else None
     _lib.check(getattr(_lib.load(), "mlrs_linear_" + s)(
         _ptr(x), x.numel(), n, d_in, _ptr(w), w.numel(), d_out, _ptr(bias), _len(bias), _ptr(residual), _len(residual),
         act, _ptr(y), y.numel(), _ptr(z), _len(z), _stream(x.device)))
@@ -532,7 +532,7 @@ def linear_grad(dy, x, w, preact=None, activation="none", bias=True, need_dx=Tru
     d_out = w.shape[0]
     dx = torch.empty_like(x) if need_dx else None
     dw = torch.empty_like(w) if need_dw else None
-    db = torch.empty(d_out, dtype=x.dtype, device=x.device) if bias else None
+    db = x.new_empty(d_out) if bias else None
     _lib.check(getattr(_lib.load(), "mlrs_linear_grad_" + s)(
         _ptr(dy), dy.numel(), _ptr(x), x.numel(), n, d_in, _ptr(w), w.numel(), d_out, _ptr(z), _len(z), act, _ptr(dx),
         _len(dx), _ptr(dw), _len(dw), _ptr(db), _len(db), _stream(x.device)))
@@ -558,8 +558,8 @@ def softmax_xent(h, w, target, bias=None, ignore_index=-100):
     _dev_check(h, target)
     n, d = h.shape
     _check_rows(target, "target", torch.int64, n)
-    loss = torch.empty(n, dtype=torch.float32, device=h.device)
-    lse = torch.empty(n, dtype=torch.float32, device=h.device)
+    loss = h.new_empty(n, dtype=torch.float32)
+    lse = torch.empty_like(loss)
     _lib.check(getattr(_lib.load(), "mlrs_softmax_xent_" + s)(
         _ptr(h), h.numel(), n, d, _ptr(w), w.numel(), w.shape[0], _ptr(bias), _len(bias), _ptr(target),
         target.numel(), int(ignore_index), _ptr(loss), _ptr(lse), n, _stream(h.device)))

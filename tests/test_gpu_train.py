@@ -439,6 +439,26 @@ def test_the_same_call_gives_the_same_bits_on_any_stream(dtype):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_calls_alternate_between_streams():
+    """Calls on the null stream and on another one, in turn and without waiting,
+    share a workspace: each starts after the one before."""
+    n, v, k = 2048, 30011, 256
+    hs, w = [dev(rand(1 + i, n, k, dtype=BF16)) for i in range(8)], dev(rand(20, v, k, dtype=BF16, std=0.2))
+    t = dev(targets(3, n, v))
+    want = []
+    for h in hs:
+        want.append(prims.softmax_xent(h, w, t))
+        torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = []
+    for i, h in enumerate(hs):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.default_stream()):
+            got.append(prims.softmax_xent(h, w, t))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 # f32 products large enough to run in three bf16 parts: whole and ragged sizes,
 # parts of the contraction (the gradients), rows aligned to four bytes alone
 @pytest.mark.parametrize("n,k,m,offset", [(4100, 1040, 4096, 0), (4100, 1031, 4100, 0), (4099, 1040, 4101, 1)])
