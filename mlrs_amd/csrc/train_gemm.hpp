@@ -348,15 +348,7 @@ __device__ __forceinline__ void wait_copies() {
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// A workgroup of every product.  8192 x 8192 x 8192 in bf16: 729 us forwards (K x
-// K), 764 for dx (R x K), 740 for dw (R x R), 1508, 1439 and 1486 TFLOP/s, where
-// the matrix instructions alone would do 2080 at the clock that the chip's power
-// allows; with the copies left out it was 1576 in 32 x 32 blocks.  In 256 x 256
-// tiles eight waves of 128 x 64 read 192 KB of fragments and copy 64 KB for 2048
-// cycles of matrix work a staged width, the LDS being busy for as long; one
-// workgroup fills a CU.  Four waves of 128 x 128 read a third less and are no
-// faster (756 us), as a wave alone on its SIMD waits for itself.
-// buf: gemm_lds bytes, the kernel's only LDS.
+// Panels that a tile keeps in LDS, and their bytes.
 template <int MB, int NB>
 __host__ __device__ constexpr int gemm_slots() {
     return MB * NB == 4 ? 6 : 5;
@@ -365,6 +357,17 @@ template <int WM, int MB, int NB>
 __host__ __device__ constexpr int gemm_lds() {
     return gemm_slots<MB, NB>() * WM * MB * 16 * kStageBytes;
 }
+
+// A workgroup of every product.  8192 x 8192 x 8192 in bf16: 729 us forwards (K x
+// K), 764 for dx (R x K), 740 for dw (R x R) on one card, 744, 827 and 799 on
+// another, 1330 to 1508 TFLOP/s, where the matrix instructions alone would do 2080
+// at the clock that the chip's power allows; with the copies left out it was 1576
+// in 32 x 32 blocks.  In 256 x 256 tiles eight waves of 128 x 64 read 192 KB of
+// fragments and copy 64 KB for 2048 cycles of matrix work a staged width, the LDS
+// being busy for as long; one workgroup fills a CU.  Four waves of 128 x 128 read a
+// third less and are no faster (756 us), as a wave alone on its SIMD waits for
+// itself.
+// buf: gemm_lds bytes, the kernel's only LDS.
 template <typename T, bool AKC, bool BKC, int WM, int WN, int MB, int NB, typename Epi, int BYTES = 16>
 __device__ __forceinline__ void gemm_workgroup(const GemmArgs& g, const Epi& epi, uint32_t wg, char* buf) {
     constexpr int BM = WM * MB * 16, BN = WN * NB * 16, WAVES = WM * WN;
