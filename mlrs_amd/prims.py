@@ -75,6 +75,14 @@ def _metric_id(metric):
 
 
 def _dev_check(*ts):
+    if ts:  # nothing to complain of, in half the time of finding out what
+        index = ts[0].get_device()
+        if index >= 0 and index == torch._C._cuda_getDevice():
+            for t in ts:
+                if t.get_device() != index or not t.is_contiguous():
+                    break
+            else:
+                return
     for t in ts:
         if not t.is_cuda:
             raise ValueError("mlrs_amd prims take device tensors (got a %s tensor)" % t.device)
@@ -469,20 +477,21 @@ def _layer_operands(a, w, a_name, *others):
     """The checks a layer and a loss share: device, contiguity, one element
     type, two dimensions.  The C ABI checks the sizes.  `others`: (tensor or
     None, name) pairs."""
-    given = [t for t, _ in others if t is not None]
-    _dev_check(a, w, *given)
+    given = [(t, name) for t, name in others if t is not None]
+    _dev_check(a, w, *[t for t, _ in given])
     s = _train_suffix(a)
     dtype = a.dtype
     if w.dtype != dtype:
         raise TypeError("%s and w dtypes differ (%s, %s)" % (a_name, dtype, w.dtype))
-    for t, name in others:
-        if t is not None and t.dtype != dtype:
+    for t, name in given:
+        if t.dtype != dtype:
             raise TypeError("%s and %s dtypes differ (%s, %s)" % (a_name, name, dtype, t.dtype))
-    if a.dim() != 2 or w.dim() != 2:
+    a_shape, w_shape = a.shape, w.shape
+    if len(a_shape) != 2 or len(w_shape) != 2:
         raise ValueError("%s and w must have two dimensions, got %s and %s"
-                         % (a_name, tuple(a.shape), tuple(w.shape)))
-    if a.shape[1] != w.shape[1]:
-        raise ValueError("%s has %d columns, w %d" % (a_name, a.shape[1], w.shape[1]))
+                         % (a_name, tuple(a_shape), tuple(w_shape)))
+    if a_shape[1] != w_shape[1]:
+        raise ValueError("%s has %d columns, w %d" % (a_name, a_shape[1], w_shape[1]))
     return s
 
 
