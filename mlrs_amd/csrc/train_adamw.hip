@@ -1,10 +1,10 @@
 // The optimizer step over many tensors: the norm of all gradients with the
 // factor that clips it, and AdamW with its two moments in 32 or in 8 bits.
 //
-// A launch takes up to kTensors tensors, whose addresses and sizes travel in
-// its arguments (no table in memory, nothing kept between calls), and cuts
-// them into runs of kRun elements, one per workgroup; a workgroup finds its
-// tensor by bisection of the running counts.
+// A launch takes as many tensors as its arguments have room for with their
+// addresses and sizes (45 of a step, 135 of a norm; no table in memory, nothing
+// kept between calls), and cuts them into runs of kRun elements, one per
+// workgroup; a workgroup finds its tensor by bisection of the running counts.
 #include <algorithm>
 #include <cmath>
 
@@ -14,14 +14,15 @@
 namespace mlrs {
 namespace train {
 
-constexpr int kTensors = 40;    // in a launch: their descriptors fit in 4 KB of arguments
-constexpr int kRun = 4096;      // elements of a workgroup: 16 per thread
-constexpr int kBlock = 256;     // elements that share a scale of an 8-bit state
+constexpr int kTableBytes = 3800;  // of the 4 KB of a launch's arguments
+constexpr int kRun = 4096;         // elements of a workgroup: 16 per thread
+constexpr int kBlock = 256;        // elements that share a scale of an 8-bit state
 
 enum { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
 template <typename Item>
 struct Batch {
+    static constexpr int kTensors = kTableBytes / (int)(sizeof(Item) + 4);
     Item item[kTensors];
     int32_t first[kTensors + 1];  // running counts of runs
     int32_t count;
@@ -127,7 +128,7 @@ static hipError_t in_batches(int64_t count, Len len, Add add, Go go) {
     for (int64_t i = 0; i < count; ++i) {
         const int64_t r = runs_of(len(i));
         if (r == 0) continue;
-        if (n == kTensors || (n > 0 && runs + r > INT32_MAX)) {
+        if (n == Batch<Item>::kTensors || (n > 0 && runs + r > INT32_MAX)) {
             b.first[n] = (int32_t)runs;
             b.count = n;
             const hipError_t e = go(b, runs);

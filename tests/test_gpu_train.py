@@ -728,6 +728,13 @@ def test_clip_scale(dtype, offset):
         assert abs(float(scale) / want - 1) <= 16 * ref.U32
 
 
+def test_clip_scale_of_more_gradients_than_a_launch():
+    gs = [rand(i, (13 * i) % 300, dtype=TYPES[i % 3]) for i in range(600)]
+    square = sum(float(g.double().square().sum()) for g in gs)
+    norm, _ = prims.clip_scale([dev(g) for g in gs], 1.0)
+    assert abs(float(norm) / square ** 0.5 - 1) <= 16 * ref.U32
+
+
 def test_clip_scale_of_nothing_and_of_infinities():
     norm, scale = prims.clip_scale([torch.empty(0, device="cuda"), torch.zeros(5, device="cuda")], 1.0)
     assert float(norm) == 0.0 and float(scale) == 1.0
