@@ -392,20 +392,27 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
                 parts = stats_parts(tile, v);
             }
         }
+        // few tiles and long rows: the logits in parts
+        const Cut zc = choose_cut((int)sizeof(T), v, n, d, cus, 64, words);
+        const bool in_parts = !split && zc.splits > 1;
         // the statistics of as many rows at a time as their parts have room for
         const int64_t room = std::max(parts, parts_s);
         const int64_t rows = std::min(n, std::max<int64_t>(256, kStatsBytes / (8 * room) / 256 * 256));
         Op<T> ho(h, n, d, words), wo(w, v, d, words);
-        float *top = nullptr, *total = nullptr, *hit = nullptr;
+        float *top = nullptr, *total = nullptr, *hit = nullptr, *z = nullptr;
         char *hs = nullptr, *ws = nullptr;
         Sides sides;
         Scratch sc;
         for (int pass = 0; pass < 2; ++pass) {
             ho.plan(sc);
             wo.plan(sc);
-            top = sc.take<float>((size_t)(room * rows));
-            total = sc.take<float>((size_t)(room * rows));
-            hit = sc.take<float>((size_t)rows);
+            if (in_parts) {
+                z = sc.take<float>(zc.part_bytes(v, n) / 4);
+            } else {
+                top = sc.take<float>((size_t)(room * rows));
+                total = sc.take<float>((size_t)(room * rows));
+                hit = sc.take<float>((size_t)rows);
+            }
             if (split) {
                 hs = sc.take<char>(split_bytes(n, d));
                 ws = sc.take<char>(split_bytes(v, d));
@@ -428,6 +435,11 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         MLRS_TRY(launch_pack<T>(ho.job(), wo.job(), plain, s));
         const Mat hm = ho.mat();
         capi::Timed timed(s, "softmax_xent");
+        if (in_parts) {
+            MLRS_TRY(launch_logit_parts<T>(hm, wo.mat(), n, v, d, zc, z, s));
+            MLRS_TRY(launch_xent_rows<T>(z, zc, bias, target, n, v, ignore, loss, lse, s));
+            return MLRS_OK;
+        }
         for (int64_t r0 = 0; r0 < n; r0 += rows) {
             const int64_t r = std::min(rows, n - r0);
             if constexpr (std::is_same<T, float>::value) {
@@ -521,10 +533,12 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                           choose_cut((int)sizeof(T), d, most, n, cus, 64, words), false, 0.0};
         // one tile for every piece: its column sums are of as many parts
         const int z_tile = split_z ? kPlainCut.tile : choose_cut((int)sizeof(T), most, n, d, cus, 1, words).tile;
-        const int parts = (int)logit_grad_parts(z_tile, n);
+        const Cut zc = choose_cut((int)sizeof(T), most, n, d, cus, 64, words);
+        const bool in_parts = !split && pieces == 1 && zc.splits > 1;  // as the loss
+        const int parts = in_parts ? column_parts(n, most, cus) : (int)logit_grad_parts(z_tile, n);
         Op<T> ho(h, n, d, words), wo(w, v, d, words);
         T* dz = nullptr;
-        float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr;
+        float *acc = nullptr, *part = nullptr, *sums = nullptr, *up = nullptr, *z = nullptr;
         char *h_k = nullptr, *w_k = nullptr, *h_r = nullptr, *w_r = nullptr, *dz_k = nullptr, *dz_r = nullptr;
         Sides sides;
         Scratch sc;
@@ -534,6 +548,7 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             dz = sc.take<T>((size_t)(n * ld));
             if (dh && pieces > 1) acc = sc.take<float>((size_t)(n * dh_ld));
             if (db) sums = sc.take<float>((size_t)parts * (size_t)most);
+            if (in_parts) z = sc.take<float>(zc.part_bytes(most, n) / 4);
             if (scaled) up = sc.take<float>(2);
             size_t bytes = cut.part_bytes(d, n, d, most);
             if (split_h) bytes = std::max(bytes, sh.part_bytes(d, n));
@@ -590,9 +605,14 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
                     MLRS_TRY(launch_logit_grad_split(split_mat(h_k, d, false), split_mat(w_k, d, false), bias, target,
                                                      lse, grad, n, v0, vp, v, d, ignore, dz, ld, sums, sides.split(), s));
             }
-            MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld, sums,
-                                          z_tile,
-                                          split_z ? plain : Only{}, s));
+            if (in_parts) {
+                MLRS_TRY(launch_logit_parts<T>(hm, wm, n, v, d, zc, z, s));
+                MLRS_TRY(launch_logit_grad_rows<T>(z, zc, bias, target, lse, grad, up, n, v, ignore, dz, ld, sums,
+                                                   parts, s));
+            } else {
+                MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld, sums,
+                                              z_tile, split_z ? plain : Only{}, s));
+            }
             const StoreTo to_w{dw ? dw + v0 * d : nullptr, d, nullptr, nullptr, 0, down};
             StoreTo to_h{};
             to_h.ld = d;

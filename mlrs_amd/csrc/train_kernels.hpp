@@ -134,6 +134,20 @@ hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target,
                              int64_t ignore, T* out, int64_t ld, float* sums, int tile, const Only& only,
                              hipStream_t s);
 
+// The logits in parts of their contraction (cut.splits > 1, cut.part_bytes(classes,
+// n)), and what joins them: every row's loss, or the gradient with `parts` runs of
+// rows' column sums (sums may be null).
+template <typename T>
+hipError_t launch_logit_parts(Mat h, Mat w, int64_t n, int64_t classes, int64_t k, const Cut& cut, float* part,
+                              hipStream_t s);
+template <typename T>
+hipError_t launch_xent_rows(const float* part, const Cut& cut, const T* bias, const int64_t* target, int64_t n,
+                            int64_t classes, int64_t ignore, float* loss, float* lse, hipStream_t s);
+template <typename T>
+hipError_t launch_logit_grad_rows(const float* part, const Cut& cut, const T* bias, const int64_t* target,
+                                  const float* lse, const float* grad, const float* up, int64_t n, int64_t classes,
+                                  int64_t ignore, T* out, int64_t ld, float* sums, int parts, hipStream_t s);
+
 // f32 products on the bf16 matrix cores (train_split.hpp).  K layout: ld is
 // bytes, split_row_bytes of the columns; R layout: ld is elements, a multiple of
 // 8, of the three rows of one k.

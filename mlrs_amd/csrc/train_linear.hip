@@ -168,6 +168,13 @@ hipError_t launch_linear(Mat x, Mat w, int64_t n, int64_t m, int64_t k, const Li
     return launch_join(part, cut.splits, m, n, LinearPoint<T>{e}, only, s);
 }
 
+template <typename T>
+hipError_t launch_logit_parts(Mat h, Mat w, int64_t n, int64_t classes, int64_t k, const Cut& cut, float* part,
+                              hipStream_t s) {
+    return launch_gemm<T>(cut.tile, w, h, classes, n, k, cut.splits, cut.k_split, Only{},
+                          parts_epi<T>(part, classes, n), s);
+}
+
 // A few rows: the weights are read once, straight into registers as the
 // fragments of the matrix instructions.  A workgroup computes
 // sixteen outputs of every row; its waves take the contraction axis in turn
@@ -437,6 +444,8 @@ hipError_t launch_products(const Product& x, const Product& w, const PairCut& cu
     template hipError_t launch_pack<T>(const PackJob&, const PackJob&, const Only&, hipStream_t);                  \
     template hipError_t launch_linear<T>(Mat, Mat, int64_t, int64_t, int64_t, const LinearOut&, const Cut&, float*, \
                                          const Only&, hipStream_t);                                                \
+    template hipError_t launch_logit_parts<T>(Mat, Mat, int64_t, int64_t, int64_t, const Cut&, float*,             \
+                                              hipStream_t);                                                        \
     template hipError_t launch_linear_few<T>(const T*, const T*, int64_t, int64_t, int64_t, const LinearOut&,      \
                                              hipStream_t);                                                         \
     template hipError_t launch_act_grad<T>(const T*, const T*, int, int64_t, int64_t, T*, int64_t,                 \

@@ -127,12 +127,156 @@ hipError_t launch_logit_grad(Mat h, Mat w, const T* bias, const int64_t* target,
     return launch_gemm<T>(tile, wp, h, piece, n, k, 1, 0, only, e, s);
 }
 
+// ---------------------------------------------------------------------------
+// few classes and few rows, long rows
+// ---------------------------------------------------------------------------
+// A dozen tiles would leave most CUs idle, and statistics need whole sums: the
+// logits' contraction is split, and a second kernel joins its parts on the way to
+// the loss or the gradient, as small a matrix as they are then.  76 x 344 by 3473
+// in f32: 92 us in twelve tiles, 21 so; 64 x 1000 by 2048 48 and 18.
+template <typename T>
+struct LogitParts {
+    const float* part;
+    int splits;
+    int64_t stride, ld;
+    const T* bias;
+    __device__ __forceinline__ f32x4 at(int64_t row, int64_t c, int64_t classes) const {
+        const float* from = part + row * ld + c;
+        f32x4 z = *reinterpret_cast<const f32x4*>(from);
+        for (int s = 1; s < splits; ++s) z += *reinterpret_cast<const f32x4*>(from + s * stride);
+        if (bias) z += load4(bias, c, classes);
+        return z;
+    }
+};
+template <typename T>
+static LogitParts<T> logit_parts(const float* part, const Cut& cut, const T* bias, int64_t n, int64_t classes) {
+    const int64_t ld = (classes + 3) & ~(int64_t)3;
+    return LogitParts<T>{part, cut.splits, n * ld, ld, bias};
+}
+
+// A workgroup computes a row's loss, in two walks over its logits.
+template <typename T>
+__global__ __launch_bounds__(256) void xent_rows_kernel(LogitParts<T> z, const int64_t* __restrict__ target,
+                                                        int64_t classes, int64_t ignore, float* __restrict__ loss,
+                                                        float* __restrict__ lse) {
+    __shared__ float join[4];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float none = -__builtin_huge_valf();
+    float mx = none;
+    for (int64_t c = threadIdx.x * 4; c < classes; c += 1024) {
+        const f32x4 v = z.at(row, c, classes);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < classes) mx = fmaxf(mx, v[e]);
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s));
+    if (lane == 0) join[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(join[0], join[1]), fmaxf(join[2], join[3]));
+    __syncthreads();
+    // as in the tiles' statistics: a NaN logit reaches the sum
+    const float base = mx == none ? 0.0f : mx;
+    float sum = 0.0f;
+    for (int64_t c = threadIdx.x * 4; c < classes; c += 1024) {
+        const f32x4 v = z.at(row, c, classes);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < classes) sum += exp_fast(v[e] - base);
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+    if (lane == 0) join[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    const float l = base + logf((join[0] + join[1]) + (join[2] + join[3]));
+    lse[row] = l;
+    const int64_t t = target[row];
+    float v = 0.0f;
+    if (t != ignore) v = __builtin_nanf("");
+    if (t != ignore && t >= 0 && t < classes) {
+        const f32x4 q = z.at(row, t & ~(int64_t)3, classes);
+        const int e = (int)(t & 3);
+        v = l - (e == 0 ? q[0] : e == 1 ? q[1] : e == 2 ? q[2] : q[3]);
+    }
+    loss[row] = v;
+}
+
+// The gradient of the logits, as LogitGradEpi's; 256 columns and a run of rows to
+// a workgroup, whose column sums are left as its part.
+template <typename T>
+__global__ __launch_bounds__(256) void logit_grad_rows_kernel(LogitParts<T> z, const int64_t* __restrict__ target,
+                                                              const float* __restrict__ lse,
+                                                              const float* __restrict__ grad,
+                                                              const float* __restrict__ up, int64_t n, int64_t classes,
+                                                              int64_t ignore, T* __restrict__ out, int64_t ld,
+                                                              float* __restrict__ sums, int64_t rows_per) {
+    __shared__ f32x4 join[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per;
+    const int64_t r1 = r0 + rows_per < n ? r0 + rows_per : n;
+    const float scale = up ? *up : 1.0f;
+    f32x4 sum = {};
+    if (c < ld) {
+        for (int64_t r = r0 + wave; r < r1; r += 4) {
+            const int64_t t = target[r];
+            const bool valid = t >= 0 && t < classes;
+            const float l = lse[r], by = valid ? grad[r] * scale : __builtin_nanf("");
+            typename Elem<T>::Vec4 v = {};
+            if (t != ignore && c < classes) {
+                const f32x4 q = z.at(r, c, classes);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = sizeof(T) == 2 ? __builtin_amdgcn_exp2f(__builtin_fmaf(q[e], kLog2E, -l * kLog2E))
+                                                   : exp_fast(q[e] - l);
+                    if (c + e < classes) v[e] = (T)((p - (t == c + e ? 1.0f : 0.0f)) * by);
+                }
+            }
+            *reinterpret_cast<typename Elem<T>::Vec4*>(out + r * ld + c) = v;
+            sum += widen(v);
+        }
+    }
+    if (!sums) return;
+    join[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && c < classes) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) sum += join[i][lane];
+        store4(sums + (int64_t)blockIdx.y * classes, c, classes, sum);
+    }
+}
+
+template <typename T>
+hipError_t launch_xent_rows(const float* part, const Cut& cut, const T* bias, const int64_t* target, int64_t n,
+                            int64_t classes, int64_t ignore, float* loss, float* lse, hipStream_t s) {
+    xent_rows_kernel<T><<<dim3((unsigned)n), 256, 0, s>>>(logit_parts(part, cut, bias, n, classes), target, classes,
+                                                          ignore, loss, lse);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_logit_grad_rows(const float* part, const Cut& cut, const T* bias, const int64_t* target,
+                                  const float* lse, const float* grad, const float* up, int64_t n, int64_t classes,
+                                  int64_t ignore, T* out, int64_t ld, float* sums, int parts, hipStream_t s) {
+    const int64_t rows_per = (n + parts - 1) / parts;
+    logit_grad_rows_kernel<T><<<dim3((unsigned)((ld + 255) / 256), (unsigned)parts), 256, 0, s>>>(
+        logit_parts(part, cut, bias, n, classes), target, lse, grad, up, n, classes, ignore, out, ld, sums, rows_per);
+    return hipGetLastError();
+}
+
 #define MLRS_INST(T)                                                                                              \
     template hipError_t launch_xent_stats<T>(Mat, Mat, const T*, const int64_t*, int64_t, int64_t, int64_t, int,  \
                                              float*, float*, float*, const Only&, hipStream_t);                   \
     template hipError_t launch_logit_grad<T>(Mat, Mat, const T*, const int64_t*, const float*, const float*,      \
                                              const float*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,  \
-                                             T*, int64_t, float*, int, const Only&, hipStream_t);
+                                             T*, int64_t, float*, int, const Only&, hipStream_t);                 \
+    template hipError_t launch_xent_rows<T>(const float*, const Cut&, const T*, const int64_t*, int64_t, int64_t, \
+                                            int64_t, float*, float*, hipStream_t);                                \
+    template hipError_t launch_logit_grad_rows<T>(const float*, const Cut&, const T*, const int64_t*,             \
+                                                  const float*, const float*, const float*, int64_t, int64_t,     \
+                                                  int64_t, T*, int64_t, float*, int, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)

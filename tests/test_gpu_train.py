@@ -278,6 +278,37 @@ def test_xent_unaligned_and_every_tile(dtype):
     check_xent(1030, 1100, 40, dtype, seed=2)
 
 
+# a few tiles of logits, each a long sum: computed in parts of the contraction
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,k", [(1, 5, 4096), (17, 1000, 2048), (76, 344, 3473), (129, 66, 5003)])
+def test_xent_few_classes_and_long_rows(dtype, n, v, k):
+    check_xent(n, v, k, dtype, seed=n + v + k)
+    check_xent(n, v, k, dtype, bias=False, offset=1, seed=n + v)
+    if v > 300:
+        check_xent(n, v, k, dtype, masked=list(range(0, 260)) + [v - 1], seed=n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_xent_long_rows_that_are_not_finite(dtype):
+    """A row with a NaN, one whose logits are all -inf and one whose target is no
+    class leave the others as they are."""
+    n, v, k = 70, 130, 4000
+    h, w, t = rand(1, n, k, dtype=dtype), rand(2, v, k, dtype=dtype, std=0.03), targets(3, n, v, ignored=0.0)
+    g = torch.full((n,), 1.0 / n)
+    plain = prims.softmax_xent(dev(h), dev(w), dev(t))
+    dz = prims.softmax_xent_grad(dev(h), dev(w), dev(t), plain[1], dev(g), need_dw=False)[0]
+    w[:, 7], h[:, 7] = w[:, 7].abs() + 0.5, 0.0
+    base = prims.softmax_xent(dev(h), dev(w), dev(t))
+    h[5, 9], h[6, 7], t[8] = float("nan"), float("-inf"), v
+    loss, lse = prims.softmax_xent(dev(h), dev(w), dev(t))
+    dh = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, dev(g), need_dw=False)[0]
+    assert loss[5].isnan() and lse[5].isnan() and lse[6] == float("-inf") and loss[8].isnan()
+    assert dh[5].isnan().all() and dh[8].isnan().all()
+    kept = [i for i in range(n) if i not in (5, 6, 8)]
+    assert torch.equal(loss[kept], base[0][kept]) and torch.equal(lse[kept], base[1][kept])
+    assert dh[kept].isfinite().all() and dz.isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_xent_wide_logits(dtype):
     """Logits tens apart: one class has nearly all of a row, others nothing."""
