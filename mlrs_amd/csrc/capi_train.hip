@@ -579,7 +579,9 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
         const Only plain = split ? sides.plain() : Only{};
         const bool all_split = split_z && (!dh || split_h) && (!dw || split_w);
         if (scaled) MLRS_TRY(launch_grad_scale(grad, target, n, ignore, up, s));
-        const float* down = scaled ? up + 1 : nullptr;
+        const bool first_row = std::is_same<T, __bf16>::value;
+        const float* down = scaled ? up + 1 : first_row ? grad : nullptr;
+        const float* lift = scaled ? up : down;
         const Mat hm = ho.mat(), wm = wo.mat();
         capi::Timed timed(s, "softmax_xent_grad");
         if constexpr (std::is_same<T, float>::value) {
@@ -607,10 +609,10 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             }
             if (in_parts) {
                 MLRS_TRY(launch_logit_parts<T>(hm, wm, n, v, d, zc, z, s));
-                MLRS_TRY(launch_logit_grad_rows<T>(z, zc, bias, target, lse, grad, up, n, v, ignore, dz, ld, sums,
+                MLRS_TRY(launch_logit_grad_rows<T>(z, zc, bias, target, lse, grad, lift, n, v, ignore, dz, ld, sums,
                                                    parts, s));
             } else {
-                MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, up, n, v0, vp, v, d, ignore, dz, ld, sums,
+                MLRS_TRY(launch_logit_grad<T>(hm, wm, bias, target, lse, grad, lift, n, v0, vp, v, d, ignore, dz, ld, sums,
                                               z_tile, split_z ? plain : Only{}, s));
             }
             const StoreTo to_w{dw ? dw + v0 * d : nullptr, d, nullptr, nullptr, 0, down};

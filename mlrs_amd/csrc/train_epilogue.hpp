@@ -96,6 +96,27 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
     }
 }
 
+// A 16-bit gradient of the logits is rounded before its products.  The rows of a
+// mean share one gradient, 1 / n, and where the other classes' shares are small the
+// target's element is nearly that in every row: its rounding error, up to 2^-8 of
+// bf16's, would be common to all and show in the results as it is.  So the
+// gradients are divided by the fraction of one of them (1 <= f < 2), which puts such
+// elements just below a power of two, where a rounding error is 2^-9 at most and
+// goes by each row's probability; the products and the sums are multiplied by it.
+// bf16 takes the first row's gradient's; f16 a factor from memory that also lifts
+// the gradients into the type's range.
+__device__ __forceinline__ float fraction_of(float x) {
+    return __uint_as_float((__float_as_uint(x) & 0x7FFFFFu) | 0x3F800000u);  // in [1, 2), whatever x is
+}
+template <typename T>
+__device__ __forceinline__ float up_factor(const float* p) {
+    return __is_same(T, __bf16) ? 1.0f / fraction_of(*p) : *p;
+}
+template <typename T>
+__device__ __forceinline__ float down_factor(const float* p) {
+    return __is_same(T, __bf16) ? fraction_of(*p) : *p;
+}
+
 // Four consecutive elements of a row from m on, those at or past `end` left
 // out.  Global accesses need no more than their elements' alignment, so rows of
 // any length are read and written four elements at a time.
@@ -291,7 +312,7 @@ struct StoreEpi {
             for (int u = 0; u < N; ++u) v[u] += old[u];
         }
         if (out) {
-            const float by = alpha ? *alpha : 1.0f;
+            const float by = alpha ? down_factor<T>(alpha) : 1.0f;
 #pragma unroll
             for (int u = 0; u < N; ++u)
                 if (n + u * step < n_end) store4(out + (n + u * step) * ld, m, end, v[u] * by);
@@ -405,8 +426,8 @@ struct StatsEpi {
 // zero in ignored rows, NaN in rows whose target is no class.  Rounded to the
 // operands' type, as it goes into two matrix products with them: the products
 // still add in f32, and a 16-bit gradient's own rounding is of the same size.
-// `up` scales it by a power of two first (f16: the gradients of a mean over a
-// batch times the probabilities of a large vocabulary lie below f16's range).
+// `up` scales it first (f16: the gradients of a mean over a batch times the
+// probabilities of a large vocabulary lie below f16's range).
 template <typename T>
 struct LogitGradEpi {
     const T* bias;
@@ -431,7 +452,7 @@ struct LogitGradEpi {
         constexpr int kPieces = kRow / 16;
         constexpr int kStep = 64 / kPieces;             // rows that the lanes cover together
         const int g = p.lane >> 4, r = p.lane & 15;
-        const float scale = up ? *up : 1.0f;
+        const float scale = up ? up_factor<T>(up) : 1.0f;
         float l[NB], by[NB];
         int32_t hot[NB];    // the target's place among the wave's classes
         uint32_t keep[NB];  // all ones, or none in an ignored row

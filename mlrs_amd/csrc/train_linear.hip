@@ -336,7 +336,7 @@ __device__ __forceinline__ void sum_parts(const ColumnSums<T>& to, int64_t m, in
     if (slice != 0 || c >= m) return;
 #pragma unroll
     for (int i = 1; i < kSlices; ++i) v += join[i * 16 + col];
-    if (to.alpha) v *= *to.alpha;
+    if (to.alpha) v *= down_factor<T>(to.alpha);
     to.out[c] = (T)v;
 }
 template <typename T>

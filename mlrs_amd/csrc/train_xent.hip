@@ -83,9 +83,9 @@ hipError_t launch_xent_join(const float* top, const float* total, int64_t parts,
     return hipGetLastError();
 }
 
-// up_down[0]: the power of two that brings the largest |gradient| of a kept row
-// to 2^13 .. 2^14, so that the products of it with probabilities down to 2^-28
-// are normal numbers of half precision; up_down[1]: its inverse.
+// up_down[0]: the factor that brings the largest |gradient| of a kept row to 2^13,
+// so that the products of it with probabilities down to 2^-27 are normal numbers of
+// half precision; up_down[1]: its inverse.
 __global__ __launch_bounds__(1024) void grad_scale_kernel(const float* __restrict__ grad,
                                                           const int64_t* __restrict__ target, int64_t n,
                                                           int64_t ignore, float* __restrict__ up_down) {
@@ -101,11 +101,12 @@ __global__ __launch_bounds__(1024) void grad_scale_kernel(const float* __restric
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, most[i]);
     int e = (int)((__float_as_uint(mx) >> 23) & 255u) - 127;  // mx in 2^e .. 2^(e+1)
     // nothing to scale, or nothing finite; and both factors stay normal
-    if (mx == 0.0f || e == 128) e = 13;
-    e = 13 - e;
+    const bool as_is = mx == 0.0f || e == 128;
+    const float f = as_is ? 1.0f : fraction_of(mx);
+    e = as_is ? 0 : 13 - e;
     e = e < -120 ? -120 : e > 120 ? 120 : e;
-    up_down[0] = __uint_as_float((uint32_t)(127 + e) << 23);
-    up_down[1] = __uint_as_float((uint32_t)(127 - e) << 23);
+    up_down[0] = __uint_as_float((uint32_t)(127 + e) << 23) / f;
+    up_down[1] = __uint_as_float((uint32_t)(127 - e) << 23) * f;
 }
 
 hipError_t launch_grad_scale(const float* grad, const int64_t* target, int64_t n, int64_t ignore, float* up_down,
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256) void logit_grad_rows_kernel(LogitParts<T> z, c
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
     const int64_t r0 = (int64_t)blockIdx.y * rows_per;
     const int64_t r1 = r0 + rows_per < n ? r0 + rows_per : n;
-    const float scale = up ? *up : 1.0f;
+    const float scale = up ? up_factor<T>(up) : 1.0f;
     f32x4 sum = {};
     if (c < ld) {
         for (int64_t r = r0 + wave; r < r1; r += 4) {

@@ -425,6 +425,25 @@ def test_xent_half_precision_gradient_range(size):
     ref.assert_near(dw, want["dw"], "dw")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_xent_common_gradient_is_not_rounded(dtype):
+    """Rows that share a gradient g halfway between two numbers of the type, three
+    of them to a target's class, and probabilities of 1 / v: a class's sum is
+    -3 g but for 3 g / v.  With u the type's unit its rounding costs u / 3, as
+    3 + 3 u lies a quarter of a step from 3 + 4 u; rounding p - 1 costs p at most;
+    each row's g rounded by itself would cost u."""
+    n, v, k = 24, 40000, 16
+    unit = ref.UNIT[dtype]
+    g = (1.0 + unit) / 32.0
+    h, w = rand(1, n, k, dtype=dtype), rand(2, v, k, dtype=dtype, std=0.001)
+    t, b = torch.arange(n) // 3 * 200, torch.zeros(v, dtype=dtype)
+    _, lse = prims.softmax_xent(dev(h), dev(w), dev(t), bias=dev(b))
+    _, _, db = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, torch.full((n,), g, device="cuda"), bias=dev(b))
+    classes = t.unique()
+    err = (db.cpu()[classes].double() / (-3.0 * g) - 1.0).abs()
+    assert float(err.max()) <= 0.5 * unit + (3 + n) / v
+
+
 def test_xent_gradient_against_differences():
     n, v, k, e = 30, 90, 20, 1e-5
     h, w, b, t, c = rand(1, n, k), rand(2, v, k, std=0.3), rand(3, v), targets(4, n, v), rand(5, n)
