@@ -218,10 +218,11 @@ class EmbeddingEncoder:
         return self.fit(X, y).transform(X)
 
     def predict(self, X):
-        """The class the head gives each row."""
-        x, was_numpy = self._rows(X)
+        """The class the head gives each row, as ``fit`` was given it: a NumPy
+        array, whatever holds the rows."""
+        x, _ = self._rows(X)
         code = prims.linear(self._encode(x), self._params[-2], bias=self._params[-1]).argmax(1)
-        return self.classes_[code.cpu().numpy()] if was_numpy else code
+        return self.classes_.take(code.cpu().numpy())
 
     def score(self, X, y):
         """The mean cross entropy of the rows, lower is better."""

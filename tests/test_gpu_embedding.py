@@ -85,6 +85,21 @@ def test_a_fit_is_repeatable_and_takes_labels_of_any_kind():
         a.score(x[:2], np.array(["up", "north"]))
 
 
+@pytest.mark.parametrize("labels", [[30, 10, 20, 40], ["north", "south", "east", "west"], [2.5, -1.0, 7.25, 0.5]])
+def test_predictions_are_classes_whatever_holds_the_rows(labels):
+    """Not their places among the classes: of a NumPy array, of a tensor on
+    either device."""
+    x, y = rows(4, 900)
+    names = np.array(labels)[y]
+    e = EmbeddingEncoder(n_components=4, hidden=(16,), epochs=2, batch_size=300, learning_rate=3e-3).fit(x, names)
+    want = e.predict(x[:200])
+    assert want.dtype == names.dtype and set(want) <= set(names)
+    for t in (torch.from_numpy(x[:200]), torch.from_numpy(x[:200]).cuda()):
+        got = e.predict(t)
+        assert isinstance(got, np.ndarray) and got.dtype == names.dtype and np.array_equal(got, want)
+    assert np.mean(want == names[:200]) > 0.4  # a quarter by chance
+
+
 def test_the_optimizer_refuses_what_it_cannot_hold():
     p = torch.zeros(3, 2, device="cuda")
     with pytest.raises(ValueError, match="state_bits"):
