@@ -97,7 +97,12 @@ def test_predictions_are_classes_whatever_holds_the_rows(labels):
     for t in (torch.from_numpy(x[:200]), torch.from_numpy(x[:200]).cuda()):
         got = e.predict(t)
         assert isinstance(got, np.ndarray) and got.dtype == names.dtype and np.array_equal(got, want)
-    assert np.mean(want == names[:200]) > 0.4  # a quarter by chance
+    h = e.transform(x[:200]).astype(np.float64)
+    head, bias = (p.double().cpu().numpy() for p in e._params[-2:])
+    z = h @ head.T + bias
+    near = np.sort(z, axis=1)
+    sure = near[:, -1] - near[:, -2] > 1e-4  # far beyond float32's error of logits of size 1
+    assert sure.sum() > 150 and np.array_equal(want[sure], np.unique(names)[z.argmax(1)][sure])
 
 
 def test_the_optimizer_refuses_what_it_cannot_hold():
