@@ -17,6 +17,7 @@ import torch
 from . import prims
 from .neighbors import _as_device_matrix, _check_finite
 
+_LOGITS = 1 << 26  # that predict holds at a time
 _DTYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
 
 
@@ -219,9 +220,15 @@ class EmbeddingEncoder:
 
     def predict(self, X):
         """The class the head gives each row, as ``fit`` was given it: a NumPy
-        array, whatever holds the rows."""
+        array, whatever holds the rows.  The logits are float32, as in the loss:
+        rounded to a 16-bit type, near classes would tie."""
         x, _ = self._rows(X)
-        code = prims.linear(self._encode(x), self._params[-2], bias=self._params[-1]).argmax(1)
+        h = self._encode(x)
+        head, bias = (p.float() for p in self._params[-2:])
+        code = torch.empty(len(h), dtype=torch.int64, device=h.device)
+        rows = max(1, _LOGITS // len(head))
+        for i in range(0, len(h), rows):
+            code[i:i + rows] = prims.linear(h[i:i + rows].float(), head, bias=bias).argmax(1)
         return self.classes_.take(code.cpu().numpy())
 
     def score(self, X, y):

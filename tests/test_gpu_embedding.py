@@ -105,6 +105,26 @@ def test_predictions_are_classes_whatever_holds_the_rows(labels):
     assert sure.sum() > 150 and np.array_equal(want[sure], np.unique(names)[z.argmax(1)][sure])
 
 
+@pytest.mark.parametrize("dtype,step", [("float32", 2.0 ** -18), ("float16", 2.0 ** -9), ("bfloat16", 2.0 ** -6)])
+def test_predictions_of_classes_nearer_than_the_type_tells_apart(dtype, step, monkeypatch):
+    """Logits 10, 10 + 2 s and 10 + s, s below half a step of the parameters'
+    type: the second is the largest, as it is to the loss; the same a few rows
+    at a time, and of no rows."""
+    e = EmbeddingEncoder(n_components=3, hidden=(), dtype=dtype)
+    t = getattr(torch, dtype)
+    head = torch.tensor([[1.0, 0.0, 0.0], [1.0, 2 * step, 0.0], [1.0, step, 0.0]], device="cuda", dtype=t)
+    e._params = [torch.eye(3, device="cuda", dtype=t), torch.zeros(3, device="cuda", dtype=t), head,
+                 torch.zeros(3, device="cuda", dtype=t)]
+    e.classes_, e.n_features_in_ = np.array([7, 8, 9]), 3
+    x = np.tile(np.array([[10.0, 1.0, 0.0]], dtype=np.float32), (50, 1))
+    x[::2, 1] = -1.0  # the first is the largest
+    want = np.where(np.arange(50) % 2, 8, 7)
+    assert np.array_equal(e.predict(x), want)
+    monkeypatch.setattr("mlrs_amd.embedding._LOGITS", 21)
+    assert np.array_equal(e.predict(x), want)
+    assert e.predict(x[:0]).shape == (0,)
+
+
 def test_the_optimizer_refuses_what_it_cannot_hold():
     p = torch.zeros(3, 2, device="cuda")
     with pytest.raises(ValueError, match="state_bits"):
