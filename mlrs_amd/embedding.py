@@ -157,7 +157,8 @@ class EmbeddingEncoder:
     def fit(self, X, y):
         widths = self._validate()
         x, _ = _as_device_matrix(X)
-        _check_finite(x)
+        x = x.to(_DTYPES[self.dtype])
+        _check_finite(x)  # as the layers read it: 65520 is no float16
         labels = y.cpu().numpy() if isinstance(y, torch.Tensor) else np.asarray(y)
         if labels.shape != (x.shape[0],):
             raise ValueError("y has shape %s, expected (%d,)" % (labels.shape, x.shape[0]))
@@ -171,7 +172,6 @@ class EmbeddingEncoder:
         gen = torch.Generator(device=x.device)
         gen.manual_seed(seed)
         self.n_features_in_ = d
-        x = x.to(_DTYPES[self.dtype])
         self._params = self._init_params(d, widths, len(self.classes_), x.device, gen)
         optimizer = AdamW(self._params, lr=float(self.learning_rate), weight_decay=float(self.weight_decay),
                           max_norm=self.max_norm, state_bits=self.state_bits, seed=seed)
@@ -206,8 +206,9 @@ class EmbeddingEncoder:
         if x.shape[1] != self.n_features_in_:
             raise ValueError("X has %d features, but EmbeddingEncoder is expecting %d features as input"
                              % (x.shape[1], self.n_features_in_))
+        x = x.to(_DTYPES[self.dtype])
         _check_finite(x)
-        return x.to(_DTYPES[self.dtype]), was_numpy
+        return x, was_numpy
 
     def transform(self, X):
         """The embedding of every row, float32 (n, n_components)."""

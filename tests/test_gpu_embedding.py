@@ -125,6 +125,26 @@ def test_predictions_of_classes_nearer_than_the_type_tells_apart(dtype, step, mo
     assert e.predict(x[:0]).shape == (0,)
 
 
+@pytest.mark.parametrize("dtype,big", [("float16", 65520.0), ("float32", 1e39), ("bfloat16", 3.4e38)])
+def test_features_that_the_type_cannot_hold_are_refused(dtype, big):
+    """Finite ones that round to an infinity of the element type."""
+    x, y = rows(5, 300)
+    x = x.astype(np.float64)
+    far = x.copy()
+    far[7, 3] = big
+    e = EmbeddingEncoder(n_components=4, hidden=(8,), epochs=1, batch_size=100, dtype=dtype)
+    for rows_of in (far, torch.from_numpy(far)):
+        with pytest.raises(ValueError, match="too large for dtype.*%s" % dtype):
+            e.fit(rows_of, y)
+    e.fit(x, y)
+    for call in (e.transform, e.predict, lambda r: e.score(r, y)):
+        with pytest.raises(ValueError, match="too large for dtype.*%s" % dtype):
+            call(far)
+    far[7, 3] = np.nan
+    with pytest.raises(ValueError, match="contains NaN"):
+        e.transform(far)
+
+
 def test_the_optimizer_refuses_what_it_cannot_hold():
     p = torch.zeros(3, 2, device="cuda")
     with pytest.raises(ValueError, match="state_bits"):
