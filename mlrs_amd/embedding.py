@@ -27,7 +27,9 @@ class AdamW:
 
     ``step(grads)`` takes one step in place; with ``max_norm`` the gradients are
     clipped to that norm first, and a step whose norm is not finite changes
-    nothing.  Tensors of one dimension do not decay."""
+    nothing but the count of steps; float16 parameters, whose gradients may leave
+    the type's range, have that without a ``max_norm`` too.  Tensors of one
+    dimension do not decay."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_norm=None, state_bits=32,
                  seed=0):
@@ -42,6 +44,7 @@ class AdamW:
         if any(half) != all(half):
             raise ValueError("float32 and 16-bit parameters cannot share an optimizer")
         self.masters = [p.float() for p in self.params] if half[0] else None
+        self.overflows = any(p.dtype == torch.float16 for p in self.params)
         kind = torch.float32 if state_bits == 32 else torch.uint8
         self.exp_avg = [torch.zeros_like(p, dtype=kind) for p in self.params]
         self.exp_avg_sq = [torch.zeros_like(p, dtype=kind) for p in self.params]
@@ -54,10 +57,10 @@ class AdamW:
 
     def step(self, grads):
         """One step; returns the gradients' norm (a device tensor) with
-        ``max_norm``, else None."""
+        ``max_norm`` or float16 parameters, else None."""
         norm = scale = None
-        if self.max_norm is not None:
-            norm, scale = prims.clip_scale(grads, self.max_norm)
+        if self.max_norm is not None or self.overflows:
+            norm, scale = prims.clip_scale(grads, float("inf") if self.max_norm is None else self.max_norm)
         self.steps += 1
         prims.adamw_step(self.params, grads, self.exp_avg, self.exp_avg_sq, step=self.steps, lr=self.lr,
                          betas=self.betas, eps=self.eps, weight_decay=self.decays, masters=self.masters,

@@ -145,6 +145,22 @@ def test_features_that_the_type_cannot_hold_are_refused(dtype, big):
         e.transform(far)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_half_precision_gradients_past_its_range_change_nothing(bits):
+    """Also where no norm clips them."""
+    p = [torch.ones(300, 2, dtype=torch.float16, device="cuda"), torch.ones(5, dtype=torch.float16, device="cuda")]
+    o = AdamW(p, max_norm=None, state_bits=bits, lr=0.1)
+    g = [torch.ones_like(t) for t in p]
+    held = p + o.masters + o.exp_avg + o.exp_avg_sq
+    before = [t.clone() for t in held]
+    g[1][2] = float("inf")
+    o.step(g)
+    assert all(torch.equal(a, b) for a, b in zip(held, before))
+    g[1][2] = 1.0
+    o.step(g)
+    assert all(bool((t < 1.0).all()) for t in p + o.masters)
+
+
 def test_the_optimizer_refuses_what_it_cannot_hold():
     p = torch.zeros(3, 2, device="cuda")
     with pytest.raises(ValueError, match="state_bits"):
