@@ -11,6 +11,8 @@ the loss over the classes and the optimizer's step are the library's kernels
 ``clip_scale``, ``adamw_step``): the logits of a batch are never in memory, and
 a step reads nothing back.
 """
+import warnings
+
 import numpy as np
 import torch
 
@@ -80,7 +82,8 @@ class EmbeddingEncoder:
     the number of passes over the rows.  ``random_state=None`` is seed 0.
 
     After ``fit``: ``classes_``, ``loss_curve_`` (the mean loss of each epoch),
-    ``n_features_in_``.
+    ``n_features_in_``.  Steps whose gradients are not finite are skipped (with
+    ``max_norm`` or float16), and a warning tells how many they were.
     """
 
     def __init__(self, n_components=64, hidden=(256,), activation="gelu", epochs=10, batch_size=1024,
@@ -185,7 +188,7 @@ class EmbeddingEncoder:
             optimizer.eps *= up
             if optimizer.max_norm is not None:
                 optimizer.max_norm *= up
-        self.loss_curve_ = []
+        self.loss_curve_, norms, skipped, steps = [], [], [], 0
         for _ in range(int(self.epochs)):
             order = torch.randperm(n, device=x.device, generator=gen)
             total = torch.zeros((), device=x.device)
@@ -193,10 +196,20 @@ class EmbeddingEncoder:
                 rows = order[start:start + int(self.batch_size)]
                 weight = torch.full((len(rows),), up / len(rows), device=x.device)
                 loss, grads = self._loss_and_grads(x[rows], target[rows], weight)
-                optimizer.step(grads)
+                norm = optimizer.step(grads)
+                steps += 1
+                if norm is not None:
+                    norms.append(norm)
                 total += loss.sum()
             self.loss_curve_.append(total / n)
+            if norms:
+                skipped.append((~torch.cat(norms).isfinite()).sum())
+                norms = []
         self.loss_curve_ = torch.stack(self.loss_curve_).cpu().tolist()
+        skipped = int(sum(skipped))
+        if skipped:
+            warnings.warn("%d of %d steps were skipped: their gradients are not finite in %s (scale the features down, "
+                          "or use another dtype)" % (skipped, steps, self.dtype), RuntimeWarning, stacklevel=2)
         return self
 
     def _check_fitted(self):

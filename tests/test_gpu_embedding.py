@@ -1,5 +1,7 @@
 """EmbeddingEncoder: its gradients against automatic differentiation in 64
 bits, and a search over what it learns."""
+import warnings
+
 import numpy as np
 import pytest
 import torch
@@ -159,6 +161,21 @@ def test_half_precision_gradients_past_its_range_change_nothing(bits):
     g[1][2] = 1.0
     o.step(g)
     assert all(bool((t < 1.0).all()) for t in p + o.masters)
+
+
+@pytest.mark.parametrize("max_norm", [1.0, None])
+def test_steps_that_fit_skips_are_told(max_norm):
+    """Rows within half precision's range whose products are past it: no step is
+    taken, the parameters stay finite, and a warning says so."""
+    x, y = rows(6, 300)
+    kw = dict(n_components=4, hidden=(8,), epochs=2, batch_size=100, dtype="float16", max_norm=max_norm)
+    far = x * np.float32(60000.0) / np.abs(x).max(1, keepdims=True)
+    with pytest.warns(RuntimeWarning, match="6 of 6 steps"):
+        e = EmbeddingEncoder(**kw).fit(np.abs(far), y)
+    assert all(p.isfinite().all() for p in e._params)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        EmbeddingEncoder(**kw).fit(x, y)
 
 
 def test_the_optimizer_refuses_what_it_cannot_hold():
