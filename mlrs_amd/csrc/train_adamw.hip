@@ -67,23 +67,22 @@ struct NormItem {
     int32_t dtype;
 };
 
-// A workgroup's sum of squares.  Each thread adds its sixteen in f32 (their
-// relative error stays under 2^-20); the threads' and then the workgroups'
-// sums are added in f64, in a fixed order.
+// A workgroup's sum of squares, in f64 from the squares on, as f32 and bf16
+// elements past 2^64 or below 2^-75 have squares that f32 cannot hold.  Added in a
+// fixed order: a thread's sixteen, the threads', the workgroups'.
 __global__ __launch_bounds__(256) void norm_kernel(Batch<NormItem> b, double* __restrict__ parts) {
     const int t = find_item(b, (int32_t)blockIdx.x);
     const NormItem& it = b.item[t];
     const int64_t at = (int64_t)((int32_t)blockIdx.x - b.first[t]) * kRun;
-    float sum = 0.0f;
+    double d = 0.0;
 #pragma unroll
     for (int u = 0; u < kRun / 1024; ++u) {
         const int64_t i = at + u * 1024 + threadIdx.x * 4;
         if (i >= it.len) continue;
         const f32x4 v = load_any(it.g, it.dtype, i, it.len);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += v[e] * v[e];
+        for (int e = 0; e < 4; ++e) d = __builtin_fma((double)v[e], (double)v[e], d);
     }
-    double d = (double)sum;
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) d += __shfl_xor(d, s);
     __shared__ double join[4];
@@ -106,7 +105,7 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(const double* __restric
     for (int i = 1; i < 16; ++i) d += join[i];
     const double root = sqrt(d);
     *norm = (float)root;
-    const bool finite = root < __builtin_huge_val();  // false for NaN too
+    const bool finite = (float)root < __builtin_huge_valf();  // false for NaN too
     *scale = !finite ? __builtin_nanf("") : root > max_norm ? (float)(max_norm / root) : 1.0f;
 }
 

@@ -793,3 +793,18 @@ def test_clip_scale_of_nothing_and_of_infinities():
         g[4321] = bad
         norm, scale = prims.clip_scale([torch.ones(3, device="cuda"), g], 1.0)
         assert not norm.isfinite().any() and scale.isnan().all()
+
+
+@pytest.mark.parametrize("dtype,size", [(F32, 1e20), (F32, 1e-25), (F32, 3e38), (BF16, 1e20), (BF16, 1e-25), (F16, 6e4)])
+def test_clip_scale_of_gradients_whose_squares_f32_cannot_hold(dtype, size):
+    gs = [(rand(i, n).clamp(-1, 1) * 0.01 * size).to(dtype) for i, n in enumerate((5000, 3))]
+    gs[0][77] = size
+    want = sum(float(g.double().square().sum()) for g in gs) ** 0.5
+    norm, scale = prims.clip_scale([dev(g) for g in gs], size / 2)
+    assert abs(float(norm) / want - 1) <= 16 * ref.U32
+    assert abs(float(scale) / (size / 2 / want) - 1) <= 16 * ref.U32
+
+
+def test_clip_scale_of_a_norm_that_f32_cannot_hold():
+    norm, scale = prims.clip_scale([torch.full((100,), 3e38, device="cuda")], 1.0)
+    assert float(norm) == float("inf") and scale.isnan().all()
