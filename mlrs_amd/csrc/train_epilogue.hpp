@@ -85,8 +85,9 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
         return cdf + z * (0.5f * kGeluC) * bell;
     }
     case kActGeluTanh: {
+        // from |z| = 16 on s is 0 or 1, and z^2 may leave f32's range
         const float s = sigmoid(2.0f * kGeluC * (z + kGeluB * z * z * z));
-        return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluB * z * z);
+        return s + z * s * (1.0f - s) * 2.0f * kGeluC * (1.0f + 3.0f * kGeluB * fminf(z * z, 256.0f));
     }
     case kActSilu: {
         const float s = sigmoid(z);

@@ -209,6 +209,23 @@ def test_linear_grad_parts_asked_for():
             assert torch.equal(part, whole) if asked else part is None
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_of_the_largest_numbers(dtype, act):
+    """Far from zero an activation is z or 0 and its slope 1 or 0, up to the
+    largest finite number, whose square and cube f32 cannot hold."""
+    most = torch.finfo(dtype).max
+    far = torch.tensor([t for t in (300.0, 6e4, 1e10, 1e13, 2e19, 1e20, 1e38, most) if t <= most], dtype=dtype)
+    z = torch.cat([far, -far])
+    one = torch.ones(1, 1, dtype=dtype)
+    y, kept = prims.linear(dev(z[:, None]), dev(one), activation=act, keep_preact=True)
+    assert torch.equal(kept.cpu()[:, 0], z)
+    on = torch.cat([torch.ones_like(far), torch.zeros_like(far) if act != "none" else torch.ones_like(far)])
+    assert torch.equal(y.cpu()[:, 0], z * on)
+    dx, dw, db = prims.linear_grad(torch.ones_like(y), torch.ones_like(y), dev(one), preact=kept, activation=act)
+    assert torch.equal(dx.cpu()[:, 0], on) and float(dw) == float(db) == float(on.sum())
+
+
 def test_linear_grad_against_differences():
     """Along random directions, the loss sum(c * y) in 64 bits changes by what
     the kernel's float32 gradient says."""
