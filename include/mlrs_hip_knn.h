@@ -462,7 +462,9 @@ int32_t mlrs_pool_stats_reset(void);
  * multiple of 16 bytes) cost a copy of the operand into the workspace.
  * Results do not depend on the stream or on other calls, and the same call
  * gives the same bits.  Row, column and class counts are limited to 2^31 - 1
- * and a row to 2^22 bytes (MLRS_ERR_UNSUPPORTED "features").
+ * and a row to 2^22 bytes (MLRS_ERR_UNSUPPORTED "features").  What a call
+ * writes overlaps neither its operands nor its other outputs (InvalidParam with
+ * the output's name, after the other checks), but where it says so.
  */
 #define MLRS_ACT_NONE 0
 #define MLRS_ACT_RELU 1

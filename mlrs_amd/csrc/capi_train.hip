@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/mlrs_hip_knn.h"
 #include "capi_shared.hpp"
@@ -126,6 +127,27 @@ int32_t grid_error(int64_t m, int64_t n) {
     return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, m, 0, "the product has more tiles than a launch");
 }
 
+// What a call writes may be no part of what it reads or else writes: workgroups
+// read operands while others write results.
+struct Span {
+    const void* p;
+    int64_t bytes;
+    template <typename T>
+    Span(const T* t, int64_t len) : p(t), bytes(t ? len * (int64_t)sizeof(T) : 0) {}
+    bool meets(const Span& o) const {
+        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
+        return bytes > 0 && o.bytes > 0 && a < b + (uintptr_t)o.bytes && b < a + (uintptr_t)bytes;
+    }
+    bool meets(std::initializer_list<Span> others) const {
+        for (const Span& o : others)
+            if (meets(o)) return true;
+        return false;
+    }
+};
+int32_t overlap_error(const char* out) {
+    return capi::error(MLRS_ERR_INVALID_PARAM, out, 0, 0, 0, "an output overlaps another operand");
+}
+
 #define MLRS_TRY(call)                                      \
     do {                                                    \
         const hipError_t e_ = (call);                       \
@@ -151,6 +173,9 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
         if (n == 0) return MLRS_OK;
         if (!x || !w || !y) return null_error(!x ? "x" : !w ? "w" : "out");
         if (!grid_fits(m, n)) return grid_error(m, n);
+        const Span sx(x, x_len), sw(w, w_len), sb(bias, bias_len), sr(residual, residual_len), sy(y, y_len);
+        if (sy.meets({sx, sw, sb}) || (y != residual && sy.meets(sr))) return overlap_error("out");
+        if (Span(z, z_len).meets({sx, sw, sb, sr, sy})) return overlap_error("preact");
         const hipStream_t s = (hipStream_t)stream;
         const LinearOut o{bias, residual, y, z, act};
         int cus = 0;
@@ -239,6 +264,10 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
         }
         if (dx && !w) return null_error("w");
         if (!grid_fits(k, n) || !grid_fits(k, m)) return grid_error(k, std::max(m, n));
+        const Span ody(dy, dy_len), ox(x, x_len), ow(w, w_len), oz(z, z_len), odx(dx, dx_len), odw(dw, dw_len);
+        if (odx.meets({ody, ox, ow, oz})) return overlap_error("dx");
+        if (odw.meets({ody, ox, ow, oz, odx})) return overlap_error("dw");
+        if (Span(db, db_len).meets({ody, ox, ow, oz, odx, odw})) return overlap_error("dbias");
         const hipStream_t s = (hipStream_t)stream;
         int cus = 0;
         rc = capi::cu_count(&cus);
@@ -369,6 +398,8 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         if (n == 0) return MLRS_OK;
         if (!h || !w || !target || !loss || !lse)
             return null_error(!h ? "h" : !w ? "w" : !target ? "target" : "out");
+        const Span sh(h, h_len), sw(w, w_len), sb(bias, bias_len), st(target, target_len), sl(loss, out_len);
+        if (sl.meets({sh, sw, sb, st}) || Span(lse, out_len).meets({sh, sw, sb, st, sl})) return overlap_error("out");
         const hipStream_t s = (hipStream_t)stream;
         int cus = 0;
         rc = capi::cu_count(&cus);
@@ -476,6 +507,11 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
         if (!w) return null_error("w");
         if (n > 0 && (!h || !target || !lse || !grad))
             return null_error(!h ? "h" : !target ? "target" : !lse ? "lse" : "grad");
+        const Span oh(h, h_len), ow(w, w_len), ob(bias, bias_len), ot(target, target_len), ol(lse, out_len),
+            og(grad, out_len), odh(dh, dh_len), odw(dw, dw_len);
+        if (odh.meets({oh, ow, ob, ot, ol, og})) return overlap_error("dh");
+        if (odw.meets({oh, ow, ob, ot, ol, og, odh})) return overlap_error("dw");
+        if (Span(db, db_len).meets({oh, ow, ob, ot, ol, og, odh, odw})) return overlap_error("dbias");
         const hipStream_t s = (hipStream_t)stream;
         int cus = 0;
         rc = capi::cu_count(&cus);

@@ -507,7 +507,8 @@ def linear(x, w, bias=None, activation="none", residual=None, keep_preact=False,
     float32 and each output rounded once.  ``activation``: "none", "relu",
     "gelu" (the erf form), "gelu_tanh" or "silu".  Returns ``y`` (n, d_out), or
     ``(y, z)`` with ``keep_preact``: z = x w^T + bias, what ``linear_grad``
-    takes.  ``out`` receives y (it may be ``residual`` itself)."""
+    takes.  ``out`` receives y (it may be ``residual`` itself, and otherwise
+    overlaps no operand)."""
     s = _layer_operands(x, w, "x", (bias, "bias"), (residual, "residual"))
     act = _activation_id(activation)
     n, d_in = x.shape

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import train_reference as ref
-from mlrs_amd import prims
+from mlrs_amd import _lib, prims
 
 pytestmark = pytest.mark.gpu
 
@@ -96,6 +96,15 @@ def test_linear_no_rows_and_in_place():
     y = prims.linear(dev(x), w, residual=r, out=r)
     assert y.data_ptr() == r.data_ptr()
     ref.assert_near(y, ref.linear(x, w.cpu(), None, "none", res)[0], "residual's buffer")
+
+
+def test_linear_out_is_no_operand():
+    x, w, r = (dev(rand(i, 64, 64)) for i in range(3))
+    both = torch.empty(65, 64, device="cuda")
+    for kw in (dict(out=x), dict(out=w), dict(out=both[1:], residual=both[:-1])):
+        with pytest.raises(_lib.InvalidParam, match="overlaps"):
+            prims.linear(x, w, **kw)
+    ref.assert_near(prims.linear(x, w, residual=r), ref.linear(x.cpu(), w.cpu(), None, "none", r.cpu())[0], "after")
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -47,6 +47,66 @@ def test_linear_with_nothing_to_do_touches_no_device():
     assert linear(n=0, r_len=0, y_len=0, z_len=0, x=None)[0] == _lib.MLRS_OK
 
 
+def apart(count, step=1 << 20):
+    return [0x100000 + i * step for i in range(count)]
+
+
+SIZE = dict(f32=4, f16=2, bf16=2)
+
+
+@pytest.mark.parametrize("s", TYPES)
+def test_linear_outputs_overlap_no_operand(s):
+    """4 x 3 by 3 x 5: each output a byte into, or a byte short of leaving, each
+    operand; the residual's own buffer is refused only where it is another's too."""
+    x, w, b, r, y, z = apart(6)
+    at = dict(x=(x, 12), w=(w, 15), b=(b, 5), r=(r, 20), y=(y, 20), z=(z, 20))
+    for out, name in (("y", "out"), ("z", "preact")):
+        for other, (start, n) in at.items():
+            if other == out:
+                continue
+            size = 20 * SIZE[s]
+            for p in (start - size + 1, start + n * SIZE[s] - 1) + ((start,) if (out, other) != ("y", "r") else ()):
+                got = linear(s, **{**dict(x=x, w=w, b=b, r=r, y=y, z=z), out: p})
+                assert got[0] == PARAM and got[1] == (name if other != "z" else "preact"), (out, other, got)
+
+
+@pytest.mark.parametrize("s", TYPES)
+def test_gradients_overlap_no_operand(s):
+    lib = _lib.load()
+    names = ["dy", "x", "w", "z", "dx", "dw", "db"]
+    lens = dict(dy=20, x=12, w=15, z=20, dx=12, dw=15, db=5)
+    base = dict(zip(names, apart(7)))
+    for out, name in (("dx", "dx"), ("dw", "dw"), ("db", "dbias")):
+        for other in names:
+            if other != out:
+                p = {**base, out: base[other] + (lens[other] - 1) * SIZE[s]}
+                got = failed(getattr(lib, "mlrs_linear_grad_" + s)(
+                    p["dy"], 20, p["x"], 12, 4, 3, p["w"], 15, 5, p["z"], 20, 1, p["dx"], 12, p["dw"], 15, p["db"], 5,
+                    None))
+                assert got[0] == PARAM and got[1] in (name, "dx", "dw", "dbias"), (out, other, got)
+    names = ["h", "w", "b", "t", "lse", "g", "dh", "dw", "db"]
+    size = {**{n: SIZE[s] for n in names}, "t": 8, "lse": 4, "g": 4}
+    lens = dict(h=12, w=15, b=5, t=4, lse=4, g=4, dh=12, dw=15, db=5)
+    base = dict(zip(names, apart(9)))
+    for out in ("dh", "dw", "db"):
+        for other in names:
+            if other != out:
+                p = {**base, out: base[other] + lens[other] * size[other] - 1}
+                got = failed(getattr(lib, "mlrs_softmax_xent_grad_" + s)(
+                    p["h"], 12, 4, 3, p["w"], 15, 5, p["b"], 5, p["t"], 4, -100, p["lse"], p["g"], 4, p["dh"], 12,
+                    p["dw"], 15, p["db"], 5, None))
+                assert got[0] == PARAM and got[1] in ("dh", "dw", "dbias"), (out, other, got)
+    names = ["h", "w", "b", "t", "loss", "lse"]
+    base = dict(zip(names, apart(6)))
+    for out in ("loss", "lse"):
+        for other in names:
+            if other != out:
+                p = {**base, out: base[other] - 15}
+                got = failed(getattr(lib, "mlrs_softmax_xent_" + s)(
+                    p["h"], 12, 4, 3, p["w"], 15, 5, p["b"], 5, p["t"], 4, -100, p["loss"], p["lse"], 4, None))
+                assert got[0] == PARAM and got[1] == "out", (out, other, got)
+
+
 @pytest.mark.parametrize("s", TYPES)
 @pytest.mark.parametrize("kw,rc,operand", [
     (dict(x_len=13), SHAPE, "x"), (dict(w_len=14), SHAPE, "w"), (dict(k=0, x_len=0, w_len=0), SHAPE, "features"),
