@@ -625,8 +625,8 @@ typedef struct mlrs_adamw_tensor {
  * the state before the first step.  `tensors` is host memory, read before the
  * call returns; no tensor may appear twice.
  * Errors: MLRS_ERR_NULL_POINTER ("master" for a 16-bit parameter without one),
- *   ShapeMismatch "tensors", MLRS_ERR_UNSUPPORTED "dtype" / "state_bits",
- *   InvalidParam "lr" / "betas" / "eps" / "weight_decay" / "step".
+ *   ShapeMismatch "tensors", MLRS_ERR_UNSUPPORTED "dtype" / "state_bits" /
+ *   "tensors" (one of more than 2^36 - 4096 elements), InvalidParam "lr" / "betas" / "eps" / "weight_decay" / "step".
  */
 int32_t mlrs_adamw_step(const mlrs_adamw_tensor *tensors, int64_t count, int32_t state_bits, double lr, double beta1,
                         double beta2, double eps, int64_t step, const float *scale, uint32_t seed, void *stream);

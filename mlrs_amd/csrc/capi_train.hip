@@ -121,8 +121,8 @@ int32_t check_sizes(const char* a_name, int64_t a_len, int64_t n, int64_t d, int
     return MLRS_OK;
 }
 
-// A product's grid must fit: tiles of the smallest size, every part of k.
-bool grid_fits(int64_t m, int64_t n) { return ((m + 63) / 64) * ((n + 63) / 64) <= INT32_MAX / 64; }
+// A product's grid must fit, in the largest tiles.
+bool grid_fits(int64_t m, int64_t n) { return launchable(((m + 255) / 256) * ((n + 255) / 256), 512); }
 int32_t grid_error(int64_t m, int64_t n) {
     return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, m, 0, "the product has more tiles than a launch");
 }
@@ -190,7 +190,7 @@ int32_t linear_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const T* w,
         bool split = false, words = false;
         if constexpr (std::is_same<T, float>::value) {
             const Cut other = choose_cut_split(m, n, k, cus);
-            split = other.us + split_us((double)(n + m) * (double)k) < cut.us;
+            split = split_launchable(m, n) && other.us + split_us((double)(n + m) * (double)k) < cut.us;
             if (split) cut = other;
             const bool rx = readable(x, k), rw = readable(w, k);
             const Cut by = choose_cut((int)sizeof(T), m, n, k, cus, 64, true);
@@ -284,8 +284,8 @@ int32_t linear_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_len,
             const Cut cx = choose_cut((int)sizeof(T), k, n, m, cus), cw = choose_cut((int)sizeof(T), k, m, n, cus);
             sx = choose_cut_split(k, n, m, cus);
             sw = choose_cut_split(k, m, n, cus);
-            split_x = want_x && sx.us + split_us((double)(n + k) * (double)m) < cx.us;
-            split_w = dw && n > 0 && sw.us + split_us((double)(m + k) * (double)n) < cw.us;
+            split_x = want_x && split_launchable(k, n) && sx.us + split_us((double)(n + k) * (double)m) < cx.us;
+            split_w = dw && n > 0 && split_launchable(k, m) && sw.us + split_us((double)(m + k) * (double)n) < cw.us;
             if (split_x || split_w) cut = PairCut{cx, cw, false, 0.0};
             const bool rw = !want_x || readable(w, k), rx = !dw || readable(x, k);
             const PairCut by = choose_pair((int)sizeof(T), k, n, m, k, m, n, cus, true);
@@ -383,7 +383,6 @@ int32_t check_xent(int64_t h_len, int64_t n, int64_t d, int64_t w_len, int64_t v
     if (bias ? bias_len != v : bias_len != 0) return capi::shape_error("bias", 1, v, bias_len);
     if (target_len != n) return capi::shape_error("target", n, 1, target_len);
     if (out_len != n) return capi::shape_error("out", n, 1, out_len);
-    if (!grid_fits(v, n)) return grid_error(v, n);
     return MLRS_OK;
 }
 
@@ -409,7 +408,9 @@ int32_t xent_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T* w, i
         int64_t parts = stats_parts(tile, v), parts_s = 0;
         bool split = false, words = false;
         if constexpr (std::is_same<T, float>::value) {
-            split = choose_cut_split(v, n, d, cus, 1).us + split_us((double)(n + v) * (double)d) < cut.us;
+            // (256 rows, or as many as leave a few tiles)
+            split = split_launchable(v, std::min<int64_t>(n, 256)) &&
+                    choose_cut_split(v, n, d, cus, 1).us + split_us((double)(n + v) * (double)d) < cut.us;
             if (split) {
                 tile = kPlainCut.tile;
                 parts = stats_parts(tile, v);
@@ -521,11 +522,12 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             if (dw) {
                 const StoreTo o{dw, d, nullptr, nullptr, 0, nullptr};
                 const Product p{Mat{w, padded<T>(d)}, Mat{w, padded<T>(v)}, d, v, 0, o};
-                const Cut c{2, 1, 0, 0.0};
+                const Cut c{0, 1, 0, 0.0};
                 MLRS_TRY(launch_products<T>(Product{}, p, PairCut{c, c, false, 0.0}, nullptr, ColumnSums<T>{}, 0, Only{}, s));
             }
-            if (db)
-                MLRS_TRY(launch_sum_parts<T>(ColumnSums<T>{db, nullptr, 0, nullptr}, v, s));
+            constexpr int64_t kMost = (int64_t)1 << 27;  // columns of a launch
+            for (int64_t c = 0; db && c < v; c += kMost)
+                MLRS_TRY(launch_sum_parts<T>(ColumnSums<T>{db + c, nullptr, 0, nullptr}, std::min(kMost, v - c), s));
             return MLRS_OK;
         }
         // classes of a piece: a multiple of 256, at least one tile, and a row of
@@ -547,10 +549,10 @@ int32_t xent_grad_impl(const T* h, int64_t h_len, int64_t n, int64_t d, const T*
             const Cut ch = choose_cut((int)sizeof(T), d, n, most, cus), cw = choose_cut((int)sizeof(T), d, most, n, cus);
             sh = choose_cut_split(d, n, most, cus);
             sw = choose_cut_split(d, most, n, cus);
-            split_z = choose_cut_split(most, n, d, cus, 1).us + split_us(nd + vd) <
+            split_z = split_launchable(most, n) && choose_cut_split(most, n, d, cus, 1).us + split_us(nd + vd) <
                       choose_cut((int)sizeof(T), most, n, d, cus, 1).us;
-            split_h = dh && sh.us + split_us(nv + vd) < ch.us;
-            split_w = dw && sw.us + split_us(nv + nd) < cw.us;
+            split_h = dh && split_launchable(d, n) && sh.us + split_us(nv + vd) < ch.us;
+            split_w = dw && split_launchable(d, most) && sw.us + split_us(nv + nd) < cw.us;
             if (split_h || split_w) cut = PairCut{ch, cw, false, 0.0};
         }
         const bool split = split_z || split_h || split_w;
@@ -788,6 +790,8 @@ int32_t mlrs_adamw_step(const mlrs_adamw_tensor* tensors, int64_t count, int32_t
                                    "unknown element type");
             if (!(t.weight_decay >= 0.0) || std::isinf(t.weight_decay))
                 return invalid("weight_decay", "weight_decay is invalid (must be finite and >= 0)");
+            if (!adamw_launchable(t.len))
+                return capi::error(MLRS_ERR_UNSUPPORTED, "tensors", i, 1, t.len, "a tensor has at most 2^36 - 4096 elements");
             if (t.len == 0) continue;
             if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return null_error("tensors");
             if (t.param_dtype != MLRS_DTYPE_F32 && !t.master) return null_error("master");

@@ -17,6 +17,7 @@ namespace train {
 constexpr int kTableBytes = 3800;  // of the 4 KB of a launch's arguments
 constexpr int kRun = 4096;         // elements of a workgroup: 16 per thread
 constexpr int kBlock = 256;        // elements that share a scale of an 8-bit state
+constexpr int64_t kMostRuns = ((int64_t)1 << 24) - 1;  // of a launch: 2^32 threads are one too many
 
 enum { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
@@ -117,28 +118,31 @@ int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count) {
     return n;
 }
 
-// Fills batches of tensors and launches each: add(batch, index) describes a
-// tensor, go(batch, runs) launches.
+// Fills batches of tensors and launches each: add(item, index, from, len) describes
+// `len` elements of a tensor, all of them but where a launch cannot hold as many;
+// go(batch, runs) launches.
 template <typename Item, typename Len, typename Add, typename Go>
 static hipError_t in_batches(int64_t count, Len len, Add add, Go go) {
     Batch<Item> b;
     int n = 0;
     int64_t runs = 0;
     for (int64_t i = 0; i < count; ++i) {
-        const int64_t r = runs_of(len(i));
-        if (r == 0) continue;
-        if (n == Batch<Item>::kTensors || (n > 0 && runs + r > INT32_MAX)) {
+        const int64_t whole = len(i);
+        for (int64_t from = 0; from < whole; from += kMostRuns * kRun) {
+            const int64_t part = std::min(whole - from, kMostRuns * kRun), r = runs_of(part);
+            if (n == Batch<Item>::kTensors || (n > 0 && runs + r > kMostRuns)) {
+                b.first[n] = (int32_t)runs;
+                b.count = n;
+                const hipError_t e = go(b, runs);
+                if (e != hipSuccess) return e;
+                n = 0;
+                runs = 0;
+            }
             b.first[n] = (int32_t)runs;
-            b.count = n;
-            const hipError_t e = go(b, runs);
-            if (e != hipSuccess) return e;
-            n = 0;
-            runs = 0;
+            add(b.item[n], i, from, part);
+            ++n;
+            runs += r;
         }
-        b.first[n] = (int32_t)runs;
-        add(b.item[n], i);
-        ++n;
-        runs += r;
     }
     if (n == 0) return hipSuccess;
     b.first[n] = (int32_t)runs;
@@ -151,9 +155,9 @@ hipError_t launch_clip_scale(const mlrs_grad_tensor* t, int64_t count, double ma
     int64_t at = 0;
     hipError_t e = in_batches<NormItem>(
         count, [&](int64_t i) { return t[i].len; },
-        [&](NormItem& it, int64_t i) {
-            it.g = t[i].grad;
-            it.len = t[i].len;
+        [&](NormItem& it, int64_t i, int64_t from, int64_t len) {
+            it.g = (const char*)t[i].grad + from * (t[i].dtype == kF32 ? 4 : 2);
+            it.len = len;
             it.dtype = t[i].dtype;
         },
         [&](const Batch<NormItem>& b, int64_t runs) {
@@ -346,11 +350,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(Batch<AdamwItem> b, AdamwHyp
     }
 }
 
+bool adamw_launchable(int64_t len) { return runs_of(len) <= kMostRuns; }
+
 hipError_t launch_adamw(const mlrs_adamw_tensor* t, int64_t count, int bits, const AdamwHyper& hy, const float* scale,
                         hipStream_t s) {
     return in_batches<AdamwItem>(
         count, [&](int64_t i) { return t[i].len; },
-        [&](AdamwItem& it, int64_t i) {
+        [&](AdamwItem& it, int64_t i, int64_t, int64_t) {  // whole: mlrs_adamw_step has checked
             const mlrs_adamw_tensor& x = t[i];
             it.param = x.param;
             it.grad = x.grad;

@@ -9,6 +9,10 @@
 namespace mlrs {
 namespace train {
 
+// Whether a launch may have so many workgroups: a grid holds fewer than 2^32
+// threads along an axis, and a larger one is cut short without an error.
+inline bool launchable(int64_t workgroups, int threads) { return workgroups * threads < (int64_t)1 << 32; }
+
 // A row-major matrix the matrix-core kernels can read: 16-byte aligned, rows
 // a multiple of 16 bytes apart (of f32 in tiles copied by words, any).
 struct Mat {
@@ -26,6 +30,7 @@ struct Cut {
         return splits > 1 ? (size_t)splits * (size_t)n * (size_t)((m + 3) & ~(int64_t)3) * 4 : 0;
     }
 };
+// Of choices whose grid is launchable, and the largest tiles in any case.
 Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64, bool words = false);
 
 // A launch that runs only where (*flag == mark) == wanted (flag null: always).
@@ -164,6 +169,7 @@ inline size_t split_bytes(int64_t rows, int64_t cols) { return (size_t)rows * (s
 inline Mat split_mat(const void* p, int64_t cols, bool r_layout) {
     return Mat{p, r_layout ? (cols + 7) / 8 * 8 : split_row_bytes(cols)};
 }
+inline bool split_launchable(int64_t m, int64_t n) { return launchable(((m + 255) / 256) * ((n + 127) / 128), 512); }
 Cut choose_cut_split(int64_t m, int64_t n, int64_t k, int cus, int max_splits = 64);
 // *flag := mark where an element is not finite.
 hipError_t launch_pack_split(const SplitJob& a, const SplitJob& b, uint32_t* flag, uint32_t mark, hipStream_t s);
@@ -189,6 +195,7 @@ struct AdamwHyper {
     double lr;
     uint32_t seed;
 };
+bool adamw_launchable(int64_t len);  // elements of a tensor
 hipError_t launch_adamw(const mlrs_adamw_tensor* t, int64_t count, int bits, const AdamwHyper& hy, const float* scale,
                         hipStream_t s);
 hipError_t launch_state_values(const uint8_t* codes, const float* scales, int64_t len, int which, float* out,

@@ -9,6 +9,7 @@ namespace mlrs {
 namespace train {
 
 constexpr int kTileRows[4] = {256, 128, 64, 64};
+constexpr int kTileThreads[4] = {512, 256, 256, 256};
 
 // Tiles of m walked together along n.  The workgroups that run at once on an
 // XCD (32 CUs) then share about as many panels of either operand.
@@ -39,7 +40,7 @@ hipError_t launch_gemm(int tile, Mat a, Mat b, int64_t m, int64_t n, int64_t k, 
                        const Only& only, const Epi& epi, hipStream_t s) {
     GemmArgs g;
     const int64_t blocks = gemm_args(g, tile, a, b, m, n, k, splits, k_split, only);
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
+    if (!launchable(blocks, kTileThreads[tile])) return hipErrorInvalidConfiguration;  // the caller has checked
     const dim3 grid((unsigned)blocks);
     if (tile == 0)
         gemm_kernel<T, 2, 4, 8, 4, Epi><<<grid, 512, 0, s>>>(g, epi);

@@ -37,6 +37,7 @@ Cut choose_cut(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int max
         for (int64_t sp = 1; sp <= max_splits && sp <= stages; sp = sp < 4 ? sp + 1 : sp * 2) {
             const int64_t each = (stages + sp - 1) / sp;
             if (sp > 1 && (each < 3 || (sp - 1) * each >= stages)) continue;
+            if ((t > 0 || sp > 1) && !launchable(tiles * sp, kTileThreads[t])) continue;
             const int64_t on_cu = (tiles * sp + cus - 1) / cus;  // tiles that the busiest CU computes
             const int64_t rounds = on_cu / kResident[t], rest = on_cu % kResident[t];
             double cost = (double)rounds * ((double)each * stage[kResident[t] - 1] + kRoundUs[t]);
@@ -101,6 +102,7 @@ PairCut choose_pair(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t 
                 const int64_t ew = (ws + sw - 1) / sw;
                 if (sw > 1 && (ew < 3 || (sw - 1) * ew >= ws || wt * sw > 8 * cus)) continue;
                 const int64_t count = xt * sx + wt * sw;
+                if (!launchable(count, kTileThreads[t])) continue;
                 const int64_t full = std::min<int64_t>(kResident[t], (count + cus - 1) / cus), slots = full * cus;
                 const double ux = (double)ex * stage[full - 1] + kRoundUs[t], uw = (double)ew * stage[full - 1] + kRoundUs[t];
                 const double all = ((double)(xt * sx) * ux + (double)(wt * sw) * uw) / (double)slots;
@@ -194,13 +196,14 @@ __device__ __forceinline__ typename Elem<T>::Frag chunk_at(const T* row, int64_t
 
 template <typename T, int NB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restrict__ x, const T* __restrict__ w,
-                                                                int32_t n, int32_t m, int64_t k, LinearEpi<T> epi) {
+                                                                int32_t n, int32_t m, int64_t k, int32_t first,
+                                                                LinearEpi<T> epi) {
     constexpr int E = 16 / (int)sizeof(T);
     constexpr int STEP = 4 * E;  // of k per wave and step
     __shared__ f32x4 sums[WAVES][NB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int32_t m0 = blockIdx.x * 16;
+    const int32_t m0 = first + (int32_t)blockIdx.x * 16;
     const T* wr = w + (int64_t)(m0 + r < m ? m0 + r : m - 1) * k;
     const T* xr[NB];
 #pragma unroll
@@ -236,9 +239,15 @@ __global__ __launch_bounds__(WAVES * 64) void linear_few_kernel(const T* __restr
 template <typename T, int NB>
 static hipError_t launch_few_nb(const T* x, const T* w, int64_t n, int64_t m, int64_t k, const LinearEpi<T>& e,
                                 hipStream_t s) {
-    linear_few_kernel<T, NB, 8>
-        <<<dim3((unsigned)((m + 15) / 16)), 512, 0, s>>>(x, w, (int32_t)n, (int32_t)m, k, e);
-    return hipGetLastError();
+    constexpr int64_t kMost = (int64_t)1 << 26;  // outputs of a launch: half of what its threads could be
+    for (int64_t first = 0; first < m; first += kMost) {
+        const int64_t here = std::min(kMost, m - first);
+        linear_few_kernel<T, NB, 8><<<dim3((unsigned)((here + 15) / 16)), 512, 0, s>>>(x, w, (int32_t)n, (int32_t)m, k,
+                                                                                      (int32_t)first, e);
+        const hipError_t r = hipGetLastError();
+        if (r != hipSuccess) return r;
+    }
+    return hipSuccess;
 }
 
 template <typename T>
@@ -359,6 +368,7 @@ hipError_t launch_act_grad(const T* dy, const T* z, int act, int64_t n, int64_t 
 template <typename T>
 hipError_t launch_sum_parts(const ColumnSums<T>& to, int64_t m, hipStream_t s) {
     if (!to.out) return hipSuccess;
+    if (!launchable((m + 15) / 16, 256)) return hipErrorInvalidConfiguration;  // the caller has checked
     sum_parts_kernel<T><<<dim3((unsigned)((m + 15) / 16)), 256, 0, s>>>(to, m);
     return hipGetLastError();
 }
@@ -410,9 +420,14 @@ static hipError_t launch_pair(const Product& x, const Product& w, const Cut& cx,
     q.x_first = q.x.k_split >= q.w.k_split;
     q.sums = sums;
     q.columns = columns;
-    const int64_t blocks = wgs[0] + wgs[1] + (sums.out ? (columns + 15) / 16 : 0);
+    int64_t blocks = wgs[0] + wgs[1] + (sums.out ? (columns + 15) / 16 : 0);
     if (blocks == 0) return hipSuccess;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
+    if (sums.out && !launchable(blocks, kTileThreads[tile])) {
+        const hipError_t e = launch_sum_parts(sums, columns, s);
+        if (e != hipSuccess) return e;
+        blocks = wgs[0] + wgs[1];
+    }
+    if (!launchable(blocks, kTileThreads[tile])) return hipErrorInvalidConfiguration;  // the caller has checked
     const dim3 grid((unsigned)blocks);
     if (tile == 0)
         pair_kernel<T, 2, 4, 8, 4><<<grid, 512, 0, s>>>(q);

@@ -93,7 +93,7 @@ static hipError_t launch_split(Mat a, Mat b, int64_t m, int64_t n, int64_t k, co
     g.mark = only.mark;
     g.wanted = only.wanted;
     const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * cut.splits;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;  // the caller has checked
+    if (!launchable(blocks, 512)) return hipErrorInvalidConfiguration;  // the caller has checked
     gemm_split_kernel<AKC, BKC, Epi><<<dim3((unsigned)blocks), 512, 0, s>>>(g, epi);
     return hipGetLastError();
 }

@@ -78,6 +78,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float* __restrict_
 hipError_t launch_xent_join(const float* top, const float* total, int64_t parts, const float* hit,
                             const int64_t* target, int64_t n, int64_t classes, int64_t ignore, float* loss, float* lse,
                             const Only& only, hipStream_t s) {
+    if (!launchable((n + 15) / 16, 256)) return hipErrorInvalidConfiguration;  // the caller's chunks are shorter
     xent_join_kernel<<<dim3((unsigned)((n + 15) / 16)), 256, 0, s>>>(top, total, parts, hit, target, n, classes,
                                                                     ignore, loss, lse, only);
     return hipGetLastError();
@@ -252,6 +253,7 @@ __global__ __launch_bounds__(256) void logit_grad_rows_kernel(LogitParts<T> z, c
 template <typename T>
 hipError_t launch_xent_rows(const float* part, const Cut& cut, const T* bias, const int64_t* target, int64_t n,
                             int64_t classes, int64_t ignore, float* loss, float* lse, hipStream_t s) {
+    if (!launchable(n, 256)) return hipErrorInvalidConfiguration;  // so many rows are no few tiles
     xent_rows_kernel<T><<<dim3((unsigned)n), 256, 0, s>>>(logit_parts(part, cut, bias, n, classes), target, classes,
                                                           ignore, loss, lse);
     return hipGetLastError();

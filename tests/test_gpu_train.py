@@ -398,6 +398,83 @@ def test_xent_many_rows_in_pieces(dtype):
     assert (db.double() - want_db).abs().max() <= (4 * ref.UNIT[dtype] + 2.0 ** -16) * want_db.abs().max()
 
 
+def test_xent_of_more_logits_than_a_launch_has_tiles_for():
+    """4,300,800 rows of 128,003 classes: the loss in chunks of rows, the gradient
+    in pieces of the vocabulary, neither of them a launch's worth of all tiles.
+    Some rows and some classes are held to 64 bits."""
+    n, v, k = 4300800, 128003, 8
+    h, w = rand(1, n, k, dtype=BF16).cuda(), rand(2, v, k, dtype=BF16, std=0.4).cuda()
+    t = targets(3, n, v).cuda()
+    g = torch.full((n,), 1.0 / n, device="cuda")
+    loss, lse = prims.softmax_xent(h, w, t)
+    dh, dw, _ = prims.softmax_xent_grad(h, w, t, lse, g)
+    rows = torch.cat([torch.arange(a, a + 40) for a in (0, 255 * 256, n // 2, n - 40)]).cuda()
+    want = ref.xent(h[rows].cpu(), w.cpu(), None, t[rows].cpu(), IGNORE, g[rows].cpu(), BF16)
+    for name, got in (("loss", loss), ("lse", lse), ("dh", dh)):
+        ref.assert_near(got[rows], want[name], name)
+    for c in (0, 64000, v - 32):
+        p = torch.exp(h.double() @ w[c:c + 32].double().t() - lse.double()[:, None])
+        hot = (t[:, None] == torch.arange(c, c + 32, device="cuda")).double()
+        dz = (p - hot) * (t != IGNORE).double()[:, None] * g.double()[:, None]
+        room = (2 * ref.UNIT[BF16] + ref.dot_bound(n)) * (dz.abs().t() @ h.double().abs())
+        assert bool(((dw[c:c + 32].double() - dz.t() @ h.double()).abs() <= room).all())
+
+
+def test_layer_of_more_outputs_than_a_launch_has_threads_for():
+    """Few rows by 2^27 + 40 outputs, sixteen to a workgroup."""
+    m = 2 ** 27 + 40
+    w = torch.arange(m, device="cuda").remainder_(2039).half()[:, None]
+    for n in (1, 17):
+        x = torch.arange(1, n + 1, device="cuda").half()[:, None]
+        y = prims.linear(x, w)
+        assert all(torch.equal(y[i], w[:, 0] * x[i, 0]) for i in (0, n - 1))
+        del y
+
+
+def test_layers_and_losses_of_more_rows_than_a_launch_has_threads_for():
+    """2^30 + 77 rows of eight features, 64 of them to a small tile.  Zero but for
+    runs of 300 rows, of small whole numbers: every sum is exact."""
+    n, k, m = 2 ** 30 + 77, 8, 8
+    runs = [slice(a, a + 300) for a in (0, 2 ** 24, 2 ** 29, n - 300)]
+    small = [rand(i, 4, 300, k).mul(2).round().clamp(-7, 7).to(BF16).cuda() for i in (1, 2)]
+    w = rand(3, m, k).mul(2).round().clamp(-7, 7).to(BF16).cuda()
+    x = torch.zeros(n, k, dtype=BF16, device="cuda")
+    for r, t in zip(runs, small[0]):
+        x[r].copy_(t)
+    y = prims.linear(x, w)
+    for r, t in zip(runs, small[0]):
+        assert torch.equal(y[r].double(), (t.double() @ w.double().t()).bfloat16().double())
+    assert not y[300:2 ** 24].any() and not y[2 ** 24 + 300:2 ** 24 + 3000].any()
+    dy = y.zero_()
+    for r, t in zip(runs, small[1]):
+        dy[r].copy_(t)
+    dx, dw, db = prims.linear_grad(dy, x, w)
+    for r, t in zip(runs, small[1]):
+        assert torch.equal(dx[r].double(), (t.double() @ w.double()).bfloat16().double())
+    assert not dx[300:2 ** 24].any() and not dx[2 ** 24 + 300:2 ** 24 + 3000].any()
+    flat = [t.reshape(-1, k).double() for t in small]
+    assert torch.equal(dw, (flat[1].t() @ flat[0]).bfloat16()) and torch.equal(db, flat[1].sum(0).bfloat16())
+    del dx, dy, y
+    t = torch.zeros(n, dtype=torch.int64, device="cuda")
+    loss, lse = prims.softmax_xent(x, w[:2], t)
+    for r, h in zip(runs, small[0]):
+        want = ref.xent(h.cpu(), w[:2].cpu(), None, t[r].cpu(), IGNORE, torch.ones(300), BF16)
+        ref.assert_near(loss[r], want["loss"], "loss")
+        ref.assert_near(lse[r], want["lse"], "lse")
+    assert float((lse[300:2 ** 24] - 0.6931472).abs().max()) < 2.0 ** -20  # log 2 of zero rows
+    del x, t, loss, lse
+    torch.cuda.empty_cache()
+
+
+def test_gradients_of_no_rows_and_many_classes():
+    """2^28 + 40 of them: their zeros are sixteen to a workgroup."""
+    w = torch.ones(2 ** 28 + 40, 1, dtype=BF16, device="cuda")
+    e = torch.empty(0, device="cuda")
+    dh, dw, db = prims.softmax_xent_grad(torch.empty(0, 1, dtype=BF16, device="cuda"), w,
+                                         torch.empty(0, dtype=torch.int64, device="cuda"), e, e, bias=w[:, 0])
+    assert dh.shape == (0, 1) and not dw.any() and not db.any()
+
+
 def test_xent_target_that_is_masked_or_no_class():
     h, w = rand(1, 6, 16), rand(2, 50, 16)
     b = torch.zeros(50)
@@ -834,3 +911,20 @@ def test_clip_scale_of_gradients_whose_squares_f32_cannot_hold(dtype, size):
 def test_clip_scale_of_a_norm_that_f32_cannot_hold():
     norm, scale = prims.clip_scale([torch.full((100,), 3e38, device="cuda")], 1.0)
     assert float(norm) == float("inf") and scale.isnan().all()
+
+
+def test_clip_scale_of_more_elements_than_a_launch_has_threads_for():
+    """Many large gradients, and one by itself."""
+    g = torch.ones(2 ** 32, dtype=F16, device="cuda")
+    norm, _ = prims.clip_scale([g] * 17, 1.0)
+    assert abs(float(norm) / (17 * 2.0 ** 32) ** 0.5 - 1) <= 16 * ref.U32
+    del g
+    torch.cuda.empty_cache()
+    g = torch.zeros(2 ** 36 + 5000, dtype=F16, device="cuda")
+    g[::2 ** 27] = 2.0
+    g[-1] = 3.0
+    norm, scale = prims.clip_scale([g], 1.0)
+    want = (4.0 * 513 + 9.0) ** 0.5
+    assert abs(float(norm) / want - 1) <= 16 * ref.U32 and abs(float(scale) * want - 1) <= 16 * ref.U32
+    del g
+    torch.cuda.empty_cache()

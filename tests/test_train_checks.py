@@ -169,6 +169,10 @@ def test_adamw_validation(kw, rc, operand):
     assert adamw(**kw)[:2] == (rc, operand)
 
 
+def test_adamw_of_more_elements_than_a_launch_has_threads_for():
+    assert adamw(len=2 ** 36 - 4095)[:2] == (UNSUPPORTED, "tensors")
+
+
 def test_adamw_with_nothing_to_do_touches_no_device():
     assert adamw(count=0, tensors=False)[0] == _lib.MLRS_OK
     assert adamw(len=0, param=None)[0] == _lib.MLRS_OK
