@@ -398,6 +398,66 @@ def test_xent_many_rows_in_pieces(dtype):
     assert (db.double() - want_db).abs().max() <= (4 * ref.UNIT[dtype] + 2.0 ** -16) * want_db.abs().max()
 
 
+def pieces_inputs(n, v, k, dtype):
+    h, w, b = rand(1, n, k, dtype=dtype).cuda(), rand(2, v, k, dtype=dtype, std=1.5 * k ** -0.5).cuda(), rand(
+        3, v, dtype=dtype, std=0.5).cuda()
+    return h, w, b, targets(4, n, v).cuda(), (rand(5, n).abs() / n).cuda()
+
+
+def check_pieces(got, want, names, rows=slice(None)):
+    for name, g in got.items():
+        if name in names:
+            value, bound = want[name]
+            one = name in ("loss", "lse", "dh")
+            ref.assert_near(g[rows] if one else g, (value[rows].cpu(), bound[rows].cpu()) if one else (
+                value.cpu(), bound.cpu()), name)
+
+
+def all_outputs(h, w, t, g, b):
+    loss, lse = prims.softmax_xent(h, w, t, bias=b)
+    dh, dw, db = prims.softmax_xent_grad(h, w, t, lse, g, bias=b)
+    return dict(loss=loss, lse=lse, dh=dh, dw=dw, db=db)
+
+
+# Gradients of two to four pieces, the last of them shorter and odd; the 64-bit
+# reference is computed on the GPU.  f32: all three products in three bf16 parts,
+# rows in place or packed; dh in parts of its contraction, of which the last piece
+# has fewer; the logits alone in bf16 parts; none.
+@pytest.mark.parametrize("n,v,k,dtype", [
+    (16384, 20011, 512, F32), (16384, 20011, 511, F32), (40000, 7003, 512, F32), (20000, 16001, 300, F32),
+    (270001, 1101, 61, F32), (270001, 2103, 24, F16), (270001, 2103, 24, BF16), (100003, 6007, 40, F16),
+])
+def test_xent_gradients_of_several_pieces(n, v, k, dtype):
+    h, w, b, t, g = pieces_inputs(n, v, k, dtype)
+    want = ref.xent(h, w, b, t, IGNORE, g, dtype)
+    check_pieces(all_outputs(h, w, t, g, b), want, want)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,v,k", [(16384, 20011, 512), (16384, 20011, 511), (20000, 16001, 300)])
+def test_xent_pieces_that_f32_takes_over(n, v, k):
+    """A class of the last piece with an element that has no bf16 parts (all rows
+    are 0 there), and a row whose target is no class: the f32 kernels take over
+    in the middle of the call, and everything beside them is what it was."""
+    h, w, b, t, g = pieces_inputs(n, v, k, F32)
+    h[:, 3] = 0.0
+    want = ref.xent(h, w, b, t, IGNORE, g, F32)
+    w[v - 5, 3] = torch.finfo(F32).max
+    got = all_outputs(h, w, t, g, b)
+    cols = [i for i in range(k) if i != 3]
+    got["dh"], want["dh"] = got["dh"][:, cols], tuple(x[:, cols] for x in want["dh"])
+    check_pieces(got, want, want)
+    w[v - 5, 3] = 0.0
+    t[77] = v
+    got = all_outputs(h, w, t, g, b)
+    rows = torch.arange(n, device="cuda") != 77
+    got["dh"] = got["dh"][:, cols]
+    check_pieces(got, want, ("loss", "lse", "dh"), rows)
+    assert got["loss"][77].isnan() and got["dh"][77].isnan().all()
+    assert got["dw"].isnan().all() and got["db"].isnan().all()
+    torch.cuda.empty_cache()
+
+
 def test_xent_of_more_logits_than_a_launch_has_tiles_for():
     """4,300,800 rows of 128,003 classes: the loss in chunks of rows, the gradient
     in pieces of the vocabulary, neither of them a launch's worth of all tiles.
