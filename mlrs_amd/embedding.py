@@ -53,8 +53,8 @@ class AdamW:
         self.avg_scales = self.avg_sq_scales = None
         if state_bits == 8:
             self.avg_scales, self.avg_sq_scales = (
-                [torch.zeros(-(-p.numel() // prims.STATE_BLOCK), device=p.device) for p in self.params]
-                for _ in range(2))
+                [torch.zeros(-(-p.numel() // prims.STATE_BLOCK), dtype=torch.float32, device=p.device)
+                 for p in self.params] for _ in range(2))
         self.steps = 0
 
     def step(self, grads):
@@ -120,7 +120,7 @@ class EmbeddingEncoder:
         the class head last."""
         out = []
         for wide in widths + [classes]:
-            w = torch.empty(wide, d, device=device).normal_(0.0, d ** -0.5, generator=gen)
+            w = torch.empty(wide, d, dtype=torch.float32, device=device).normal_(0.0, d ** -0.5, generator=gen)
             out += [w.to(_DTYPES[self.dtype]), torch.zeros(wide, dtype=_DTYPES[self.dtype], device=device)]
             d = wide
         return out
@@ -191,10 +191,10 @@ class EmbeddingEncoder:
         self.loss_curve_, norms, skipped, steps = [], [], [], 0
         for _ in range(int(self.epochs)):
             order = torch.randperm(n, device=x.device, generator=gen)
-            total = torch.zeros((), device=x.device)
+            total = torch.zeros((), dtype=torch.float32, device=x.device)
             for start in range(0, n, int(self.batch_size)):
                 rows = order[start:start + int(self.batch_size)]
-                weight = torch.full((len(rows),), up / len(rows), device=x.device)
+                weight = torch.full((len(rows),), up / len(rows), dtype=torch.float32, device=x.device)
                 loss, grads = self._loss_and_grads(x[rows], target[rows], weight)
                 norm = optimizer.step(grads)
                 steps += 1

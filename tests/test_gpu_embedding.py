@@ -178,6 +178,20 @@ def test_steps_that_fit_skips_are_told(max_norm):
         EmbeddingEncoder(**kw).fit(x, y)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_default_dtype_is_not_asked(bits):
+    x, y = rows(7, 300)
+    kw = dict(n_components=4, hidden=(8,), epochs=2, batch_size=100, state_bits=bits)
+    want = EmbeddingEncoder(**kw).fit(x, y).transform(x)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = EmbeddingEncoder(**kw).fit(x, y).transform(x)
+    finally:
+        torch.set_default_dtype(before)
+    assert got.dtype == np.float32 and np.array_equal(got, want)
+
+
 def test_the_optimizer_refuses_what_it_cannot_hold():
     p = torch.zeros(3, 2, device="cuda")
     with pytest.raises(ValueError, match="state_bits"):
