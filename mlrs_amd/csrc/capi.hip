@@ -118,13 +118,16 @@ static size_t aligned_bytes(size_t n) { return (n + 255) & ~(size_t)255; }
 // the previous call's work (an event recorded at the end of every call that
 // touched a cached buffer): calls on one device run in call order, as on the
 // reference's single stream (crates/mlrs-backend/src/stream_cap.rs:69).  The
-// null stream is there for good, so the event of a call on it is recorded only
-// once a call on another stream has to wait for it: calls that stay on it pay
-// nothing (recording and waiting cost 4 us of a call's 11).
+// null stream is there for good and in order: a call on it waits for no event of
+// another on it, and records none until a call has come on another stream
+// (recording and waiting cost 4 us of a call's 11).  The first of those records
+// the null stream's event itself and so waits for all that is on it by then;
+// from there on each call on it records its own end, and others wait for no more.
 struct DevOrder {
     hipEvent_t ev = nullptr;
-    bool have = false;     // ev stands for the last call's end
-    bool on_null = false;  // the last call ran on the null stream, and nothing is recorded
+    bool have = false;      // ev stands for the last call's end
+    bool on_null = false;   // the last call ran on the null stream
+    bool streams = false;   // a call has come on another stream
 };
 DevOrder g_order[kMaxDevices];
 
@@ -149,12 +152,11 @@ struct CallGuard {
     ~CallGuard() {
         if (st.armed) {
             DevOrder& O = g_order[st.dev];
-            if (!st.s) {
-                O.on_null = true;
-            } else if (hipEventRecord(O.ev, st.s) == hipSuccess) {
+            if ((st.s || O.streams) && hipEventRecord(O.ev, st.s) == hipSuccess)
                 O.have = true;
-                O.on_null = false;
-            }
+            else if (!st.s)
+                O.have = false;
+            O.on_null = !st.s;
         }
         g_call = nullptr;
     }
@@ -174,16 +176,16 @@ int32_t order_after_last_call(int dev, hipStream_t s) {
             return hip_err(e, "hipEventCreateWithFlags");
         }
     }
-    if (O.on_null && s) {
+    if (s) O.streams = true;
+    if (O.on_null && s && !O.have) {
         e = hipEventRecord(O.ev, nullptr);
         if (e != hipSuccess) return hip_err(e, "hipEventRecord");
         O.have = true;
-        O.on_null = false;
     }
     // Waited for even when the stream handle equals the last call's: a
     // destroyed stream's handle can be handed out again while its work is
     // pending, and waiting on an event the stream itself recorded is free.
-    if (O.have && !O.on_null) {
+    if (O.have && !(O.on_null && !s)) {
         e = hipStreamWaitEvent(s, O.ev, 0);
         if (e != hipSuccess) return hip_err(e, "hipStreamWaitEvent");
     }

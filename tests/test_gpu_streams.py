@@ -79,3 +79,33 @@ def test_two_streams_mixed_entry_points():
     _same(kd, wkd)
     _same(ki, wki)
     _same(pw, oracle.pairwise(q, c, "cosine"))
+
+
+def test_a_call_waits_for_calls_and_not_for_what_else_the_null_stream_does():
+    """A call on another stream after one on the null stream, which has ~0.2 s
+    of unrelated matrix products to do since: the call is done before they are."""
+    rng = np.random.default_rng(14)
+    q = rng.standard_normal((300, 32)).astype(np.float32)
+    x = rng.standard_normal((5000, 32)).astype(np.float32)
+    dq, dx = _t(q), _t(x)
+    a = torch.randn((4096, 4096), device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        prims.knn_topk(dq, dx, 5)
+    torch.cuda.synchronize()
+    null = torch.cuda.default_stream()
+    with torch.cuda.stream(null):
+        first = prims.knn_topk(dq, dx, 5)
+        for _ in range(200):
+            a = torch.mm(a, a) * 1e-3
+    with torch.cuda.stream(side):
+        second = prims.knn_topk(dq, dx, 7)
+    side.synchronize()
+    busy = not null.query()
+    torch.cuda.synchronize()
+    assert busy, "the call waited for the null stream's other work"
+    for got, k in ((first, 5), (second, 7)):
+        wd, wi = oracle.knn_topk(q, x, k)
+        _same(got[0], wd)
+        _same(got[1], wi)
