@@ -455,13 +455,13 @@ int32_t mlrs_pool_stats_reset(void);
  * gradient, and the optimizer step.  No counterpart in the reference.
  *
  * Element types: _f32 (float), _f16 (IEEE half) and _bf16 (bfloat16; 16-bit
- * elements are passed as uint16_t).  Products, sums, softmax statistics and
- * norms are held in f32 whatever the type; a result is rounded to its type
+ * elements are passed as uint16_t).  Products, sums and softmax statistics are
+ * held in f32 whatever the type, norms in f64; a result is rounded to its type
  * once, to nearest even.  Matrices are contiguous and row-major, aligned to
  * their element size; other alignments than 16 bytes (or rows that are no
  * multiple of 16 bytes) cost a copy of the operand into the workspace.
  * Results do not depend on the stream or on other calls, and the same call
- * gives the same bits.  Row, column and class counts are limited to 2^31 - 1
+ * gives the same bits.  Row, column and class counts are limited to 2^31 - 513
  * and a row to 2^22 bytes (MLRS_ERR_UNSUPPORTED "features").  What a call
  * writes overlaps neither its operands nor its other outputs (InvalidParam with
  * the output's name, after the other checks), but where it says so.
@@ -522,11 +522,13 @@ int32_t mlrs_linear_grad_bf16(const uint16_t *dy, int64_t dy_len, const uint16_t
 
 /*
  * Softmax cross entropy of z = h w^T + bias: lse_i = log sum_v e^(z_iv) and
- * loss_i = lse_i - z_i,target(i), without z in memory.  h is n x d, w
+ * loss_i = lse_i - z_i,target(i), without z in memory (but for a few tiles of
+ * long rows, whose z is computed in parts in the workspace).  h is n x d, w
  * classes x d, bias `classes` long (may be NULL; -inf leaves a class out);
  * target, loss and lse hold n elements.  A row whose target is `ignore_index`
  * has loss 0 (its lse is still written); a target that is no class, loss NaN.
- * A row all of whose logits are -inf has lse -inf, and loss NaN.
+ * A row all of whose logits are -inf has lse -inf, and loss NaN; one with a
+ * logit of +inf or NaN has NaN for both (a loss of 0 where it is ignored).
  * Errors, in this order: ShapeMismatch "h" / "w", "features" (d or classes
  *   < 1), MLRS_ERR_UNSUPPORTED "features" / "rows", ShapeMismatch "bias" /
  *   "target" / "out".
@@ -550,9 +552,14 @@ int32_t mlrs_softmax_xent_bf16(const uint16_t *h, int64_t h_len, int64_t n, int6
  * (classes x d) and dbias = the column sums of dz.  lse is mlrs_softmax_xent's
  * of the same operands; z is computed again, in pieces of the vocabulary (256
  * classes at least) whose dz takes at most MLRS_XENT_PIECE_BYTES of workspace;
- * of several pieces, dh is added up in f32.  Any of dh, dw and dbias
- * may be NULL (length 0).  16-bit types: dz is rounded to the type before the
- * products (f16: scaled by a power of two first, by the largest |grad|).
+ * of several pieces, dh is added up in f32.  f32's large products take dz in six
+ * bytes an element more each, up to four times MLRS_XENT_PIECE_BYTES with it.  Any
+ * of dh, dw and dbias may be NULL (length 0).
+ * 16-bit types: dz is rounded to the type before the products, and dbias adds up
+ * what is rounded.  It is scaled for that, and the results back: divided by the
+ * fraction (1 to 2) of grad_0 in bf16, of the largest |grad_i| of a row that is not
+ * ignored in f16, where a power of two also lifts that to 2^13.  So how an
+ * element of one row is rounded depends on another row's grad.
  * n = 0 gives dw = 0 and dbias = 0.
  * Errors, in this order: as mlrs_softmax_xent ("out" being lse's and grad's
  *   length), then ShapeMismatch "dh" / "dw" / "dbias".
@@ -626,7 +633,8 @@ typedef struct mlrs_adamw_tensor {
  * call returns; no tensor may appear twice.
  * Errors: MLRS_ERR_NULL_POINTER ("master" for a 16-bit parameter without one),
  *   ShapeMismatch "tensors", MLRS_ERR_UNSUPPORTED "dtype" / "state_bits" /
- *   "tensors" (one of more than 2^36 - 4096 elements), InvalidParam "lr" / "betas" / "eps" / "weight_decay" / "step".
+ *   "tensors" (one of more than 2^36 - 4096 elements), InvalidParam "lr" /
+ *   "betas" / "eps" / "weight_decay" / "step".
  */
 int32_t mlrs_adamw_step(const mlrs_adamw_tensor *tensors, int64_t count, int32_t state_bits, double lr, double beta1,
                         double beta2, double eps, int64_t step, const float *scale, uint32_t seed, void *stream);

@@ -427,6 +427,8 @@ struct StatsEpi {
 // zero in ignored rows, NaN in rows whose target is no class.  Rounded to the
 // operands' type, as it goes into two matrix products with them: the products
 // still add in f32, and a 16-bit gradient's own rounding is of the same size.
+// The column sums add up the rounded elements, as they leave LDS in lines (within
+// 2.7e-4 of the sums of unrounded ones in f16, as the products are).
 // `up` scales it first (f16: the gradients of a mean over a batch times the
 // probabilities of a large vocabulary lie below f16's range).
 template <typename T>

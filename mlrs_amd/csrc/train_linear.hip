@@ -280,6 +280,11 @@ int column_parts(int64_t n, int64_t m, int cus) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 256), (n + 7) / 8));
 }
 
+// dz leaves in the operands' type, as the matrix instructions of the two products
+// take it; the column sums add it up in f32, unrounded.  With a 16-bit dz the
+// products' error against 64 bits is 2.3e-3 in bf16 (8192 x 2048 by 8192) and
+// 2.9e-4 in f16, where rounding the results alone makes 1.7e-3 and 2.1e-4; a dz in
+// two parts would double the products.
 template <typename T>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy, const T* __restrict__ z, int act,
                                                        int64_t n, int64_t m, T* __restrict__ dz, int64_t ld,

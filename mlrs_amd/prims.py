@@ -563,7 +563,8 @@ def softmax_xent(h, w, target, bias=None, ignore_index=-100):
     ``h`` (n, d), ``w`` (classes, d) and ``bias`` (classes,; -inf leaves a class
     out) share one dtype; ``target`` (n,) is int64.  ``lse`` is the logarithm of
     the sum of exponentials, ``loss = lse - z[target]``, 0 where the target is
-    ``ignore_index`` and NaN where it is no class."""
+    ``ignore_index`` and NaN where it is no class.  A few tiles of long rows have
+    their logits computed in parts, in the workspace."""
     s = _layer_operands(h, w, "h", (bias, "bias"))
     _dev_check(h, target)
     n, d = h.shape
@@ -583,7 +584,9 @@ def softmax_xent_grad(h, w, target, lse, grad, bias=None, ignore_index=-100, nee
 
     ``lse`` is what ``softmax_xent`` returned for the same operands, ``grad``
     float32 (n,) the gradient of each row's loss (1 / n for their mean).  The
-    logits are computed again, a piece of the vocabulary at a time."""
+    logits are computed again, a piece of the vocabulary at a time.  16-bit types:
+    the logits' gradient is rounded to the type before the two products, scaled by
+    a common factor, and ``dbias`` sums what is rounded."""
     s = _layer_operands(h, w, "h", (bias, "bias"))
     _dev_check(h, target, lse, grad)
     n, d = h.shape

@@ -573,6 +573,22 @@ def test_xent_rows_with_nan_stay_alone():
     assert loss[3].isnan() and lse[3].isnan()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,k", [(70, 300, 32), (70, 130, 4000)])
+def test_xent_rows_with_infinite_logits_stay_alone(dtype, n, v, k):
+    h, w, t = rand(1, n, k, dtype=dtype), rand(2, v, k, dtype=dtype, std=k ** -0.5), targets(3, n, v, 0.0)
+    w[:, 5] = w[:, 5].abs() + 0.1
+    t[9] = IGNORE
+    clean = prims.softmax_xent(dev(h), dev(w), dev(t))
+    h[3, 5] = h[9, 5] = float("inf")
+    loss, lse = prims.softmax_xent(dev(h), dev(w), dev(t))
+    dh, _, _ = prims.softmax_xent_grad(dev(h), dev(w), dev(t), lse, torch.ones(n, device="cuda"), need_dw=False)
+    keep = [i for i in range(n) if i not in (3, 9)]
+    assert torch.equal(loss[keep], clean[0][keep]) and torch.equal(lse[keep], clean[1][keep])
+    assert loss[3].isnan() and lse[3].isnan() and loss[9] == 0 and lse[9].isnan()
+    assert dh[3].isnan().all() and not dh[9].any() and dh[keep].isfinite().all()
+
+
 @pytest.mark.parametrize("size", [1e-6, 1.0, 3e4])
 def test_xent_half_precision_gradient_range(size):
     """Gradients far below and above half precision's range times probabilities
