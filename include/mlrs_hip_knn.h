@@ -581,6 +581,99 @@ int32_t mlrs_softmax_xent_grad_bf16(const uint16_t *h, int64_t h_len, int64_t n,
                                     const float *grad, int64_t out_len, uint16_t *dh, int64_t dh_len, uint16_t *dw,
                                     int64_t dw_len, uint16_t *dbias, int64_t dbias_len, void *stream);
 
+/*
+ * ---- the rest of an encoder's layer ----
+ * Dropout, and group norm with an activation and dropout.  Element types,
+ * overlaps and errors as above.  No call here synchronizes or reads back.  A call
+ * that takes no workspace can be captured into a graph and replayed; one that
+ * does is refused there (MLRS_ERR_UNSUPPORTED "stream").
+ *
+ * Random bits come from a counter: element i of the tensor takes 16 bits of
+ * Philox 4x32 with seven rounds (Salmon et al., SC 2011), key `seed`, counter
+ * (i / 8, offset): the low half of word (i % 8) / 2 where i is even, else the
+ * high one.  It is kept where they are at least t = round(65536 p) (65535 at
+ * most), and then multiplied by 65536 / (65536 - t); else it is 0, whatever it
+ * held.  So the mask is not stored: the backward pass takes the same seed and
+ * offset.  `step` may be NULL, or an int64_t on the device that is added to
+ * `offset` when the call runs (a replayed graph then draws other bits each time).
+ */
+
+/*
+ * y = drop(x) + residual; all hold x_len elements, residual may be NULL.  y may
+ * be x's or the residual's buffer.  The gradient of x is drop(dy), of the
+ * residual dy.
+ * Errors, in this order: ShapeMismatch "x" / "residual" / "out", InvalidParam
+ *   "p" (not in [0, 1)).
+ */
+int32_t mlrs_dropout_f32(const float *x, int64_t x_len, double p, uint64_t seed, uint64_t offset, const int64_t *step,
+                         const float *residual, int64_t residual_len, float *y, int64_t y_len, void *stream);
+int32_t mlrs_dropout_f16(const uint16_t *x, int64_t x_len, double p, uint64_t seed, uint64_t offset,
+                         const int64_t *step, const uint16_t *residual, int64_t residual_len, uint16_t *y,
+                         int64_t y_len, void *stream);
+int32_t mlrs_dropout_bf16(const uint16_t *x, int64_t x_len, double p, uint64_t seed, uint64_t offset,
+                          const int64_t *step, const uint16_t *residual, int64_t residual_len, uint16_t *y,
+                          int64_t y_len, void *stream);
+
+/*
+ * Group norm, channels last: x is n x positions x channels, in `groups` groups of
+ * adjacent channels (8192 at most).  With mean and variance (over all of them, not
+ * one less) of a sample's group over its positions, and rstd = 1 / sqrt(var + eps):
+ *   z = (x - mean) rstd weight + bias,  y = drop(act(z)).
+ * weight and bias hold `channels` elements and may be NULL (1 and 0).  mean and
+ * rstd (n x groups, f32) may both be NULL; the gradient takes them.
+ * Errors, in this order: ShapeMismatch "x" / "features" (positions or channels
+ *   < 1) / "groups" (< 1, or channels no multiple), MLRS_ERR_UNSUPPORTED "groups"
+ *   / "features" (channels > 2^22, positions > 2^31, n > 2^40), ShapeMismatch
+ *   "weight" / "bias" / "out" / "stats", MLRS_ERR_UNSUPPORTED "activation",
+ *   InvalidParam "eps" / "p".
+ */
+int32_t mlrs_group_norm_f32(const float *x, int64_t x_len, int64_t n, int64_t positions, int64_t channels,
+                            int64_t groups, const float *weight, int64_t weight_len, const float *bias,
+                            int64_t bias_len, double eps, int32_t activation, double p, uint64_t seed,
+                            uint64_t offset, const int64_t *step, float *y, int64_t y_len, float *mean, float *rstd,
+                            int64_t stats_len, void *stream);
+int32_t mlrs_group_norm_f16(const uint16_t *x, int64_t x_len, int64_t n, int64_t positions, int64_t channels,
+                            int64_t groups, const uint16_t *weight, int64_t weight_len, const uint16_t *bias,
+                            int64_t bias_len, double eps, int32_t activation, double p, uint64_t seed,
+                            uint64_t offset, const int64_t *step, uint16_t *y, int64_t y_len, float *mean,
+                            float *rstd, int64_t stats_len, void *stream);
+int32_t mlrs_group_norm_bf16(const uint16_t *x, int64_t x_len, int64_t n, int64_t positions, int64_t channels,
+                             int64_t groups, const uint16_t *weight, int64_t weight_len, const uint16_t *bias,
+                             int64_t bias_len, double eps, int32_t activation, double p, uint64_t seed,
+                             uint64_t offset, const int64_t *step, uint16_t *y, int64_t y_len, float *mean,
+                             float *rstd, int64_t stats_len, void *stream);
+
+/*
+ * Its gradient: with dz = drop(dy) act'(z) and t = dz weight, dbias = the sums of
+ * dz over samples and positions, dweight those of dz (x - mean) rstd, and dx =
+ * rstd (t - (mean of t) - (x - mean) rstd (mean of t (x - mean) rstd)), the means
+ * over the sample's group.  z is computed again.  Any of dx, dweight and dbias may
+ * be NULL (length 0); n = 0 gives dweight = 0 and dbias = 0.
+ * Errors, in this order: as mlrs_group_norm to "bias", ShapeMismatch "dy" /
+ *   "stats" / "dx" / "dweight" / "dbias", MLRS_ERR_UNSUPPORTED "activation",
+ *   InvalidParam "p".
+ */
+int32_t mlrs_group_norm_grad_f32(const float *dy, int64_t dy_len, const float *x, int64_t x_len, int64_t n,
+                                 int64_t positions, int64_t channels, int64_t groups, const float *weight,
+                                 int64_t weight_len, const float *bias, int64_t bias_len, const float *mean,
+                                 const float *rstd, int64_t stats_len, int32_t activation, double p, uint64_t seed,
+                                 uint64_t offset, const int64_t *step, float *dx, int64_t dx_len, float *dweight,
+                                 int64_t dweight_len, float *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_group_norm_grad_f16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                                 int64_t positions, int64_t channels, int64_t groups, const uint16_t *weight,
+                                 int64_t weight_len, const uint16_t *bias, int64_t bias_len, const float *mean,
+                                 const float *rstd, int64_t stats_len, int32_t activation, double p, uint64_t seed,
+                                 uint64_t offset, const int64_t *step, uint16_t *dx, int64_t dx_len,
+                                 uint16_t *dweight, int64_t dweight_len, uint16_t *dbias, int64_t dbias_len,
+                                 void *stream);
+int32_t mlrs_group_norm_grad_bf16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                                  int64_t positions, int64_t channels, int64_t groups, const uint16_t *weight,
+                                  int64_t weight_len, const uint16_t *bias, int64_t bias_len, const float *mean,
+                                  const float *rstd, int64_t stats_len, int32_t activation, double p, uint64_t seed,
+                                  uint64_t offset, const int64_t *step, uint16_t *dx, int64_t dx_len,
+                                  uint16_t *dweight, int64_t dweight_len, uint16_t *dbias, int64_t dbias_len,
+                                  void *stream);
+
 #define MLRS_DTYPE_F32 0
 #define MLRS_DTYPE_F16 1
 #define MLRS_DTYPE_BF16 2

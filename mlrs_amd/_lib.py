@@ -109,6 +109,7 @@ class AdamwTensor(ctypes.Structure):
 
 # (name, restype, argtypes) of every exported symbol in include/mlrs_hip_knn.h
 _i32, _i64, _vp, _f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
+_u64 = ctypes.c_uint64
 SIGNATURES = {
     "mlrs_last_error": (_i32, [ctypes.POINTER(ErrorInfo)]),
     "mlrs_status_string": (ctypes.c_char_p, [_i32]),
@@ -168,6 +169,13 @@ for _s in ("f32", "f16", "bf16"):
                                                     _vp, _vp, _i64, _vp])
     SIGNATURES["mlrs_softmax_xent_grad_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                                                          _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp])
+
+    SIGNATURES["mlrs_dropout_" + _s] = (_i32, [_vp, _i64, _f64, _u64, _u64, _vp, _vp, _i64, _vp, _i64, _vp])
+    SIGNATURES["mlrs_group_norm_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _f64, _i32,
+                                                  _f64, _u64, _u64, _vp, _vp, _i64, _vp, _vp, _i64, _vp])
+    SIGNATURES["mlrs_group_norm_grad_" + _s] = (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
+                                                       _i64, _vp, _vp, _i64, _i32, _f64, _u64, _u64, _vp, _vp, _i64,
+                                                       _vp, _i64, _vp, _i64, _vp])
 
 _lib = None
 

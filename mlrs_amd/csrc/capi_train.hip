@@ -4,10 +4,9 @@
 
 #include <algorithm>
 #include <cmath>
-#include <initializer_list>
 
 #include "../../include/mlrs_hip_knn.h"
-#include "capi_shared.hpp"
+#include "capi_train.hpp"
 #include "train_kernels.hpp"
 
 using namespace mlrs;
@@ -19,24 +18,6 @@ constexpr int64_t kMaxCount = 0x7FFFFFFF - 512;  // a tile past it must not over
 constexpr int64_t kMaxRowBytes = (int64_t)1 << 22;  // 256 rows of a tile within a buffer descriptor's 2^31
 
 constexpr int64_t kStatsBytes = (int64_t)256 << 20;  // of a loss's partial statistics
-
-int32_t null_error(const char* operand) {
-    return capi::error(MLRS_ERR_NULL_POINTER, operand, 0, 0, 0, "null pointer");
-}
-
-// Carves a call's scratch: first a pass that only adds up, then one that hands
-// out addresses.
-struct Scratch {
-    char* base = nullptr;
-    size_t used = 0;
-    template <typename T>
-    T* take(size_t n) {
-        used = (used + 255) & ~(size_t)255;
-        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
-        used += n * sizeof(T);
-        return p;
-    }
-};
 
 template <typename T>
 int64_t padded(int64_t cols) {
@@ -126,33 +107,6 @@ bool grid_fits(int64_t m, int64_t n) { return launchable(((m + 255) / 256) * ((n
 int32_t grid_error(int64_t m, int64_t n) {
     return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, m, 0, "the product has more tiles than a launch");
 }
-
-// What a call writes may be no part of what it reads or else writes: workgroups
-// read operands while others write results.
-struct Span {
-    const void* p;
-    int64_t bytes;
-    template <typename T>
-    Span(const T* t, int64_t len) : p(t), bytes(t ? len * (int64_t)sizeof(T) : 0) {}
-    bool meets(const Span& o) const {
-        const uintptr_t a = (uintptr_t)p, b = (uintptr_t)o.p;
-        return bytes > 0 && o.bytes > 0 && a < b + (uintptr_t)o.bytes && b < a + (uintptr_t)bytes;
-    }
-    bool meets(std::initializer_list<Span> others) const {
-        for (const Span& o : others)
-            if (meets(o)) return true;
-        return false;
-    }
-};
-int32_t overlap_error(const char* out) {
-    return capi::error(MLRS_ERR_INVALID_PARAM, out, 0, 0, 0, "an output overlaps another operand");
-}
-
-#define MLRS_TRY(call)                                      \
-    do {                                                    \
-        const hipError_t e_ = (call);                       \
-        if (e_ != hipSuccess) return capi::hip_error(e_, where); \
-    } while (0)
 
 // ---------------------------------------------------------------------------
 template <typename T>

@@ -186,6 +186,38 @@ hipError_t launch_logit_grad_split(Mat h, Mat w, const float* bias, const int64_
                                    int64_t k, int64_t ignore, float* out, int64_t ld, float* sums,
                                    const Only& only, hipStream_t s);
 
+// Dropout: an element is kept where its sixteen random bits are at least
+// `threshold` (0: all are), and multiplied by `factor` then.
+struct Drop {
+    uint32_t threshold;
+    float factor;
+    uint32_t k0, k1;      // the seed
+    uint64_t offset;
+    const int64_t* step;  // device scalar that is added to the offset; may be null
+};
+template <typename T>
+hipError_t launch_dropout(const T* x, const T* residual, T* y, int64_t len, const Drop& drop, int cus, hipStream_t s);
+
+// Group norm, channels last: x is n x s x c.  Backwards y is dx, and dy, dw and db
+// are its other operands; y, dw and db may be null then, mean and rstd forwards.
+constexpr int64_t kNormGroup = 8192;  // channels of a group, at most
+struct NormCall {
+    const void *x, *w, *b, *dy;
+    void* y;
+    float *mean, *rstd;
+    void *dw, *db;
+    int64_t n, s, c, g;
+    float eps;
+    int act;
+    Drop drop;
+};
+size_t norm_scratch(int elem_bytes, const NormCall& k, int cus);
+template <typename T>
+hipError_t launch_norm(const NormCall& k, float* scratch, int cus, hipStream_t s);
+size_t norm_grad_scratch(int elem_bytes, const NormCall& k, int cus);
+template <typename T>
+hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStream_t s);
+
 // Optimizer.
 int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);
 hipError_t launch_clip_scale(const mlrs_grad_tensor* t, int64_t count, double max_norm, double* parts, float* norm,

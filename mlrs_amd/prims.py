@@ -34,6 +34,9 @@ it takes float32, float16 and bfloat16 tensors:
 | ``clip_scale``           | the norm of many gradients and the factor that clips it    |
 | ``adamw_step``           | AdamW over many tensors, states in 32 or 8 bits            |
 | ``adamw_state_values``   | the values that an 8-bit state stands for                  |
+| ``dropout``              | dropout whose mask is computed, not stored; a residual     |
+| ``group_norm``           | group norm, channels last, with an activation and dropout  |
+| ``group_norm_grad``      | its gradient                                               |
 """
 import ctypes
 import itertools
@@ -763,3 +766,122 @@ def adamw_state_values(codes, scales, which):
                                                    int(which == "exp_avg_sq"), _ptr(out), out.numel(),
                                                    _stream(codes.device)))
     return out
+
+
+# ---- the rest of an encoder's layer ----
+
+_WORD64 = (1 << 64) - 1
+
+
+def _drop_args(p, seed, offset, device):
+    """(p, seed, offset, pointer to the offset on the device or None)."""
+    p = float(p)
+    if isinstance(offset, torch.Tensor):
+        _check_out(offset, "offset", (torch.int64,), 1, device)
+        return p, int(seed) & _WORD64, 0, _ptr(offset)
+    return p, int(seed) & _WORD64, int(offset) & _WORD64, None
+
+
+def dropout(x, p, seed, offset=0, residual=None, out=None):
+    """``x`` with each element 0 with probability ``p`` and divided by ``1 - p``
+    else, plus ``residual`` (mlrs_dropout_*).
+
+    The mask is a function of ``seed``, ``offset`` and the element's index and is
+    not stored: the gradient of x is ``dropout(dy, p, seed, offset)``, the
+    residual's ``dy``.  Give every call of a step its own ``offset`` (or ``seed``).
+    ``offset`` may be an int64 (1,) device tensor, read when the call runs: a call
+    captured into a graph then draws other bits in each replay.  ``p`` in [0, 1) is
+    taken to the nearest multiple of 2^-16.  ``out`` receives the result; it may be
+    ``x`` or ``residual`` itself."""
+    others = () if residual is None else (residual,)
+    _dev_check(x, *others)
+    s = _train_suffix(x)
+    if residual is not None:
+        if residual.dtype != x.dtype:
+            raise TypeError("x and residual dtypes differ (%s, %s)" % (x.dtype, residual.dtype))
+        if residual.shape != x.shape:
+            raise ValueError("residual has shape %s, x %s" % (tuple(residual.shape), tuple(x.shape)))
+    if out is None:
+        y = torch.empty_like(x)
+    else:
+        _check_out(out, "out", (x.dtype,), x.numel(), x.device)
+        y = out
+    p, seed, offset, step = _drop_args(p, seed, offset, x.device)
+    _lib.check(getattr(_lib.load(), "mlrs_dropout_" + s)(
+        _ptr(x), x.numel(), p, seed, offset, step, _ptr(residual), _len(residual), _ptr(y), y.numel(),
+        _stream(x.device)))
+    return y
+
+
+def _norm_operands(x, *others):
+    """The checks that group norm and its gradient share; `others`: (tensor or
+    None, name) pairs of x's element type.  (suffix, samples, positions, channels)."""
+    given = [(t, name) for t, name in others if t is not None]
+    _dev_check(x, *[t for t, _ in given])
+    s = _train_suffix(x)
+    for t, name in given:
+        if t.dtype != x.dtype:
+            raise TypeError("x and %s dtypes differ (%s, %s)" % (name, x.dtype, t.dtype))
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError("x must have two dimensions at least (samples, ..., channels), got %s" % (tuple(shape),))
+    positions = 1
+    for k in shape[1:-1]:
+        positions *= k
+    return s, shape[0], positions, shape[-1]
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="none", p=0.0, seed=0, offset=0,
+               keep_stats=False):
+    """Group norm, channels last, with an activation and dropout
+    (mlrs_group_norm_*): ``drop(act((x - mean) * rstd * weight + bias))``.
+
+    ``x`` (n, ..., channels) has its channels in ``groups`` groups of adjacent ones;
+    mean and rstd = 1 / sqrt(variance + eps) are those of a sample's group over all
+    positions between the first dimension and the last.  One group of a
+    two-dimensional x is layer norm.  ``weight`` and ``bias`` (channels,) have x's
+    dtype; ``activation`` as in ``linear``; ``p``, ``seed`` and ``offset`` as in
+    ``dropout``.  Returns y, or ``(y, mean, rstd)`` with ``keep_stats``, float32 (n,
+    groups) each: what ``group_norm_grad`` takes."""
+    s, n, positions, c = _norm_operands(x, (weight, "weight"), (bias, "bias"))
+    act = _activation_id(activation)
+    groups = int(groups)
+    y = torch.empty_like(x)
+    mean = rstd = None
+    if keep_stats:
+        mean = x.new_empty((n, max(groups, 0)), dtype=torch.float32)
+        rstd = torch.empty_like(mean)
+    p, seed, offset, step = _drop_args(p, seed, offset, x.device)
+    _lib.check(getattr(_lib.load(), "mlrs_group_norm_" + s)(
+        _ptr(x), x.numel(), n, positions, c, groups, _ptr(weight), _len(weight), _ptr(bias), _len(bias), float(eps),
+        act, p, seed, offset, step, _ptr(y), y.numel(), _ptr(mean), _ptr(rstd), _len(mean), _stream(x.device)))
+    return (y, mean, rstd) if keep_stats else y
+
+
+def group_norm_grad(dy, x, mean, rstd, weight=None, bias=None, activation="none", p=0.0, seed=0, offset=0,
+                    need_dx=True):
+    """The gradient of ``group_norm`` (mlrs_group_norm_grad_*): ``(dx, dweight,
+    dbias)``, None in the place of what is not asked for (``dweight`` without a
+    ``weight``, ``dbias`` without a ``bias``).
+
+    ``dy`` is the gradient of y; ``mean`` and ``rstd`` are what ``group_norm`` kept,
+    and the other arguments are that call's."""
+    s, n, positions, c = _norm_operands(x, (dy, "dy"), (weight, "weight"), (bias, "bias"))
+    _dev_check(x, mean, rstd)
+    if dy.shape != x.shape:
+        raise ValueError("dy has shape %s, x %s" % (tuple(dy.shape), tuple(x.shape)))
+    if mean.dim() != 2 or mean.shape[0] != n:
+        raise ValueError("mean must be (%d, groups), got %s" % (n, tuple(mean.shape)))
+    groups = mean.shape[1]
+    _check_rows(mean, "mean", torch.float32, n * groups)
+    _check_rows(rstd, "rstd", torch.float32, n * groups)
+    act = _activation_id(activation)
+    dx = torch.empty_like(x) if need_dx else None
+    dw = torch.empty_like(weight) if weight is not None else None
+    db = torch.empty_like(bias) if bias is not None else None
+    p, seed, offset, step = _drop_args(p, seed, offset, x.device)
+    _lib.check(getattr(_lib.load(), "mlrs_group_norm_grad_" + s)(
+        _ptr(dy), dy.numel(), _ptr(x), x.numel(), n, positions, c, groups, _ptr(weight), _len(weight), _ptr(bias),
+        _len(bias), _ptr(mean), _ptr(rstd), mean.numel(), act, p, seed, offset, step, _ptr(dx), _len(dx), _ptr(dw),
+        _len(dw), _ptr(db), _len(db), _stream(x.device)))
+    return dx, dw, db
