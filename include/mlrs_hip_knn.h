@@ -583,7 +583,8 @@ int32_t mlrs_softmax_xent_grad_bf16(const uint16_t *h, int64_t h_len, int64_t n,
 
 /*
  * ---- the rest of an encoder's layer ----
- * Dropout, and group norm with an activation and dropout.  Element types,
+ * Dropout, group norm with an activation and dropout, and the layer in 8-bit
+ * floating point.  Element types,
  * overlaps and errors as above.  No call here synchronizes or reads back.  A call
  * that takes no workspace can be captured into a graph and replayed; one that
  * does is refused there (MLRS_ERR_UNSUPPORTED "stream").
@@ -673,6 +674,91 @@ int32_t mlrs_group_norm_grad_bf16(const uint16_t *dy, int64_t dy_len, const uint
                                   uint64_t offset, const int64_t *step, uint16_t *dx, int64_t dx_len,
                                   uint16_t *dweight, int64_t dweight_len, uint16_t *dbias, int64_t dbias_len,
                                   void *stream);
+
+/*
+ * ---- a layer in 8-bit floating point ----
+ * Values are held as e4m3 codes (OCP: largest 448, no infinities, a NaN) with a
+ * power of two for every block of 128 elements of a contraction axis, the least
+ * with which no finite magnitude of the block passes 448 (1 for a block of zeros);
+ * a code is the value over its scale, rounded to nearest even, so that a value is
+ * rounded once.  Infinities and NaN have code NaN and no part in the scale.
+ * Weights: one scale for each 128 x 128.  codes: d_out x C bytes, C = d_in rounded
+ * up to 128, zeros behind a row; scales: a byte (the exponent + 127) for each tile,
+ * ceil(d_out / 128) rows of S bytes, S = ceil(d_in / 128) rounded up to 4, 127
+ * behind a row.  codes_t / scales_t: the same of the transpose (d_in rows), which
+ * the gradient takes.  Codes are aligned to 16 bytes, scales to 4.
+ */
+
+/*
+ * The codes of weights w (d_out x d_in); codes_t and scales_t may both be NULL
+ * (lengths 0).
+ * Errors, in this order: ShapeMismatch "w" / "features", MLRS_ERR_UNSUPPORTED
+ *   "features" (> 2^22), ShapeMismatch and then InvalidParam (alignment) "codes" /
+ *   "scales", "codes_t" / "scales_t".
+ */
+int32_t mlrs_fp8_weight_f32(const float *w, int64_t w_len, int64_t d_out, int64_t d_in, uint8_t *codes,
+                            int64_t codes_len, uint8_t *scales, int64_t scales_len, uint8_t *codes_t,
+                            int64_t codes_t_len, uint8_t *scales_t, int64_t scales_t_len, void *stream);
+int32_t mlrs_fp8_weight_f16(const uint16_t *w, int64_t w_len, int64_t d_out, int64_t d_in, uint8_t *codes,
+                            int64_t codes_len, uint8_t *scales, int64_t scales_len, uint8_t *codes_t,
+                            int64_t codes_t_len, uint8_t *scales_t, int64_t scales_t_len, void *stream);
+int32_t mlrs_fp8_weight_bf16(const uint16_t *w, int64_t w_len, int64_t d_out, int64_t d_in, uint8_t *codes,
+                             int64_t codes_len, uint8_t *scales, int64_t scales_len, uint8_t *codes_t,
+                             int64_t codes_t_len, uint8_t *scales_t, int64_t scales_t_len, void *stream);
+
+/*
+ * mlrs_linear with such weights: z = x' w'^T + bias, y = act(z) + residual, where x'
+ * is what 8 bits hold of x, a scale for each 128 of a row, and w' what the codes
+ * stand for.  Products are exact.  f16, bf16: the matrix instruction adds eight
+ * adjacent products after cutting off what lies below 2^-13 of the largest one's
+ * power of two, all else in f32.  f32: added up in f32, the values of more than 32
+ * rows in bf16's range.  Up to 32 rows take no workspace.
+ * Errors, in this order: ShapeMismatch "x" / "features", MLRS_ERR_UNSUPPORTED
+ *   "features" / "rows", "codes" and "scales" as above, then as mlrs_linear from
+ *   "bias" on.
+ */
+int32_t mlrs_linear_fp8_f32(const float *x, int64_t x_len, int64_t n, int64_t d_in, const uint8_t *codes,
+                            int64_t codes_len, const uint8_t *scales, int64_t scales_len, int64_t d_out,
+                            const float *bias, int64_t bias_len, const float *residual, int64_t residual_len,
+                            int32_t activation, float *y, int64_t y_len, float *preact, int64_t preact_len,
+                            void *stream);
+int32_t mlrs_linear_fp8_f16(const uint16_t *x, int64_t x_len, int64_t n, int64_t d_in, const uint8_t *codes,
+                            int64_t codes_len, const uint8_t *scales, int64_t scales_len, int64_t d_out,
+                            const uint16_t *bias, int64_t bias_len, const uint16_t *residual, int64_t residual_len,
+                            int32_t activation, uint16_t *y, int64_t y_len, uint16_t *preact, int64_t preact_len,
+                            void *stream);
+int32_t mlrs_linear_fp8_bf16(const uint16_t *x, int64_t x_len, int64_t n, int64_t d_in, const uint8_t *codes,
+                             int64_t codes_len, const uint8_t *scales, int64_t scales_len, int64_t d_out,
+                             const uint16_t *bias, int64_t bias_len, const uint16_t *residual, int64_t residual_len,
+                             int32_t activation, uint16_t *y, int64_t y_len, uint16_t *preact, int64_t preact_len,
+                             void *stream);
+
+/*
+ * Its gradient, of the values in 8 bits as if they were x and w: dz = dy
+ * act'(preact), dx = dz' w' with a scale for each 128 of a row of dz, dw = dz''^T
+ * x'' with one for each 128 rows of a column of dz and of x; dbias = the column sums
+ * of dz itself.  Any of dx, dw and dbias may be NULL (length 0); codes_t and scales_t
+ * may be where dx is.  n is limited to 2^22; n = 0 gives dw = 0 and dbias = 0.
+ * Errors, in this order: as mlrs_linear_fp8 to "scales" ("codes_t" / "scales_t"
+ *   where they are given), ShapeMismatch "dy" / "dx" / "dw" / "dbias",
+ *   MLRS_ERR_UNSUPPORTED "activation", ShapeMismatch "preact", MLRS_ERR_UNSUPPORTED
+ *   "rows".
+ */
+int32_t mlrs_linear_fp8_grad_f32(const float *dy, int64_t dy_len, const float *x, int64_t x_len, int64_t n,
+                                 int64_t d_in, const uint8_t *codes_t, int64_t codes_t_len, const uint8_t *scales_t,
+                                 int64_t scales_t_len, int64_t d_out, const float *preact, int64_t preact_len,
+                                 int32_t activation, float *dx, int64_t dx_len, float *dw, int64_t dw_len,
+                                 float *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_linear_fp8_grad_f16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                                 int64_t d_in, const uint8_t *codes_t, int64_t codes_t_len, const uint8_t *scales_t,
+                                 int64_t scales_t_len, int64_t d_out, const uint16_t *preact, int64_t preact_len,
+                                 int32_t activation, uint16_t *dx, int64_t dx_len, uint16_t *dw, int64_t dw_len,
+                                 uint16_t *dbias, int64_t dbias_len, void *stream);
+int32_t mlrs_linear_fp8_grad_bf16(const uint16_t *dy, int64_t dy_len, const uint16_t *x, int64_t x_len, int64_t n,
+                                  int64_t d_in, const uint8_t *codes_t, int64_t codes_t_len, const uint8_t *scales_t,
+                                  int64_t scales_t_len, int64_t d_out, const uint16_t *preact, int64_t preact_len,
+                                  int32_t activation, uint16_t *dx, int64_t dx_len, uint16_t *dw, int64_t dw_len,
+                                  uint16_t *dbias, int64_t dbias_len, void *stream);
 
 #define MLRS_DTYPE_F32 0
 #define MLRS_DTYPE_F16 1

@@ -176,6 +176,12 @@ for _s in ("f32", "f16", "bf16"):
     SIGNATURES["mlrs_group_norm_grad_" + _s] = (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp,
                                                        _i64, _vp, _vp, _i64, _i32, _f64, _u64, _u64, _vp, _vp, _i64,
                                                        _vp, _i64, _vp, _i64, _vp])
+    SIGNATURES["mlrs_fp8_weight_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                                  _vp])
+    SIGNATURES["mlrs_linear_fp8_" + _s] = (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp,
+                                                  _i64, _i32, _vp, _i64, _vp, _i64, _vp])
+    SIGNATURES["mlrs_linear_fp8_grad_" + _s] = (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64,
+                                                       _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp])
 
 _lib = None
 

@@ -218,6 +218,51 @@ size_t norm_grad_scratch(int elem_bytes, const NormCall& k, int cus);
 template <typename T>
 hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStream_t s);
 
+// Products in 8-bit floating point (train_fp8.hpp).  Codes: rows x fp8_columns(k),
+// scales fp8_scale_row(k) bytes for every row or, `tile`, for every 128.  f32 calls
+// have the values as bf16 in the codes' place, without scales.
+struct Fp8Mat {
+    const void* codes;
+    const uint8_t* scales;
+    bool tile;
+};
+inline int64_t fp8_columns(int64_t k) { return (k + 127) / 128 * 128; }
+inline int64_t fp8_scale_row(int64_t k) { return (k + 511) / 512 * 4; }
+// Codes of weights, and of their transpose where to_t has some.
+template <typename T>
+hipError_t launch_fp8_weight(const T* w, int64_t rows, int64_t cols, const Fp8Mat& to, const Fp8Mat& to_t, hipStream_t s);
+// The values of weights' codes.
+hipError_t launch_fp8_values(const Fp8Mat& w, int64_t rows, int64_t k, void* out, hipStream_t s);
+template <typename T>
+hipError_t launch_fp8_rows(const T* x, int64_t n, int64_t k, const Fp8Mat& to, hipStream_t s);
+// Codes of dz = dy act'(z) (z may be null) and of its transpose, its column sums of
+// every 128 rows, and codes of the transpose of x; each may be null.
+template <typename T>
+hipError_t launch_fp8_grad_codes(const T* dy, const T* z, int act, int64_t n, int64_t m, const Fp8Mat& dz,
+                                 const Fp8Mat& dz_t, float* sums, const T* x, int64_t k, const Fp8Mat& x_t,
+                                 hipStream_t s);
+// k_split is a multiple of 512.  tile: a choice of it, or -1.
+Cut choose_cut_fp8(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int tile = -1);
+void choose_pair_fp8(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus,
+                     Cut* x, Cut* w);
+template <typename T>
+hipError_t launch_fp8_linear(const Fp8Mat& x, const Fp8Mat& w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
+                             const Cut& cut, float* part, hipStream_t s);
+// The same for at most kFp8Few rows, from the rows themselves.
+constexpr int64_t kFp8Few = 32;
+template <typename T>
+hipError_t launch_fp8_few(const T* x, const Fp8Mat& w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
+                          hipStream_t s);
+// The two products of a gradient, both operands with k contiguous; m = 0: not wanted.
+struct Fp8Product {
+    Fp8Mat a, b;
+    int64_t m, n, k;
+    StoreTo to;
+};
+template <typename T>
+hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const Cut& cx, const Cut& cw, float* part,
+                               hipStream_t s);
+
 // Optimizer.
 int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);
 hipError_t launch_clip_scale(const mlrs_grad_tensor* t, int64_t count, double max_norm, double* parts, float* norm,

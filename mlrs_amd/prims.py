@@ -37,10 +37,14 @@ it takes float32, float16 and bfloat16 tensors:
 | ``dropout``              | dropout whose mask is computed, not stored; a residual     |
 | ``group_norm``           | group norm, channels last, with an activation and dropout  |
 | ``group_norm_grad``      | its gradient                                               |
+| ``fp8_weight``           | weights in 8-bit floating point, a scale per 128 x 128     |
+| ``linear_fp8``           | a layer with such weights                                  |
+| ``linear_fp8_grad``      | its gradient                                               |
 """
 import ctypes
 import itertools
 import struct
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -884,4 +888,119 @@ def group_norm_grad(dy, x, mean, rstd, weight=None, bias=None, activation="none"
         _ptr(dy), dy.numel(), _ptr(x), x.numel(), n, positions, c, groups, _ptr(weight), _len(weight), _ptr(bias),
         _len(bias), _ptr(mean), _ptr(rstd), mean.numel(), act, p, seed, offset, step, _ptr(dx), _len(dx), _ptr(dw),
         _len(dw), _ptr(db), _len(db), _stream(x.device)))
+    return dx, dw, db
+
+
+# ---- a layer in 8-bit floating point ----
+
+class Fp8Weight(NamedTuple):
+    """Weights (d_out, d_in) in 8-bit floating point, as ``fp8_weight`` lays them
+    out: float8_e4m3fn ``codes`` (d_out, d_in rounded up to 128), zeros behind each
+    row, and uint8 ``scales``, the exponent + 127 of the power of two of each 128 x
+    128 (ceil(d_out / 128) rows of ceil(d_in / 128) bytes, rounded up to 4).
+    ``codes_t`` and ``scales_t`` are those of the transpose, or None."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    codes_t: Optional[torch.Tensor]
+    scales_t: Optional[torch.Tensor]
+    d_in: int
+
+
+def _fp8_empty(rows, cols, device):
+    return (torch.empty((rows, -(-cols // 128) * 128), dtype=torch.float8_e4m3fn, device=device),
+            torch.empty((-(-rows // 128), -(-cols // 512) * 4), dtype=torch.uint8, device=device))
+
+
+def fp8_weight(w, backward=False):
+    """``w`` (d_out, d_in) as an ``Fp8Weight`` (mlrs_fp8_weight_*); with ``backward``
+    its transpose too, which ``linear_fp8_grad`` takes.
+
+    A 128 x 128's scale is the least power of two with which no finite magnitude
+    passes 448, the largest code, so that a value is rounded once, to nearest even
+    (relative error 2^-4 at most, but below 2^-6 of the scale).  Infinities and NaN
+    become NaN."""
+    _dev_check(w)
+    s = _train_suffix(w)
+    if w.dim() != 2:
+        raise ValueError("w must have two dimensions, got %s" % (tuple(w.shape),))
+    m, k = w.shape
+    codes, scales = _fp8_empty(m, k, w.device)
+    codes_t, scales_t = _fp8_empty(k, m, w.device) if backward else (None, None)
+    _lib.check(getattr(_lib.load(), "mlrs_fp8_weight_" + s)(
+        _ptr(w), w.numel(), m, k, _ptr(codes), codes.numel(), _ptr(scales), scales.numel(), _ptr(codes_t),
+        _len(codes_t), _ptr(scales_t), _len(scales_t), _stream(w.device)))
+    return Fp8Weight(codes, scales, codes_t, scales_t, k)
+
+
+def _fp8_operands(x, w8, codes, scales, *others):
+    """The checks that a layer in 8 bits and its gradient share: (suffix, n, d_in,
+    d_out)."""
+    given = [(t, name) for t, name in others if t is not None]
+    _dev_check(x, w8.codes, codes, scales, *[t for t, _ in given])
+    s = _train_suffix(x)
+    for t, name in given:
+        if t.dtype != x.dtype:
+            raise TypeError("x and %s dtypes differ (%s, %s)" % (name, x.dtype, t.dtype))
+    for t in (w8.codes, codes):
+        if t.dtype != torch.float8_e4m3fn or t.dim() != 2:
+            raise TypeError("codes must be two-dimensional float8_e4m3fn, got %s %s" % (tuple(t.shape), t.dtype))
+    if scales.dtype != torch.uint8:
+        raise TypeError("scales must be uint8, got %s" % scales.dtype)
+    if x.dim() != 2:
+        raise ValueError("x must have two dimensions, got %s" % (tuple(x.shape),))
+    if x.shape[1] != w8.d_in:
+        raise ValueError("x has %d columns, w8 %d" % (x.shape[1], w8.d_in))
+    return s, x.shape[0], x.shape[1], w8.codes.shape[0]
+
+
+def linear_fp8(x, w8, bias=None, activation="none", residual=None, keep_preact=False, out=None):
+    """``linear`` with weights in 8-bit floating point (mlrs_linear_fp8_*):
+    ``act(x' w'^T + bias) + residual``, with x' what 8 bits hold of ``x`` (a scale
+    for each 128 of a row, made in the call) and w' what ``w8``, an ``Fp8Weight``,
+    stands for.
+
+    Products are exact.  float16 and bfloat16: the matrix instruction adds eight
+    adjacent ones after cutting off what lies below 2^-13 of the largest one's power
+    of two, all else in float32; float32 calls add up in float32, at half the rate.
+    The other arguments and the result are ``linear``'s.  Up to 32 rows take one
+    launch and no workspace."""
+    s, n, d_in, d_out = _fp8_operands(x, w8, w8.codes, w8.scales, (bias, "bias"), (residual, "residual"))
+    act = _activation_id(activation)
+    if out is None:
+        y = x.new_empty((n, d_out))
+    else:
+        _check_out(out, "out", (x.dtype,), n * d_out, x.device)
+        y = out
+    z = x.new_empty((n, d_out)) if keep_preact else None
+    _lib.check(getattr(_lib.load(), "mlrs_linear_fp8_" + s)(
+        _ptr(x), x.numel(), n, d_in, _ptr(w8.codes), w8.codes.numel(), _ptr(w8.scales), w8.scales.numel(), d_out,
+        _ptr(bias), _len(bias), _ptr(residual), _len(residual), act, _ptr(y), y.numel(), _ptr(z), _len(z),
+        _stream(x.device)))
+    return (y, z) if keep_preact else y
+
+
+def linear_fp8_grad(dy, x, w8, preact=None, activation="none", bias=True, need_dx=True, need_dw=True):
+    """The gradient of ``linear_fp8`` (mlrs_linear_fp8_grad_*): ``(dx, dw, dbias)``,
+    None in the place of what is not asked for.
+
+    The gradient is that of the 8-bit values as if they were ``x`` and the weights:
+    dz = dy * act'(preact) goes into dx in 8 bits with a scale for each 128 of a row
+    (``w8`` must hold its transpose), and into dw with one for each 128 rows of a
+    column, as x does; ``dbias`` sums dz itself.  The arguments are ``linear_grad``'s."""
+    act = _activation_id(activation)
+    z = preact if act else None
+    if act and z is None:
+        raise ValueError("activation %r needs preact, the z that linear_fp8 kept" % (activation,))
+    if need_dx and (w8.codes_t is None or w8.scales_t is None):
+        raise ValueError("dx needs the transposed weights: fp8_weight(w, backward=True)")
+    codes_t, scales_t = (w8.codes_t, w8.scales_t) if need_dx else (None, None)
+    s, n, d_in, d_out = _fp8_operands(x, w8, codes_t if need_dx else w8.codes, scales_t if need_dx else w8.scales,
+                                      (dy, "dy"), (z, "preact"))
+    dx = torch.empty_like(x) if need_dx else None
+    dw = x.new_empty((d_out, d_in)) if need_dw else None
+    db = x.new_empty(d_out) if bias else None
+    _lib.check(getattr(_lib.load(), "mlrs_linear_fp8_grad_" + s)(
+        _ptr(dy), dy.numel(), _ptr(x), x.numel(), n, d_in, _ptr(codes_t), _len(codes_t), _ptr(scales_t),
+        _len(scales_t), d_out, _ptr(z), _len(z), act, _ptr(dx), _len(dx), _ptr(dw), _len(dw), _ptr(db), _len(db),
+        _stream(x.device)))
     return dx, dw, db
