@@ -3,12 +3,16 @@ dense encoder whose outputs separate given classes, for ``NearestNeighbors``,
 ``KNeighborsClassifier`` or ``KMeans`` over ``transform(X)``.  No counterpart in
 the reference.
 
-The network is layers ``act(x w^T + b)``, a layer as wide as its input adding
-it (``+ x``), a last linear layer to ``n_components`` columns, and a class head
-``h w^T + b`` under a softmax.  Every product, its activation and its gradient,
-the loss over the classes and the optimizer's step are the library's kernels
-(``prims.linear``, ``linear_grad``, ``softmax_xent``, ``softmax_xent_grad``,
-``clip_scale``, ``adamw_step``): the logits of a batch are never in memory, and
+The network is layers ``drop(act(x w^T + b))``, a layer as wide as its input
+adding it (``+ x``), a last linear layer to ``n_components`` columns, and a class
+head ``h w^T + b`` under a softmax.  With ``norm_groups`` a layer is
+``drop(act(group_norm(x w^T + b)))``; with ``products="fp8"`` the products of all
+layers but the head are those of 8-bit values, forwards and backwards.  Every
+product, norm, activation and gradient, dropout, the loss over the classes and the
+optimizer's step are the library's kernels (``prims.linear``, ``linear_grad``,
+``group_norm``, ``group_norm_grad``, ``dropout``, ``fp8_weight``, ``linear_fp8``,
+``linear_fp8_grad``, ``softmax_xent``, ``softmax_xent_grad``, ``clip_scale``,
+``adamw_step``): the logits of a batch and dropout's masks are never in memory, and
 a step reads nothing back.
 """
 import warnings
@@ -78,7 +82,12 @@ class EmbeddingEncoder:
     embedding; ``activation`` one of ``prims.ACTIVATIONS``; ``dtype`` the
     element type of the parameters and the products ("float32", "float16" or
     "bfloat16", the 16-bit types with float32 masters); ``state_bits`` that of
-    the optimizer's moments.  A step takes ``batch_size`` rows; ``epochs`` is
+    the optimizer's moments.  ``norm_groups``: None, or the groups of a group norm
+    (1: layer norm) between a hidden layer's product and its activation, a divisor of
+    every hidden width.  ``dropout`` in [0, 1) is a hidden layer's, in ``fit`` alone.
+    ``products``: "native", or "fp8" for 8-bit floating point with a scale for each
+    128 elements; the weights are kept in ``dtype`` and made into codes every step,
+    and once for the fitted encoder.  A step takes ``batch_size`` rows; ``epochs`` is
     the number of passes over the rows.  ``random_state=None`` is seed 0.
 
     After ``fit``: ``classes_``, ``loss_curve_`` (the mean loss of each epoch),
@@ -88,7 +97,7 @@ class EmbeddingEncoder:
 
     def __init__(self, n_components=64, hidden=(256,), activation="gelu", epochs=10, batch_size=1024,
                  learning_rate=1e-3, weight_decay=0.01, max_norm=1.0, dtype="float32", state_bits=32,
-                 random_state=None, output_type="input"):
+                 random_state=None, output_type="input", norm_groups=None, dropout=0.0, products="native"):
         self.n_components = n_components
         self.hidden = hidden
         self.activation = activation
@@ -101,6 +110,9 @@ class EmbeddingEncoder:
         self.state_bits = state_bits
         self.random_state = random_state
         self.output_type = output_type
+        self.norm_groups = norm_groups
+        self.dropout = dropout
+        self.products = products
 
     def _validate(self):
         if self.dtype not in _DTYPES:
@@ -113,51 +125,112 @@ class EmbeddingEncoder:
         for name in ("epochs", "batch_size"):
             if int(getattr(self, name)) < 1:
                 raise ValueError("%s should be > 0, got %r" % (name, getattr(self, name)))
+        if self.norm_groups is not None:
+            if int(self.norm_groups) < 1 or any(w % int(self.norm_groups) for w in widths[:-1]):
+                raise ValueError("norm_groups should divide every hidden width %r, got %r"
+                                 % (widths[:-1], self.norm_groups))
+        if not 0.0 <= float(self.dropout) < 1.0:
+            raise ValueError("dropout should be in [0, 1), got %r" % (self.dropout,))
+        if self.products not in ("native", "fp8"):
+            raise ValueError("products should be 'native' or 'fp8', got %r" % (self.products,))
         return widths
 
     def _init_params(self, d, widths, classes, device, gen):
-        """Weights of variance 1 / inputs, biases zero: [w, b] of every layer,
+        """Weights of variance 1 / inputs, biases zero, the norms' weights one: [w, b]
+        of every layer, of a hidden one with a norm [w, b, norm's weight, its bias];
         the class head last."""
         out = []
-        for wide in widths + [classes]:
+        dtype = _DTYPES[self.dtype]
+        for i, wide in enumerate(widths + [classes]):
             w = torch.empty(wide, d, dtype=torch.float32, device=device).normal_(0.0, d ** -0.5, generator=gen)
-            out += [w.to(_DTYPES[self.dtype]), torch.zeros(wide, dtype=_DTYPES[self.dtype], device=device)]
+            out += [w.to(dtype), torch.zeros(wide, dtype=dtype, device=device)]
+            if self.norm_groups is not None and i < len(widths) - 1:
+                out += [torch.ones(wide, dtype=dtype, device=device), torch.zeros(wide, dtype=dtype, device=device)]
             d = wide
         return out
 
     def _layers(self):
-        """(w, b, activation, whether the input is added) of every layer but the head."""
-        pairs = list(zip(self._params[0:-2:2], self._params[1:-2:2]))
-        last = len(pairs) - 1
-        return [(w, b, self.activation if i < last else "none", i < last and w.shape[0] == w.shape[1])
-                for i, (w, b) in enumerate(pairs)]
+        """(w, b, norm's weight and bias or None, activation, whether the input is
+        added) of every layer but the head; the last has neither norm, activation
+        nor sum."""
+        out, at = [], 0
+        each = 2 if self.norm_groups is None else 4
+        while at < len(self._params) - 4:
+            w, b = self._params[at:at + 2]
+            norm = None if each == 2 else self._params[at + 2:at + 4]
+            out.append((w, b, norm, self.activation, w.shape[0] == w.shape[1]))
+            at += each
+        w, b = self._params[at:at + 2]
+        return out + [(w, b, None, "none", False)]
+
+    def _codes(self, backward):
+        """The layers' weights in 8 bits, None for each with native products."""
+        return [prims.fp8_weight(layer[0], backward=backward) if self.products == "fp8" else None
+                for layer in self._layers()]
+
+    @staticmethod
+    def _product(x, w, w8, **kw):
+        return prims.linear(x, w, **kw) if w8 is None else prims.linear_fp8(x, w8, **kw)
 
     def _encode(self, x):
-        for w, b, act, skip in self._layers():
-            x = prims.linear(x, w, bias=b, activation=act, residual=x if skip else None)
+        layers = self._layers()
+        codes = self._weight_codes if self.products == "fp8" else [None] * len(layers)
+        for (w, b, norm, act, skip), w8 in zip(layers, codes):
+            if norm is None:
+                x = self._product(x, w, w8, bias=b, activation=act, residual=x if skip else None)
+                continue
+            y = prims.group_norm(self._product(x, w, w8, bias=b), int(self.norm_groups), weight=norm[0], bias=norm[1],
+                                 activation=act)
+            x = y.add_(x) if skip else y
         return x
 
-    def _loss_and_grads(self, x, target, weight):
+    def _loss_and_grads(self, x, target, weight, seed=0, step=0):
         """The rows' losses, and the gradients of sum(weight * loss) in the order
-        of the parameters."""
-        layers = self._layers()
+        of the parameters.  `seed` and `step` decide dropout's masks."""
+        layers, codes = self._layers(), self._codes(backward=True)
+        p = float(self.dropout)
         kept = []
-        for w, b, act, skip in layers:
-            y, z = prims.linear(x, w, bias=b, activation=act, residual=x if skip else None, keep_preact=True)
-            kept.append((x, z))
+        for i, ((w, b, norm, act, skip), w8) in enumerate(zip(layers, codes)):
+            hidden = i < len(layers) - 1
+            drop = dict(p=p if hidden else 0.0, seed=seed, offset=step * len(layers) + i)
+            # where the input is added, dropout comes with the sum, after the layer
+            late = hidden and p > 0.0 and (skip or norm is None)
+            if norm is None:
+                y, z = self._product(x, w, w8, bias=b, activation=act, keep_preact=True,
+                                     residual=x if skip and not late else None)
+                stats = None
+            else:
+                z = self._product(x, w, w8, bias=b)
+                within = {} if late else drop
+                y, *stats = prims.group_norm(z, int(self.norm_groups), weight=norm[0], bias=norm[1], activation=act,
+                                             keep_stats=True, **within)
+                if skip and not late:
+                    y += x
+            if late:
+                y = prims.dropout(y, residual=x if skip else None, **drop)
+            kept.append((x, z, stats, drop, late))
             x = y
         head, bias = self._params[-2:]
         loss, lse = prims.softmax_xent(x, head, target, bias=bias)
         dx, dw, db = prims.softmax_xent_grad(x, head, target, lse, weight, bias=bias)
         grads = [dw, db]
         for i in range(len(layers) - 1, -1, -1):
-            w, b, act, skip = layers[i]
-            x, z = kept[i]
+            w, b, norm, act, skip = layers[i]
+            x, z, stats, drop, late = kept[i]
             dy = dx
-            dx, dw, db = prims.linear_grad(dy, x, w, preact=z, activation=act, need_dx=i > 0)
+            inner = prims.dropout(dy, **drop) if late else dy
+            more = []
+            if norm is not None:
+                inner, *more = prims.group_norm_grad(inner, z, *stats, weight=norm[0], bias=norm[1], activation=act,
+                                                     **({} if late else drop))
+                z, act = None, "none"
+            if codes[i] is None:
+                dx, dw, db = prims.linear_grad(inner, x, w, preact=z, activation=act, need_dx=i > 0)
+            else:
+                dx, dw, db = prims.linear_fp8_grad(inner, x, codes[i], preact=z, activation=act, need_dx=i > 0)
             if skip and i > 0:
                 dx += dy
-            grads = [dw, db] + grads
+            grads = [dw, db] + more + grads
         return loss, grads
 
     def fit(self, X, y):
@@ -195,7 +268,7 @@ class EmbeddingEncoder:
             for start in range(0, n, int(self.batch_size)):
                 rows = order[start:start + int(self.batch_size)]
                 weight = torch.full((len(rows),), up / len(rows), dtype=torch.float32, device=x.device)
-                loss, grads = self._loss_and_grads(x[rows], target[rows], weight)
+                loss, grads = self._loss_and_grads(x[rows], target[rows], weight, seed, steps)
                 norm = optimizer.step(grads)
                 steps += 1
                 if norm is not None:
@@ -205,6 +278,7 @@ class EmbeddingEncoder:
             if norms:
                 skipped.append((~torch.cat(norms).isfinite()).sum())
                 norms = []
+        self._weight_codes = self._codes(backward=False)
         self.loss_curve_ = torch.stack(self.loss_curve_).cpu().tolist()
         skipped = int(sum(skipped))
         if skipped:
