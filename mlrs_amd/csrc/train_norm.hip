@@ -108,6 +108,7 @@ __device__ __forceinline__ void forward_oct(const NormOperands<T>& a, uint64_t o
         for (int e = 0; e < 8; ++e) v[e] = activate(v[e], decltype(act)::id);
     });
     if (a.drop.threshold) drop_oct(a.drop, offset, i, v);
+    __builtin_amdgcn_sched_barrier(0);  // one after another: interleaved, they take twice the registers
 }
 
 // dz of eight elements: dy becomes it.
@@ -122,6 +123,7 @@ __device__ __forceinline__ void backward_oct(const NormOperands<T>& a, uint64_t 
             for (int e = 0; e < 8; ++e)
                 dy[e] *= activate_slope(__builtin_fmaf(xh[e], w[e], b[e]), decltype(act)::id);
         });
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // ---------------------------------------------------------------------------
@@ -329,12 +331,24 @@ __device__ __forceinline__ SlabPlace slab_place(const NormOperands<T>& a, const 
     return q;
 }
 
-// The sums over every group of N values of each of a thread's channels: out
-// (N x groups), in LDS.  `lds`: N * rows * octs * 8 floats.  Channels past the
-// slab's end hold zeros.
-template <int N>
-__device__ __forceinline__ void group_sums(const float (&v)[N][8], const SlabPlan& p, const SlabPlace& q, int32_t d,
-                                           int threads, float* lds, float* out) {
+// Where sums of the slab's groups are: few groups are added up by several waves each.
+struct GroupSums {
+    float* at;      // N x parts x groups
+    int32_t parts, groups;
+    __device__ __forceinline__ float get(int i, int32_t g) const {
+        float v = at[i * parts * groups + g];
+        for (int k = 1; k < parts; ++k) v += at[(i * parts + k) * groups + g];
+        return v;
+    }
+};
+
+// The sums over every group of N values of each of a thread's channels, in LDS.
+// `lds`: N * rows * octs * 8 floats.  What channels past the slab's end hold is not
+// read.
+template <int N, int THREADS>
+__device__ __forceinline__ GroupSums group_sums(const float (&v)[N][8], const SlabPlan& p, const SlabPlace& q,
+                                                int32_t d, float* lds, float* out) {
+    constexpr int kWaves = THREADS / 64;
     const int32_t line = p.octs * 8, size = p.rows * line;
     __syncthreads();  // what was there has been read
     if ((int)threadIdx.x < p.rows * p.octs) {
@@ -347,23 +361,58 @@ __device__ __forceinline__ void group_sums(const float (&v)[N][8], const SlabPla
                     f32x4{v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = threads >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int parts = 1;
+    while (parts * 2 * p.groups <= kWaves) parts *= 2;
     // the lanes of a wave side by side over the group's channels, and over rows
-    int span = 1;
-    while (span < 64 && span < d) span *= 2;
-    const int side = 64 / span, lc = lane & (span - 1), lr = lane / span;
-    for (int g = wave; g < q.groups; g += waves) {
+    int span = 1, shift = 0;
+    while (span < 64 && span < d) {
+        span *= 2;
+        ++shift;
+    }
+    const int side = (64 >> shift) * parts, lc = lane & (span - 1);
+    constexpr int U = 4;  // rows under way
+    for (int w = wave; w < q.groups * parts; w += kWaves) {
+        const int g = w / parts, part = w - g * parts;
+        const int lr = (lane >> shift) * parts + part;
         float sum[N] = {};
-        for (int r = lr; r < p.rows; r += side)
-            for (int c = lc; c < d; c += span)
+        for (int c = lc; c < d; c += span) {
+            const float* from = lds + g * d + c;
+            for (int r = lr; r < p.rows; r += U * side) {
+                float u[U][N] = {};
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += lds[i * size + r * line + g * d + c];
+                for (int k = 0; k < U; ++k)
+                    if (r + k * side < p.rows)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) u[k][i] = from[i * size + (r + k * side) * line];
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] += u[k][i];
+            }
+        }
         lane_sums(sum, 64);
         if (lane == 0)
 #pragma unroll
-            for (int i = 0; i < N; ++i) out[i * p.groups + g] = sum[i];
+            for (int i = 0; i < N; ++i) out[(i * parts + part) * p.groups + g] = sum[i];
     }
     __syncthreads();
+    return GroupSums{out, parts, p.groups};
+}
+
+// The groups of a thread's eight channels, of the slab (0 past its end).
+template <typename F>
+__device__ __forceinline__ void each_group(const SlabPlace& q, int32_t d, F f) {
+    const int32_t c0 = 8 * q.oct;
+    int32_t g = q.row >= 0 ? c0 / d : 0, in = c0 - g * d;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f(e, q.row >= 0 && c0 + e < q.width ? g : 0);
+        if (++in == d) {
+            in = 0;
+            ++g;
+        }
+    }
 }
 
 // The same sums over the rows alone, to memory.
@@ -399,14 +448,14 @@ template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[THREADS * 8];
     __shared__ float sums[kSlabGroups];
-    const int64_t items = a.n * p.slabs;
     const uint64_t offset = drop_offset(a.drop);
     const float count = (float)a.s * (float)a.d, inv = 1.0f / count;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t n = item / p.slabs;
-        const int32_t slab = (int32_t)(item - n * p.slabs);
-        const SlabPlace q = slab_place(a, p, slab);
-        const int32_t d = (int32_t)a.d;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const SlabPlace q = slab_place(a, p, slab);
+    const int32_t d = (int32_t)a.d;
+    int32_t gi[8];
+    each_group(q, d, [&](int e, int32_t g) { gi[e] = g; });
+    for (int64_t n = blockIdx.y; n < a.n; n += gridDim.y) {
         const int64_t c0 = 8 * (int64_t)q.oct;  // within the slab
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> raw[M] = {};
@@ -422,14 +471,11 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
         for (int i = 0; i < M; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[0][e] += (float)raw[i][e];
-        group_sums(v, p, q, d, THREADS, lds, sums);
+        GroupSums total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
         float mean[8], rstd[8];
-        int32_t gi[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int32_t c = (int32_t)c0 + e;
-            gi[e] = q.row >= 0 && c < q.width ? c / d : 0;
-            mean[e] = sums[gi[e]] / count;
+            mean[e] = total.get(0, gi[e]) / count;
             v[0][e] = 0.0f;
         }
         if (q.row >= 0) {
@@ -443,16 +489,17 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
                 }
             }
         }
-        group_sums(v, p, q, d, THREADS, lds, sums);
+        total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rstd[e] = 1.0f / sqrtf(__builtin_fmaf(sums[gi[e]], inv, a.eps));
+        for (int e = 0; e < 8; ++e) rstd[e] = 1.0f / sqrtf(__builtin_fmaf(total.get(0, gi[e]), inv, a.eps));
         if (q.row < 0) continue;
         if (a.mean && q.row == 0) {
+            const int64_t at = n * a.g + (int64_t)slab * p.groups;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c0 + e < q.width && ((int32_t)c0 + e) % d == 0) {
-                    a.mean[n * a.g + q.c0 / d + gi[e]] = mean[e];
-                    a.rstd[n * a.g + q.c0 / d + gi[e]] = rstd[e];
+                if (c0 + e < q.width && (int32_t)c0 + e == gi[e] * d) {
+                    a.mean[at + gi[e]] = mean[e];
+                    a.rstd[at + gi[e]] = rstd[e];
                 }
         }
         float w[8], b[8];
@@ -475,8 +522,8 @@ template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[2 * THREADS * 8];
     __shared__ float sums[2 * kSlabGroups];
-    const int32_t slab = (int32_t)(blockIdx.x % (uint32_t)p.slabs);
-    const int64_t place = blockIdx.x / (uint32_t)p.slabs;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const int64_t place = blockIdx.y;
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
     const SlabPlace q = slab_place(a, p, slab);
@@ -485,15 +532,14 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
     float w[8], b[8], total[2][8] = {};
     int32_t gi[8];
     load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) gi[e] = q.row >= 0 && c0 + e < q.width ? ((int32_t)c0 + e) / d : 0;
+    each_group(q, d, [&](int e, int32_t g) { gi[e] = g; });
     for (int64_t n = place; n < a.n; n += p.across) {
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> rx[M] = {}, rd[M] = {};
         float mean[8], rstd[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int64_t at = n * a.g + q.c0 / d + gi[e];
+            const int64_t at = n * a.g + (int64_t)slab * p.groups + gi[e];
             mean[e] = a.mean[at];
             rstd[e] = a.rstd[at];
         }
@@ -533,13 +579,13 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
                 v[k][e] *= w[e];
             }
         if (!a.y) continue;
-        group_sums(v, p, q, d, THREADS, lds, sums);
+        const GroupSums group = group_sums<2, THREADS>(v, p, q, d, lds, sums);
         if (q.row < 0) continue;
         float m1[8], m2[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            m1[e] = sums[gi[e]] * inv;
-            m2[e] = sums[p.groups + gi[e]] * inv;
+            m1[e] = group.get(0, gi[e]) * inv;
+            m2[e] = group.get(1, gi[e]) * inv;
         }
 #pragma unroll
         for (int i = 0; i < M; ++i) {
@@ -571,17 +617,15 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
 // thread sums differences from its first row, a channel of its own, so that a
 // large mean costs nothing.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<T> a, SlabPlan p, float* part) {
+__global__ __launch_bounds__(THREADS, 4) void norm_split_stats_kernel(NormOperands<T> a, SlabPlan p, float* part) {
     __shared__ __attribute__((aligned(16))) float lds[THREADS * 8];
     __shared__ float sums[kSlabGroups];
-    const int64_t per = (int64_t)p.slabs * p.across;
-    for (int64_t item = blockIdx.x; item < a.n * per; item += gridDim.x) {
-        const int64_t n = item / per, in = item - n * per;
-        const int64_t run = in / p.slabs;
-        const int32_t slab = (int32_t)(in - run * p.slabs);
-        const SlabPlace q = slab_place(a, p, slab);
-        const int32_t d = (int32_t)a.d;
-        const int64_t c0 = 8 * (int64_t)q.oct;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const int64_t run = blockIdx.y;
+    const SlabPlace q = slab_place(a, p, slab);
+    const int32_t d = (int32_t)a.d;
+    const int64_t c0 = 8 * (int64_t)q.oct;
+    for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
         const T* from = a.x + n * a.s * a.c + q.c0;
         float first[8] = {}, sum[8] = {}, square[8] = {};
@@ -617,72 +661,72 @@ __global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<
             const float m = count ? sum[e] / (float)count : 0.0f;
             about[e] = square[e] - sum[e] * m;
             first[e] += m;  // the channel's mean
-            v[0][e] = c0 + e < q.width ? first[e] * (float)count : 0.0f;
+            v[0][e] = first[e] * (float)count;
         }
-        group_sums(v, p, q, d, THREADS, lds, sums);
+        GroupSums total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
         const float size = (float)(s1 - s0) * (float)d;
-        float mean[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int32_t c = (int32_t)c0 + e;
-            mean[e] = sums[q.row >= 0 && c < q.width ? c / d : 0] / size;
-            const float far = first[e] - mean[e];
-            v[0][e] = count && c < q.width ? __builtin_fmaf(far * far, (float)count, about[e]) : 0.0f;
-        }
-        const int64_t at = (n * p.across + run) * a.g + q.c0 / d;
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g)] = sums[g] / size;
-        group_sums(v, p, q, d, THREADS, lds, sums);
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g) + 1] = sums[g];
+        each_group(q, d, [&](int e, int32_t g) {
+            const float far = first[e] - total.get(0, g) / size;
+            v[0][e] = count ? __builtin_fmaf(far * far, (float)count, about[e]) : 0.0f;
+        });
+        const int64_t at = (n * p.across + run) * a.g + (int64_t)slab * p.groups;
+        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g)] = total.get(0, g) / size;
+        total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
+        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g) + 1] = total.get(0, g);
     }
+}
+
+// A run's share of the positions.
+__device__ __forceinline__ float run_share(const SlabPlan& p, int64_t s, int64_t r) {
+    return (float)(r + 1 < p.across ? p.run : s - r * p.run) / (float)s;
 }
 
 // Joins the runs of a sample's groups: the mean, and the squares about it.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
+__global__ __launch_bounds__(THREADS, 4) void norm_split_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float means[kSlabGroups], rstds[kSlabGroups];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t offset = drop_offset(a.drop);
-    const int64_t per = (int64_t)p.slabs * p.across;
-    for (int64_t item = blockIdx.x; item < a.n * per; item += gridDim.x) {
-        const int64_t n = item / per, in = item - n * per;
-        const int64_t run = in / p.slabs;
-        const int32_t slab = (int32_t)(in - run * p.slabs);
-        const SlabPlace q = slab_place(a, p, slab);
-        const int32_t d = (int32_t)a.d;
-        const int64_t c0 = 8 * (int64_t)q.oct;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const int64_t run = blockIdx.y;
+    const SlabPlace q = slab_place(a, p, slab);
+    const int32_t d = (int32_t)a.d;
+    const int64_t c0 = 8 * (int64_t)q.oct;
+    for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) {
-            const float* f = part + 2 * (n * p.across * a.g + q.c0 / d + g);
+        // a wave to a group, its lanes over the runs
+        for (int g = wave; g < q.groups; g += THREADS / 64) {
+            const float* f = part + 2 * (n * p.across * a.g + (int64_t)slab * p.groups + g);
             const int64_t step = 2 * a.g;
-            float mean = 0.0f;  // as what it is beyond the first run's
-            for (int64_t r = 1; r < p.across; ++r) {
-                const int64_t count = r + 1 < p.across ? p.run : a.s - r * p.run;
-                mean += (f[r * step] - f[0]) * ((float)count / (float)a.s);
-            }
-            mean += f[0];
-            float square = 0.0f;
-            for (int64_t r = 0; r < p.across; ++r) {
-                const int64_t count = r + 1 < p.across ? p.run : a.s - r * p.run;
+            const float first = f[0];
+            float sum[1] = {0.0f};  // what the mean is beyond the first run's
+            for (int64_t r = lane; r < p.across; r += 64)
+                sum[0] = __builtin_fmaf(f[r * step] - first, run_share(p, a.s, r), sum[0]);
+            lane_sums(sum, 64);
+            const float mean = first + sum[0];
+            sum[0] = 0.0f;
+            for (int64_t r = lane; r < p.across; r += 64) {
                 const float far = f[r * step] - mean;
-                square += __builtin_fmaf(far * far, (float)count * (float)d, f[r * step + 1]);
+                sum[0] += __builtin_fmaf(far * far, run_share(p, a.s, r) * (float)a.s * (float)d, f[r * step + 1]);
             }
-            const float rstd = 1.0f / sqrtf(square / ((float)a.s * (float)d) + a.eps);
+            lane_sums(sum, 64);
+            const float rstd = 1.0f / sqrtf(sum[0] / ((float)a.s * (float)d) + a.eps);
+            if (lane) continue;
             means[g] = mean;
             rstds[g] = rstd;
             if (a.mean && run == 0) {
-                a.mean[n * a.g + q.c0 / d + g] = mean;
-                a.rstd[n * a.g + q.c0 / d + g] = rstd;
+                a.mean[n * a.g + (int64_t)slab * p.groups + g] = mean;
+                a.rstd[n * a.g + (int64_t)slab * p.groups + g] = rstd;
             }
         }
         __syncthreads();
         if (q.row < 0) continue;
         float w[8], b[8], mean[8], rstd[8];
         load_affine(a, q.c0 + c0, q.c0 + q.width, w, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int32_t c = (int32_t)c0 + e, g = c < q.width ? c / d : 0;
+        each_group(q, d, [&](int e, int32_t g) {
             mean[e] = means[g];
             rstd[e] = rstds[g];
-        }
+        });
         const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
         const int64_t base = n * a.s * a.c + q.c0;
         constexpr int U = 4;
@@ -707,29 +751,24 @@ __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, 
 
 // Backwards: of every run the groups' two sums (part), and the channels' (pw, pb).
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_split_sums_kernel(NormOperands<T> a, SlabPlan p, float* part) {
+__global__ __launch_bounds__(THREADS, 4) void norm_split_sums_kernel(NormOperands<T> a, SlabPlan p, float* part) {
     __shared__ __attribute__((aligned(16))) float lds[2 * THREADS * 8];
     __shared__ float sums[2 * kSlabGroups];
     const uint64_t offset = drop_offset(a.drop);
-    const int64_t per = (int64_t)p.slabs * p.across;
-    for (int64_t item = blockIdx.x; item < a.n * per; item += gridDim.x) {
-        const int64_t n = item / per, in = item - n * per;
-        const int64_t run = in / p.slabs;
-        const int32_t slab = (int32_t)(in - run * p.slabs);
-        const SlabPlace q = slab_place(a, p, slab);
-        const int32_t d = (int32_t)a.d;
-        const int64_t c0 = 8 * (int64_t)q.oct;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const int64_t run = blockIdx.y;
+    const SlabPlace q = slab_place(a, p, slab);
+    const int32_t d = (int32_t)a.d;
+    const int64_t c0 = 8 * (int64_t)q.oct;
+    for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
         const int64_t base = n * a.s * a.c + q.c0;
         float w[8], b[8], mean[8], rstd[8], v[2][8] = {};
         load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int32_t c = (int32_t)c0 + e;
-            const int64_t at = n * a.g + q.c0 / d + (q.row >= 0 && c < q.width ? c / d : 0);
-            mean[e] = a.mean[at];
-            rstd[e] = a.rstd[at];
-        }
+        each_group(q, d, [&](int e, int32_t g) {
+            mean[e] = a.mean[n * a.g + (int64_t)slab * p.groups + g];
+            rstd[e] = a.rstd[n * a.g + (int64_t)slab * p.groups + g];
+        });
         if (q.row >= 0) {
             constexpr int U = 2;
             for (int64_t pos = s0 + q.row; pos < s1; pos += U * p.rows) {
@@ -767,50 +806,50 @@ __global__ __launch_bounds__(THREADS) void norm_split_sums_kernel(NormOperands<T
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[k][e] *= w[e];
-        group_sums(v, p, q, d, THREADS, lds, sums);
+        const GroupSums group = group_sums<2, THREADS>(v, p, q, d, lds, sums);
         for (int g = threadIdx.x; g < q.groups; g += THREADS) {
-            part[2 * (at * a.g + q.c0 / d + g)] = sums[g];
-            part[2 * (at * a.g + q.c0 / d + g) + 1] = sums[p.groups + g];
+            float* const to2 = part + 2 * (at * a.g + (int64_t)slab * p.groups + g);
+            to2[0] = group.get(0, g);
+            to2[1] = group.get(1, g);
         }
     }
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_split_grad_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
+__global__ __launch_bounds__(THREADS, 4) void norm_split_grad_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float m1s[kSlabGroups], m2s[kSlabGroups];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
-    const int64_t per = (int64_t)p.slabs * p.across;
-    for (int64_t item = blockIdx.x; item < a.n * per; item += gridDim.x) {
-        const int64_t n = item / per, in = item - n * per;
-        const int64_t run = in / p.slabs;
-        const int32_t slab = (int32_t)(in - run * p.slabs);
-        const SlabPlace q = slab_place(a, p, slab);
-        const int32_t d = (int32_t)a.d;
-        const int64_t c0 = 8 * (int64_t)q.oct;
+    const int32_t slab = (int32_t)blockIdx.x;
+    const int64_t run = blockIdx.y;
+    const SlabPlace q = slab_place(a, p, slab);
+    const int32_t d = (int32_t)a.d;
+    const int64_t c0 = 8 * (int64_t)q.oct;
+    for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) {
-            const float* f = part + 2 * (n * p.across * a.g + q.c0 / d + g);
-            float s1 = 0.0f, s2 = 0.0f;
-            for (int64_t r = 0; r < p.across; ++r) {
-                s1 += f[2 * r * a.g];
-                s2 += f[2 * r * a.g + 1];
+        for (int g = wave; g < q.groups; g += THREADS / 64) {  // a wave to a group, its lanes over the runs
+            const float* f = part + 2 * (n * p.across * a.g + (int64_t)slab * p.groups + g);
+            float sum[2] = {0.0f, 0.0f};
+            for (int64_t r = lane; r < p.across; r += 64) {
+                sum[0] += f[2 * r * a.g];
+                sum[1] += f[2 * r * a.g + 1];
             }
-            m1s[g] = s1 * inv;
-            m2s[g] = s2 * inv;
+            lane_sums(sum, 64);
+            if (lane) continue;
+            m1s[g] = sum[0] * inv;
+            m2s[g] = sum[1] * inv;
         }
         __syncthreads();
         if (q.row < 0) continue;
         float w[8], b[8], mean[8], rstd[8], m1[8], m2[8];
         load_affine(a, q.c0 + c0, q.c0 + q.width, w, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int32_t c = (int32_t)c0 + e, g = c < q.width ? c / d : 0;
-            mean[e] = a.mean[n * a.g + q.c0 / d + g];
-            rstd[e] = a.rstd[n * a.g + q.c0 / d + g];
+        each_group(q, d, [&](int e, int32_t g) {
+            mean[e] = a.mean[n * a.g + (int64_t)slab * p.groups + g];
+            rstd[e] = a.rstd[n * a.g + (int64_t)slab * p.groups + g];
             m1[e] = m1s[g];
             m2[e] = m2s[g];
-        }
+        });
         const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
         const int64_t base = n * a.s * a.c + q.c0;
         constexpr int U = 2;
@@ -883,7 +922,8 @@ struct Way {
     int m;             // resident: positions of a thread
     RowPlan row;
     SlabPlan slab;
-    int64_t blocks;
+    int64_t blocks;  // rows
+    int64_t side;    // slabs: samples side by side
     int64_t parts;  // rows of the parameters' partial sums
 };
 
@@ -900,13 +940,13 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
             o.row.lanes = 1;
             while (o.row.lanes < octs) o.row.lanes *= 2;
             units = 4 * (64 / o.row.lanes);
-        } else if (octs <= 256) {
-            o.cpl = octs <= 128 ? 2 : 4;
+        } else if (octs <= 128) {
+            o.cpl = 2;
             o.row.lanes = 64;
             units = 4;
         } else {
-            o.cpl = octs <= 512 ? 2 : 4;
-            o.threads = 256;
+            o.cpl = octs <= 256 ? 1 : 2;
+            o.threads = octs <= 512 ? 256 : 512;
             units = 1;
         }
         const int64_t most = std::max(ceil_div((int64_t)cus * (grad ? 4 : 8), 1), ceil_div(g, units));
@@ -929,7 +969,7 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
     };
     const int64_t line = std::min<int64_t>(g, std::max<int64_t>(1, ceil_div(128 / elem_bytes, d)));
     const int most = elem_bytes == 4 && grad ? 4 : 8;
-    for (int threads : {256, 1024}) {
+    for (int threads : {256, 512}) {
         const SlabPlan p = slab(threads, std::min<int64_t>(line, kSlabGroups));
         if (p.octs > threads || ceil_div(s, p.rows) > most) continue;
         o.kind = Way::kResident;
@@ -937,9 +977,9 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         const int64_t m = ceil_div(s, p.rows);
         o.m = m <= 2 ? 2 : m <= 4 ? 4 : 8;
         o.slab = p;
-        const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 256 ? 4 : 1) / p.slabs);
-        o.slab.across = grad ? ceil_div(n, ceil_div(n, std::min(n, side))) : n;
-        o.blocks = grad ? o.slab.across * p.slabs : std::min<int64_t>(n * p.slabs, (int64_t)cus * 16);
+        const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 256 ? 4 : 2) / p.slabs);
+        o.slab.across = grad ? ceil_div(n, ceil_div(n, std::min<int64_t>({n, side, 65535}))) : n;
+        o.side = std::min<int64_t>(grad ? o.slab.across : n, 65535);
         o.parts = o.slab.across;
         return o;
     }
@@ -952,7 +992,7 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
     const int64_t rows = std::max<int64_t>(ceil_div(s, std::max<int64_t>(1, want)), 4 * (int64_t)o.slab.rows);
     o.slab.run = std::min(rows, s);
     o.slab.across = ceil_div(s, o.slab.run);
-    o.blocks = std::min<int64_t>(n * o.slab.slabs * o.slab.across, (int64_t)cus * 16);
+    o.side = std::min<int64_t>(n, 65535);
     o.parts = n * o.slab.across;
     return o;
 }
@@ -973,16 +1013,16 @@ hipError_t launch_rows(const NormOperands<T>& a, const Way& o, hipStream_t s) {
     }
     MLRS_ROWS(1, 0)
     MLRS_ROWS(2, 0)
-    MLRS_ROWS(4, 0)
+    MLRS_ROWS(1, 256)
     MLRS_ROWS(2, 256)
-    MLRS_ROWS(4, 256)
+    MLRS_ROWS(2, 512)
 #undef MLRS_ROWS
     return hipErrorInvalidValue;
 }
 
 template <typename T, bool GRAD>
 hipError_t launch_resident(const NormOperands<T>& a, const Way& o, hipStream_t s) {
-    const dim3 grid((unsigned)o.blocks);
+    const dim3 grid((unsigned)o.slab.slabs, (unsigned)o.side);
     auto go = [&](auto kernel) {
         kernel<<<grid, o.threads, 0, s>>>(a, o.slab);
         return hipGetLastError();
@@ -996,11 +1036,11 @@ hipError_t launch_resident(const NormOperands<T>& a, const Way& o, hipStream_t s
     }
     MLRS_SLAB(2, 256)
     MLRS_SLAB(4, 256)
-    MLRS_SLAB(2, 1024)
-    MLRS_SLAB(4, 1024)
+    MLRS_SLAB(2, 512)
+    MLRS_SLAB(4, 512)
     if constexpr (!GRAD || sizeof(T) == 2) {
         MLRS_SLAB(8, 256)
-        MLRS_SLAB(8, 1024)
+        MLRS_SLAB(8, 512)
     }
 #undef MLRS_SLAB
     return hipErrorInvalidValue;
@@ -1040,7 +1080,7 @@ hipError_t launch_norm(const NormCall& k, float* scratch, int cus, hipStream_t s
     const NormOperands<T> a = operands<T>(k);
     if (o.kind == Way::kRows) return launch_rows<T, false>(a, o, s);
     if (o.kind == Way::kResident) return launch_resident<T, false>(a, o, s);
-    const dim3 grid((unsigned)o.blocks);
+    const dim3 grid((unsigned)o.slab.slabs, (unsigned)o.slab.across, (unsigned)o.side);
     if (o.threads == 512)
         norm_split_stats_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, scratch);
     else
@@ -1085,7 +1125,7 @@ hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStrea
     } else if (o.kind == Way::kResident) {
         e = launch_resident<T, true>(a, o, s);
     } else {
-        const dim3 grid((unsigned)o.blocks);
+        const dim3 grid((unsigned)o.slab.slabs, (unsigned)o.slab.across, (unsigned)o.side);
         if (o.threads == 512)
             norm_split_sums_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, at);
         else
