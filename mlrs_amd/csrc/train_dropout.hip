@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* resid
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = (float)v[u][e];
-            if (drop.threshold) drop_oct(drop, offset, at * 8, f);
+            if (drop.threshold) drop_oct(drop, offset, at * 8, true, f);
             if (residual) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] += (float)r[u][e];

@@ -40,30 +40,176 @@ struct NormOperands {
     int64_t n, s, c, g, d;
     float eps;
     int act;
+    bool aligned;  // every thread's eight channels are whole and one block of random bits
     Drop drop;
 };
 
-template <int A>
-struct Act {
-    static constexpr int id = A;
-};
-template <typename F>
-__device__ __forceinline__ void with_activation(int act, F f) {
-    switch (act) {
-    case kActRelu: f(Act<kActRelu>{}); break;
-    case kActGelu: f(Act<kActGelu>{}); break;
-    case kActGeluTanh: f(Act<kActGeluTanh>{}); break;
-    case kActSilu: f(Act<kActSilu>{}); break;
-    default: f(Act<kActNone>{}); break;
+// ---------------------------------------------------------------------------
+// what is done with an element
+// ---------------------------------------------------------------------------
+// gelu is z Phi(z) = max(z, 0) - |z| Phi(-|z|), and Phi(-u) = e^(-u^2/2) q(t) with t =
+// 1 / (1 + c u), as train_epilogue.hpp's: a polynomial fitted to the scaled
+// complementary error function for u in 0 .. 40.  f32: degree 9, relative error 3.8e-7
+// as it is computed; 16-bit types: degree 6, 1.1e-5, which is a fiftieth of f16's
+// rounding and saves three of some sixteen instructions an element, where these
+// kernels are bound by instructions.
+template <typename T>
+__device__ __forceinline__ float normal_tail(float u, float& bell) {
+    bell = __builtin_amdgcn_exp2f(u * u * (-0.5f * kLog2E));
+    float q;
+    if constexpr (sizeof(T) == 4) {
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, u, 1.0f));
+        q = -0.030237516661021768f;
+        q = __builtin_fmaf(q, t, 0.13950534889597813f);
+        q = __builtin_fmaf(q, t, -0.22359445728159374f);
+        q = __builtin_fmaf(q, t, 0.10736457851476656f);
+        q = __builtin_fmaf(q, t, -0.00038397830051628453f);
+        q = __builtin_fmaf(q, t, 0.09603661840218482f);
+        q = __builtin_fmaf(q, t, 0.1240098852248856f);
+        q = __builtin_fmaf(q, t, 0.14368186910198438f);
+        q = __builtin_fmaf(q, t, 0.14361766520603944f);
+        return q * t * bell;
+    } else {
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.32f, u, 1.0f));
+        q = -0.06677426336821958f;
+        q = __builtin_fmaf(q, t, 0.13958546063672428f);
+        q = __builtin_fmaf(q, t, 0.04961394871763218f);
+        q = __builtin_fmaf(q, t, 0.12305164080264364f);
+        q = __builtin_fmaf(q, t, 0.12682801098738777f);
+        q = __builtin_fmaf(q, t, 0.1276897246494251f);
+        return q * t * bell;
     }
 }
 
-// Sums over the lanes of a unit (a power of two of them, up to a wave).
+template <typename T, int ACT>
+__device__ __forceinline__ float value_of(float z) {
+    if constexpr (ACT == kActGelu) {
+        float bell;
+        const float tail = normal_tail<T>(fabsf(z), bell);
+        return z != z ? z : __builtin_fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));
+    } else {
+        return activate(z, ACT);
+    }
+}
+template <typename T, int ACT>
+__device__ __forceinline__ float slope_of(float z) {
+    if constexpr (ACT == kActGelu) {
+        float bell;
+        const float tail = normal_tail<T>(fabsf(z), bell);
+        const float cdf = 0.5f + __builtin_copysignf(0.5f - tail, z);
+        return __builtin_fmaf(z * (0.5f * kGeluC), bell, cdf);
+    } else {
+        return activate_slope(z, ACT);
+    }
+}
+
+// One switch for eight elements: v = value(z), or v *= slope(z).
+template <typename T>
+__device__ __forceinline__ void values_of(int act, float (&v)[8]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
+    };
+    switch (act) {
+    case kActRelu: each([](float z) { return value_of<T, kActRelu>(z); }); break;
+    case kActGelu: each([](float z) { return value_of<T, kActGelu>(z); }); break;
+    case kActGeluTanh: each([](float z) { return value_of<T, kActGeluTanh>(z); }); break;
+    case kActSilu: each([](float z) { return value_of<T, kActSilu>(z); }); break;
+    default: break;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void times_slopes(int act, const float (&xh)[8], const float (&w)[8], const float (&b)[8],
+                                             float (&v)[8]) {
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f(__builtin_fmaf(xh[e], w[e], b[e]));
+    };
+    switch (act) {
+    case kActRelu: each([](float z) { return slope_of<T, kActRelu>(z); }); break;
+    case kActGelu: each([](float z) { return slope_of<T, kActGelu>(z); }); break;
+    case kActGeluTanh: each([](float z) { return slope_of<T, kActGeluTanh>(z); }); break;
+    case kActSilu: each([](float z) { return slope_of<T, kActSilu>(z); }); break;
+    default: break;
+    }
+}
+
+// y of eight elements from their xh.
+template <typename T>
+__device__ __forceinline__ void forward_oct(const NormOperands<T>& a, uint64_t offset, int64_t i, const float (&w)[8],
+                                            const float (&b)[8], float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], w[e], b[e]);
+    values_of<T>(a.act, v);
+    if (a.drop.threshold) drop_oct(a.drop, offset, i, a.aligned, v);
+}
+
+// dz of eight elements: dy becomes it.
+template <typename T>
+__device__ __forceinline__ void backward_oct(const NormOperands<T>& a, uint64_t offset, int64_t i,
+                                             const float (&w)[8], const float (&b)[8], const float (&xh)[8],
+                                             float (&dy)[8]) {
+    if (a.drop.threshold) drop_oct(a.drop, offset, i, a.aligned, dy);
+    times_slopes<T>(a.act, xh, w, b, dy);
+}
+
+// 1 / sqrt(v): the hardware's, to one unit, and a step of Newton's.
+__device__ __forceinline__ float inverse_root(float v) {
+    const float y = __builtin_amdgcn_rsqf(v);
+    const float better = y * __builtin_fmaf(-0.5f * v * y, y, 1.5f);
+    return y < 1e18f && y > 1e-18f ? better : y;  // v y is out of range beyond, or v 0 or infinite
+}
+// sum / count, by its reciprocal and a step: the quotient rounded, so that the mean of
+// equal elements is theirs where their sum is exact.
+__device__ __forceinline__ float mean_of(float sum, float count, float inv) {
+    const float m = sum * inv;
+    const float rest = __builtin_fmaf(-m, count, sum);
+    return rest - rest == 0.0f ? __builtin_fmaf(rest, inv, m) : m;
+}
+
+// ---------------------------------------------------------------------------
+// sums
+// ---------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(float,
+                              __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+#else
+    return v;
+#endif
+}
+__device__ __forceinline__ float other_rows(float v, bool halves) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const unsigned u = __float_as_uint(v);
+    if (halves) {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const unsigned lo = r[0], hi = r[1];
+        return __uint_as_float(lo) + __uint_as_float(hi);
+    }
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned even = r[0], odd = r[1];
+    return __uint_as_float(even) + __uint_as_float(odd);
+#else
+    (void)halves;
+    return v;
+#endif
+}
+
+// Sums over the lanes of a unit (a power of two of them, up to a wave), in every one
+// of them, by moves within the vector unit: neighbours, pairs, mirrored halves of
+// eight and of sixteen, rows of sixteen, halves of the wave.
 template <int N>
 __device__ __forceinline__ void lane_sums(float (&v)[N], int lanes) {
-    for (int o = lanes >> 1; o; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    for (int i = 0; i < N; ++i) {
+        if (lanes > 1) v[i] += from_lane<0xB1>(v[i]);
+        if (lanes > 2) v[i] += from_lane<0x4E>(v[i]);
+        if (lanes > 4) v[i] += from_lane<0x141>(v[i]);
+        if (lanes > 8) v[i] += from_lane<0x140>(v[i]);
+        if (lanes > 16) v[i] = other_rows(v[i], false);
+        if (lanes > 32) v[i] = other_rows(v[i], true);
+    }
 }
 
 // The same over a workgroup of THREADS; `lds` holds N * THREADS / 64 floats that
@@ -97,35 +243,6 @@ __device__ __forceinline__ void load_affine(const NormOperands<T>& a, int64_t at
     }
 }
 
-// y of eight elements from their xh.
-template <typename T>
-__device__ __forceinline__ void forward_oct(const NormOperands<T>& a, uint64_t offset, int64_t i, const float (&w)[8],
-                                            const float (&b)[8], float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], w[e], b[e]);
-    with_activation(a.act, [&](auto act) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activate(v[e], decltype(act)::id);
-    });
-    if (a.drop.threshold) drop_oct(a.drop, offset, i, v);
-    __builtin_amdgcn_sched_barrier(0);  // one after another: interleaved, they take twice the registers
-}
-
-// dz of eight elements: dy becomes it.
-template <typename T>
-__device__ __forceinline__ void backward_oct(const NormOperands<T>& a, uint64_t offset, int64_t i,
-                                             const float (&w)[8], const float (&b)[8], const float (&xh)[8],
-                                             float (&dy)[8]) {
-    if (a.drop.threshold) drop_oct(a.drop, offset, i, dy);
-    if (a.act != kActNone)
-        with_activation(a.act, [&](auto act) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                dy[e] *= activate_slope(__builtin_fmaf(xh[e], w[e], b[e]), decltype(act)::id);
-        });
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 // ---------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------
@@ -138,34 +255,55 @@ struct RowPlan {
     int64_t passes;  // samples side by side: places / g
 };
 
-template <typename T, int CPL, int THREADS>
-__global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(NormOperands<T> a, RowPlan plan) {
+struct RowPlace {
+    int li;      // the lane in its unit
+    int step;    // channels from one of a lane's octs to the next
+    int64_t row0, gi;
+    bool live;
+};
+template <int THREADS, typename T>
+__device__ __forceinline__ RowPlace row_place(const NormOperands<T>& a, const RowPlan& plan) {
     constexpr bool kWide = THREADS > 0;
-    constexpr int kWaves = kWide ? THREADS / 64 : 1;
-    __shared__ float lds[2][2][kWaves];
-    int turn = 0;
+    RowPlace q;
     const int lane = threadIdx.x & 63;
-    const int li = kWide ? threadIdx.x : lane & (plan.lanes - 1);
+    q.li = kWide ? threadIdx.x : lane & (plan.lanes - 1);
+    q.step = 8 * (kWide ? THREADS : plan.lanes);
     const int per = 64 / (kWide ? 64 : plan.lanes);
     const int64_t place = kWide ? (int64_t)blockIdx.x
                                 : ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per + lane / plan.lanes;
-    const int64_t row0 = place / a.g, gi = place - row0 * a.g;
-    const bool live = place < plan.places;
+    q.row0 = place / a.g;
+    q.gi = place - q.row0 * a.g;
+    q.live = place < plan.places;
+    return q;
+}
+
+template <typename T, int CPL, int THREADS>
+__global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(NormOperands<T> a, RowPlan plan) {
+    constexpr bool kWide = THREADS > 0;
+    __shared__ float lds[2][2][kWide ? THREADS / 64 : 1];
+    const RowPlace q = row_place<THREADS>(a, plan);
     const uint64_t offset = drop_offset(a.drop);
-    const float inv = 1.0f / (float)a.d;
-    const int step = 8 * (kWide ? THREADS : plan.lanes);
+    const float count = (float)a.d, inv = 1.0f / count;
+    const int32_t d = (int32_t)a.d;
+    float w[CPL][8], b[CPL][8];
+#pragma unroll
+    for (int j = 0; j < CPL; ++j) {
+        const int32_t c = 8 * q.li + j * q.step;
+        load_affine(a, q.gi * a.d + c, q.live && c < d ? (q.gi + 1) * a.d : 0, w[j], b[j]);
+    }
+    int turn = 0;
     for (int64_t r0 = 0; r0 < a.n; r0 += plan.passes, turn ^= 1) {
-        const int64_t row = r0 + row0;
-        const bool ok = live && row < a.n;
+        const int64_t row = r0 + q.row0;
+        const bool ok = q.live && row < a.n;
         if (kWide && !ok) break;  // the whole workgroup
-        const int64_t base = (row * a.g + gi) * a.d;
+        const int64_t unit = row * a.g + q.gi, base = unit * a.d;
         float v[CPL][8];
         float sum[1] = {0.0f};
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
+            const int32_t c = 8 * q.li + j * q.step;
             Oct<T> raw = {};
-            if (ok && c < a.d) raw = load_oct(a.x + base, c, a.d);
+            if (ok && c < d) raw = load_oct(a.x + base, c, d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[j][e] = (float)raw[e];
@@ -176,41 +314,39 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(Norm
             block_sums<1, THREADS>(sum, lds[turn][0]);
         else
             lane_sums(sum, plan.lanes);
-        const float mean = sum[0] / (float)a.d;  // exact where all are equal and few
+        const float mean = mean_of(sum[0], count, inv);
         sum[0] = 0.0f;
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
+            const int32_t c = 8 * q.li + j * q.step;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[j][e] -= mean;
-            if (c + 8 <= a.d) {
+            if (c + 8 <= d) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[0] = __builtin_fmaf(v[j][e], v[j][e], sum[0]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (c + e < a.d) sum[0] = __builtin_fmaf(v[j][e], v[j][e], sum[0]);
+                    if (c + e < d) sum[0] = __builtin_fmaf(v[j][e], v[j][e], sum[0]);
             }
         }
         if constexpr (kWide)
             block_sums<1, THREADS>(sum, lds[turn][1]);
         else
             lane_sums(sum, plan.lanes);
-        const float rstd = 1.0f / sqrtf(__builtin_fmaf(sum[0], inv, a.eps));
-        if (ok && li == 0 && a.mean) {
-            a.mean[row * a.g + gi] = mean;
-            a.rstd[row * a.g + gi] = rstd;
+        const float rstd = inverse_root(__builtin_fmaf(sum[0], inv, a.eps));
+        if (ok && q.li == 0 && a.mean) {
+            a.mean[unit] = mean;
+            a.rstd[unit] = rstd;
         }
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
-            if (!ok || c >= a.d) continue;
-            float w[8], b[8];
-            load_affine(a, gi * a.d + c, (gi + 1) * a.d, w, b);
+            const int32_t c = 8 * q.li + j * q.step;
+            if (!ok || c >= d) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[j][e] *= rstd;
-            forward_oct(a, offset, base + c, w, b, v[j]);
-            store_oct(a.y + base, c, a.d, v[j]);
+            forward_oct(a, offset, base + c, w[j], b[j], v[j]);
+            store_oct(a.y + base, c, d, v[j]);
         }
     }
 }
@@ -218,53 +354,48 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(Norm
 template <typename T, int CPL, int THREADS>
 __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_grad_kernel(NormOperands<T> a, RowPlan plan) {
     constexpr bool kWide = THREADS > 0;
-    constexpr int kWaves = kWide ? THREADS / 64 : 1;
-    __shared__ float lds[2][2 * kWaves];
-    const int lane = threadIdx.x & 63;
-    const int li = kWide ? threadIdx.x : lane & (plan.lanes - 1);
-    const int per = 64 / (kWide ? 64 : plan.lanes);
-    const int64_t place = kWide ? (int64_t)blockIdx.x
-                                : ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per + lane / plan.lanes;
-    const int64_t row0 = place / a.g, gi = place - row0 * a.g;
-    const bool live = place < plan.places;
+    __shared__ float lds[2][2 * (kWide ? THREADS / 64 : 1)];
+    const RowPlace q = row_place<THREADS>(a, plan);
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / (float)a.d;
-    const int step = 8 * (kWide ? THREADS : plan.lanes);
+    const int32_t d = (int32_t)a.d;
     float w[CPL][8], b[CPL][8], dw[CPL][8] = {}, db[CPL][8] = {};
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
-        const int64_t c = 8 * li + j * step;
-        load_affine(a, gi * a.d + c, live && c < a.d ? (gi + 1) * a.d : 0, w[j], b[j]);
+        const int32_t c = 8 * q.li + j * q.step;
+        load_affine(a, q.gi * a.d + c, q.live && c < d ? (q.gi + 1) * a.d : 0, w[j], b[j]);
     }
     int turn = 0;
     for (int64_t r0 = 0; r0 < a.n; r0 += plan.passes, turn ^= 1) {
-        const int64_t row = r0 + row0;
-        const bool ok = live && row < a.n;
+        const int64_t row = r0 + q.row0;
+        const bool ok = q.live && row < a.n;
         if (kWide && !ok) break;  // the whole workgroup
-        const int64_t unit = row * a.g + gi, base = unit * a.d;
+        const int64_t unit = row * a.g + q.gi, base = unit * a.d;
         float xh[CPL][8], t[CPL][8];
         const float mean = ok ? a.mean[unit] : 0.0f, rstd = ok ? a.rstd[unit] : 0.0f;
         Oct<T> rx[CPL] = {}, rd[CPL] = {};
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
-            if (ok && c < a.d) {
-                rx[j] = load_oct(a.x + base, c, a.d);
-                rd[j] = load_oct(a.dy + base, c, a.d);
+            const int32_t c = 8 * q.li + j * q.step;
+            if (ok && c < d) {
+                rx[j] = load_oct(a.x + base, c, d);
+                rd[j] = load_oct(a.dy + base, c, d);
             }
         }
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
+            const int32_t c = 8 * q.li + j * q.step;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 xh[j][e] = ((float)rx[j][e] - mean) * rstd;
                 t[j][e] = (float)rd[j][e];
-                // past the group's end dy is zero, and so is what comes of it
-                if (c + 8 > a.d && c + e >= a.d) xh[j][e] = 0.0f;
             }
-            if (!ok || c >= a.d) continue;
+            if (c + 8 > d)  // past the group's end dy is zero, and so is what comes of it
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e >= d) xh[j][e] = 0.0f;
+            if (!ok || c >= d) continue;
             backward_oct(a, offset, base + c, w[j], b[j], xh[j], t[j]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -282,20 +413,20 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_grad_kernel
         const float m1 = sum[0] * inv, m2 = sum[1] * inv;
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int64_t c = 8 * li + j * step;
-            if (!a.y || !ok || c >= a.d) continue;
+            const int32_t c = 8 * q.li + j * q.step;
+            if (!a.y || !ok || c >= d) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[j][e] = rstd * (t[j][e] - __builtin_fmaf(xh[j][e], m2, m1));
-            store_oct(a.y + base, c, a.d, t[j]);
+            store_oct(a.y + base, c, d, t[j]);
         }
     }
-    if (!live) return;
+    if (!q.live) return;
 #pragma unroll
     for (int j = 0; j < CPL; ++j) {
-        const int64_t c = 8 * li + j * step;
-        if (c >= a.d) continue;
-        if (a.pw) store_oct(a.pw + row0 * a.c + gi * a.d, c, a.d, dw[j]);
-        if (a.pb) store_oct(a.pb + row0 * a.c + gi * a.d, c, a.d, db[j]);
+        const int32_t c = 8 * q.li + j * q.step;
+        if (c >= d) continue;
+        if (a.pw) store_oct(a.pw + q.row0 * a.c + q.gi * a.d, c, d, dw[j]);
+        if (a.pb) store_oct(a.pb + q.row0 * a.c + q.gi * a.d, c, d, db[j]);
     }
 }
 
@@ -311,118 +442,66 @@ struct SlabPlan {
     int64_t run;      // split: positions of a run
 };
 
-// A thread's place in a slab.
+constexpr int kSlabGroups = 256;  // of a slab, at most
+
+// A thread's place in a slab: eight channels of every so-manieth position; and, where
+// the threads' sums are added up, a channel (or several) of a slice of those.
 struct SlabPlace {
-    int32_t oct, row;   // row: -1 where the thread has nothing to do
-    int32_t c0, width;  // the slab's first channel, and its channels
-    int32_t groups;
+    int32_t oct, row;       // row: -1 where the thread has nothing to do
+    int32_t width;          // channels of the slab
+    int32_t groups, d;
+    int32_t slices;         // 1 where there are more channels than threads
+    int32_t slice, column;  // column: the first of the thread's, then + THREADS
+    int64_t c0, g0;         // the slab's first channel and group
 };
-template <typename T>
+template <int THREADS, typename T>
 __device__ __forceinline__ SlabPlace slab_place(const NormOperands<T>& a, const SlabPlan& p, int32_t slab) {
     SlabPlace q;
     const int t = threadIdx.x;
     q.row = t / p.octs;
     q.oct = t - q.row * p.octs;
-    const int64_t left = a.g - (int64_t)slab * p.groups;
+    q.d = (int32_t)a.d;
+    q.g0 = (int64_t)slab * p.groups;
+    q.c0 = q.g0 * a.d;
+    const int64_t left = a.g - q.g0;
     q.groups = (int32_t)(left < p.groups ? left : p.groups);
-    q.c0 = (int32_t)(slab * p.groups * a.d);
-    q.width = (int32_t)(q.groups * a.d);
+    q.width = q.groups * q.d;
     if (q.row >= p.rows || q.oct * 8 >= q.width) q.row = -1;
+    q.slices = THREADS / q.width;
+    if (q.slices > p.rows) q.slices = p.rows;
+    if (q.slices < 1) q.slices = 1;
+    q.slice = q.slices > 1 ? t / q.width : 0;
+    q.column = t - q.slice * q.width;
     return q;
-}
-
-// Where sums of the slab's groups are: few groups are added up by several waves each.
-struct GroupSums {
-    float* at;      // N x parts x groups
-    int32_t parts, groups;
-    __device__ __forceinline__ float get(int i, int32_t g) const {
-        float v = at[i * parts * groups + g];
-        for (int k = 1; k < parts; ++k) v += at[(i * parts + k) * groups + g];
-        return v;
-    }
-};
-
-// The sums over every group of N values of each of a thread's channels, in LDS.
-// `lds`: N * rows * octs * 8 floats.  What channels past the slab's end hold is not
-// read.
-template <int N, int THREADS>
-__device__ __forceinline__ GroupSums group_sums(const float (&v)[N][8], const SlabPlan& p, const SlabPlace& q,
-                                                int32_t d, float* lds, float* out) {
-    constexpr int kWaves = THREADS / 64;
-    const int32_t line = p.octs * 8, size = p.rows * line;
-    __syncthreads();  // what was there has been read
-    if ((int)threadIdx.x < p.rows * p.octs) {
-        const int t = threadIdx.x;  // row * octs + oct
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4)
-                *reinterpret_cast<f32x4*>(lds + i * size + t * 8 + e) =
-                    f32x4{v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int parts = 1;
-    while (parts * 2 * p.groups <= kWaves) parts *= 2;
-    // the lanes of a wave side by side over the group's channels, and over rows
-    int span = 1, shift = 0;
-    while (span < 64 && span < d) {
-        span *= 2;
-        ++shift;
-    }
-    const int side = (64 >> shift) * parts, lc = lane & (span - 1);
-    constexpr int U = 4;  // rows under way
-    for (int w = wave; w < q.groups * parts; w += kWaves) {
-        const int g = w / parts, part = w - g * parts;
-        const int lr = (lane >> shift) * parts + part;
-        float sum[N] = {};
-        for (int c = lc; c < d; c += span) {
-            const float* from = lds + g * d + c;
-            for (int r = lr; r < p.rows; r += U * side) {
-                float u[U][N] = {};
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (r + k * side < p.rows)
-#pragma unroll
-                        for (int i = 0; i < N; ++i) u[k][i] = from[i * size + (r + k * side) * line];
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) sum[i] += u[k][i];
-            }
-        }
-        lane_sums(sum, 64);
-        if (lane == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i) out[(i * parts + part) * p.groups + g] = sum[i];
-    }
-    __syncthreads();
-    return GroupSums{out, parts, p.groups};
 }
 
 // The groups of a thread's eight channels, of the slab (0 past its end).
 template <typename F>
-__device__ __forceinline__ void each_group(const SlabPlace& q, int32_t d, F f) {
+__device__ __forceinline__ void each_group(const SlabPlace& q, F f) {
     const int32_t c0 = 8 * q.oct;
-    int32_t g = q.row >= 0 ? c0 / d : 0, in = c0 - g * d;
+    int32_t g = q.row >= 0 ? c0 / q.d : 0, in = c0 - g * q.d;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         f(e, q.row >= 0 && c0 + e < q.width ? g : 0);
-        if (++in == d) {
+        if (++in == q.d) {
             in = 0;
             ++g;
         }
     }
 }
 
-// The same sums over the rows alone, to memory.
-template <int N>
-__device__ __forceinline__ void channel_sums(const float (&v)[N][8], const SlabPlan& p, const SlabPlace& q,
-                                             int threads, float* lds, float* const (&to)[N]) {
+// Adds up N values of each of the threads' channels over the rows: first over every
+// `slices`th row, a channel's and slice's handed to seen(place in a row of lds, sums);
+// then over slices and a group's channels, times what weight(channel) says, and
+// done(group, sums) once for each.  `lds`: N * rows *
+// octs * 8 floats; what channels past the slab's end hold is not read.
+template <int N, int THREADS, typename Seen, typename Weight, typename Done>
+__device__ __forceinline__ void group_sums(const float (&v)[N][8], const SlabPlan& p, const SlabPlace& q, float* lds,
+                                           bool groups, Seen seen, Weight weight, Done done) {
     const int32_t line = p.octs * 8, size = p.rows * line;
-    __syncthreads();
-    if ((int)threadIdx.x < p.rows * p.octs) {
-        const int t = threadIdx.x;
+    const int t = threadIdx.x;
+    __syncthreads();  // what was there has been read
+    if (t < p.rows * p.octs) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -431,32 +510,79 @@ __device__ __forceinline__ void channel_sums(const float (&v)[N][8], const SlabP
                     f32x4{v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]};
     }
     __syncthreads();
+    if (q.slice < q.slices) {
+        constexpr int U = 4;  // rows under way
+#pragma unroll 1
+        for (int c = q.column; c < q.width; c += THREADS) {
+            float sum[N] = {};
+#pragma unroll 1
+            for (int r = q.slice; r < p.rows; r += U * q.slices) {
+                float u[U][N] = {};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (!to[i]) continue;
-        for (int c = threadIdx.x; c < q.width; c += threads) {
-            float sum = 0.0f;
-            for (int r = 0; r < p.rows; ++r) sum += lds[i * size + r * line + c];
-            to[i][q.c0 + c] = sum;
+                for (int j = 0; j < U; ++j)
+                    if (r + j * q.slices < p.rows)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) u[j][i] = lds[i * size + (r + j * q.slices) * line + c];
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] += u[j][i];
+            }
+            // row `slice` of the column is this thread's own
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds[i * size + q.slice * line + c] = sum[i];
+            seen(q.slice * line + c, sum);
         }
     }
+    if (!groups) return;
+    __syncthreads();
+    if (q.slices * q.d <= 32) {  // a thread to a group
+        if (t < q.groups) {
+            float sum[N] = {};
+#pragma unroll 1
+            for (int c = t * q.d; c < (t + 1) * q.d; ++c) {
+                const float by = weight(c);
+                for (int r = 0; r < q.slices; ++r)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sum[i] = __builtin_fmaf(lds[i * size + r * line + c], by, sum[i]);
+            }
+            done(t, sum);
+        }
+    } else {  // a wave to a group
+        const int lane = t & 63, wave = t >> 6;
+        for (int g = wave; g < q.groups; g += THREADS / 64) {
+            float sum[N] = {};
+            for (int r = 0; r < q.slices; ++r)
+                for (int c = lane; c < q.d; c += 64)
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        sum[i] = __builtin_fmaf(lds[i * size + r * line + g * q.d + c], weight(g * q.d + c), sum[i]);
+            lane_sums(sum, 64);
+            if (lane == 0) done(g, sum);
+        }
+    }
+    __syncthreads();
 }
 
-constexpr int kSlabGroups = 256;  // of a slab, at most
+__device__ __forceinline__ float weight_one(int) { return 1.0f; }
+struct Nothing {
+    template <int N>
+    __device__ __forceinline__ void operator()(int, const float (&)[N]) const {}
+};
 
 template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[THREADS * 8];
-    __shared__ float sums[kSlabGroups];
+    __shared__ float means[kSlabGroups], rstds[kSlabGroups];
     const uint64_t offset = drop_offset(a.drop);
     const float count = (float)a.s * (float)a.d, inv = 1.0f / count;
-    const int32_t slab = (int32_t)blockIdx.x;
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;  // within the slab
     int32_t gi[8];
-    each_group(q, d, [&](int e, int32_t g) { gi[e] = g; });
+    each_group(q, [&](int e, int32_t g) { gi[e] = g; });
+    float w[8], b[8];
+    load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.y; n < a.n; n += gridDim.y) {
-        const int64_t c0 = 8 * (int64_t)q.oct;  // within the slab
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> raw[M] = {};
         if (q.row >= 0) {
@@ -471,11 +597,12 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
         for (int i = 0; i < M; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[0][e] += (float)raw[i][e];
-        GroupSums total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
-        float mean[8], rstd[8];
+        group_sums<1, THREADS>(v, p, q, lds, true, Nothing{}, weight_one,
+                               [&](int g, const float (&sum)[1]) { means[g] = mean_of(sum[0], count, inv); });
+        float mean[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            mean[e] = total.get(0, gi[e]) / count;
+            mean[e] = means[gi[e]];
             v[0][e] = 0.0f;
         }
         if (q.row >= 0) {
@@ -485,25 +612,22 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float u = (float)raw[i][e] - mean[e];
-                    if (c0 + e < q.width) v[0][e] = __builtin_fmaf(u, u, v[0][e]);
+                    v[0][e] = __builtin_fmaf(u, u, v[0][e]);
                 }
             }
         }
-        total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) rstd[e] = 1.0f / sqrtf(__builtin_fmaf(total.get(0, gi[e]), inv, a.eps));
+        group_sums<1, THREADS>(v, p, q, lds, true, Nothing{}, weight_one, [&](int g, const float (&sum)[1]) {
+            const float rstd = inverse_root(__builtin_fmaf(sum[0], inv, a.eps));
+            rstds[g] = rstd;
+            if (a.mean) {
+                a.mean[n * a.g + q.g0 + g] = means[g];
+                a.rstd[n * a.g + q.g0 + g] = rstd;
+            }
+        });
         if (q.row < 0) continue;
-        if (a.mean && q.row == 0) {
-            const int64_t at = n * a.g + (int64_t)slab * p.groups;
+        float rstd[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c0 + e < q.width && (int32_t)c0 + e == gi[e] * d) {
-                    a.mean[at + gi[e]] = mean[e];
-                    a.rstd[at + gi[e]] = rstd[e];
-                }
-        }
-        float w[8], b[8];
-        load_affine(a, q.c0 + c0, q.c0 + q.width, w, b);
+        for (int e = 0; e < 8; ++e) rstd[e] = rstds[gi[e]];
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             const int64_t pos = q.row + (int64_t)i * p.rows;
@@ -517,29 +641,37 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
     }
 }
 
+// The weights of a slab's channels, for what is added up of each of them.
+template <int THREADS, typename T>
+__device__ __forceinline__ void slab_weights(const NormOperands<T>& a, const SlabPlace& q, float* lds) {
+    for (int c = threadIdx.x; c < q.width; c += THREADS) lds[c] = a.w ? (float)a.w[q.c0 + c] : 1.0f;
+}
+
 // Workgroup (slab, place): samples place, place + across, ...
 template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[2 * THREADS * 8];
-    __shared__ float sums[2 * kSlabGroups];
-    const int32_t slab = (int32_t)blockIdx.x;
+    __shared__ float totals[2 * THREADS * 8];  // of the channels' slices, each its thread's own
+    __shared__ float weights[THREADS * 8], m1s[kSlabGroups], m2s[kSlabGroups];
+    constexpr int kSize = THREADS * 8;
     const int64_t place = blockIdx.y;
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
-    const int64_t c0 = 8 * (int64_t)q.oct;
-    float w[8], b[8], total[2][8] = {};
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;
+    slab_weights<THREADS>(a, q, weights);
+    for (int i = threadIdx.x; i < 2 * kSize; i += THREADS) totals[i] = 0.0f;
+    float w[8], b[8];
     int32_t gi[8];
     load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
-    each_group(q, d, [&](int e, int32_t g) { gi[e] = g; });
+    each_group(q, [&](int e, int32_t g) { gi[e] = g; });
     for (int64_t n = place; n < a.n; n += p.across) {
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> rx[M] = {}, rd[M] = {};
         float mean[8], rstd[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int64_t at = n * a.g + (int64_t)slab * p.groups + gi[e];
+            const int64_t at = n * a.g + q.g0 + gi[e];
             mean[e] = a.mean[at];
             rstd[e] = a.rstd[at];
         }
@@ -571,21 +703,23 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
                 }
             }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                total[k][e] += v[k][e];
-                v[k][e] *= w[e];
-            }
-        if (!a.y) continue;
-        const GroupSums group = group_sums<2, THREADS>(v, p, q, d, lds, sums);
-        if (q.row < 0) continue;
+        group_sums<2, THREADS>(
+            v, p, q, lds, a.y != nullptr,
+            [&](int at, const float (&sum)[2]) {
+                totals[at] += sum[0];
+                totals[kSize + at] += sum[1];
+            },
+            [&](int c) { return weights[c]; },
+            [&](int g, const float (&sum)[2]) {
+                m1s[g] = sum[0] * inv;
+                m2s[g] = sum[1] * inv;
+            });
+        if (!a.y || q.row < 0) continue;
         float m1[8], m2[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            m1[e] = group.get(0, gi[e]) * inv;
-            m2[e] = group.get(1, gi[e]) * inv;
+            m1[e] = m1s[gi[e]];
+            m2[e] = m2s[gi[e]];
         }
 #pragma unroll
         for (int i = 0; i < M; ++i) {
@@ -605,46 +739,53 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
         }
     }
     if (!a.pw && !a.pb) return;
-    float* const to[2] = {a.pb ? a.pb + place * a.c : nullptr, a.pw ? a.pw + place * a.c : nullptr};
-    channel_sums(total, p, q, THREADS, lds, to);
+    __syncthreads();
+    for (int c = threadIdx.x; c < q.width; c += THREADS) {
+        float sum[2] = {0.0f, 0.0f};
+        for (int r = 0; r < q.slices; ++r) {
+            sum[0] += totals[r * p.octs * 8 + c];
+            sum[1] += totals[kSize + r * p.octs * 8 + c];
+        }
+        if (a.pb) a.pb[place * a.c + q.c0 + c] = sum[0];
+        if (a.pw) a.pw[place * a.c + q.c0 + c] = sum[1];
+    }
 }
 
 // ---------------------------------------------------------------------------
 // split
 // ---------------------------------------------------------------------------
-// A run's statistics of every group: three floats, its mean, the sum of squares
-// about it, and nothing else is needed: the counts follow from the run.  Each
-// thread sums differences from its first row, a channel of its own, so that a
-// large mean costs nothing.
+// A run's statistics of every group: its mean, and the sum of squares about it; the
+// counts follow from the run.  Each thread sums differences from its first row, a
+// channel of its own, so that a large mean costs nothing.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void norm_split_stats_kernel(NormOperands<T> a, SlabPlan p, float* part) {
+__global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<T> a, SlabPlan p, float* part) {
     __shared__ __attribute__((aligned(16))) float lds[THREADS * 8];
-    __shared__ float sums[kSlabGroups];
-    const int32_t slab = (int32_t)blockIdx.x;
+    __shared__ float means[kSlabGroups];
     const int64_t run = blockIdx.y;
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
-    const int64_t c0 = 8 * (int64_t)q.oct;
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;
+    const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
+    const float size = (float)(s1 - s0) * (float)a.d, inv = 1.0f / size;
+    const int64_t step = (int64_t)p.rows * a.c;
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
-        const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
-        const T* from = a.x + n * a.s * a.c + q.c0;
         float first[8] = {}, sum[8] = {}, square[8] = {};
-        int32_t count = 0;
+        int32_t rows = 0;
         if (q.row >= 0 && s0 + q.row < s1) {
-            const Oct<T> raw = load_oct(from + (s0 + q.row) * a.c, c0, q.width);
+            const T* from = a.x + (n * a.s + s0 + q.row) * a.c + q.c0;
+            rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
+            constexpr int U = 4;
+            const Oct<T> raw = load_oct(from, c0, q.width);
 #pragma unroll
             for (int e = 0; e < 8; ++e) first[e] = (float)raw[e];
-            count = 1;
-            constexpr int U = 4;
-            for (int64_t pos = s0 + q.row + p.rows; pos < s1; pos += U * p.rows) {
+            from += step;
+            for (int32_t r = 1; r < rows; r += U, from += U * step) {
                 Oct<T> v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (pos + u * p.rows < s1) v[u] = load_oct(from + (pos + u * p.rows) * a.c, c0, q.width);
+                    if (r + u < rows) v[u] = load_oct(from + u * step, c0, q.width);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (pos + u * p.rows >= s1) continue;
-                    ++count;
+                    if (r + u >= rows) continue;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float t = (float)v[u][e] - first[e];
@@ -655,24 +796,26 @@ __global__ __launch_bounds__(THREADS, 4) void norm_split_stats_kernel(NormOperan
             }
         }
         // to each channel's own mean, then to the group's
-        float v[1][8], about[8];
+        float v[1][8];
+        const float by = rows ? 1.0f / (float)rows : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float m = count ? sum[e] / (float)count : 0.0f;
-            about[e] = square[e] - sum[e] * m;
+            const float m = sum[e] * by;
+            square[e] -= sum[e] * m;
             first[e] += m;  // the channel's mean
-            v[0][e] = first[e] * (float)count;
+            v[0][e] = first[e] * (float)rows;
         }
-        GroupSums total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
-        const float size = (float)(s1 - s0) * (float)d;
-        each_group(q, d, [&](int e, int32_t g) {
-            const float far = first[e] - total.get(0, g) / size;
-            v[0][e] = count ? __builtin_fmaf(far * far, (float)count, about[e]) : 0.0f;
+        const int64_t at = (n * p.across + run) * a.g + q.g0;
+        group_sums<1, THREADS>(v, p, q, lds, true, Nothing{}, weight_one, [&](int g, const float (&total)[1]) {
+            means[g] = mean_of(total[0], size, inv);
+            part[2 * (at + g)] = means[g];
         });
-        const int64_t at = (n * p.across + run) * a.g + (int64_t)slab * p.groups;
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g)] = total.get(0, g) / size;
-        total = group_sums<1, THREADS>(v, p, q, d, lds, sums);
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) part[2 * (at + g) + 1] = total.get(0, g);
+        each_group(q, [&](int e, int32_t g) {
+            const float far = first[e] - means[g];
+            v[0][e] = rows ? __builtin_fmaf(far * far, (float)rows, square[e]) : 0.0f;
+        });
+        group_sums<1, THREADS>(v, p, q, lds, true, Nothing{}, weight_one,
+                               [&](int g, const float (&total)[1]) { part[2 * (at + g) + 1] = total[0]; });
     }
 }
 
@@ -681,155 +824,156 @@ __device__ __forceinline__ float run_share(const SlabPlan& p, int64_t s, int64_t
     return (float)(r + 1 < p.across ? p.run : s - r * p.run) / (float)s;
 }
 
-// Joins the runs of a sample's groups: the mean, and the squares about it.
+// Joins the runs of a sample's groups: the mean, and the squares about it; then y.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void norm_split_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
+__global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float means[kSlabGroups], rstds[kSlabGroups];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t offset = drop_offset(a.drop);
-    const int32_t slab = (int32_t)blockIdx.x;
     const int64_t run = blockIdx.y;
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
-    const int64_t c0 = 8 * (int64_t)q.oct;
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;
+    const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
+    const int64_t step = (int64_t)p.rows * a.c;
+    float w[8], b[8];
+    load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
         // a wave to a group, its lanes over the runs
         for (int g = wave; g < q.groups; g += THREADS / 64) {
-            const float* f = part + 2 * (n * p.across * a.g + (int64_t)slab * p.groups + g);
-            const int64_t step = 2 * a.g;
+            const float* f = part + 2 * (n * p.across * a.g + q.g0 + g);
+            const int64_t next = 2 * a.g;
             const float first = f[0];
             float sum[1] = {0.0f};  // what the mean is beyond the first run's
             for (int64_t r = lane; r < p.across; r += 64)
-                sum[0] = __builtin_fmaf(f[r * step] - first, run_share(p, a.s, r), sum[0]);
+                sum[0] = __builtin_fmaf(f[r * next] - first, run_share(p, a.s, r), sum[0]);
             lane_sums(sum, 64);
             const float mean = first + sum[0];
             sum[0] = 0.0f;
             for (int64_t r = lane; r < p.across; r += 64) {
-                const float far = f[r * step] - mean;
-                sum[0] += __builtin_fmaf(far * far, run_share(p, a.s, r) * (float)a.s * (float)d, f[r * step + 1]);
+                const float far = f[r * next] - mean;
+                sum[0] += __builtin_fmaf(far * far, run_share(p, a.s, r) * (float)a.s * (float)a.d, f[r * next + 1]);
             }
             lane_sums(sum, 64);
-            const float rstd = 1.0f / sqrtf(sum[0] / ((float)a.s * (float)d) + a.eps);
+            const float rstd = inverse_root(sum[0] / ((float)a.s * (float)a.d) + a.eps);
             if (lane) continue;
             means[g] = mean;
             rstds[g] = rstd;
             if (a.mean && run == 0) {
-                a.mean[n * a.g + (int64_t)slab * p.groups + g] = mean;
-                a.rstd[n * a.g + (int64_t)slab * p.groups + g] = rstd;
+                a.mean[n * a.g + q.g0 + g] = mean;
+                a.rstd[n * a.g + q.g0 + g] = rstd;
             }
         }
         __syncthreads();
-        if (q.row < 0) continue;
-        float w[8], b[8], mean[8], rstd[8];
-        load_affine(a, q.c0 + c0, q.c0 + q.width, w, b);
-        each_group(q, d, [&](int e, int32_t g) {
+        if (q.row < 0 || s0 + q.row >= s1) continue;
+        float mean[8], rstd[8];
+        each_group(q, [&](int e, int32_t g) {
             mean[e] = means[g];
             rstd[e] = rstds[g];
         });
-        const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
-        const int64_t base = n * a.s * a.c + q.c0;
-        constexpr int U = 4;
-        for (int64_t pos = s0 + q.row; pos < s1; pos += U * p.rows) {
-            Oct<T> v[U];
+        int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
+        const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
+        // the next row under way while one is worked on: unrolled, the code of every
+        // activation takes the registers of as many waves
+        Oct<T> v = load_oct(a.x + at, c0, q.width), next = {};
+#pragma unroll 1
+        for (int32_t r = 0; r < rows; ++r, at += step) {
+            if (r + 1 < rows) next = load_oct(a.x + at + step, c0, q.width);
+            float f[8];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (pos + u * p.rows < s1) v[u] = load_oct(a.x + base + (pos + u * p.rows) * a.c, c0, q.width);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t at = pos + u * p.rows;
-                if (at >= s1) continue;
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = ((float)v[u][e] - mean[e]) * rstd[e];
-                forward_oct(a, offset, base + at * a.c + c0, w, b, f);
-                store_oct(a.y + base + at * a.c, c0, q.width, f);
-            }
+            for (int e = 0; e < 8; ++e) f[e] = ((float)v[e] - mean[e]) * rstd[e];
+            forward_oct(a, offset, at + c0, w, b, f);
+            store_oct(a.y + at, c0, q.width, f);
+            v = next;
         }
     }
 }
 
 // Backwards: of every run the groups' two sums (part), and the channels' (pw, pb).
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void norm_split_sums_kernel(NormOperands<T> a, SlabPlan p, float* part) {
+__global__ __launch_bounds__(THREADS) void norm_split_sums_kernel(NormOperands<T> a, SlabPlan p, float* part) {
     __shared__ __attribute__((aligned(16))) float lds[2 * THREADS * 8];
-    __shared__ float sums[2 * kSlabGroups];
+    __shared__ float weights[THREADS * 8];
     const uint64_t offset = drop_offset(a.drop);
-    const int32_t slab = (int32_t)blockIdx.x;
     const int64_t run = blockIdx.y;
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
-    const int64_t c0 = 8 * (int64_t)q.oct;
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;
+    const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
+    const int64_t step = (int64_t)p.rows * a.c;
+    slab_weights<THREADS>(a, q, weights);
+    float w[8], b[8];
+    load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
-        const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
-        const int64_t base = n * a.s * a.c + q.c0;
-        float w[8], b[8], mean[8], rstd[8], v[2][8] = {};
-        load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
-        each_group(q, d, [&](int e, int32_t g) {
-            mean[e] = a.mean[n * a.g + (int64_t)slab * p.groups + g];
-            rstd[e] = a.rstd[n * a.g + (int64_t)slab * p.groups + g];
+        float mean[8], rstd[8], v[2][8] = {};
+        each_group(q, [&](int e, int32_t g) {
+            mean[e] = a.mean[n * a.g + q.g0 + g];
+            rstd[e] = a.rstd[n * a.g + q.g0 + g];
         });
-        if (q.row >= 0) {
-            constexpr int U = 2;
-            for (int64_t pos = s0 + q.row; pos < s1; pos += U * p.rows) {
-                Oct<T> rx[U], rd[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (pos + u * p.rows < s1) {
-                        rx[u] = load_oct(a.x + base + (pos + u * p.rows) * a.c, c0, q.width);
-                        rd[u] = load_oct(a.dy + base + (pos + u * p.rows) * a.c, c0, q.width);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int64_t at = pos + u * p.rows;
-                    if (at >= s1) continue;
-                    float xh[8], t[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        xh[e] = ((float)rx[u][e] - mean[e]) * rstd[e];
-                        t[e] = (float)rd[u][e];
-                    }
-                    backward_oct(a, offset, base + at * a.c + c0, w, b, xh, t);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        v[0][e] += t[e];
-                        v[1][e] = __builtin_fmaf(t[e], xh[e], v[1][e]);
-                    }
+        if (q.row >= 0 && s0 + q.row < s1) {
+            int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
+            const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
+            Oct<T> rx = load_oct(a.x + at, c0, q.width), rd = load_oct(a.dy + at, c0, q.width), nx = {}, nd = {};
+#pragma unroll 1
+            for (int32_t r = 0; r < rows; ++r, at += step) {
+                if (r + 1 < rows) {
+                    nx = load_oct(a.x + at + step, c0, q.width);
+                    nd = load_oct(a.dy + at + step, c0, q.width);
                 }
+                float xh[8], t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    xh[e] = ((float)rx[e] - mean[e]) * rstd[e];
+                    t[e] = (float)rd[e];
+                }
+                backward_oct(a, offset, at + c0, w, b, xh, t);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[0][e] += t[e];
+                    v[1][e] = __builtin_fmaf(t[e], xh[e], v[1][e]);
+                }
+                rx = nx;
+                rd = nd;
             }
         }
-        const int64_t at = n * p.across + run;
-        float* const to[2] = {a.pb ? a.pb + at * a.c : nullptr, a.pw ? a.pw + at * a.c : nullptr};
-        channel_sums(v, p, q, THREADS, lds, to);
-        if (!a.y) continue;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[k][e] *= w[e];
-        const GroupSums group = group_sums<2, THREADS>(v, p, q, d, lds, sums);
-        for (int g = threadIdx.x; g < q.groups; g += THREADS) {
-            float* const to2 = part + 2 * (at * a.g + (int64_t)slab * p.groups + g);
-            to2[0] = group.get(0, g);
-            to2[1] = group.get(1, g);
+        const int64_t line = n * p.across + run;
+        group_sums<2, THREADS>(
+            v, p, q, lds, true, Nothing{}, [&](int c) { return weights[c]; },
+            [&](int g, const float (&sum)[2]) {
+                float* const to = part + 2 * (line * a.g + q.g0 + g);
+                to[0] = sum[0];
+                to[1] = sum[1];
+            });
+        if (!a.pw && !a.pb) continue;
+        const int32_t row = p.octs * 8, size = p.rows * row;  // where the slices' sums are
+        for (int c = threadIdx.x; c < q.width; c += THREADS) {
+            float sum[2] = {0.0f, 0.0f};
+            for (int r = 0; r < q.slices; ++r) {
+                sum[0] += lds[r * row + c];
+                sum[1] += lds[size + r * row + c];
+            }
+            if (a.pb) a.pb[line * a.c + q.c0 + c] = sum[0];
+            if (a.pw) a.pw[line * a.c + q.c0 + c] = sum[1];
         }
     }
 }
 
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void norm_split_grad_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
+__global__ __launch_bounds__(THREADS) void norm_split_grad_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float m1s[kSlabGroups], m2s[kSlabGroups];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
-    const int32_t slab = (int32_t)blockIdx.x;
     const int64_t run = blockIdx.y;
-    const SlabPlace q = slab_place(a, p, slab);
-    const int32_t d = (int32_t)a.d;
-    const int64_t c0 = 8 * (int64_t)q.oct;
+    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const int32_t c0 = 8 * q.oct;
+    const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
+    const int64_t step = (int64_t)p.rows * a.c;
+    float w[8], b[8];
+    load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
         for (int g = wave; g < q.groups; g += THREADS / 64) {  // a wave to a group, its lanes over the runs
-            const float* f = part + 2 * (n * p.across * a.g + (int64_t)slab * p.groups + g);
+            const float* f = part + 2 * (n * p.across * a.g + q.g0 + g);
             float sum[2] = {0.0f, 0.0f};
             for (int64_t r = lane; r < p.across; r += 64) {
                 sum[0] += f[2 * r * a.g];
@@ -841,42 +985,35 @@ __global__ __launch_bounds__(THREADS, 4) void norm_split_grad_kernel(NormOperand
             m2s[g] = sum[1] * inv;
         }
         __syncthreads();
-        if (q.row < 0) continue;
-        float w[8], b[8], mean[8], rstd[8], m1[8], m2[8];
-        load_affine(a, q.c0 + c0, q.c0 + q.width, w, b);
-        each_group(q, d, [&](int e, int32_t g) {
-            mean[e] = a.mean[n * a.g + (int64_t)slab * p.groups + g];
-            rstd[e] = a.rstd[n * a.g + (int64_t)slab * p.groups + g];
+        if (q.row < 0 || s0 + q.row >= s1) continue;
+        float mean[8], rstd[8], m1[8], m2[8];
+        each_group(q, [&](int e, int32_t g) {
+            mean[e] = a.mean[n * a.g + q.g0 + g];
+            rstd[e] = a.rstd[n * a.g + q.g0 + g];
             m1[e] = m1s[g];
             m2[e] = m2s[g];
         });
-        const int64_t s0 = run * p.run, s1 = s0 + p.run < a.s ? s0 + p.run : a.s;
-        const int64_t base = n * a.s * a.c + q.c0;
-        constexpr int U = 2;
-        for (int64_t pos = s0 + q.row; pos < s1; pos += U * p.rows) {
-            Oct<T> rx[U], rd[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (pos + u * p.rows < s1) {
-                    rx[u] = load_oct(a.x + base + (pos + u * p.rows) * a.c, c0, q.width);
-                    rd[u] = load_oct(a.dy + base + (pos + u * p.rows) * a.c, c0, q.width);
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t at = pos + u * p.rows;
-                if (at >= s1) continue;
-                float xh[8], t[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    xh[e] = ((float)rx[u][e] - mean[e]) * rstd[e];
-                    t[e] = (float)rd[u][e];
-                }
-                backward_oct(a, offset, base + at * a.c + c0, w, b, xh, t);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    t[e] = rstd[e] * (t[e] * w[e] - __builtin_fmaf(xh[e], m2[e], m1[e]));
-                store_oct(a.y + base + at * a.c, c0, q.width, t);
+        int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
+        const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
+        Oct<T> rx = load_oct(a.x + at, c0, q.width), rd = load_oct(a.dy + at, c0, q.width), nx = {}, nd = {};
+#pragma unroll 1
+        for (int32_t r = 0; r < rows; ++r, at += step) {
+            if (r + 1 < rows) {
+                nx = load_oct(a.x + at + step, c0, q.width);
+                nd = load_oct(a.dy + at + step, c0, q.width);
             }
+            float xh[8], t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                xh[e] = ((float)rx[e] - mean[e]) * rstd[e];
+                t[e] = (float)rd[e];
+            }
+            backward_oct(a, offset, at + c0, w, b, xh, t);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = rstd[e] * (t[e] * w[e] - __builtin_fmaf(xh[e], m2[e], m1[e]));
+            store_oct(a.y + at, c0, q.width, t);
+            rx = nx;
+            rd = nd;
         }
     }
 }
@@ -983,8 +1120,8 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.parts = o.slab.across;
         return o;
     }
-    o.kind = Way::kSplit;
-    o.threads = octs <= 512 ? 512 : 1024;
+    o.kind = Way::kSplit;  // four workgroups to a CU: a run's first and last steps cost as much as its rows
+    o.threads = octs <= 256 ? 256 : 1024;
     // as many whole groups as the threads have room for
     const int64_t groups = std::max<int64_t>(1, std::min<int64_t>({g, kSlabGroups, (int64_t)o.threads * 8 / d}));
     o.slab = slab(o.threads, groups);
@@ -1047,7 +1184,7 @@ hipError_t launch_resident(const NormOperands<T>& a, const Way& o, hipStream_t s
 }
 
 template <typename T>
-NormOperands<T> operands(const NormCall& k) {
+NormOperands<T> operands(const NormCall& k, const Way& o) {
     NormOperands<T> a{};
     a.x = (const T*)k.x;
     a.w = (const T*)k.w;
@@ -1064,6 +1201,7 @@ NormOperands<T> operands(const NormCall& k) {
     a.eps = k.eps;
     a.act = k.act;
     a.drop = k.drop;
+    a.aligned = k.c % 8 == 0 && (o.kind == Way::kRows ? a.d : o.slab.groups * a.d) % 8 == 0;
     return a;
 }
 
@@ -1077,18 +1215,18 @@ size_t norm_scratch(int elem_bytes, const NormCall& k, int cus) {
 template <typename T>
 hipError_t launch_norm(const NormCall& k, float* scratch, int cus, hipStream_t s) {
     const Way o = choose((int)sizeof(T), k.n, k.s, k.c, k.g, false, cus);
-    const NormOperands<T> a = operands<T>(k);
+    const NormOperands<T> a = operands<T>(k, o);
     if (o.kind == Way::kRows) return launch_rows<T, false>(a, o, s);
     if (o.kind == Way::kResident) return launch_resident<T, false>(a, o, s);
     const dim3 grid((unsigned)o.slab.slabs, (unsigned)o.slab.across, (unsigned)o.side);
-    if (o.threads == 512)
-        norm_split_stats_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, scratch);
+    if (o.threads == 256)
+        norm_split_stats_kernel<T, 256><<<grid, 256, 0, s>>>(a, o.slab, scratch);
     else
         norm_split_stats_kernel<T, 1024><<<grid, 1024, 0, s>>>(a, o.slab, scratch);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (o.threads == 512)
-        norm_split_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, scratch);
+    if (o.threads == 256)
+        norm_split_kernel<T, 256><<<grid, 256, 0, s>>>(a, o.slab, scratch);
     else
         norm_split_kernel<T, 1024><<<grid, 1024, 0, s>>>(a, o.slab, scratch);
     return hipGetLastError();
@@ -1108,7 +1246,7 @@ template <typename T>
 hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStream_t s) {
     Way o{};  // of no samples, the parameters' sums have no parts
     if (k.n) o = choose((int)sizeof(T), k.n, k.s, k.c, k.g, true, cus);
-    NormOperands<T> a = operands<T>(k);
+    NormOperands<T> a = operands<T>(k, o);
     float* at = scratch;
     if (k.dw) {
         a.pw = at;
@@ -1126,14 +1264,14 @@ hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStrea
         e = launch_resident<T, true>(a, o, s);
     } else {
         const dim3 grid((unsigned)o.slab.slabs, (unsigned)o.slab.across, (unsigned)o.side);
-        if (o.threads == 512)
-            norm_split_sums_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, at);
+        if (o.threads == 256)
+            norm_split_sums_kernel<T, 256><<<grid, 256, 0, s>>>(a, o.slab, at);
         else
             norm_split_sums_kernel<T, 1024><<<grid, 1024, 0, s>>>(a, o.slab, at);
         e = hipGetLastError();
         if (e == hipSuccess && k.y) {
-            if (o.threads == 512)
-                norm_split_grad_kernel<T, 512><<<grid, 512, 0, s>>>(a, o.slab, at);
+            if (o.threads == 256)
+                norm_split_grad_kernel<T, 256><<<grid, 256, 0, s>>>(a, o.slab, at);
             else
                 norm_split_grad_kernel<T, 1024><<<grid, 1024, 0, s>>>(a, o.slab, at);
             e = hipGetLastError();

@@ -87,13 +87,13 @@ __device__ __forceinline__ uint64_t drop_offset(const Drop& d) {
 }
 
 // Multiplies elements i .. i + 7 by their factor, 0 (whatever they hold) or
-// d.factor.  i is a multiple of 8 wherever rows and groups are; else the eight
-// lie in two blocks.
-__device__ __forceinline__ void drop_oct(const Drop& d, uint64_t offset, int64_t i, float (&v)[8]) {
+// d.factor.  aligned: i is a multiple of 8, in every lane; else the eight may lie
+// in two blocks.
+__device__ __forceinline__ void drop_oct(const Drop& d, uint64_t offset, int64_t i, bool aligned, float (&v)[8]) {
     RandomWords w;
     random_block((uint64_t)i >> 3, offset, d.k0, d.k1, w);
     const int r = (int)(i & 7);
-    if (r) {
+    if (!aligned) {
         RandomWords next;
         random_block(((uint64_t)i >> 3) + 1, offset, d.k0, d.k1, next);
         uint32_t all[8];
