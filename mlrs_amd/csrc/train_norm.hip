@@ -85,8 +85,9 @@ template <typename T, int ACT>
 __device__ __forceinline__ float value_of(float z) {
     if constexpr (ACT == kActGelu) {
         float bell;
-        const float tail = normal_tail<T>(fabsf(z), bell);
-        return z != z ? z : __builtin_fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));
+        const float u = __builtin_elementwise_minimum(fabsf(z), 1e18f);  // these two keep a NaN
+        const float tail = normal_tail<T>(u, bell);
+        return __builtin_fmaf(-u, tail, __builtin_elementwise_maximum(z, 0.0f));
     } else {
         return activate(z, ACT);
     }
@@ -95,7 +96,7 @@ template <typename T, int ACT>
 __device__ __forceinline__ float slope_of(float z) {
     if constexpr (ACT == kActGelu) {
         float bell;
-        const float tail = normal_tail<T>(fabsf(z), bell);
+        const float tail = normal_tail<T>(__builtin_elementwise_minimum(fabsf(z), 1e18f), bell);
         const float cdf = 0.5f + __builtin_copysignf(0.5f - tail, z);
         return __builtin_fmaf(z * (0.5f * kGeluC), bell, cdf);
     } else {
@@ -292,6 +293,15 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(Norm
         load_affine(a, q.gi * a.d + c, q.live && c < d ? (q.gi + 1) * a.d : 0, w[j], b[j]);
     }
     int turn = 0;
+    Oct<T> raw[CPL] = {};
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+            const int32_t c = 8 * q.li + j * q.step;
+            if (q.live && row < a.n && c < d) raw[j] = load_oct(a.x + (row * a.g + q.gi) * a.d, c, d);
+        }
+    };
+    load(q.row0);
     for (int64_t r0 = 0; r0 < a.n; r0 += plan.passes, turn ^= 1) {
         const int64_t row = r0 + q.row0;
         const bool ok = q.live && row < a.n;
@@ -300,16 +310,13 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_kernel(Norm
         float v[CPL][8];
         float sum[1] = {0.0f};
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-            const int32_t c = 8 * q.li + j * q.step;
-            Oct<T> raw = {};
-            if (ok && c < d) raw = load_oct(a.x + base, c, d);
+        for (int j = 0; j < CPL; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[j][e] = (float)raw[e];
+                v[j][e] = (float)raw[j][e];
                 sum[0] += v[j][e];
             }
-        }
+        load(row + plan.passes);  // under way while this one is worked on
         if constexpr (kWide)
             block_sums<1, THREADS>(sum, lds[turn][0]);
         else
@@ -366,31 +373,43 @@ __global__ __launch_bounds__(THREADS ? THREADS : 256) void norm_rows_grad_kernel
         load_affine(a, q.gi * a.d + c, q.live && c < d ? (q.gi + 1) * a.d : 0, w[j], b[j]);
     }
     int turn = 0;
+    Oct<T> rx[CPL] = {}, rd[CPL] = {};
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    auto load = [&](int64_t row) {
+        if (!q.live || row >= a.n) return;
+        const int64_t unit = row * a.g + q.gi;
+        next_mean = a.mean[unit];
+        next_rstd = a.rstd[unit];
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+            const int32_t c = 8 * q.li + j * q.step;
+            if (c < d) {
+                rx[j] = load_oct(a.x + unit * a.d, c, d);
+                rd[j] = load_oct(a.dy + unit * a.d, c, d);
+            }
+        }
+    };
+    load(q.row0);
     for (int64_t r0 = 0; r0 < a.n; r0 += plan.passes, turn ^= 1) {
         const int64_t row = r0 + q.row0;
         const bool ok = q.live && row < a.n;
         if (kWide && !ok) break;  // the whole workgroup
-        const int64_t unit = row * a.g + q.gi, base = unit * a.d;
+        const int64_t base = (row * a.g + q.gi) * a.d;
         float xh[CPL][8], t[CPL][8];
-        const float mean = ok ? a.mean[unit] : 0.0f, rstd = ok ? a.rstd[unit] : 0.0f;
-        Oct<T> rx[CPL] = {}, rd[CPL] = {};
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-            const int32_t c = 8 * q.li + j * q.step;
-            if (ok && c < d) {
-                rx[j] = load_oct(a.x + base, c, d);
-                rd[j] = load_oct(a.dy + base, c, d);
-            }
-        }
+        const float mean = next_mean, rstd = next_rstd;
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < CPL; ++j) {
-            const int32_t c = 8 * q.li + j * q.step;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 xh[j][e] = ((float)rx[j][e] - mean) * rstd;
                 t[j][e] = (float)rd[j][e];
             }
+        }
+        load(row + plan.passes);  // under way while this one is worked on
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+            const int32_t c = 8 * q.li + j * q.step;
             if (c + 8 > d)  // past the group's end dy is zero, and so is what comes of it
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -773,7 +792,7 @@ __global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<
         if (q.row >= 0 && s0 + q.row < s1) {
             const T* from = a.x + (n * a.s + s0 + q.row) * a.c + q.c0;
             rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
-            constexpr int U = 4;
+            constexpr int U = sizeof(T) == 2 ? 8 : 4;
             const Oct<T> raw = load_oct(from, c0, q.width);
 #pragma unroll
             for (int e = 0; e < 8; ++e) first[e] = (float)raw[e];
@@ -819,16 +838,55 @@ __global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<
     }
 }
 
-// A run's share of the positions.
-__device__ __forceinline__ float run_share(const SlabPlan& p, int64_t s, int64_t r) {
-    return (float)(r + 1 < p.across ? p.run : s - r * p.run) / (float)s;
+// Rows under way: the first of DEPTH is worked on while the others are loaded.  Rows
+// are moved up rather than the loop unrolled, as the code of every activation times
+// the depth takes the registers of as many waves.
+template <typename T, int DEPTH>
+struct RowQueue {
+    Oct<T> v[DEPTH];
+    __device__ __forceinline__ void fill(const T* from, int64_t step, int32_t c, int32_t width, int32_t rows) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            v[i] = Oct<T>{};
+            if (i < rows) v[i] = load_oct(from + i * step, c, width);
+        }
+    }
+    // the row in front is done; `left` rows from it on
+    __device__ __forceinline__ void next(const T* from, int64_t step, int32_t c, int32_t width, int32_t left) {
+#pragma unroll
+        for (int i = 0; i + 1 < DEPTH; ++i) v[i] = v[i + 1];
+        if (left > DEPTH) v[DEPTH - 1] = load_oct(from + DEPTH * step, c, width);
+    }
+};
+
+template <typename T>
+constexpr int kRowsAhead = sizeof(T) == 2 ? 4 : 3;
+
+// A run's positions.
+__device__ __forceinline__ float run_count(const SlabPlan& p, int64_t s, int64_t r) {
+    return (float)(r + 1 < p.across ? p.run : s - r * p.run);
+}
+
+// The lanes that add up a group's runs: so many that the workgroup has all groups at
+// once, a power of two.
+template <int THREADS>
+__device__ __forceinline__ int join_lanes(const SlabPlan& p) {
+    int lanes = 64;
+    while (lanes > 1 && lanes * p.groups > THREADS) lanes >>= 1;
+    return lanes;
+}
+template <typename F>
+__device__ __forceinline__ void each_join(const SlabPlace& q, int lanes, F f) {
+    const int g = threadIdx.x / lanes;
+    if (g < q.groups) f(g, threadIdx.x & (lanes - 1));
 }
 
 // Joins the runs of a sample's groups: the mean, and the squares about it; then y.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float means[kSlabGroups], rstds[kSlabGroups];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lanes = join_lanes<THREADS>(p);
+    const float inv = 1.0f / ((float)a.s * (float)a.d);
     const uint64_t offset = drop_offset(a.drop);
     const int64_t run = blockIdx.y;
     const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
@@ -839,31 +897,30 @@ __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, 
     load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
-        // a wave to a group, its lanes over the runs
-        for (int g = wave; g < q.groups; g += THREADS / 64) {
+        // as a sum over the first run's mean: sum of n (m - m0), and of the squares
+        // about m0, from which what the mean is off m0 is taken
+        each_join(q, lanes, [&](int g, int li) {
             const float* f = part + 2 * (n * p.across * a.g + q.g0 + g);
             const int64_t next = 2 * a.g;
             const float first = f[0];
-            float sum[1] = {0.0f};  // what the mean is beyond the first run's
-            for (int64_t r = lane; r < p.across; r += 64)
-                sum[0] = __builtin_fmaf(f[r * next] - first, run_share(p, a.s, r), sum[0]);
-            lane_sums(sum, 64);
-            const float mean = first + sum[0];
-            sum[0] = 0.0f;
-            for (int64_t r = lane; r < p.across; r += 64) {
-                const float far = f[r * next] - mean;
-                sum[0] += __builtin_fmaf(far * far, run_share(p, a.s, r) * (float)a.s * (float)a.d, f[r * next + 1]);
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll 4
+            for (int64_t r = li; r < p.across; r += lanes) {
+                const float far = f[r * next] - first, count = run_count(p, a.s, r) * (float)a.d;
+                sum[0] = __builtin_fmaf(far, count, sum[0]);
+                sum[1] += __builtin_fmaf(far * far, count, f[r * next + 1]);
             }
-            lane_sums(sum, 64);
-            const float rstd = inverse_root(sum[0] / ((float)a.s * (float)a.d) + a.eps);
-            if (lane) continue;
+            lane_sums(sum, lanes);
+            if (li) return;
+            const float beyond = sum[0] * inv, mean = first + beyond;
+            const float rstd = inverse_root(fmaxf(__builtin_fmaf(-beyond, beyond, sum[1] * inv), 0.0f) + a.eps);
             means[g] = mean;
             rstds[g] = rstd;
             if (a.mean && run == 0) {
                 a.mean[n * a.g + q.g0 + g] = mean;
                 a.rstd[n * a.g + q.g0 + g] = rstd;
             }
-        }
+        });
         __syncthreads();
         if (q.row < 0 || s0 + q.row >= s1) continue;
         float mean[8], rstd[8];
@@ -873,18 +930,16 @@ __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, 
         });
         int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
         const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
-        // the next row under way while one is worked on: unrolled, the code of every
-        // activation takes the registers of as many waves
-        Oct<T> v = load_oct(a.x + at, c0, q.width), next = {};
+        RowQueue<T, kRowsAhead<T>> rows_x;
+        rows_x.fill(a.x + at, step, c0, q.width, rows);
 #pragma unroll 1
         for (int32_t r = 0; r < rows; ++r, at += step) {
-            if (r + 1 < rows) next = load_oct(a.x + at + step, c0, q.width);
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = ((float)v[e] - mean[e]) * rstd[e];
+            for (int e = 0; e < 8; ++e) f[e] = ((float)rows_x.v[0][e] - mean[e]) * rstd[e];
+            rows_x.next(a.x + at, step, c0, q.width, rows - r);
             forward_oct(a, offset, at + c0, w, b, f);
             store_oct(a.y + at, c0, q.width, f);
-            v = next;
         }
     }
 }
@@ -912,27 +967,25 @@ __global__ __launch_bounds__(THREADS) void norm_split_sums_kernel(NormOperands<T
         if (q.row >= 0 && s0 + q.row < s1) {
             int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
             const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
-            Oct<T> rx = load_oct(a.x + at, c0, q.width), rd = load_oct(a.dy + at, c0, q.width), nx = {}, nd = {};
+            RowQueue<T, 3> rows_x, rows_d;
+            rows_x.fill(a.x + at, step, c0, q.width, rows);
+            rows_d.fill(a.dy + at, step, c0, q.width, rows);
 #pragma unroll 1
             for (int32_t r = 0; r < rows; ++r, at += step) {
-                if (r + 1 < rows) {
-                    nx = load_oct(a.x + at + step, c0, q.width);
-                    nd = load_oct(a.dy + at + step, c0, q.width);
-                }
                 float xh[8], t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    xh[e] = ((float)rx[e] - mean[e]) * rstd[e];
-                    t[e] = (float)rd[e];
+                    xh[e] = ((float)rows_x.v[0][e] - mean[e]) * rstd[e];
+                    t[e] = (float)rows_d.v[0][e];
                 }
+                rows_x.next(a.x + at, step, c0, q.width, rows - r);
+                rows_d.next(a.dy + at, step, c0, q.width, rows - r);
                 backward_oct(a, offset, at + c0, w, b, xh, t);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[0][e] += t[e];
                     v[1][e] = __builtin_fmaf(t[e], xh[e], v[1][e]);
                 }
-                rx = nx;
-                rd = nd;
             }
         }
         const int64_t line = n * p.across + run;
@@ -960,7 +1013,7 @@ __global__ __launch_bounds__(THREADS) void norm_split_sums_kernel(NormOperands<T
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_split_grad_kernel(NormOperands<T> a, SlabPlan p, const float* part) {
     __shared__ float m1s[kSlabGroups], m2s[kSlabGroups];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lanes = join_lanes<THREADS>(p);
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
     const int64_t run = blockIdx.y;
@@ -972,18 +1025,19 @@ __global__ __launch_bounds__(THREADS) void norm_split_grad_kernel(NormOperands<T
     load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
-        for (int g = wave; g < q.groups; g += THREADS / 64) {  // a wave to a group, its lanes over the runs
+        each_join(q, lanes, [&](int g, int li) {
             const float* f = part + 2 * (n * p.across * a.g + q.g0 + g);
             float sum[2] = {0.0f, 0.0f};
-            for (int64_t r = lane; r < p.across; r += 64) {
+#pragma unroll 4
+            for (int64_t r = li; r < p.across; r += lanes) {
                 sum[0] += f[2 * r * a.g];
                 sum[1] += f[2 * r * a.g + 1];
             }
-            lane_sums(sum, 64);
-            if (lane) continue;
+            lane_sums(sum, lanes);
+            if (li) return;
             m1s[g] = sum[0] * inv;
             m2s[g] = sum[1] * inv;
-        }
+        });
         __syncthreads();
         if (q.row < 0 || s0 + q.row >= s1) continue;
         float mean[8], rstd[8], m1[8], m2[8];
@@ -995,25 +1049,23 @@ __global__ __launch_bounds__(THREADS) void norm_split_grad_kernel(NormOperands<T
         });
         int64_t at = (n * a.s + s0 + q.row) * a.c + q.c0;
         const int32_t rows = (int32_t)((s1 - s0 - q.row + p.rows - 1) / p.rows);
-        Oct<T> rx = load_oct(a.x + at, c0, q.width), rd = load_oct(a.dy + at, c0, q.width), nx = {}, nd = {};
+        RowQueue<T, 3> rows_x, rows_d;
+        rows_x.fill(a.x + at, step, c0, q.width, rows);
+        rows_d.fill(a.dy + at, step, c0, q.width, rows);
 #pragma unroll 1
         for (int32_t r = 0; r < rows; ++r, at += step) {
-            if (r + 1 < rows) {
-                nx = load_oct(a.x + at + step, c0, q.width);
-                nd = load_oct(a.dy + at + step, c0, q.width);
-            }
             float xh[8], t[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                xh[e] = ((float)rx[e] - mean[e]) * rstd[e];
-                t[e] = (float)rd[e];
+                xh[e] = ((float)rows_x.v[0][e] - mean[e]) * rstd[e];
+                t[e] = (float)rows_d.v[0][e];
             }
+            rows_x.next(a.x + at, step, c0, q.width, rows - r);
+            rows_d.next(a.dy + at, step, c0, q.width, rows - r);
             backward_oct(a, offset, at + c0, w, b, xh, t);
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = rstd[e] * (t[e] * w[e] - __builtin_fmaf(xh[e], m2[e], m1[e]));
             store_oct(a.y + at, c0, q.width, t);
-            rx = nx;
-            rd = nd;
         }
     }
 }

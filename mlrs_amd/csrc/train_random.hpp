@@ -94,6 +94,7 @@ __device__ __forceinline__ void drop_oct(const Drop& d, uint64_t offset, int64_t
     random_block((uint64_t)i >> 3, offset, d.k0, d.k1, w);
     const int r = (int)(i & 7);
     if (!aligned) {
+        asm volatile("");  // not to be computed where it is not needed
         RandomWords next;
         random_block(((uint64_t)i >> 3) + 1, offset, d.k0, d.k1, next);
         uint32_t all[8];
