@@ -75,6 +75,35 @@ __host__ __device__ constexpr int fp8_lds() {
     return fp8_depth<MB>() * (WM * MB + WN * NB) * 16 * kStageBytes + 2 * (WM * MB + WN * NB) * 16 * 4;
 }
 
+// A wave's copies of a panel of codes into LDS, in the places of train_gemm.hpp's
+// Stager: eight rows an instruction, a lane the chunk that the swizzle of its row puts
+// there.  What that adds to an instruction's first row is the same for every second
+// instruction, and for both operands, whose rows are as long: two registers a lane,
+// where the accumulators leave few.
+struct CodeStager {
+    const char* base;  // the wave's first row, at k = 0
+    int64_t bytes;     // from base to the operand's end
+    int64_t pair;      // bytes of sixteen rows
+    __device__ __forceinline__ void init(const Operand& o, int32_t row0, int32_t rows, int32_t wave_rows, int wave) {
+        const int64_t first = (int64_t)row0 + (int64_t)wave * wave_rows;
+        base = reinterpret_cast<const char*>(o.p) + first * o.ld;
+        bytes = ((int64_t)rows - first) * o.ld;
+        pair = 16 * o.ld;
+    }
+    // Instruction I of the wave's, at k0; past the end come zeros.
+    template <int I>
+    __device__ __forceinline__ void load(char* lds, int64_t k0, const uint32_t (&off)[2]) const {
+        const int64_t skip = k0 + (I / 2) * pair, left = bytes - skip;
+        const uint64_t at = (uint64_t)(base + skip);
+        u32x4 rsrc;
+        rsrc[0] = (uint32_t)at;
+        rsrc[1] = (uint32_t)(at >> 32) & 0xFFFFu;
+        rsrc[2] = left < 0x7FFFFFFF ? (left > 0 ? (uint32_t)left : 0u) : 0x7FFFFFFFu;
+        rsrc[3] = 0x00027000u;
+        copy_to_lds(rsrc, lds + I * 1024, off[I & 1]);
+    }
+};
+
 // The words of 64 rows' scales into LDS.
 struct ScaleCopy {
     const uint8_t* base;  // of the tile's first row (or its 128)
@@ -124,11 +153,19 @@ __device__ __forceinline__ void fp8_workgroup(const Fp8Args& q, const Epi& epi, 
     const int32_t k_hi = g.k - k_lo < g.k_split ? g.k : k_lo + g.k_split;
     const int32_t widths = (k_hi - k_lo) / kStageBytes;
 
-    Stager<uint8_t, true, BM, WAVES> sa;
-    Stager<uint8_t, true, BN, WAVES> sb;
-    sa.init(g.a, m0, g.m, k_hi, wave, lane);
-    sb.init(g.b, n0, g.n, k_hi, wave, lane);
-    constexpr int kCopies = decltype(sa)::kInstr + decltype(sb)::kInstr;
+    static_assert(BM == BN, "both operands' panels alike");
+    constexpr int kInstr = BM / 8 / WAVES, kCopies = 2 * kInstr;  // of an operand, of both
+    static_assert(kInstr % 2 == 0, "sixteen rows at a time");
+    CodeStager sa, sb;
+    sa.init(g.a, m0, g.m, kInstr * 8, wave);
+    sb.init(g.b, n0, g.n, kInstr * 8, wave);
+    uint32_t off[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        off[i] = (uint32_t)r * (uint32_t)g.a.ld + 16u * (uint32_t)((lane & 7) ^ k_swizzle(r));
+    }
+    char* const panel = buf + wave * kInstr * 1024;  // the wave's part of a panel
     ScaleCopy sc;
     const int part = wave & (kScaleWaves - 1);  // of the words; small tiles have more waves
     if (part < BM / 64)
@@ -144,11 +181,28 @@ __device__ __forceinline__ void fp8_workgroup(const Fp8Args& q, const Epi& epi, 
     // does with the scales goes by its place U = p % 4.
     // Copies of width p, the scales of four before them: they are the older ones
     // where it is waited for all but the last.
-    auto copy = [&](int32_t p, int at, auto u) {
+    // Instructions I of them alone, FROM <= I < TO of either operand.
+    auto copy_some = [&](int32_t p, int at, auto from, auto to) {
+        const int64_t k0 = p < widths ? k_lo + p * kStageBytes : (int64_t)1 << 40;  // past the end: zeros
+        auto one = [&](auto i) {
+            if constexpr (decltype(i)::v >= decltype(from)::v && decltype(i)::v < decltype(to)::v) {
+                sa.template load<decltype(i)::v>(panel + at, k0, off);
+                sb.template load<decltype(i)::v>(panel + at + kA, k0, off);
+            }
+        };
+        one(Set<0>{});
+        one(Set<1>{});
+        one(Set<2>{});
+        one(Set<3>{});
+    };
+    static_assert(kInstr <= 4, "four are spelled out");
+    auto copy_scales = [&](int32_t p, auto u) {
         if constexpr ((decltype(u)::v & 3) == 0)
             sc.load(scales + __builtin_amdgcn_readfirstlane(((p >> 2) & 1) * kScales + part * 256), (k_lo >> 7) + p);
-        sa.template load<0, 1>(buf + at, k_lo + p * kStageBytes, k_hi, wave);
-        sb.template load<0, 1>(buf + at + kA, k_lo + p * kStageBytes, k_hi, wave);
+    };
+    auto copy = [&](int32_t p, int at, auto u) {
+        copy_scales(p, u);
+        copy_some(p, at, Set<0>{}, Set<kInstr>{});
     };
     auto next = [&](int at) { return at + kPair >= kDepth * kPair ? 0 : at + kPair; };
     auto frag_a = [&](const char* from, int i) { return join_halves(ra.get(from, 0, i), ra.get(from, 1, i)); };
@@ -227,6 +281,7 @@ __device__ __forceinline__ void fp8_workgroup(const Fp8Args& q, const Epi& epi, 
         // widths too: the barrier that publishes width p + 1 stands before the last
         // part of width p.  After it width p + 2 is copied where p was.
         constexpr int kParts = MB / 2;
+        static_assert(NB == 4, "four steps of the last part");
         i32x8 fa[2][2], fb[NB];
         auto fetch_a = [&](const char* from, int part) {
 #pragma unroll
