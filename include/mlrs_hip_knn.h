@@ -711,8 +711,8 @@ int32_t mlrs_fp8_weight_bf16(const uint16_t *w, int64_t w_len, int64_t d_out, in
  * is what 8 bits hold of x, a scale for each 128 of a row, and w' what the codes
  * stand for.  Products are exact.  f16, bf16: the matrix instruction adds eight
  * adjacent products after cutting off what lies below 2^-13 of the largest one's
- * power of two, all else in f32.  f32: added up in f32, the values of more than 32
- * rows in bf16's range.  Up to 32 rows take no workspace.
+ * power of two, all else in f32.  f32: added up in f32, the values of more than 16
+ * rows in bf16's range.  Up to 16 rows take no workspace.
  * Errors, in this order: ShapeMismatch "x" / "features", MLRS_ERR_UNSUPPORTED
  *   "features" / "rows", "codes" and "scales" as above, then as mlrs_linear from
  *   "bias" on.

@@ -191,7 +191,7 @@ int32_t check_codes(const char* codes_name, const char* scales_name, const uint8
 }
 // A product's grid must fit, in the largest tiles.
 bool grid_fits(int64_t m, int64_t n) { return launchable(((m + 255) / 256) * ((n + 255) / 256), 512); }
-bool codes_fit(int64_t n, int64_t k) { return launchable(tiles128(n) * tiles128(k), 256); }
+bool codes_fit(int64_t n, int64_t k) { return launchable(tiles128(n) * tiles128(k), 512); }
 int32_t grid_error(int64_t m, int64_t n) {
     return capi::error(MLRS_ERR_UNSUPPORTED, "rows", n, m, 0, "the product has more tiles than a launch");
 }
@@ -256,7 +256,7 @@ int32_t linear_fp8_impl(const T* x, int64_t x_len, int64_t n, int64_t k, const u
         int cus = 0;
         rc = capi::cu_count(&cus);
         if (rc) return rc;
-        if (n <= kFp8Few) {
+        if (fp8_few_rows(n, m, k)) {
             capi::Timed timed(s, "linear_fp8_few");
             MLRS_TRY(launch_fp8_few<T>(x, w, n, m, k, o, s));
             return MLRS_OK;
@@ -317,7 +317,7 @@ int32_t linear_fp8_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_
             if (act != MLRS_ACT_NONE && !z) return null_error("preact");
         }
         if (dx && (!codes_t || !scales_t)) return null_error(!codes_t ? "codes_t" : "scales_t");
-        if (!grid_fits(k, n) || !grid_fits(k, m) || !launchable(tiles128(n) * (tiles128(m) + tiles128(k)), 256))
+        if (!grid_fits(k, n) || !grid_fits(k, m) || !launchable(tiles128(n) * (tiles128(m) + tiles128(k)), 512))
             return grid_error(k, std::max(m, n));
         const Span ody(dy, dy_len), ox(x, x_len), oc(codes_t, codes_t_len), os(scales_t, scales_t_len), oz(z, z_len),
             odx(dx, dx_len), odw(dw, dw_len);

@@ -63,13 +63,14 @@ __device__ __forceinline__ bool unbounded(float x) { return fabsf(x) == __builti
 // ---------------------------------------------------------------------------
 // making codes
 // ---------------------------------------------------------------------------
-// A workgroup takes 128 x 128 elements, a thread eight by eight of them: rows 8 (t /
+// A workgroup takes 128 x 128 elements, a thread four by eight of them: rows 4 (t /
 // 16) on and columns 8 (t % 16) on, so that it has eight adjacent codes of a row and
-// of a column.  The elements are read once, whatever is made of them: codes with a
-// scale for each row, codes of the transpose with a scale for each column (turned
-// through LDS), or both with one scale for the tile; and column sums.  Infinities and
-// NaN have code NaN and no part in the scale.  VALUES: bf16 values and no scales in
-// the codes' place.
+// four of a column (eight by eight take 210 registers and the same time: 136 to 152 us
+// for the 535 MB of a gradient of 8192 x 8192 and its x of 8192 x 4096, 3.5 to 3.9
+// TB/s).  Bound by memory.  The elements are read once, whatever is made of them: codes with a scale for each row, codes of the transpose
+// with a scale for each column (turned through LDS), or both with one scale for the
+// tile; and column sums.  Infinities and NaN have code NaN and no part in the scale.
+// VALUES: bf16 values and no scales in the codes' place.
 template <typename T>
 struct CodeJob {
     const T *src, *z;  // z: null, or src is multiplied by act'(z)
@@ -82,36 +83,39 @@ struct CodeJob {
     __host__ __device__ int64_t tiles() const { return (rows + 127) / 128 * tiles_c(); }
 };
 
+constexpr int kCodeThreads = 512;
+
 template <typename T, bool VALUES>
-__global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T> second) {
+__global__ __launch_bounds__(kCodeThreads, 4) void codes_kernel(CodeJob<T> first, CodeJob<T> second) {
+    constexpr int R = 4, WAVES = kCodeThreads / 64;
     __shared__ __attribute__((aligned(16))) char turn[128 * 128 * (VALUES ? 2 : 1)];
-    __shared__ float tops[4][128], sums[4][128];
+    __shared__ float tops[WAVES][128], sums[WAVES][128];
     const bool one = (int64_t)blockIdx.x < first.tiles();
     const CodeJob<T>& j = one ? first : second;
     const int64_t t = one ? blockIdx.x : blockIdx.x - first.tiles();
     const int64_t tr = t / j.tiles_c(), tc = t - tr * j.tiles_c();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int o = threadIdx.x & 15, p = threadIdx.x >> 4;
-    const int64_t r0 = tr * 128 + 8 * p, c0 = tc * 128 + 8 * o;
-    float v[8][8];
+    const int64_t r0 = tr * 128 + R * p, c0 = tc * 128 + 8 * o;
+    float v[R][8];
     {
-        Oct<T> raw[8] = {}, z[8] = {};
+        Oct<T> raw[R] = {}, z[R] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
             if (r0 + i < j.rows && c0 < j.cols) raw[i] = load_oct(j.src + (r0 + i) * j.cols, c0, j.cols);
         if (j.z) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < R; ++i)
                 if (r0 + i < j.rows && c0 < j.cols) z[i] = load_oct(j.z + (r0 + i) * j.cols, c0, j.cols);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = (float)raw[i][e];
         if (j.z) {
             auto slope = [&](auto f) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < R; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[i][e] *= f((float)z[i][e]);
             };
@@ -125,12 +129,12 @@ __global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T>
         }
     }
     // the largest magnitudes; maxima leave out NaN by themselves
-    float row_top[8], col_top[8], col_sum[8] = {};
+    float row_top[R], col_top[8], col_sum[8] = {};
     auto maxima = [&](auto magnitude) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) col_top[e] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < R; ++i) {
             row_top[i] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -142,30 +146,32 @@ __global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T>
     };
     if (j.sums) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e) col_sum[e] += v[i][e];
     }
     maxima([](float x) { return fabsf(x); });
     bool odd = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) odd |= unbounded(row_top[i]);
+    for (int i = 0; i < R; ++i) odd |= unbounded(row_top[i]);
     if (odd) {
         maxima([](float x) { return unbounded(x) ? 0.0f : fabsf(x); });
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (unbounded(v[i][e])) v[i][e] = __builtin_nanf("");
     }
+    if (j.codes_t || j.tile) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        col_top[e] = fmaxf(col_top[e], __shfl_xor(col_top[e], 16));
-        col_top[e] = fmaxf(col_top[e], __shfl_xor(col_top[e], 32));
+        for (int e = 0; e < 8; ++e) {
+            col_top[e] = fmaxf(col_top[e], __shfl_xor(col_top[e], 16));
+            col_top[e] = fmaxf(col_top[e], __shfl_xor(col_top[e], 32));
+        }
+        if (lane < 16)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tops[wave][8 * o + e] = col_top[e];
     }
-    if (lane < 16)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) tops[wave][8 * o + e] = col_top[e];
     if (j.sums) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -176,30 +182,35 @@ __global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T>
 #pragma unroll
             for (int e = 0; e < 8; ++e) sums[wave][8 * o + e] = col_sum[e];
     }
-    __syncthreads();
-    if (j.sums && threadIdx.x < 128) {
-        const int c = threadIdx.x;
-        if (tc * 128 + c < j.cols)
-            j.sums[tr * j.cols + tc * 128 + c] = ((sums[0][c] + sums[1][c]) + sums[2][c]) + sums[3][c];
-    }
     float whole = 0.0f;
+    if (j.codes_t || j.tile || j.sums) {
+        __syncthreads();
+        if (j.sums && threadIdx.x < 128) {
+            const int c = threadIdx.x;
+            float sum = sums[0][c];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        col_top[e] = fmaxf(fmaxf(tops[0][8 * o + e], tops[1][8 * o + e]), fmaxf(tops[2][8 * o + e], tops[3][8 * o + e]));
-        whole = fmaxf(whole, col_top[e]);
+            for (int w = 1; w < WAVES; ++w) sum += sums[w][c];
+            if (tc * 128 + c < j.cols) j.sums[tr * j.cols + tc * 128 + c] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            col_top[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) col_top[e] = fmaxf(col_top[e], tops[w][8 * o + e]);
+            whole = fmaxf(whole, col_top[e]);
+        }
     }
     if (j.tile) {
+        whole = max16(whole);
 #pragma unroll
-        for (int s = 1; s < 16; s <<= 1) whole = fmaxf(whole, __shfl_xor(whole, s));
+        for (int e = 0; e < 8; ++e) col_top[e] = whole;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) row_top[e] = col_top[e] = whole;
+        for (int i = 0; i < R; ++i) row_top[i] = whole;
     } else if (j.codes) {
 #pragma unroll
-        for (int s = 1; s < 16; s <<= 1)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row_top[i] = fmaxf(row_top[i], __shfl_xor(row_top[i], s));
+        for (int i = 0; i < R; ++i) row_top[i] = max16(row_top[i]);
     }
-    // a row of scales in whole words: the last tile writes what is behind it
+    // weights' rows of scales are whole words: the last tile writes what is behind it
     auto put_scale = [](uint8_t* row, int64_t at, int64_t blocks, int e) {
         row[at] = (uint8_t)(e + 127);
         if (at + 1 == blocks)
@@ -209,7 +220,7 @@ __global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T>
     const int64_t ld = (blocks + 3) / 4 * 4, ld_t = (blocks_t + 3) / 4 * 4;
     if (j.codes) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < R; ++i) {
             const int e = scale_exponent(row_top[i]);
             const float by = scale_inverse(e);
             if (r0 + i >= j.rows) continue;
@@ -221,44 +232,37 @@ __global__ __launch_bounds__(256) void codes_kernel(CodeJob<T> first, CodeJob<T>
                 continue;
             }
             *reinterpret_cast<uint64_t*>(j.codes + at) = lo | (uint64_t)hi << 32;
-            if (!j.tile && o == 0) put_scale(j.scales + (r0 + i) * ld, tc, blocks, e);
+            if (!j.tile && o == 0) j.scales[((tc >> 2) * j.rows + r0 + i) * 4 + (tc & 3)] = (uint8_t)(e + 127);
         }
         if (!VALUES && j.tile && threadIdx.x == 0) put_scale(j.scales + tr * ld, tc, blocks, scale_exponent(whole));
     }
     if (!j.codes_t) return;
-    // column c's eight codes of rows 8 p on are piece p ^ (c / 8) of its line
+    // column c's line in LDS: its pieces of sixteen bytes at piece ^ (c / 8), so that the
+    // lanes that write one row's eighths of the columns are in different banks
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int x = scale_exponent(col_top[e]);
         const float by = scale_inverse(x);
-        const uint32_t lo = codes4(v[0][e] * by, v[1][e] * by, v[2][e] * by, v[3][e] * by);
-        const uint32_t hi = codes4(v[4][e] * by, v[5][e] * by, v[6][e] * by, v[7][e] * by);
+        const uint32_t w = codes4(v[0][e] * by, v[1][e] * by, v[2][e] * by, v[3][e] * by);
         if constexpr (VALUES) {
-            *reinterpret_cast<bf16x8*>(turn + (8 * o + e) * 256 + ((p ^ o) << 4)) = values8(lo, hi, scale_of(x));
+            const bf16x8 u = values8(w, 0, scale_of(x));
+            *reinterpret_cast<bf16x4*>(turn + (8 * o + e) * 256 + (((p >> 1) ^ o) << 4) + (p & 1) * 8) =
+                __builtin_shufflevector(u, u, 0, 1, 2, 3);
             continue;
         }
-        *reinterpret_cast<uint64_t*>(turn + (8 * o + e) * 128 + ((p ^ o) << 3)) = lo | (uint64_t)hi << 32;
-        if (!j.tile && p == 0 && c0 + e < j.cols) put_scale(j.scales_t + (c0 + e) * ld_t, tr, blocks_t, x);
+        *reinterpret_cast<uint32_t*>(turn + (8 * o + e) * 128 + (((p >> 2) ^ (o & 7)) << 4) + (p & 3) * 4) = w;
+        if (!j.tile && p == 0 && c0 + e < j.cols)
+            j.scales_t[((tr >> 2) * j.cols + c0 + e) * 4 + (tr & 3)] = (uint8_t)(x + 127);
     }
     if (!VALUES && j.tile && threadIdx.x == 0) put_scale(j.scales_t + tc * ld_t, tr, blocks_t, scale_exponent(whole));
     __syncthreads();
-    if constexpr (VALUES) {
+    constexpr int kPieces = VALUES ? 16 : 8;  // of a line
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int at = threadIdx.x + 256 * i, c = at >> 4, piece = at & 15;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(turn + c * 256 + ((piece ^ (c >> 3)) << 4));
-            if (tc * 128 + c < j.cols)
-                *reinterpret_cast<u32x4*>(j.codes_t + ((tc * 128 + c) * blocks_t * 128 + tr * 128) * 2 + 16 * piece) = w;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = threadIdx.x + 256 * i, c = at >> 3, piece = at & 7, x = c >> 3;
-        u32x4 w = *reinterpret_cast<const u32x4*>(turn + c * 128 + ((piece ^ (x >> 1)) << 4));
-        if (x & 1) w = __builtin_shufflevector(w, w, 2, 3, 0, 1);
+    for (int i = 0; i < 128 * kPieces / kCodeThreads; ++i) {
+        const int at = threadIdx.x + kCodeThreads * i, c = at / kPieces, piece = at % kPieces;
+        const u32x4 w = *reinterpret_cast<const u32x4*>(turn + c * 16 * kPieces + ((piece ^ ((c >> 3) & (kPieces - 1))) << 4));
         if (tc * 128 + c < j.cols)
-            *reinterpret_cast<u32x4*>(j.codes_t + (tc * 128 + c) * blocks_t * 128 + tr * 128 + 16 * piece) = w;
+            *reinterpret_cast<u32x4*>(j.codes_t + ((tc * 128 + c) * blocks_t * 128 + tr * 128) * (VALUES ? 2 : 1) + 16 * piece) = w;
     }
 }
 
@@ -266,8 +270,8 @@ template <bool VALUES, typename T>
 hipError_t launch_codes(const CodeJob<T>& a, const CodeJob<T>& b, hipStream_t s) {
     const int64_t tiles = a.tiles() + b.tiles();
     if (tiles == 0) return hipSuccess;
-    if (!launchable(tiles, 256)) return hipErrorInvalidConfiguration;  // the caller has checked
-    codes_kernel<T, VALUES><<<dim3((unsigned)tiles), 256, 0, s>>>(a, b);
+    if (!launchable(tiles, kCodeThreads)) return hipErrorInvalidConfiguration;  // the caller has checked
+    codes_kernel<T, VALUES><<<dim3((unsigned)tiles), kCodeThreads, 0, s>>>(a, b);
     return hipGetLastError();
 }
 
@@ -290,45 +294,27 @@ __global__ __launch_bounds__(256) void values_kernel(const uint8_t* __restrict__
 // ---------------------------------------------------------------------------
 // Bound by reading the codes of the weights, once, straight into registers as the
 // fragments of the matrix instructions.  A workgroup computes sixteen outputs of
-// every row; its waves take blocks of k in turn, make the codes of the rows' blocks
-// themselves (the four lanes of a row hold a block), and their sums are joined in
-// LDS, in the order of the waves.  No launch and no workspace besides.
-template <typename T>
-__device__ __forceinline__ void few_codes(const T* row, int64_t c0, int64_t k, int g, i32x8& codes, int& scale) {
-    float v[32];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        const int64_t c = c0 + (h >> 1) * 64 + 16 * g + (h & 1) * 8;
-        Oct<T> raw = {};
-        if (c < k) raw = load_oct(row, c, k);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * h + e] = (float)raw[e];
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(v[e]));
-    if (unbounded(top)) {
-        top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            if (unbounded(v[e])) v[e] = __builtin_nanf("");
-            top = fmaxf(top, fabsf(v[e]));
-        }
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const int e = scale_exponent(top);
-    const float by = scale_inverse(e);
-    scale = e + 127;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) codes[w] = (int)codes4(v[4 * w] * by, v[4 * w + 1] * by, v[4 * w + 2] * by, v[4 * w + 3] * by);
+// every row.  In passes of 1024 U columns its threads first make the codes of the rows
+// in LDS, sixteen lanes to a block, while the pass's weights are on their way; then
+// each wave multiplies its U blocks.  The waves' sums are joined in LDS, in order.  No
+// launch and no workspace besides.  (Each wave making the codes of its own blocks, as
+// it needs them, took 12.1 us of one row by 8192 x 4096: the codes of a row are then
+// made sixteen times over.)
+constexpr int kFewWaves = 8;
+template <int U>
+__host__ __device__ constexpr int few_row_bytes() {  // of a row in LDS: codes and scales
+    return kFewWaves * U * (128 + 4);
 }
 
-template <typename T, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const T* __restrict__ x, const uint8_t* __restrict__ codes,
-                                                             const uint8_t* __restrict__ scales, int32_t n, int32_t m,
-                                                             int64_t k, LinearEpi<T> epi) {
-    __shared__ f32x4 sums[WAVES][NB][64];
+template <typename T, int NB, int U>
+__global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(const T* __restrict__ x,
+                                                                 const uint8_t* __restrict__ codes,
+                                                                 const uint8_t* __restrict__ scales, int32_t n,
+                                                                 int32_t m, int64_t k, LinearEpi<T> epi) {
+    extern __shared__ __attribute__((aligned(16))) char rows[];  // n rows of few_row_bytes
+    __shared__ f32x4 sums[kFewWaves][NB][64];
+    constexpr int kBlocks = kFewWaves * U, kOcts = kBlocks * 16;  // of a pass
+    char* const row_scales = rows + n * kBlocks * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int32_t m0 = (int32_t)blockIdx.x * 16;
@@ -336,8 +322,8 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const T* __restrict
     const uint8_t* wr = codes + (int64_t)(m0 + r < m ? m0 + r : m - 1) * blocks * 128 + 16 * g;
     const uint8_t* ws = scales + (m0 >> 7) * ((blocks + 3) / 4 * 4);
     f32x4 acc[NB] = {};
-    constexpr int U = 2;  // blocks in flight
-    for (int64_t b0 = (int64_t)wave * U; b0 < blocks; b0 += (int64_t)WAVES * U) {
+    for (int64_t pass = 0; pass < blocks; pass += kBlocks) {
+        const int64_t b0 = pass + wave * U;
         u32x4 lo[U] = {}, hi[U] = {};
         int sw[U] = {};
 #pragma unroll
@@ -347,24 +333,54 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const T* __restrict
                 hi[u] = *reinterpret_cast<const u32x4*>(wr + (b0 + u) * 128 + 64);
                 sw[u] = ws[b0 + u];
             }
+        if (pass) __syncthreads();  // the last pass's codes have been read
+        for (int at = threadIdx.x; at < n * kOcts; at += kFewWaves * 64) {
+            const int row = at / kOcts, oct = at % kOcts;
+            const int64_t c = pass * 128 + 8 * oct;
+            Oct<T> raw = {};
+            if (c < k) raw = load_oct(x + row * k, c, k);
+            float v[8], top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = (float)raw[e];
+                top = fmaxf(top, fabsf(v[e]));
+            }
+            if (unbounded(top)) {
+                top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (unbounded(v[e])) v[e] = __builtin_nanf("");
+                    top = fmaxf(top, fabsf(v[e]));
+                }
+            }
+            const int e = scale_exponent(max16(top));
+            const float by = scale_inverse(e);
+            const uint64_t w = codes4(v[0] * by, v[1] * by, v[2] * by, v[3] * by) |
+                               (uint64_t)codes4(v[4] * by, v[5] * by, v[6] * by, v[7] * by) << 32;
+            *reinterpret_cast<uint64_t*>(rows + (row * kBlocks + oct / 16) * 128 +
+                                         ((((oct >> 1) & 7) ^ k_swizzle(row)) << 4) + (oct & 1) * 8) = w;
+            if ((oct & 15) == 0) *reinterpret_cast<int*>(row_scales + (row * kBlocks + oct / 16) * 4) = e + 127;
+        }
+        __syncthreads();
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const T* xr = x + (int64_t)(b * 16 + r < n ? b * 16 + r : n - 1) * k;
+            const int row = b * 16 + r < n ? b * 16 + r : n - 1;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (b0 + u >= blocks) continue;
-                i32x8 cx;
-                int sx;
-                few_codes(xr, (b0 + u) * 128, k, g, cx, sx);
+                const char* from = rows + (row * kBlocks + wave * U + u) * 128;
+                const u32x4 x0 = *reinterpret_cast<const u32x4*>(from + ((g ^ k_swizzle(row)) << 4));
+                const u32x4 x1 = *reinterpret_cast<const u32x4*>(from + (((4 + g) ^ k_swizzle(row)) << 4));
+                const int sx = *reinterpret_cast<const int*>(row_scales + (row * kBlocks + wave * U + u) * 4);
                 if constexpr (sizeof(T) == 2) {
-                    acc[b] = mfma_fp8(join_halves(lo[u], hi[u]), cx, acc[b], sw[u], sx);
+                    acc[b] = mfma_fp8(join_halves(lo[u], hi[u]), join_halves(x0, x1), acc[b], sw[u], sx);
                 } else {  // in f32 the codes go through the bf16 instructions, the scales to their sums
                     f32x4 block = {};
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        const u32x4& w = h < 2 ? lo[u] : hi[u];
+                        const u32x4 &w = h < 2 ? lo[u] : hi[u], &y = h < 2 ? x0 : x1;
                         block = mfma_step<__bf16>(values8(w[2 * (h & 1)], w[2 * (h & 1) + 1], 1.0f),
-                                                  values8(cx[2 * h], cx[2 * h + 1], 1.0f), block);
+                                                  values8(y[2 * (h & 1)], y[2 * (h & 1) + 1], 1.0f), block);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[b][e] += ldexpf(block[e], sw[u] + sx - 254);
@@ -375,10 +391,10 @@ __global__ __launch_bounds__(WAVES * 64) void fp8_few_kernel(const T* __restrict
 #pragma unroll
     for (int b = 0; b < NB; ++b) sums[wave][b][lane] = acc[b];
     __syncthreads();
-    for (int b = wave; b < NB; b += WAVES) {  // wave b joins the sums of rows 16 b .. 16 b + 15
+    for (int b = wave; b < NB; b += kFewWaves) {  // wave b joins the sums of rows 16 b .. 16 b + 15
         f32x4 v = sums[0][b][lane];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) v += sums[i][b][lane];
+        for (int i = 1; i < kFewWaves; ++i) v += sums[i][b][lane];
         const int32_t row = b * 16 + r, c = m0 + 4 * g;
         if (row < n && c < m) epi.point(row, c, m, v);
     }
@@ -391,14 +407,12 @@ int64_t fp8_args(Fp8Args& q, int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t
                  int32_t k_split) {
     const int64_t kp = fp8_columns(k);
     const int64_t blocks = gemm_args(q.g, tile, Mat{a.codes, kp}, Mat{b.codes, kp}, m, n, kp, splits, k_split, Only{});
-    const int64_t ld = fp8_scale_row(k);
-    q.sa = a.scales;
-    q.sb = b.scales;
-    q.sa_ld = q.sb_ld = ld;
-    q.a_shift = a.tile ? 7 : 0;
-    q.b_shift = b.tile ? 7 : 0;
-    q.sa_rows = a.tile ? (m + 127) / 128 : m;
-    q.sb_rows = b.tile ? (n + 127) / 128 : n;
+    auto where = [&](const Fp8Mat& x, int64_t rows) {
+        return x.tile ? ScaleRows{x.scales, fp8_scale_row(k), 4, (rows + 127) / 128, 7}
+                      : ScaleRows{x.scales, 4, 4 * rows, rows, 0};
+    };
+    q.sa = where(a, m);
+    q.sb = where(b, n);
     return blocks;
 }
 
@@ -537,10 +551,14 @@ hipError_t launch_fp8_few(const T* x, const Fp8Mat& w, int64_t n, int64_t m, int
                           hipStream_t s) {
     const LinearEpi<T> e = linear_epi<T>(o, m);
     const dim3 grid((unsigned)((m + 15) / 16));
-    if (n <= 16)
-        fp8_few_kernel<T, 1, 8><<<grid, 512, 0, s>>>(x, (const uint8_t*)w.codes, w.scales, (int32_t)n, (int32_t)m, k, e);
+    const uint8_t* c = (const uint8_t*)w.codes;
+    // as many columns at a time as leave several workgroups a CU
+    if (n <= 8)
+        fp8_few_kernel<T, 1, 4><<<grid, kFewWaves * 64, n * few_row_bytes<4>(), s>>>(x, c, w.scales, (int32_t)n, (int32_t)m, k, e);
+    else if (n <= 16)
+        fp8_few_kernel<T, 1, 2><<<grid, kFewWaves * 64, n * few_row_bytes<2>(), s>>>(x, c, w.scales, (int32_t)n, (int32_t)m, k, e);
     else
-        fp8_few_kernel<T, 2, 8><<<grid, 512, 0, s>>>(x, (const uint8_t*)w.codes, w.scales, (int32_t)n, (int32_t)m, k, e);
+        fp8_few_kernel<T, 2, 1><<<grid, kFewWaves * 64, n * few_row_bytes<1>(), s>>>(x, c, w.scales, (int32_t)n, (int32_t)m, k, e);
     return hipGetLastError();
 }
 

@@ -17,9 +17,11 @@
 // do without: their operands are made as bf16 values (a code times its power of two
 // has four bits) and multiplied by train_gemm.hpp's instructions, at half the rate.
 //
-// Operands.  Codes have k contiguous, rows padded with zeros to whole blocks; a row's
-// scales are bytes (the exponent + 127), padded to whole words, of every row (shift 0)
-// or of every 128 rows (shift 7).  All three products of a layer have this layout, as
+// Operands.  Codes have k contiguous, rows padded with zeros to whole blocks.  Scales
+// are bytes (the exponent + 127) in words of four blocks: of weights, words of every 128
+// rows in turn; of rows made for a product, the rows' words of the same four blocks
+// side by side, so that a workgroup that makes the codes of 128 x 128 writes its 128
+// bytes into four lines.  All three products of a layer have this layout, as
 // the kernel that makes the codes writes them transposed where that is wanted.
 //
 // Tile.  As train_gemm.hpp's, with the same swizzles: 128 bytes of k are one staged
@@ -41,12 +43,17 @@ struct Elem<uint8_t> {
     typedef u32x4 Frag;
 };
 
+// Where the scales of an operand are: the word of four blocks of row r, or of 128 rows
+// (shift 7), is at s + (r >> shift) * step + word * plane.
+struct ScaleRows {
+    const uint8_t* s;
+    int64_t step, plane, rows;  // bytes, bytes, and how many of r >> shift
+    int shift;
+};
+
 struct Fp8Args {
     GemmArgs g;
-    const uint8_t *sa, *sb;   // scales
-    int64_t sa_ld, sb_ld;     // bytes
-    int64_t sa_rows, sb_rows;
-    int a_shift, b_shift;
+    ScaleRows sa, sb;
 };
 
 __device__ __forceinline__ f32x4 mfma_fp8(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
@@ -107,21 +114,23 @@ struct CodeStager {
 // The words of 64 rows' scales into LDS.
 struct ScaleCopy {
     const uint8_t* base;  // of the tile's first row (or its 128)
-    int64_t bytes;        // from base to the end
+    int64_t plane;
+    uint32_t bytes;       // of a plane, from base to its end
     uint32_t off;         // the lane's
-    __device__ __forceinline__ void init(const uint8_t* s, int64_t ld, int64_t rows, int shift, int32_t row0, int32_t row) {
-        const int64_t first = row0 >> shift;
-        base = s + first * ld;
-        bytes = (rows - first) * ld;
-        off = (uint32_t)((((int64_t)row0 + row) >> shift) - first) * (uint32_t)ld;
+    __device__ __forceinline__ void init(const ScaleRows& s, int32_t row0, int32_t row) {
+        const int64_t first = row0 >> s.shift, left = (s.rows - first) * s.step;
+        base = s.s + first * s.step;
+        plane = s.plane;
+        bytes = left < 0x7FFFFFFF ? (left > 0 ? (uint32_t)left : 0u) : 0x7FFFFFFFu;
+        off = (uint32_t)((((int64_t)row0 + row) >> s.shift) - first) * (uint32_t)s.step;
     }
-    __device__ __forceinline__ void load(char* lds, int32_t at) const {
-        const int64_t left = bytes - at;
-        const uint64_t from = (uint64_t)(base + at);
+    // Word w; past the last one zeros.
+    __device__ __forceinline__ void load(char* lds, int32_t w, bool past) const {
+        const uint64_t from = (uint64_t)(base + w * plane);
         // uniform, which the compiler must see
         const int lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)from);
         const int hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(from >> 32));
-        const int records = __builtin_amdgcn_readfirstlane(left < 0x7FFFFFFF ? (left > 0 ? (int)left : 0) : 0x7FFFFFFF);
+        const int records = __builtin_amdgcn_readfirstlane(past ? 0 : (int)bytes);
         u32x4 rsrc;
         rsrc[0] = (uint32_t)lo;
         rsrc[1] = (uint32_t)hi & 0xFFFFu;
@@ -169,9 +178,9 @@ __device__ __forceinline__ void fp8_workgroup(const Fp8Args& q, const Epi& epi, 
     ScaleCopy sc;
     const int part = wave & (kScaleWaves - 1);  // of the words; small tiles have more waves
     if (part < BM / 64)
-        sc.init(q.sa, q.sa_ld, q.sa_rows, q.a_shift, m0, part * 64 + lane);
+        sc.init(q.sa, m0, part * 64 + lane);
     else
-        sc.init(q.sb, q.sb_ld, q.sb_rows, q.b_shift, n0, (part - BM / 64) * 64 + lane);
+        sc.init(q.sb, n0, (part - BM / 64) * 64 + lane);
     Reader<uint8_t, true, BM, MB> ra;
     Reader<uint8_t, true, BN, NB> rb;
     ra.init(wm * MB * 16, lane);
@@ -198,7 +207,8 @@ __device__ __forceinline__ void fp8_workgroup(const Fp8Args& q, const Epi& epi, 
     static_assert(kInstr <= 4, "four are spelled out");
     auto copy_scales = [&](int32_t p, auto u) {
         if constexpr ((decltype(u)::v & 3) == 0)
-            sc.load(scales + __builtin_amdgcn_readfirstlane(((p >> 2) & 1) * kScales + part * 256), (k_lo >> 7) + p);
+            sc.load(scales + __builtin_amdgcn_readfirstlane(((p >> 2) & 1) * kScales + part * 256),
+                    (k_lo >> 9) + (p >> 2), p >= widths);
     };
     auto copy = [&](int32_t p, int at, auto u) {
         copy_scales(p, u);

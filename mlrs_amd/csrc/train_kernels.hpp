@@ -219,7 +219,8 @@ template <typename T>
 hipError_t launch_norm_grad(const NormCall& k, float* scratch, int cus, hipStream_t s);
 
 // Products in 8-bit floating point (train_fp8.hpp).  Codes: rows x fp8_columns(k),
-// scales fp8_scale_row(k) bytes for every row or, `tile`, for every 128.  f32 calls
+// scales fp8_scale_row(k) bytes for every row (words of four side by side) or,
+// `tile`, for every 128 (rows of words).  f32 calls
 // have the values as bf16 in the codes' place, without scales.
 struct Fp8Mat {
     const void* codes;
@@ -248,8 +249,12 @@ void choose_pair_fp8(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t
 template <typename T>
 hipError_t launch_fp8_linear(const Fp8Mat& x, const Fp8Mat& w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                              const Cut& cut, float* part, hipStream_t s);
-// The same for at most kFp8Few rows, from the rows themselves.
-constexpr int64_t kFp8Few = 32;
+// The same for at most 32 rows, from the rows themselves, and whether that is the
+// faster way: up to 16 rows always; more by 4096 x 8192 take 30 us, tiles 21; by 1024 x
+// 1024 9.5 and 13.
+inline bool fp8_few_rows(int64_t n, int64_t m, int64_t k) {
+    return n <= 16 || (n <= 32 && m * k <= (int64_t)1 << 23);
+}
 template <typename T>
 hipError_t launch_fp8_few(const T* x, const Fp8Mat& w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                           hipStream_t s);

@@ -171,15 +171,6 @@ __device__ __forceinline__ float mean_of(float sum, float count, float inv) {
 // ---------------------------------------------------------------------------
 // sums
 // ---------------------------------------------------------------------------
-template <int CTRL>
-__device__ __forceinline__ float from_lane(float v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    return __builtin_bit_cast(float,
-                              __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-#else
-    return v;
-#endif
-}
 __device__ __forceinline__ float other_rows(float v, bool halves) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const unsigned u = __float_as_uint(v);
@@ -204,10 +195,10 @@ template <int N>
 __device__ __forceinline__ void lane_sums(float (&v)[N], int lanes) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (lanes > 1) v[i] += from_lane<0xB1>(v[i]);
-        if (lanes > 2) v[i] += from_lane<0x4E>(v[i]);
-        if (lanes > 4) v[i] += from_lane<0x141>(v[i]);
-        if (lanes > 8) v[i] += from_lane<0x140>(v[i]);
+        if (lanes > 1) v[i] += from_lane<kNeighbour>(v[i]);
+        if (lanes > 2) v[i] += from_lane<kPair>(v[i]);
+        if (lanes > 4) v[i] += from_lane<kMirror8>(v[i]);
+        if (lanes > 8) v[i] += from_lane<kMirror16>(v[i]);
         if (lanes > 16) v[i] = other_rows(v[i], false);
         if (lanes > 32) v[i] = other_rows(v[i], true);
     }

@@ -60,6 +60,26 @@ __device__ __forceinline__ void store_oct(T* row, int64_t c, int64_t end, const 
     }
 }
 
+// Another lane's value, by a move within the vector unit: the neighbour's, that of the
+// other pair of four, that of the mirror image in eight or sixteen lanes.
+enum { kNeighbour = 0xB1, kPair = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140 };
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(float,
+                              __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+#else
+    return v;
+#endif
+}
+// The largest of sixteen adjacent lanes' values, in each of them.
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, from_lane<kNeighbour>(v));
+    v = fmaxf(v, from_lane<kPair>(v));
+    v = fmaxf(v, from_lane<kMirror8>(v));
+    return fmaxf(v, from_lane<kMirror16>(v));
+}
+
 typedef uint32_t RandomWords[4];
 
 __device__ __forceinline__ void random_block(uint64_t block, uint64_t offset, uint32_t k0, uint32_t k1,

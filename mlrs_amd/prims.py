@@ -962,7 +962,7 @@ def linear_fp8(x, w8, bias=None, activation="none", residual=None, keep_preact=F
     Products are exact.  float16 and bfloat16: the matrix instruction adds eight
     adjacent ones after cutting off what lies below 2^-13 of the largest one's power
     of two, all else in float32; float32 calls add up in float32, at half the rate.
-    The other arguments and the result are ``linear``'s.  Up to 32 rows take one
+    The other arguments and the result are ``linear``'s.  Up to 16 rows take one
     launch and no workspace."""
     s, n, d_in, d_out = _fp8_operands(x, w8, w8.codes, w8.scales, (bias, "bias"), (residual, "residual"))
     act = _activation_id(activation)

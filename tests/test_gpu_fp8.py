@@ -113,6 +113,13 @@ def test_linear_sizes(dtype, n, k, m):
     check_linear(n, k, m, dtype, "gelu", seed=n + k + m)
 
 
+# the rows from which weights of this size go in tiles, and the last before them
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [8, 16, 17, 31])
+def test_linear_few_rows_of_large_weights(dtype, n):
+    check_linear(n, 2100, 4100, dtype, "silu", seed=n)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bias,residual,keep", [(False, False, False), (True, False, True), (False, True, False)])
 @pytest.mark.parametrize("n", [9, 130])
