@@ -459,11 +459,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_pair_kernel(Fp8Pair<T> q) 
 }
 
 // The time of each choice, in microseconds, as of the 16-bit products: a staged width
-// (128 of k) of the one, two, ... tiles that a CU holds, and a round's other costs.
-constexpr double kStage8[3][3] = {{1.35}, {0.6, 0.95}, {0.3, 0.55, 0.8}};
-constexpr double kRound8[3] = {6.0, 4.5, 4.0};
+// (128 of k) of the one, two, ... tiles that a CU holds, a round's other costs, and the
+// join of split sums.  Measured over every tile and count of splits of 17 products from
+// 64 x 4096 x 8192 to 4096^3: the choice is the fastest or within 6 % of it, for a
+// gradient's two within 16 %, where others take up to 8 times as long.
+constexpr double kStage8[3][3] = {{1.31}, {0.67, 0.96}, {0.265, 0.43, 0.6}};
+constexpr double kRound8[3] = {6.0, 4.0, 3.4};
 constexpr int kResident8[3] = {1, 2, 3};
-double join_us(int64_t elements) { return elements ? 10.0 + (double)elements * 8.0 / 4.5e6 : 0.0; }
+double join_us(int64_t elements) { return elements ? 4.5 + (double)elements * 8.0 / 4.5e6 : 0.0; }
 
 }  // namespace
 
