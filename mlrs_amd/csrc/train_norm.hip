@@ -560,10 +560,12 @@ __device__ __forceinline__ void group_sums(const float (&v)[N][8], const SlabPla
         }
     } else {  // a wave to a group
         const int lane = t & 63, wave = t >> 6;
+        // as many slices side by side as the lanes have room for
+        const int wide = q.d < 64 ? q.d : 64, side = 64 / wide, first = lane / wide;
         for (int g = wave; g < q.groups; g += THREADS / 64) {
             float sum[N] = {};
-            for (int r = 0; r < q.slices; ++r)
-                for (int c = lane; c < q.d; c += 64)
+            for (int r = first < side ? first : q.slices; r < q.slices; r += side)
+                for (int c = lane - first * wide; c < q.d; c += 64)
 #pragma unroll
                     for (int i = 0; i < N; ++i)
                         sum[i] = __builtin_fmaf(lds[i * size + r * line + g * q.d + c], weight(g * q.d + c), sum[i]);
@@ -580,19 +582,45 @@ struct Nothing {
     __device__ __forceinline__ void operator()(int, const float (&)[N]) const {}
 };
 
+// What was made of these elements is made again from here on: 16-bit ones would be
+// kept as f32 besides, in twice the registers.
+template <typename T, int M>
+__device__ __forceinline__ void forget(Oct<T> (&v)[M]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            u32x4 w = __builtin_bit_cast(u32x4, v[i]);
+            asm volatile("" : "+v"(w));
+            v[i] = __builtin_bit_cast(Oct<T>, w);
+        }
+    }
+}
+
+// The workgroup's slab and sample: adjacent slabs, which have lines of memory in
+// common, in one chiplet (workgroups go to the eight in turn).
+__device__ __forceinline__ void slab_of(int32_t& slab, int64_t& sample) {
+    const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x, each = gridDim.x * gridDim.y / 8;
+    const uint32_t to = id < each * 8 ? (id & 7) * each + (id >> 3) : id;
+    sample = to / gridDim.x;
+    slab = (int32_t)(to - (uint32_t)sample * gridDim.x);
+}
+
 template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[THREADS * 8];
     __shared__ float means[kSlabGroups], rstds[kSlabGroups];
     const uint64_t offset = drop_offset(a.drop);
     const float count = (float)a.s * (float)a.d, inv = 1.0f / count;
-    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    int32_t slab;
+    int64_t place;
+    slab_of(slab, place);
+    const SlabPlace q = slab_place<THREADS>(a, p, slab);
     const int32_t c0 = 8 * q.oct;  // within the slab
     int32_t gi[8];
     each_group(q, [&](int e, int32_t g) { gi[e] = g; });
     float w[8], b[8];
     load_affine(a, q.c0 + c0, q.row >= 0 ? q.c0 + q.width : 0, w, b);
-    for (int64_t n = blockIdx.y; n < a.n; n += gridDim.y) {
+    for (int64_t n = place; n < a.n; n += gridDim.y) {
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> raw[M] = {};
         if (q.row >= 0) {
@@ -609,6 +637,7 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
             for (int e = 0; e < 8; ++e) v[0][e] += (float)raw[i][e];
         group_sums<1, THREADS>(v, p, q, lds, true, Nothing{}, weight_one,
                                [&](int g, const float (&sum)[1]) { means[g] = mean_of(sum[0], count, inv); });
+        forget<T>(raw);
         float mean[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -635,6 +664,7 @@ __global__ __launch_bounds__(THREADS) void norm_resident_kernel(NormOperands<T> 
             }
         });
         if (q.row < 0) continue;
+        forget<T>(raw);
         float rstd[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) rstd[e] = rstds[gi[e]];
@@ -657,17 +687,21 @@ __device__ __forceinline__ void slab_weights(const NormOperands<T>& a, const Sla
     for (int c = threadIdx.x; c < q.width; c += THREADS) lds[c] = a.w ? (float)a.w[q.c0 + c] : 1.0f;
 }
 
-// Workgroup (slab, place): samples place, place + across, ...
+// Workgroup (slab, place): samples place, place + across, ...  dz is kept for the second
+// use of the elements where there are registers for it.
 template <typename T, int M, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperands<T> a, SlabPlan p) {
     __shared__ __attribute__((aligned(16))) float lds[2 * THREADS * 8];
     __shared__ float totals[2 * THREADS * 8];  // of the channels' slices, each its thread's own
     __shared__ float weights[THREADS * 8], m1s[kSlabGroups], m2s[kSlabGroups];
     constexpr int kSize = THREADS * 8;
-    const int64_t place = blockIdx.y;
+    constexpr bool kKeep = M <= 4;
+    int32_t slab;
+    int64_t place;
+    slab_of(slab, place);
     const uint64_t offset = drop_offset(a.drop);
     const float inv = 1.0f / ((float)a.s * (float)a.d);
-    const SlabPlace q = slab_place<THREADS>(a, p, (int32_t)blockIdx.x);
+    const SlabPlace q = slab_place<THREADS>(a, p, slab);
     const int32_t c0 = 8 * q.oct;
     slab_weights<THREADS>(a, q, weights);
     for (int i = threadIdx.x; i < 2 * kSize; i += THREADS) totals[i] = 0.0f;
@@ -678,7 +712,7 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
     for (int64_t n = place; n < a.n; n += p.across) {
         const int64_t base = n * a.s * a.c + q.c0;
         Oct<T> rx[M] = {}, rd[M] = {};
-        float mean[8], rstd[8];
+        float mean[8], rstd[8], dz[kKeep ? M : 1][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int64_t at = n * a.g + q.g0 + gi[e];
@@ -710,6 +744,7 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
                 for (int e = 0; e < 8; ++e) {
                     v[0][e] += t[e];
                     v[1][e] = __builtin_fmaf(t[e], xh[e], v[1][e]);
+                    if constexpr (kKeep) dz[i][e] = t[e];
                 }
             }
         }
@@ -725,6 +760,8 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
                 m2s[g] = sum[1] * inv;
             });
         if (!a.y || q.row < 0) continue;
+        forget<T>(rx);
+        if constexpr (!kKeep) forget<T>(rd);
         float m1[8], m2[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -739,9 +776,9 @@ __global__ __launch_bounds__(THREADS) void norm_resident_grad_kernel(NormOperand
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 xh[e] = ((float)rx[i][e] - mean[e]) * rstd[e];
-                t[e] = (float)rd[i][e];
+                t[e] = kKeep ? dz[kKeep ? i : 0][e] : (float)rd[i][e];
             }
-            backward_oct(a, offset, base + pos * a.c + c0, w, b, xh, t);
+            if constexpr (!kKeep) backward_oct(a, offset, base + pos * a.c + c0, w, b, xh, t);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 t[e] = rstd[e] * (t[e] * w[e] - __builtin_fmaf(xh[e], m2[e], m1[e]));
@@ -1107,6 +1144,9 @@ struct Way {
     int64_t parts;  // rows of the parameters' partial sums
 };
 
+// Positions of a thread of 512, as many as spill no registers.
+constexpr int most_positions(int elem_bytes, bool grad) { return !grad ? 12 : elem_bytes == 4 ? 6 : 11; }
+
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad, int cus) {
@@ -1138,7 +1178,7 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.parts = o.row.passes;
         return o;
     }
-    // the slab: whole groups, as few as make a line of memory
+    // the slab: whole groups, as few as make a line of memory, or half of one
     auto slab = [&](int threads, int64_t groups) {
         SlabPlan p{};
         p.groups = (int32_t)groups;
@@ -1147,15 +1187,29 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         p.slabs = (int32_t)ceil_div(g, groups);
         return p;
     };
-    const int64_t line = std::min<int64_t>(g, std::max<int64_t>(1, ceil_div(128 / elem_bytes, d)));
-    const int most = elem_bytes == 4 && grad ? 4 : 8;
-    for (int threads : {256, 512}) {
-        const SlabPlan p = slab(threads, std::min<int64_t>(line, kSlabGroups));
-        if (p.octs > threads || ceil_div(s, p.rows) > most) continue;
+    auto bytes = [&](int64_t line) {
+        return std::min<int64_t>({g, kSlabGroups, std::max<int64_t>(1, ceil_div(line / elem_bytes, d))});
+    };
+    const int most = most_positions(elem_bytes, grad), middle = elem_bytes == 4 && grad ? 4 : 8;
+    // Slabs of half a line, and as many positions as there are registers for, leave a CU
+    // one workgroup at a time, whose loads, sums and stores follow one another: they are
+    // taken where no CU gets a second one, whole octs first.  16 samples of 1024 positions
+    // of 640 bf16 channels in 32 groups take 17.6 us so and 28.9 backwards, split 27.8
+    // and 46.6; 64 samples 62 and 111, split 53 and 86; 16 of 600 positions of 320, slabs
+    // of 70 channels, 21.8 and 38.5, split 18.2 and 24.
+    struct { int threads, line, most; } tries[] = {
+        {256, 128, middle}, {512, 128, middle}, {512, 64, most}, {512, 128, most}, {512, 64, middle}};
+    for (int i = 0; i < 5; ++i) {
+        const auto& t = tries[i];
+        const int threads = t.threads;
+        const SlabPlan p = slab(threads, bytes(t.line));
+        if (p.octs > threads || ceil_div(s, p.rows) > t.most) continue;
+        if (i >= 2 && n * p.slabs > cus) continue;
+        if ((i == 2 || i == 3) && p.groups * d % 8) continue;
         o.kind = Way::kResident;
         o.threads = threads;
         const int64_t m = ceil_div(s, p.rows);
-        o.m = m <= 2 ? 2 : m <= 4 ? 4 : 8;
+        o.m = m <= 2 ? 2 : m <= 4 ? 4 : m <= middle ? middle : most;
         o.slab = p;
         const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 256 ? 4 : 2) / p.slabs);
         o.slab.across = grad ? ceil_div(n, ceil_div(n, std::min<int64_t>({n, side, 65535}))) : n;
@@ -1222,6 +1276,7 @@ hipError_t launch_resident(const NormOperands<T>& a, const Way& o, hipStream_t s
         MLRS_SLAB(8, 256)
         MLRS_SLAB(8, 512)
     }
+    MLRS_SLAB(most_positions((int)sizeof(T), GRAD), 512)
 #undef MLRS_SLAB
     return hipErrorInvalidValue;
 }

@@ -172,6 +172,17 @@ def test_norm_slabs(dtype, shape, groups, p):
     check_norm(shape, groups, dtype, "gelu", p=p, seed=shape[0] + shape[-1])
 
 
+# half a line of memory at many positions: as many as a thread has registers for, and
+# one more; a last slab of fewer groups; as many samples as there is room for, and more
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [
+    ((3, 1000, 100), 5), ((2, 1122, 40), 2), ((2, 1123, 40), 2), ((1, 1225, 64), 4), ((2, 1500, 64), 4),
+    ((2, 1537, 64), 4), ((1, 700, 200), 4), ((90, 700, 120), 6), ((80, 600, 96), 6),
+])
+def test_norm_slabs_of_many_positions(dtype, shape, groups):
+    check_norm(shape, groups, dtype, "silu", p=0.2, seed=shape[0] + shape[-1])
+
+
 # groups larger than a workgroup holds
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape,groups", [
