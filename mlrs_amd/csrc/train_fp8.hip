@@ -1,5 +1,6 @@
 // A layer in 8-bit floating point: making the codes, and its three products.
 #include <cmath>
+#include <type_traits>
 
 #include "train_fp8.hpp"
 #include "train_random.hpp"
@@ -403,10 +404,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(const T* __rest
 // ---------------------------------------------------------------------------
 // the products
 // ---------------------------------------------------------------------------
-int64_t fp8_args(Fp8Args& q, int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int64_t n, int64_t k, int splits,
-                 int32_t k_split) {
+int64_t product_args(GemmArgs& g, int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int64_t n, int64_t k,
+                     int splits, int32_t k_split) {
     const int64_t kp = fp8_columns(k);
-    const int64_t blocks = gemm_args(q.g, tile, Mat{a.codes, kp}, Mat{b.codes, kp}, m, n, kp, splits, k_split, Only{});
+    return gemm_args(g, tile, Mat{a.codes, kp}, Mat{b.codes, kp}, m, n, kp, splits, k_split, Only{});
+}
+int64_t product_args(Fp8Args& q, int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int64_t n, int64_t k,
+                     int splits, int32_t k_split) {
+    const int64_t blocks = product_args(q.g, tile, a, b, m, n, k, splits, k_split);
     auto where = [&](const Fp8Mat& x, int64_t rows) {
         return x.tile ? ScaleRows{x.scales, fp8_scale_row(k), 4, (rows + 127) / 128, 7}
                       : ScaleRows{x.scales, 4, 4 * rows, rows, 0};
@@ -426,7 +431,7 @@ hipError_t launch_fp8(int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int
         return launch_gemm<__bf16>(tile, Mat{a.codes, kp}, Mat{b.codes, kp}, m, n, kp, splits, k_split, Only{}, epi, s);
     } else {
         Fp8Args q;
-        const int64_t blocks = fp8_args(q, tile, a, b, m, n, k, splits, k_split);
+        const int64_t blocks = product_args(q, tile, a, b, m, n, k, splits, k_split);
         if (!launchable(blocks, kTileThreads[tile])) return hipErrorInvalidConfiguration;  // the caller has checked
         const dim3 grid((unsigned)blocks);
         if (tile == 0)
@@ -439,23 +444,28 @@ hipError_t launch_fp8(int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int
     }
 }
 
-// The two products of a gradient in one grid, as train_linear.hip's.
+// The two products of a gradient in one grid, as train_linear.hip's: of codes, or in
+// f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 45 us, in a launch each 58.
 template <typename T>
 struct Fp8Pair {
-    Fp8Args x, w;
+    std::conditional_t<sizeof(T) == 4, GemmArgs, Fp8Args> x, w;
     StoreEpi<T> to_x, to_w;
     int32_t x_wgs, w_wgs;
     bool x_first;  // the one with the longer workgroups
 };
 template <typename T, int WM, int WN, int MB, int NB>
 __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_pair_kernel(Fp8Pair<T> q) {
-    __shared__ __attribute__((aligned(1024))) char buf[fp8_lds<WM, WN, MB, NB>()];
+    constexpr int kLds = sizeof(T) == 4 ? gemm_lds<WM, MB, NB>() : fp8_lds<WM, WN, MB, NB>();
+    __shared__ __attribute__((aligned(1024))) char buf[kLds];
     int32_t wg = blockIdx.x;
     const int32_t lead = q.x_first ? q.x_wgs : q.w_wgs;
     const bool second = wg >= lead;
     if (second) wg -= lead;
     const bool is_x = second != q.x_first;
-    fp8_workgroup<WM, WN, MB, NB>(is_x ? q.x : q.w, is_x ? q.to_x : q.to_w, wg, buf);
+    if constexpr (sizeof(T) == 4)
+        gemm_workgroup<__bf16, true, true, WM, WN, MB, NB, StoreEpi<T>>(is_x ? q.x : q.w, is_x ? q.to_x : q.to_w, wg, buf);
+    else
+        fp8_workgroup<WM, WN, MB, NB>(is_x ? q.x : q.w, is_x ? q.to_x : q.to_w, wg, buf);
 }
 
 // The time of each choice, in microseconds, as of the 16-bit products: a staged width
@@ -497,6 +507,12 @@ Cut choose_cut_fp8(int elem_bytes, int64_t m, int64_t n, int64_t k, int cus, int
 
 // Both products of a gradient: in tiles of one size, so that one grid holds them.
 void choose_pair_fp8(int elem_bytes, int64_t xm, int64_t xn, int64_t xk, int64_t wm, int64_t wn, int64_t wk, int cus, Cut* x, Cut* w) {
+    if (elem_bytes == 4) {
+        const PairCut p = choose_pair(2, xm, xn, fp8_columns(xk), wm, wn, fp8_columns(wk), cus, false);
+        *x = p.x;
+        *w = p.w;
+        return;
+    }
     double best = 1e300;
     for (int t = 0; t < 3; ++t) {
         const Cut cx = choose_cut_fp8(elem_bytes, xm, xn, xk, cus, t), cw = choose_cut_fp8(elem_bytes, wm, wn, wk, cus, t);
@@ -571,17 +587,23 @@ hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const C
     const Fp8Product* ps[2] = {&x, &w};
     const Cut* cs[2] = {&cx, &cw};
     float* parts[2] = {part, part + (x.m ? cx.part_bytes(x.m, x.n) / 4 : 0)};
-    if (sizeof(T) == 2 && x.m && w.m && cx.tile == cw.tile) {
+    if (x.m && w.m && cx.tile == cw.tile) {
         Fp8Pair<T> q;
-        Fp8Args* args[2] = {&q.x, &q.w};
+        decltype(q.x)* args[2] = {&q.x, &q.w};
         StoreEpi<T>* to[2] = {&q.to_x, &q.to_w};
         int32_t* wgs[2] = {&q.x_wgs, &q.w_wgs};
         for (int i = 0; i < 2; ++i) {
             const Fp8Product& p = *ps[i];
-            *wgs[i] = (int32_t)fp8_args(*args[i], cs[i]->tile, p.a, p.b, p.m, p.n, p.k, cs[i]->splits, cs[i]->k_split);
+            *wgs[i] = (int32_t)product_args(*args[i], cs[i]->tile, p.a, p.b, p.m, p.n, p.k, cs[i]->splits, cs[i]->k_split);
             *to[i] = cs[i]->splits > 1 ? parts_epi<T>(parts[i], p.m, p.n) : store_epi<T>(p.to);
         }
-        q.x_first = q.x.g.k_split >= q.w.g.k_split;
+        auto each = [](const auto& a) {
+            if constexpr (sizeof(T) == 4)
+                return a.k_split;
+            else
+                return a.g.k_split;
+        };
+        q.x_first = each(q.x) >= each(q.w);
         const int64_t blocks = (int64_t)q.x_wgs + q.w_wgs;
         if (!launchable(blocks, kTileThreads[cx.tile])) return hipErrorInvalidConfiguration;  // the caller has checked
         const dim3 grid((unsigned)blocks);
