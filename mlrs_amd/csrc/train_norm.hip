@@ -1197,21 +1197,36 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
     // of 640 bf16 channels in 32 groups take 17.6 us so and 28.9 backwards, split 27.8
     // and 46.6; 64 samples 62 and 111, split 53 and 86; 16 of 600 positions of 320, slabs
     // of 70 channels, 21.8 and 38.5, split 18.2 and 24.
+    // A wave alone takes a row of channels that it can hold.  Where few positions would
+    // leave most of 256 threads without work, a slab has more groups, as long as every
+    // CU has four: 2499 samples of 5 positions of 2025 f16 channels in 27 groups take 266
+    // us, there and back, in slabs of a line 1015; 3302 of 4 of 18, a wave each, 34, 72.
+    auto wide = [&](int64_t groups) {
+        const int64_t line = groups;
+        for (int64_t more = 2 * groups;; more *= 2) {
+            more = std::min<int64_t>({more, g, kSlabGroups});
+            const SlabPlan p = slab(256, more);
+            if (more == groups || p.octs > 256 || ceil_div(s, p.rows) > 4 || n * p.slabs < 4 * (int64_t)cus) break;
+            groups = more;
+        }
+        return groups == line ? line : ceil_div(g, ceil_div(g, groups));  // all slabs alike
+    };
     struct { int threads, line, most; } tries[] = {
-        {256, 128, middle}, {512, 128, middle}, {512, 64, most}, {512, 128, most}, {512, 64, middle}};
-    for (int i = 0; i < 5; ++i) {
+        {64, 0, 2}, {256, 128, middle}, {512, 128, middle}, {512, 64, most}, {512, 128, most}, {512, 64, middle}};
+    for (int i = 0; i < 6; ++i) {
         const auto& t = tries[i];
         const int threads = t.threads;
-        const SlabPlan p = slab(threads, bytes(t.line));
+        const SlabPlan p = slab(threads, i == 0 ? std::min<int64_t>(g, kSlabGroups) : i == 1 ? wide(bytes(128)) : bytes(t.line));
         if (p.octs > threads || ceil_div(s, p.rows) > t.most) continue;
-        if (i >= 2 && n * p.slabs > cus) continue;
-        if ((i == 2 || i == 3) && p.groups * d % 8) continue;
+        if (i == 0 && p.slabs > 1) continue;
+        if (i >= 3 && n * p.slabs > cus) continue;
+        if ((i == 3 || i == 4) && p.groups * d % 8) continue;
         o.kind = Way::kResident;
         o.threads = threads;
         const int64_t m = ceil_div(s, p.rows);
         o.m = m <= 2 ? 2 : m <= 4 ? 4 : m <= middle ? middle : most;
         o.slab = p;
-        const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 256 ? 4 : 2) / p.slabs);
+        const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 64 ? 8 : threads == 256 ? 4 : 2) / p.slabs);
         o.slab.across = grad ? ceil_div(n, ceil_div(n, std::min<int64_t>({n, side, 65535}))) : n;
         o.side = std::min<int64_t>(grad ? o.slab.across : n, 65535);
         o.parts = o.slab.across;
@@ -1268,6 +1283,7 @@ hipError_t launch_resident(const NormOperands<T>& a, const Way& o, hipStream_t s
         else                                                             \
             return go(norm_resident_kernel<T, M, THREADS>);              \
     }
+    MLRS_SLAB(2, 64)
     MLRS_SLAB(2, 256)
     MLRS_SLAB(4, 256)
     MLRS_SLAB(2, 512)

@@ -183,6 +183,16 @@ def test_norm_slabs_of_many_positions(dtype, shape, groups):
     check_norm(shape, groups, dtype, "silu", p=0.2, seed=shape[0] + shape[-1])
 
 
+# few positions: a wave to a sample, slabs of many groups, more samples than workgroups
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [
+    ((3000, 4, 18), 6), ((70000, 2, 8), 4), ((1300, 5, 1025), 41), ((2100, 3, 300), 300), ((600, 9, 777), 7),
+    ((40, 8, 128), 16), ((40, 9, 128), 16), ((5, 64, 8), 1),
+])
+def test_norm_slabs_of_few_positions(dtype, shape, groups):
+    check_norm(shape, groups, dtype, "gelu", p=0.2, seed=shape[0] + shape[-1])
+
+
 # groups larger than a workgroup holds
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape,groups", [
