@@ -584,10 +584,10 @@ int32_t mlrs_softmax_xent_grad_bf16(const uint16_t *h, int64_t h_len, int64_t n,
 /*
  * ---- the rest of an encoder's layer ----
  * Dropout, group norm with an activation and dropout, and the layer in 8-bit
- * floating point.  Element types,
- * overlaps and errors as above.  No call here synchronizes or reads back.  A call
- * that takes no workspace can be captured into a graph and replayed; one that
- * does is refused there (MLRS_ERR_UNSUPPORTED "stream").
+ * floating point.  Element types, overlaps and errors as above.  No call here
+ * synchronizes or reads back.  A call that takes no workspace can be captured into
+ * a graph and replayed; one that does is refused there (MLRS_ERR_UNSUPPORTED
+ * "stream").
  *
  * Random bits come from a counter: element i of the tensor takes 16 bits of
  * Philox 4x32 with seven rounds (Salmon et al., SC 2011), key `seed`, counter

@@ -66,11 +66,12 @@ __device__ __forceinline__ bool unbounded(float x) { return fabsf(x) == __builti
 // ---------------------------------------------------------------------------
 // A workgroup takes 128 x 128 elements, a thread four by eight of them: rows 4 (t /
 // 16) on and columns 8 (t % 16) on, so that it has eight adjacent codes of a row and
-// four of a column (eight by eight take 210 registers and the same time: 136 to 152 us
-// for the 535 MB of a gradient of 8192 x 8192 and its x of 8192 x 4096, 3.5 to 3.9
-// TB/s).  Bound by memory.  The elements are read once, whatever is made of them: codes with a scale for each row, codes of the transpose
-// with a scale for each column (turned through LDS), or both with one scale for the
-// tile; and column sums.  Infinities and NaN have code NaN and no part in the scale.
+// four of a column (eight by eight take 210 registers and the same time).  Bound by
+// memory: the codes of 8192 x 8192 with act'(z) and of x of 8192 x 4096, 535 MB in bf16,
+// take 127 to 152 us, 3.5 to 4.2 TB/s.  The elements are read once, whatever is made of
+// them: codes with a scale for each row, codes of the transpose with a scale for each
+// column (turned through LDS), or both with one scale for the tile; and column sums.
+// Infinities and NaN have code NaN and no part in the scale.
 // VALUES: bf16 values and no scales in the codes' place.
 template <typename T>
 struct CodeJob {
@@ -445,7 +446,7 @@ hipError_t launch_fp8(int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int
 }
 
 // The two products of a gradient in one grid, as train_linear.hip's: of codes, or in
-// f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 45 us, in a launch each 58.
+// f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 38 us, in a launch each 58.
 template <typename T>
 struct Fp8Pair {
     std::conditional_t<sizeof(T) == 4, GemmArgs, Fp8Args> x, w;
