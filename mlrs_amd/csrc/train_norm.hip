@@ -1182,6 +1182,10 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.parts = o.row.passes;
         return o;
     }
+    // samples side by side, each in `blocks` workgroups: a launch has fewer than 2^32 threads
+    auto beside = [&](int64_t blocks, int threads) {
+        return std::max<int64_t>(1, std::min<int64_t>({n, 65535, ((int64_t)1 << 31) / (blocks * threads)}));
+    };
     // the slab: whole groups, as few as make a line of memory, or half of one
     auto slab = [&](int threads, int64_t groups) {
         SlabPlan p{};
@@ -1232,7 +1236,7 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.slab = p;
         const int64_t side = std::max<int64_t>(1, (int64_t)cus * (threads == 64 ? 8 : threads == 256 ? 4 : 2) / p.slabs);
         o.slab.across = grad ? ceil_div(n, ceil_div(n, std::min<int64_t>({n, side, 65535}))) : n;
-        o.side = std::min<int64_t>(grad ? o.slab.across : n, 65535);
+        o.side = grad ? o.slab.across : beside(p.slabs, threads);
         o.parts = o.slab.across;
         return o;
     }
@@ -1245,7 +1249,7 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
     const int64_t rows = std::max<int64_t>(ceil_div(s, std::max<int64_t>(1, want)), 4 * (int64_t)o.slab.rows);
     o.slab.run = std::min(rows, s);
     o.slab.across = ceil_div(s, o.slab.run);
-    o.side = std::min<int64_t>(n, 65535);
+    o.side = beside(o.slab.slabs * o.slab.across, o.threads);
     o.parts = n * o.slab.across;
     return o;
 }
