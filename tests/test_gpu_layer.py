@@ -153,7 +153,7 @@ def test_norm_activations(dtype, act):
 @pytest.mark.parametrize("n,c,groups", [
     (1, 8, 1), (1, 4, 2), (5, 30, 5), (3, 1000, 1), (7, 2000, 1), (6, 2500, 1), (4, 4100, 1), (2, 8192, 1),
     (3, 16384, 2), (1000, 64, 8), (333, 14, 7), (17, 130, 13), (2, 1024, 128), (5000, 24, 3), (9, 520, 8),
-    (300, 4104, 1), (1, 1024, 8),
+    (300, 4104, 1), (1, 1024, 8), (6000, 39, 3), (2, 16, 2), (401, 16, 1),
 ])
 @pytest.mark.parametrize("p", [0.0, 0.3])
 def test_norm_rows(dtype, n, c, groups, p):
