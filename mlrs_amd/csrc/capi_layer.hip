@@ -375,7 +375,6 @@ int32_t linear_fp8_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_
         const Fp8Mat dz{zc, zs, false}, dz_t{zct, zst, false}, x_t{xct, xst, false};
         MLRS_TRY(launch_fp8_grad_codes<T>(dy, act == MLRS_ACT_NONE ? nullptr : z, act, n, m, dz, dz_t, sums,
                                           dw ? x : nullptr, k, x_t, s));
-        if (db) MLRS_TRY(launch_sum_parts<T>(ColumnSums<T>{db, sums, (int)runs, nullptr}, m, s));
         const Fp8Mat wt{codes_t, scales_t, true};
         if (kValues && dx) MLRS_TRY(launch_fp8_values(wt, k, m, wv, s));
         capi::Timed timed(s, "linear_fp8_grad");
@@ -383,7 +382,7 @@ int32_t linear_fp8_grad_impl(const T* dy, int64_t dy_len, const T* x, int64_t x_
         Fp8Product pw{x_t, dz_t, k, m, n, StoreTo{dw, k, nullptr, nullptr, 0, nullptr}};
         if (!dx) px.m = 0;
         if (!dw) pw.m = 0;
-        MLRS_TRY(launch_fp8_products<T>(px, pw, cx, cw, part, s));
+        MLRS_TRY(launch_fp8_products<T>(px, pw, cx, cw, part, ColumnSums<T>{db, sums, (int)runs, nullptr}, m, s));
         return MLRS_OK;
     });
 }

@@ -445,14 +445,17 @@ hipError_t launch_fp8(int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int
     }
 }
 
-// The two products of a gradient in one grid, as train_linear.hip's: of codes, or in
-// f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 38 us, in a launch each 58.
+// The two products of a gradient in one grid, as train_linear.hip's, with the column
+// sums' last step: of codes, or in f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 37 us, in a launch
+// each and one for the sums 62.
 template <typename T>
 struct Fp8Pair {
     std::conditional_t<sizeof(T) == 4, GemmArgs, Fp8Args> x, w;
     StoreEpi<T> to_x, to_w;
     int32_t x_wgs, w_wgs;
     bool x_first;  // the one with the longer workgroups
+    ColumnSums<T> sums;
+    int64_t columns;
 };
 template <typename T, int WM, int WN, int MB, int NB>
 __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_pair_kernel(Fp8Pair<T> q) {
@@ -460,6 +463,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void fp8_pair_kernel(Fp8Pair<T> q) 
     __shared__ __attribute__((aligned(1024))) char buf[kLds];
     int32_t wg = blockIdx.x;
     const int32_t lead = q.x_first ? q.x_wgs : q.w_wgs;
+    if (wg >= q.x_wgs + q.w_wgs) {
+        sum_parts<T, WM * WN * 64>(q.sums, q.columns, wg - q.x_wgs - q.w_wgs, reinterpret_cast<float*>(buf));
+        return;
+    }
     const bool second = wg >= lead;
     if (second) wg -= lead;
     const bool is_x = second != q.x_first;
@@ -584,7 +591,7 @@ hipError_t launch_fp8_few(const T* x, const Fp8Mat& w, int64_t n, int64_t m, int
 
 template <typename T>
 hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const Cut& cx, const Cut& cw, float* part,
-                               hipStream_t s) {
+                               const ColumnSums<T>& sums, int64_t columns, hipStream_t s) {
     const Fp8Product* ps[2] = {&x, &w};
     const Cut* cs[2] = {&cx, &cw};
     float* parts[2] = {part, part + (x.m ? cx.part_bytes(x.m, x.n) / 4 : 0)};
@@ -605,7 +612,14 @@ hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const C
                 return a.g.k_split;
         };
         q.x_first = each(q.x) >= each(q.w);
-        const int64_t blocks = (int64_t)q.x_wgs + q.w_wgs;
+        int64_t blocks = (int64_t)q.x_wgs + q.w_wgs + (sums.out ? (columns + 15) / 16 : 0);
+        q.sums = sums;
+        q.columns = columns;
+        if (sums.out && !launchable(blocks, kTileThreads[cx.tile])) {
+            const hipError_t e = launch_sum_parts(sums, columns, s);
+            if (e != hipSuccess) return e;
+            blocks = (int64_t)q.x_wgs + q.w_wgs;
+        }
         if (!launchable(blocks, kTileThreads[cx.tile])) return hipErrorInvalidConfiguration;  // the caller has checked
         const dim3 grid((unsigned)blocks);
         if (cx.tile == 0)
@@ -617,6 +631,8 @@ hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const C
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     } else {
+        const hipError_t r = launch_sum_parts(sums, columns, s);
+        if (r != hipSuccess) return r;
         for (int i = 0; i < 2; ++i) {
             const Fp8Product& p = *ps[i];
             if (!p.m) continue;
@@ -642,7 +658,7 @@ hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const C
     template hipError_t launch_fp8_few<T>(const T*, const Fp8Mat&, int64_t, int64_t, int64_t, const LinearOut&,     \
                                           hipStream_t);                                                             \
     template hipError_t launch_fp8_products<T>(const Fp8Product&, const Fp8Product&, const Cut&, const Cut&, float*, \
-                                               hipStream_t);
+                                               const ColumnSums<T>&, int64_t, hipStream_t);
 MLRS_INST(float)
 MLRS_INST(_Float16)
 MLRS_INST(__bf16)

@@ -259,6 +259,7 @@ template <typename T>
 hipError_t launch_fp8_few(const T* x, const Fp8Mat& w, int64_t n, int64_t m, int64_t k, const LinearOut& o,
                           hipStream_t s);
 // The two products of a gradient, both operands with k contiguous; m = 0: not wanted.
+// The column sums' last step goes with them.
 struct Fp8Product {
     Fp8Mat a, b;
     int64_t m, n, k;
@@ -266,7 +267,7 @@ struct Fp8Product {
 };
 template <typename T>
 hipError_t launch_fp8_products(const Fp8Product& x, const Fp8Product& w, const Cut& cx, const Cut& cw, float* part,
-                               hipStream_t s);
+                               const ColumnSums<T>& sums, int64_t columns, hipStream_t s);
 
 // Optimizer.
 int64_t norm_parts(const mlrs_grad_tensor* t, int64_t count);

@@ -335,24 +335,6 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
     }
 }
 
-// A workgroup joins the parts of 16 columns: a sixteenth of its threads each
-// takes every so-manieth part of a column, then one of them joins theirs in order.
-template <typename T, int THREADS>
-__device__ __forceinline__ void sum_parts(const ColumnSums<T>& to, int64_t m, int32_t wg, float* join) {
-    constexpr int kSlices = THREADS / 16;
-    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const int64_t c = (int64_t)wg * 16 + col;
-    float v = 0.0f;
-    if (c < m)
-        for (int p = slice; p < to.parts; p += kSlices) v += to.sums[(int64_t)p * m + c];
-    join[threadIdx.x] = v;
-    __syncthreads();
-    if (slice != 0 || c >= m) return;
-#pragma unroll
-    for (int i = 1; i < kSlices; ++i) v += join[i * 16 + col];
-    if (to.alpha) v *= down_factor<T>(to.alpha);
-    to.out[c] = (T)v;
-}
 template <typename T>
 __global__ __launch_bounds__(256) void sum_parts_kernel(ColumnSums<T> to, int64_t m) {
     __shared__ float join[256];
