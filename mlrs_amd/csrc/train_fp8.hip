@@ -446,8 +446,8 @@ hipError_t launch_fp8(int tile, const Fp8Mat& a, const Fp8Mat& b, int64_t m, int
 }
 
 // The two products of a gradient in one grid, as train_linear.hip's, with the column
-// sums' last step: of codes, or in f32 of values.  Of 3001 x 2050 by 1000 in f32 they take 37 us, in a launch
-// each and one for the sums 62.
+// sums' last step: of codes, or in f32 of values.  Of 3001 x 2050 by 1000 in f32 they
+// take 37 us, in a launch each and one for the sums 62.
 template <typename T>
 struct Fp8Pair {
     std::conditional_t<sizeof(T) == 4, GemmArgs, Fp8Args> x, w;
