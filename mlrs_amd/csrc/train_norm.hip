@@ -1245,13 +1245,17 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.parts = o.slab.across;
         return o;
     }
-    o.kind = Way::kSplit;  // four workgroups to a CU: a run's first and last steps cost as much as its rows
+    // As many workgroups as run at once, four to a CU, backwards three, and six positions to
+    // a thread at least: a run's first and last steps cost as much as its rows.  16 x 4096
+    // x 320 f16 in 32 groups backwards: 54 us, of four to a CU 58, of eight 78; forwards 36,
+    // 36 and 51.  4 x 4096 x 320: 22 us, with four positions 27.
+    o.kind = Way::kSplit;
     o.threads = octs <= 256 ? 256 : 1024;
     // as many whole groups as the threads have room for
     const int64_t groups = std::max<int64_t>(1, std::min<int64_t>({g, kSlabGroups, (int64_t)o.threads * 8 / d}));
     o.slab = slab(o.threads, groups);
-    const int64_t want = ceil_div((int64_t)cus * 4, n * o.slab.slabs);
-    const int64_t rows = std::max<int64_t>(ceil_div(s, std::max<int64_t>(1, want)), 4 * (int64_t)o.slab.rows);
+    const int64_t want = ceil_div((int64_t)cus * (grad ? 3 : 4), n * o.slab.slabs);
+    const int64_t rows = std::max<int64_t>(ceil_div(s, std::max<int64_t>(1, want)), 6 * (int64_t)o.slab.rows);
     o.slab.run = std::min(rows, s);
     o.slab.across = ceil_div(s, o.slab.run);
     o.side = beside(o.slab.slabs * o.slab.across, o.threads);
