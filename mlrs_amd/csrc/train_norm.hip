@@ -551,17 +551,17 @@ __device__ __forceinline__ void group_sums(const float (&v)[N][8], const SlabPla
     }
     if (!groups) return;
     __syncthreads();
-    if (q.slices * q.d <= 32) {  // a thread to a group
-        if (t < q.groups) {
+    if (q.slices * q.d <= 32) {  // a thread to a group; a wave alone may have more groups than threads
+        for (int g = t; g < q.groups; g += THREADS) {
             float sum[N] = {};
 #pragma unroll 1
-            for (int c = t * q.d; c < (t + 1) * q.d; ++c) {
+            for (int c = g * q.d; c < (g + 1) * q.d; ++c) {
                 const float by = weight(c);
                 for (int r = 0; r < q.slices; ++r)
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum[i] = __builtin_fmaf(lds[i * size + r * line + c], by, sum[i]);
             }
-            done(t, sum);
+            done(g, sum);
         }
     } else {  // a wave to a group
         const int lane = t & 63, wave = t >> 6;
