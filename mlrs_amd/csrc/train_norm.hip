@@ -165,6 +165,12 @@ __device__ __forceinline__ float inverse_root(float v) {
     const float better = y * __builtin_fmaf(-0.5f * v * y, y, 1.5f);
     return y < 1e18f && y > 1e-18f ? better : y;  // v y is out of range beyond, or v 0 or infinite
 }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+// Squares about a place, less what that place is off their mean: not negative, whatever
+// is rounded; infinite where they are past f32's range, and NaN where they are.
+__device__ __forceinline__ float squares_less(float squares, float less) {
+    return __builtin_elementwise_maximum(squares - (finite(less) ? less : 0.0f), 0.0f);
+}
 // sum / count, by its reciprocal and a step: the quotient rounded, so that the mean of
 // equal elements is theirs where their sum is exact.
 __device__ __forceinline__ float mean_of(float sum, float count, float inv) {
@@ -828,7 +834,12 @@ __global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<
             constexpr int U = sizeof(T) == 2 ? 8 : 4;
             const Oct<T> raw = load_oct(from, c0, q.width);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) first[e] = (float)raw[e];
+            for (int e = 0; e < 8; ++e) {  // differences from what is no number would be none
+                sum[e] = (float)raw[e];
+                first[e] = finite(sum[e]) ? sum[e] : 0.0f;
+                sum[e] -= first[e];
+                square[e] = fabsf(sum[e]);
+            }
             from += step;
             for (int32_t r = 1; r < rows; r += U, from += U * step) {
                 Oct<T> v[U];
@@ -853,7 +864,7 @@ __global__ __launch_bounds__(THREADS) void norm_split_stats_kernel(NormOperands<
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float m = sum[e] * by;
-            square[e] -= sum[e] * m;
+            square[e] = squares_less(square[e], sum[e] * m);
             first[e] += m;  // the channel's mean
             v[0][e] = first[e] * (float)rows;
         }
@@ -931,11 +942,12 @@ __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, 
     for (int64_t n = blockIdx.z; n < a.n; n += gridDim.z) {
         __syncthreads();
         // as a sum over the first run's mean: sum of n (m - m0), and of the squares
-        // about m0, from which what the mean is off m0 is taken
+        // about m0, from which what the mean is off m0 is taken; infinities and NaN go
+        // where the definition has them
         each_join(q, lanes, [&](int g, int li) {
             const float* f = part + 2 * (n * p.across * a.g + q.g0 + g);
             const int64_t next = 2 * a.g;
-            const float first = f[0];
+            const float first = finite(f[0]) ? f[0] : 0.0f;
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll 4
             for (int64_t r = li; r < p.across; r += lanes) {
@@ -946,7 +958,7 @@ __global__ __launch_bounds__(THREADS) void norm_split_kernel(NormOperands<T> a, 
             lane_sums(sum, lanes);
             if (li) return;
             const float beyond = sum[0] * inv, mean = first + beyond;
-            const float rstd = inverse_root(fmaxf(__builtin_fmaf(-beyond, beyond, sum[1] * inv), 0.0f) + a.eps);
+            const float rstd = inverse_root(squares_less(sum[1] * inv, beyond * beyond) + a.eps);
             means[g] = mean;
             rstds[g] = rstd;
             if (a.mean && run == 0) {
