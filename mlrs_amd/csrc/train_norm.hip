@@ -53,55 +53,42 @@ struct NormOperands {
 // what is done with an element
 // ---------------------------------------------------------------------------
 // gelu is z Phi(z) = max(z, 0) - |z| Phi(-|z|), and Phi(-u) = e^(-u^2/2) q(t) with t =
-// 1 / (1 + c u), as train_epilogue.hpp's: a polynomial fitted to the scaled
-// complementary error function for u in 0 .. 40.  f32: degree 9, relative error 3.8e-7
-// as it is computed; 16-bit types: degree 6, 1.1e-5, which is a fiftieth of f16's
-// rounding and saves three of some sixteen instructions an element, where these
-// kernels are bound by instructions.
-template <typename T>
+// 1 / (1 + 0.36 u), as train_epilogue.hpp's: a polynomial of degree 9 fitted to the
+// scaled complementary error function for u in 0 .. 40, relative error 3.8e-7 as it is
+// computed: a layer's gelu is as exact with a norm as without, in every type.  (Degree 6,
+// relative error 1.1e-5, saves 3 us of 106 of 16384 x 2048 bf16 there and back, but
+// rounds 65 of 38400 f16 slopes to the wrong side.)
 __device__ __forceinline__ float normal_tail(float u, float& bell) {
     bell = __builtin_amdgcn_exp2f(u * u * (-0.5f * kLog2E));
-    float q;
-    if constexpr (sizeof(T) == 4) {
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, u, 1.0f));
-        q = -0.030237516661021768f;
-        q = __builtin_fmaf(q, t, 0.13950534889597813f);
-        q = __builtin_fmaf(q, t, -0.22359445728159374f);
-        q = __builtin_fmaf(q, t, 0.10736457851476656f);
-        q = __builtin_fmaf(q, t, -0.00038397830051628453f);
-        q = __builtin_fmaf(q, t, 0.09603661840218482f);
-        q = __builtin_fmaf(q, t, 0.1240098852248856f);
-        q = __builtin_fmaf(q, t, 0.14368186910198438f);
-        q = __builtin_fmaf(q, t, 0.14361766520603944f);
-        return q * t * bell;
-    } else {
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.32f, u, 1.0f));
-        q = -0.06677426336821958f;
-        q = __builtin_fmaf(q, t, 0.13958546063672428f);
-        q = __builtin_fmaf(q, t, 0.04961394871763218f);
-        q = __builtin_fmaf(q, t, 0.12305164080264364f);
-        q = __builtin_fmaf(q, t, 0.12682801098738777f);
-        q = __builtin_fmaf(q, t, 0.1276897246494251f);
-        return q * t * bell;
-    }
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.36f, u, 1.0f));
+    float q = -0.030237516661021768f;
+    q = __builtin_fmaf(q, t, 0.13950534889597813f);
+    q = __builtin_fmaf(q, t, -0.22359445728159374f);
+    q = __builtin_fmaf(q, t, 0.10736457851476656f);
+    q = __builtin_fmaf(q, t, -0.00038397830051628453f);
+    q = __builtin_fmaf(q, t, 0.09603661840218482f);
+    q = __builtin_fmaf(q, t, 0.1240098852248856f);
+    q = __builtin_fmaf(q, t, 0.14368186910198438f);
+    q = __builtin_fmaf(q, t, 0.14361766520603944f);
+    return q * t * bell;
 }
 
-template <typename T, int ACT>
+template <int ACT>
 __device__ __forceinline__ float value_of(float z) {
     if constexpr (ACT == kActGelu) {
         float bell;
         const float u = __builtin_elementwise_minimum(fabsf(z), 1e18f);  // these two keep a NaN
-        const float tail = normal_tail<T>(u, bell);
+        const float tail = normal_tail(u, bell);
         return __builtin_fmaf(-u, tail, __builtin_elementwise_maximum(z, 0.0f));
     } else {
         return activate(z, ACT);
     }
 }
-template <typename T, int ACT>
+template <int ACT>
 __device__ __forceinline__ float slope_of(float z) {
     if constexpr (ACT == kActGelu) {
         float bell;
-        const float tail = normal_tail<T>(__builtin_elementwise_minimum(fabsf(z), 1e18f), bell);
+        const float tail = normal_tail(__builtin_elementwise_minimum(fabsf(z), 1e18f), bell);
         const float cdf = 0.5f + __builtin_copysignf(0.5f - tail, z);
         return __builtin_fmaf(z * (0.5f * kGeluC), bell, cdf);
     } else {
@@ -110,21 +97,19 @@ __device__ __forceinline__ float slope_of(float z) {
 }
 
 // One switch for eight elements: v = value(z), or v *= slope(z).
-template <typename T>
 __device__ __forceinline__ void values_of(int act, float (&v)[8]) {
     auto each = [&](auto f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
     };
     switch (act) {
-    case kActRelu: each([](float z) { return value_of<T, kActRelu>(z); }); break;
-    case kActGelu: each([](float z) { return value_of<T, kActGelu>(z); }); break;
-    case kActGeluTanh: each([](float z) { return value_of<T, kActGeluTanh>(z); }); break;
-    case kActSilu: each([](float z) { return value_of<T, kActSilu>(z); }); break;
+    case kActRelu: each([](float z) { return value_of<kActRelu>(z); }); break;
+    case kActGelu: each([](float z) { return value_of<kActGelu>(z); }); break;
+    case kActGeluTanh: each([](float z) { return value_of<kActGeluTanh>(z); }); break;
+    case kActSilu: each([](float z) { return value_of<kActSilu>(z); }); break;
     default: break;
     }
 }
-template <typename T>
 __device__ __forceinline__ void times_slopes(int act, const float (&xh)[8], const float (&w)[8], const float (&b)[8],
                                              float (&v)[8]) {
     auto each = [&](auto f) {
@@ -132,10 +117,10 @@ __device__ __forceinline__ void times_slopes(int act, const float (&xh)[8], cons
         for (int e = 0; e < 8; ++e) v[e] *= f(__builtin_fmaf(xh[e], w[e], b[e]));
     };
     switch (act) {
-    case kActRelu: each([](float z) { return slope_of<T, kActRelu>(z); }); break;
-    case kActGelu: each([](float z) { return slope_of<T, kActGelu>(z); }); break;
-    case kActGeluTanh: each([](float z) { return slope_of<T, kActGeluTanh>(z); }); break;
-    case kActSilu: each([](float z) { return slope_of<T, kActSilu>(z); }); break;
+    case kActRelu: each([](float z) { return slope_of<kActRelu>(z); }); break;
+    case kActGelu: each([](float z) { return slope_of<kActGelu>(z); }); break;
+    case kActGeluTanh: each([](float z) { return slope_of<kActGeluTanh>(z); }); break;
+    case kActSilu: each([](float z) { return slope_of<kActSilu>(z); }); break;
     default: break;
     }
 }
@@ -146,7 +131,7 @@ __device__ __forceinline__ void forward_oct(const NormOperands<T>& a, uint64_t o
                                             const float (&b)[8], float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(v[e], w[e], b[e]);
-    values_of<T>(a.act, v);
+    values_of(a.act, v);
     if (a.drop.threshold) drop_oct(a.drop, offset, i, a.aligned, v);
 }
 
@@ -156,7 +141,7 @@ __device__ __forceinline__ void backward_oct(const NormOperands<T>& a, uint64_t 
                                              const float (&w)[8], const float (&b)[8], const float (&xh)[8],
                                              float (&dy)[8]) {
     if (a.drop.threshold) drop_oct(a.drop, offset, i, a.aligned, dy);
-    times_slopes<T>(a.act, xh, w, b, dy);
+    times_slopes(a.act, xh, w, b, dy);
 }
 
 // 1 / sqrt(v): the hardware's, to one unit, and a step of Newton's.
