@@ -174,7 +174,10 @@ class EmbeddingEncoder:
 
     def _encode(self, x):
         layers = self._layers()
-        codes = self._weight_codes if self.products == "fp8" else [None] * len(layers)
+        # the fitted weights', or, of a fit that was interrupted, those of its weights
+        codes = self._weight_codes if self.products == "fp8" else None
+        if codes is None:
+            codes = self._codes(backward=False)
         for (w, b, norm, act, skip), w8 in zip(layers, codes):
             if norm is None:
                 x = self._product(x, w, w8, bias=b, activation=act, residual=x if skip else None)
@@ -244,16 +247,17 @@ class EmbeddingEncoder:
         if x.shape[0] == 0 or x.shape[1] == 0:
             raise ValueError("Found array with shape %s: at least one row and one feature are required"
                              % (tuple(x.shape),))
-        self.classes_, codes = np.unique(labels, return_inverse=True)
+        classes, codes = np.unique(labels, return_inverse=True)
         target = torch.from_numpy(np.ascontiguousarray(codes.reshape(-1), dtype=np.int64)).to(x.device)
         n, d = x.shape
         seed = 0 if self.random_state is None else int(self.random_state)
         gen = torch.Generator(device=x.device)
         gen.manual_seed(seed)
-        self.n_features_in_ = d
-        self._params = self._init_params(d, widths, len(self.classes_), x.device, gen)
-        optimizer = AdamW(self._params, lr=float(self.learning_rate), weight_decay=float(self.weight_decay),
+        params = self._init_params(d, widths, len(classes), x.device, gen)
+        optimizer = AdamW(params, lr=float(self.learning_rate), weight_decay=float(self.weight_decay),
                           max_norm=self.max_norm, state_bits=self.state_bits, seed=seed)
+        # from here on nothing of an earlier fit is left
+        self.classes_, self.n_features_in_, self._params, self._weight_codes = classes, d, params, None
         # half precision's gradients are scaled into its range; AdamW's step does
         # not depend on a gradient's scale but through eps, which is scaled too
         up = 1024.0 if self.dtype == "float16" else 1.0
@@ -278,7 +282,8 @@ class EmbeddingEncoder:
             if norms:
                 skipped.append((~torch.cat(norms).isfinite()).sum())
                 norms = []
-        self._weight_codes = self._codes(backward=False)
+        if self.products == "fp8":
+            self._weight_codes = self._codes(backward=False)
         self.loss_curve_ = torch.stack(self.loss_curve_).cpu().tolist()
         skipped = int(sum(skipped))
         if skipped:
