@@ -620,6 +620,8 @@ int32_t mlrs_dropout_bf16(const uint16_t *x, int64_t x_len, double p, uint64_t s
  * adjacent channels (8192 at most).  With mean and variance (over all of them, not
  * one less) of a sample's group over its positions, and rstd = 1 / sqrt(var + eps):
  *   z = (x - mean) rstd weight + bias,  y = drop(act(z)).
+ * Sums are f32: a group with an infinity or a NaN has rstd NaN and so all of its y;
+ * squares past f32's range give rstd 0.
  * weight and bias hold `channels` elements and may be NULL (1 and 0).  mean and
  * rstd (n x groups, f32) may both be NULL; the gradient takes them.
  * Errors, in this order: ShapeMismatch "x" / "features" (positions or channels

@@ -13,15 +13,16 @@
 // What bounds it is memory only without an activation; with one it is the vector
 // instructions, 26 an element forwards with silu and 48 backwards.  Three ways:
 //   rows      s = 1: a group is d adjacent elements, which some lanes of a wave, or
-//             a workgroup, hold.  16384 x 2048 bf16 in 16 groups, gelu, dropout: 44 us
-//             (3.1 TB/s), backwards 62 (3.2).
+//             a workgroup, hold.  16384 x 2048 bf16 in 16 groups, gelu, dropout: 45 us
+//             (3.0 TB/s), backwards 63 (3.2).
 //   resident  a workgroup holds a slab, some whole groups of a sample: a thread has
 //             eight adjacent channels at every so-manieth position.  16 x 1024 x 640
-//             bf16 in 32 groups, silu: 18 us (2.3 TB/s), backwards 29 (2.2).
+//             bf16 in 32 groups, silu: 17 us (2.4 TB/s), backwards 32 (2.0).
 //   split     groups past that: partial sums of runs of positions, then a second
 //             pass over the elements; it reads the sums first, so that it is the
-//             second launch of two.  16 x 4096 x 320 f16 in 32 groups, silu: 14 and
-//             21 us; the second pass finds its elements in the last cache.
+//             second launch of two.  16 x 4096 x 320 f16 in 32 groups, silu: 15 and
+//             21 us, bf16 as long, f32 53 together, backwards 55 and 88; the second
+//             pass finds its elements in the last cache.
 // The parameters' gradients are added up per thread while its channels stay the
 // same over samples and positions; a last launch adds those in order.
 #include <algorithm>
@@ -1146,7 +1147,8 @@ struct Way {
     int64_t parts;  // rows of the parameters' partial sums
 };
 
-// Positions of a thread of 512, as many as spill no registers.
+// Positions of a thread of 512: backwards as many as spill no registers (11 take 254 of
+// 256, six of f32 250); forwards one more than that (12 take 179, of f32 212).
 constexpr int most_positions(int elem_bytes, bool grad) { return !grad ? 12 : elem_bytes == 4 ? 6 : 11; }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1205,8 +1207,9 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
     // one workgroup at a time, whose loads, sums and stores follow one another: they are
     // taken where no CU gets a second one, whole octs first.  16 samples of 1024 positions
     // of 640 bf16 channels in 32 groups take 17.6 us so and 28.9 backwards, split 27.8
-    // and 46.6; 64 samples 62 and 111, split 53 and 86; 16 of 600 positions of 320, slabs
-    // of 70 channels, 21.8 and 38.5, split 18.2 and 24.
+    // and 46.6 (whole calls: 17 and 36; of 17 samples, split, 29 and 41); 64 samples 62 and
+    // 111, split 53 and 86; 16 of 600 positions of 320, slabs of 70 channels, 21.8 and 38.5,
+    // split 18.2 and 24.
     // A wave alone takes a row of channels that it can hold.  Where few positions would
     // leave most of 256 threads without work, a slab has more groups, as long as every
     // CU has four: 2499 samples of 5 positions of 2025 f16 channels in 27 groups take 266
@@ -1242,10 +1245,16 @@ Way choose(int elem_bytes, int64_t n, int64_t s, int64_t c, int64_t g, bool grad
         o.parts = o.slab.across;
         return o;
     }
-    // As many workgroups as run at once, four to a CU, backwards three, and six positions to
-    // a thread at least: a run's first and last steps cost as much as its rows.  16 x 4096
-    // x 320 f16 in 32 groups backwards: 54 us, of four to a CU 58, of eight 78; forwards 36,
-    // 36 and 51.  4 x 4096 x 320: 22 us, with four positions 27.
+    // As many workgroups as run at once in the 16-bit types, four to a CU (114 to 126
+    // registers a thread), backwards three (148 to 166), and six positions to a thread at
+    // least: a run's first and last steps cost as much as its rows.  16 x 4096 x 320 f16 in
+    // 32 groups backwards: 54 us, of four to a CU 58, of eight 78; forwards 36, 36 and 51.
+    // 4 x 4096 x 320: 22 us, with four positions 27.  f32's statistics run four to a CU as
+    // well, but its second pass three (139 registers) and its gradient's two (176, 191):
+    // their grids end in a part of a round; other counts were not measured there.
+    // Groups of more than 2048 channels take 1024 threads of 128 registers, which spill
+    // but for 16-bit forwards (f32 10 of them, backwards 41 and 53; 16 bits backwards 14
+    // to 29): 2 x 300 x 20000 in 4 groups, silu, 51 us in f16 and 85 backwards, f32 59, 142.
     o.kind = Way::kSplit;
     o.threads = octs <= 256 ? 256 : 1024;
     // as many whole groups as the threads have room for
